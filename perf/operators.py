@@ -7,6 +7,7 @@ A case names the heads, the page size, the element type, how many sequences ther
 many new tokens a sequence brings at most (`new`; the first `singles` sequences bring one), how many
 tokens are cached before them at most (`ctx`), `mix` (0: every sequence has just these lengths;
 else the seed of ragged ones) and `pad`, the rows of the token-major buffers behind the last sequence.
+`window`: how many slots back a token sees, itself counted (0: all of them).
 """
 import math
 import random
@@ -23,11 +24,13 @@ CACHE = 64 * 8 * 4096 * 128 + (1 << 22)  # cached elements of K of the largest l
 
 
 def _case(name, kind, heads, kv_heads, head_dim, page, dtype, seqs, new, ctx, singles=0, mix=0, pad=0, src="f32",
-          norm=True, half=False, rotary=None):
+          norm=True, half=False, rotary=None, window=0):
     c = dict(name=name, kind=kind, heads=heads, kv_heads=kv_heads, head_dim=head_dim, page=page, dtype=dtype,
              seqs=seqs, new=new, ctx=ctx, singles=singles, mix=mix, pad=pad)
     if kind == "append":
         c.update(src=src, norm=norm, half=half, rotary=head_dim if rotary is None else rotary)
+    else:
+        c.update(window=window)
     return c
 
 
@@ -54,8 +57,8 @@ def listed():
         _case("attend chunk 512", "attend", 32, 8, 128, 16, "f16", 1, 512, 2690),
         # a mixed step: chunks of three prompts beside single tokens of thirteen conversations
         _case("attend mixed bf16", "attend", 64, 8, 128, 32, "bf16", 16, 300, 2000, singles=13, mix=7),
-        # ragged prompts of a small model with narrow heads
-        _case("attend 5 prompts hd 64", "attend", 8, 2, 64, 64, "f16", 5, 1500, 0, mix=2),
+        # ragged prompts of a small model with narrow heads and a sliding window
+        _case("attend 5 prompts hd 64", "attend", 8, 2, 64, 64, "f16", 5, 1500, 0, mix=2, window=512),
         # the last chunk of a very long prompt
         _case("attend chunk 2048 ctx 14336", "attend", 32, 8, 128, 64, "f16", 1, 2048, 14336),
     ]
@@ -80,6 +83,8 @@ def draw(rng):
         c["ctx"] //= c["seqs"]  # a pool that the new tokens are a fair part of
         c.update(src=rng.choice(["f32", "f16", "bf16"]), norm=rng.random() < 0.8, half=rng.random() < 0.5,
                  rotary=rng.choice([0, head_dim // 2, head_dim, head_dim]))
+    else:
+        c["window"] = rng.choice([0, 0, 0, _log(rng, 1, 4096)])
     # no more work or memory than the largest listed case
     while (c["seqs"] * c["new"] * (c["ctx"] + c["new"]) * heads > CELLS
            or c["seqs"] * (c["ctx"] + c["new"] + 256) * kv_heads * head_dim > CACHE
@@ -171,7 +176,7 @@ def _own(state):
         b.append(state["qkv"], state["q_out"], state["inv_freq"], c["rotary"], q_norm=state["q_norm"],
                  k_norm=state["k_norm"], eps=EPS, half=c["half"], stream=stream)
         return {"q": state["q_out"], "k": state["k_pages"], "v": state["v_pages"]}
-    b.attend(state["q"], state["q_out"], state["scratch"], stream=stream)
+    b.attend(state["q"], state["q_out"], state["scratch"], window=c["window"], stream=stream)
     return state["q_out"]
 
 
@@ -230,6 +235,8 @@ def _attend(st):
     del k
     slot = torch.arange(L, device="cuda")
     seen = (slot <= pos[..., None]) & (table >= 0).repeat_interleave(P, 1)[:, None]  # [S, N, L]
+    if c["window"]:
+        seen &= slot > pos[..., None] - c["window"]
     s.masked_fill_(~seen[:, None, None], -math.inf)
     top = s.amax(-1, keepdim=True).clamp(min=-3e38)
     p = s.sub_(top).exp_()
@@ -285,13 +292,14 @@ def _exact_attend(st):
     first = 0
     for s, (n, m) in enumerate(zip(new, kv)):
         ids = st["page_table"][s, : -(-m // P)].long()
-        later = torch.arange(m, device="cuda")[None] > torch.arange(m - n, m, device="cuda")[:, None]
+        t, p = torch.arange(m, device="cuda")[None], torch.arange(m - n, m, device="cuda")[:, None]
+        hidden = (t > p) | (t <= p - (c["window"] or m + 1))
         for h in range(K):
             k = st["k_pages"][ids, h].double().reshape(-1, D)[:m]
             v = st["v_pages"][ids, h].double().reshape(-1, D)[:m]
             for a in range(h * G, (h + 1) * G):
                 q = st["q"][first: first + n, a * D: (a + 1) * D].double()
-                w = (q @ k.T / math.sqrt(D)).masked_fill_(later, -math.inf)
+                w = (q @ k.T / math.sqrt(D)).masked_fill_(hidden, -math.inf)
                 w = torch.softmax(w, -1)
                 out[first: first + n, a * D: (a + 1) * D] = w @ v
         first += n
@@ -305,5 +313,8 @@ def work(case):
     if case["kind"] == "append":
         return {"bytes": T * (H + 2 * K) * D * (SIZE[case["src"]] + e) + (8 * D if case["norm"] else 0),
                 "flops": T * (6 * (H + K) * D)}
-    pairs = sum(n * m - n * (n - 1) // 2 for n, m in zip(new, kv))  # (token, slot) pairs that the mask leaves
-    return {"bytes": 2 * T * H * D * e + 2 * sum(kv) * K * D * e, "flops": 4 * pairs * H * D}
+    W = case["window"] or 1 << 30
+    # (token, slot) pairs that the mask leaves, and the slots that any token sees
+    pairs = sum(min(p + 1, W) for n, m in zip(new, kv) for p in range(m - n, m))
+    slots = sum(min(m, n - 1 + W) for n, m in zip(new, kv))
+    return {"bytes": 2 * T * H * D * e + 2 * slots * K * D * e, "flops": 4 * pairs * H * D}
