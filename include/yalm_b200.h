@@ -293,6 +293,73 @@ int yb_prefill_gemm_dev(float* out_f32, uint16_t* out_f16, const uint16_t* a, co
 int yb_prefill_attention_dev(uint16_t* out, const float* q, const uint16_t* k_cache, const uint16_t* v_cache, int T,
                              int pos0, int n_heads, int n_kv_heads, int head_dim, int max_seq_len, void* stream);
 
+/* ---------------------------------------------------------------- paged KV cache of many sequences
+ * No counterpart in yalm, which keeps one contiguous cache of one sequence (src/model.cpp:203-204).
+ * The kernels of a serving step: append (per-head norm, rotation, store) and attention, over a batch
+ * of sequences that each bring a whole prompt, a chunk of one, or a single token. */
+
+#define YB_DTYPE_F32 0 /* yalm's DType order, src/codec.h:15-25 */
+#define YB_DTYPE_F16 1
+#define YB_DTYPE_BF16 2
+
+/* The batch.  Rows q_start[s] .. q_start[s + 1] - 1 of the token-major buffers are sequence s's new
+ * tokens (possibly none); kv_len[s] slots are in its cache, the new tokens among them, so its i-th of n
+ * new tokens has slot kv_len[s] - n + i.  Slot t lies in row t % page_size of page page_table[s][t /
+ * page_size].  The caches are [n_pages][n_kv_heads][page_size][head_dim].
+ *
+ * q_start, kv_len and the table are read on the device when the kernel runs: a captured launch may be
+ * replayed with new contents.  q_start must not decrease; rows before q_start[0] and from
+ * q_start[n_seqs] on are left as they are.  Values out of range never lead out of a buffer: q_start is
+ * taken as clamped to [0, n_tokens], kv_len to [0, max_pages * page_size], and a table entry outside
+ * [0, n_pages) stands for a page that is not there (nothing is stored in it, its slots are masked).
+ * Two sequences may read the same page; a page that tokens are appended to belongs to one sequence. */
+typedef struct yb_paged_batch {
+  int n_seqs;     /* up to 65536; 0 is an empty batch */
+  int n_tokens;   /* rows of the token-major buffers, up to 2^20 */
+  int n_heads;
+  int n_kv_heads; /* n_heads / n_kv_heads: a whole number from 1 to 16 */
+  int head_dim;   /* 64 or 128 */
+  int dtype;      /* of the caches, q and out: YB_DTYPE_F16 or YB_DTYPE_BF16 */
+  int page_size;  /* 16, 32, 64, 128 or 256 */
+  int n_pages;    /* pages in each cache */
+  int max_pages;  /* row length of page_table; max_pages * page_size up to 2^21 */
+  const int* q_start_dev;    /* [n_seqs + 1] */
+  const int* kv_len_dev;     /* [n_seqs] */
+  const int* page_table_dev; /* [n_seqs][max_pages] */
+  void* k_pages;             /* 16-byte aligned */
+  void* v_pages;
+} yb_paged_batch;
+
+/* Both entry points run on the current device and refuse (YB_E_INVALID) buffers that are not its memory.
+ * Rows of q, q_out, out and qkv are given by their strides in elements; base addresses and row
+ * strides must be multiples of 16 bytes.  No buffer that is written may overlap another one. */
+
+/* One pass over the new tokens' projections, the epilogue that yb_qkv_dev has for one token: qkv rows
+ * [n_heads query heads | n_kv_heads key heads | n_kv_heads value heads], of qkv_dtype (YB_DTYPE_*).
+ * Every element is clipped to +-qkv_clip (FLT_MAX: not at all); with q_norm_dev / k_norm_dev (head_dim
+ * fp32 weights, each may be NULL) every query / key head x becomes x / sqrt(mean(x^2) + eps) * w; the first
+ * rotary_dim elements of it are rotated by position * inv_freq_dev[j] (rotary_dim / 2 fp32 values), with
+ * pairs (2j, 2j + 1) as yalm has them (src/infer.cpp:205), or (j, j + rotary_dim / 2) when rope_half != 0
+ * (rotary_dim then a multiple of 8); queries go to q_out, keys and values to the token's slot.  The position
+ * is the slot, or pos_dev[row] when pos_dev is not NULL.  A token whose slot is negative or on a
+ * page that is not there is not stored; its query is written all the same.  Norms, angles (64 bits)
+ * and rotation are computed before the one rounding to dtype. */
+int yb_paged_append_dev(const yb_paged_batch* b, void* q_out, long long q_out_stride, const void* qkv,
+                        long long qkv_stride, int qkv_dtype, const float* q_norm_dev, const float* k_norm_dev,
+                        float eps, const float* inv_freq_dev, int rotary_dim, int rope_half, const int* pos_dev,
+                        float qkv_clip, void* stream);
+
+/* Causal attention of the new tokens over their sequences' caches, which hold them already: the token of
+ * slot p sees slots max(0, p - window + 1) .. p (window 0: 0 .. p), less those on pages that are not
+ * there; out = sum softmax(scale * q.k) v, or zeros where it sees no slot.  Slots from kv_len on and
+ * pages that are not there may hold anything, NaN included; the slots below kv_len hold finite values.
+ * scratch_dev: yb_paged_attention_scratch_bytes(b) bytes (the same for every batch of this head_dim on a
+ * device), zero-filled before its first use and left ready by every call; calls that may run at the
+ * same time, replayed graphs among them, each need their own. */
+int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long long out_stride, const void* q,
+                           long long q_stride, float scale, int window, void* scratch_dev, void* stream);
+size_t yb_paged_attention_scratch_bytes(const yb_paged_batch* b); /* 0 for a batch that is refused */
+
 /* Number of streaming multiprocessors the kernels size their grids for (device 0 if none set). */
 int yb_num_sms(void);
 

@@ -37,6 +37,12 @@ class yb_config(ctypes.Structure):
                [(n, ctypes.c_float) for n in ("rope_theta", "norm_eps", "qkv_clip")]
 
 
+class yb_paged_batch(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("n_seqs", "n_tokens", "n_heads", "n_kv_heads", "head_dim", "dtype",
+                                            "page_size", "n_pages", "max_pages")] + \
+               [(n, ctypes.c_void_p) for n in ("q_start_dev", "kv_len_dev", "page_table_dev", "k_pages", "v_pages")]
+
+
 _P = ctypes.c_void_p
 _PP = ctypes.POINTER(ctypes.c_void_p)
 
@@ -48,7 +54,7 @@ class yb_weights(ctypes.Structure):
 
 
 _lib = None
-_I, _F, _S = ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+_I, _F, _S, _LL = ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_longlong
 
 _SIGS = {
     "yb_create": (_I, [ctypes.POINTER(yb_config), ctypes.POINTER(yb_weights), _I, _I, _I, ctypes.POINTER(_P)]),
@@ -83,6 +89,9 @@ _SIGS = {
     "yb_attention_scratch_bytes": (_S, [_I, _I, _I, _I]),
     "yb_attention_plan_info": (_I, [_I, _I, _I, _I, _P]),
     "yb_attention_dev_noalloc": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "yb_paged_append_dev": (_I, [_P, _P, _LL, _P, _LL, _I, _P, _P, _F, _P, _I, _I, _P, _F, _P]),
+    "yb_paged_attention_dev": (_I, [_P, _P, _LL, _P, _LL, _F, _I, _P, _P]),
+    "yb_paged_attention_scratch_bytes": (_S, [_P]),
     "yb_num_sms": (_I, []),
     "yb_profile_kernel": (_I, [_P, _I, _I, ctypes.POINTER(_F)]),
 }
