@@ -136,6 +136,13 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
   tma_load_2d_s(smem_u32(dst), map, x, y, smem_u32(bar));
 }
 
+__device__ __forceinline__ void tma_load_3d_s(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
 // ---------------------------------------------------------------- warp-level mma (m16n8k16, fp16)
 // Fragment layouts as the PTX ISA defines them for mma.m16n8k16 with .f16 inputs: with
 // g = lane / 4 and c = lane % 4, A (16 x 16, row) holds {(g, 2c..2c+1), (g+8, 2c..), (g, 2c+8..),

@@ -1,70 +1,772 @@
-// Attention of a batch's new tokens over the paged KV cache, the simplest form: a warp per (row, head),
-// one key at a time, online softmax.
+// Attention of a batch's new tokens over the paged KV cache on the 5th-generation tensor cores:
+//
+//   o[token, head] = sum_t 2^(c q.k_t - m) v_t / sum_t 2^(c q.k_t - m),   c = scale * log2(e),
+//
+// over the slots t that the token sees, in one pass over the keys with a running maximum m and sum.
+// Whole prompts, chunks and single tokens take the same path in one launch.
+//
+// Work.  A unit is (sequence, kv head, block of up to 2 QB queries), QB = 128 / (query heads per kv head):
+// its rows are (query, head of the group) pairs, in two row tiles of 128, so every K and V tile that is
+// loaded serves all query heads of its group.  A unit's cost is its number of 128-slot key tiles.  The
+// units of the whole batch in order make one axis of key tiles, which the blocks (one per SM) share out
+// evenly: a long cache of few rows is cut over many blocks, and ragged lengths balance themselves.
+// The cuts follow from the lengths on the device, by a closed form for a sequence's tiles (floor
+// sums), so there is no plan to be made on the host and a captured launch follows new lengths.  A unit
+// that is cut leaves (o, m, l) records in the workspace; the block that finishes it last merges them in
+// the order of the slots, so results do not depend on timing.
+//
+// Block.  Two pipelines of 128 rows share the tensor cores, one's softmax under the other's products:
+//   warp 0       loads Q (a 3-D box of queries x heads) and the ring of K and V tiles, one lane a page
+//   warp 1       issues the products: S[p] = Q . K^T into tensor memory, then O[p] += P . V with P read from
+//                tensor memory, where it took the place of S
+//   warps 4-7, 8-11   softmax of pipeline 0 / 1, a row per thread
+// A unit of two row tiles runs them as the pipelines over the same key tiles.  A unit of one row tile (single
+// tokens, short chunks) gives the pipelines alternate key tiles, and merges the two at its end.
+//
+// P is rounded to the caches' type for the tensor cores (the weights' rounding error is that of the
+// output's rounding, and averages over the slots); scores, maxima, sums and outputs are fp32.  The output is
+// rescaled only when a row's maximum grew by more than 2^8: until then the old maximum serves, and every
+// weight stays below 2^8.  fp16 weights carry a factor 2^7, which keeps the small ones above 2^-32 of the
+// largest out of the subnormal range.
 #include "paged.cuh"
 
 #include <cuda_bf16.h>
 
 #include <math.h>
+#include <type_traits>
+
+#include "launch.h"
+#include "tmap.h"
+#include "umma.cuh"
 
 namespace yb {
 
 namespace {
 
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void put(__half* p, float x) { *p = __float2half_rn(x); }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+constexpr int kKT = 128;       // slots per key tile
+constexpr int kRows = 128;     // rows per row tile = tensor-memory lanes
+constexpr int kThreads = 384;
+constexpr int kMaxGrid = 256;  // blocks the workspace has counters for
+constexpr int kMinTiles = 1;   // key tiles a block takes at least
+constexpr uint32_t kBlk = kRows * 128;  // bytes of 128 rows x 64 elements
 
-template <int HD, typename T>
-__global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) {
-  const int row = blockIdx.x, lane = threadIdx.x & 31;
-  const int h = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (h >= a.b.n_heads) return;
-  const int seq = paged_find_seq(a.b, row);
-  if (seq < 0) return;
-  const PagedSeq sq = paged_seq(a.b, seq);
-  if (row - sq.row0 >= sq.n) return;
-  const int p = sq.kv - sq.n + row - sq.row0;
-  const int g = h / (a.b.n_heads / a.b.n_kv_heads);
-  constexpr int V = HD / 32;
-  const T* qp = static_cast<const T*>(a.q) + (size_t)row * a.q_stride + (size_t)h * HD;
-  float q[V], o[V], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < V; ++i) q[i] = to_f(qp[lane + 32 * i]) * a.scale, o[i] = 0.f;
-  const int t0 = p >= a.window ? p - a.window + 1 : 0;
-  const int mask = (1 << a.b.ps_log2) - 1;
-  for (int t = t0; t <= p; ++t) {
-    const int page = __ldg(a.b.page_table + (size_t)seq * a.b.max_pages + (t >> a.b.ps_log2));
-    if (page < 0 || page >= a.b.n_pages) continue;
-    const size_t at = ((((size_t)page * a.b.n_kv_heads + g) << a.b.ps_log2) + (t & mask)) * HD;
-    const T* k = static_cast<const T*>(a.k_pages) + at;
-    const T* v = static_cast<const T*>(a.v_pages) + at;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) s += q[i] * to_f(k[lane + 32 * i]);
-    s = warp_sum(s);
-    const float mn = fmaxf(m, s), c = expf(m - mn), w = expf(s - mn);
-    l = l * c + w;
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = o[i] * c + w * to_f(v[lane + 32 * i]);
-    m = mn;
+template <int HD>
+struct Cfg {
+  static constexpr int kHalves = HD / 64;
+  static constexpr int kStages = HD == 128 ? 5 : 10;
+  static constexpr uint32_t kTile = kHalves * kBlk;  // a row tile of Q, a K tile or a V tile
+  static constexpr uint32_t kSmem = (2 + kStages) * kTile + 1024 + 1024;  // + (m, l) of pipeline 1, + alignment
+};
+
+// -------------------------------------------------------------------------------------- the work axis
+// sum_{i < n} floor((a i + b) / m), a, b >= 0: each round takes the whole parts out and swaps the roles of the
+// axes, as Euclid's algorithm does.  The arguments here keep every product below 2^32.
+__device__ __forceinline__ unsigned floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
+  unsigned s = 0;
+  while (n) {
+    s += (a / m) * (n * (n - 1) / 2) + (b / m) * n;
+    a %= m;
+    b %= m;
+    const unsigned y = a * n + b;
+    n = y / m;
+    b = y % m;
+    const unsigned t = m;
+    m = a;
+    a = t;
+    if (!m) break;
   }
-  T* out = static_cast<T*>(a.out) + (size_t)row * a.out_stride + (size_t)h * HD;
-#pragma unroll
-  for (int i = 0; i < V; ++i) put(out + lane + 32 * i, l > 0.f ? o[i] / l : 0.f);
+  return s;
 }
+// sum_{i < n} floor(max(0, a + i u) / 128)
+__device__ __forceinline__ unsigned ramp(int n, int a, int u) {
+  if (a < 0) {
+    const int skip = (-a + u - 1) / u;
+    if (skip >= n) return 0;
+    n -= skip;
+    a += skip * u;
+  }
+  return n > 0 ? floor_sum((unsigned)n, kKT, (unsigned)u, (unsigned)a) : 0u;
+}
+
+struct Unit {
+  int q0, nq;      // queries [q0, q0 + nq) of the sequence
+  int tile0;       // first key tile
+  int cost;        // key tiles, at least 1
+  bool none;       // no slot is seen: zeros
+};
+struct Axis {
+  int U, window, K;  // queries per unit, window, kv heads
+};
+__device__ __forceinline__ Unit unit_of(const Axis& x, const PagedSeq& q, int i) {
+  Unit u;
+  const int p0 = q.kv - q.n;
+  u.q0 = i * x.U;
+  u.nq = min(x.U, q.n - u.q0);
+  const int end = p0 + u.q0 + u.nq;
+  u.tile0 = max(0, p0 + u.q0 - x.window + 1) / kKT;
+  u.none = end <= 0;
+  u.cost = max(1, (end + kKT - 1) / kKT - u.tile0);
+  return u;
+}
+__device__ __forceinline__ int n_units(const Axis& x, const PagedSeq& q) { return (q.n + x.U - 1) / x.U; }
+// key tiles of the first m units of a (sequence, kv head), m < n_units: unit i ends at slot p0 + (i + 1) U
+__device__ __forceinline__ unsigned units_before(const Axis& x, const PagedSeq& q, int m) {
+  const int p0 = q.kv - q.n;
+  return (unsigned)m + ramp(m, p0 + x.U - 1, x.U) - ramp(m, p0 - x.window + 1, x.U);
+}
+__device__ __forceinline__ unsigned head_tiles(const Axis& x, const PagedSeq& q) {
+  if (q.n <= 0) return 0;
+  const int nu = n_units(x, q);
+  return units_before(x, q, nu - 1) + (unsigned)unit_of(x, q, nu - 1).cost;
+}
+
+// Where a block starts, and its share.
+struct Start {
+  int seq, head, unit, off;
+  int left;          // key tiles of this block
+  long long begin;   // first key tile on the axis
+  long long total;
+  int blocks;        // blocks that have work
+};
+// begin of block c, and the block that holds tile x
+__device__ __forceinline__ long long block_begin(long long total, int blocks, int c) { return total * c / blocks; }
+__device__ __forceinline__ int block_of(long long total, int blocks, long long x) {
+  return (int)(((x + 1) * blocks + total - 1) / total) - 1;
+}
+
+// The next piece of this block's share: tiles [t0, t1) of a unit.
+struct Piece {
+  PagedSeq sq;
+  int seq, head;
+  Unit u;
+  int t0, t1;
+};
+struct Walk {
+  Start st;
+  PagedSeq sq;
+  __device__ __forceinline__ Walk(const PagedBatch& b, const Start& s) : st(s) {
+    if (st.left > 0) sq = paged_seq(b, st.seq);
+  }
+  __device__ __forceinline__ bool next(const PagedBatch& b, const Axis& x, Piece& p) {
+    if (st.left <= 0 || st.seq >= b.n_seqs) return false;
+    p.sq = sq;
+    p.seq = st.seq;
+    p.head = st.head;
+    p.u = unit_of(x, sq, st.unit);
+    p.t0 = st.off;
+    p.t1 = min(p.u.cost, st.off + st.left);
+    st.left -= p.t1 - p.t0;
+    st.off = p.t1;
+    if (st.off == p.u.cost && st.left > 0) {
+      st.off = 0;
+      if (++st.unit >= n_units(x, sq)) {
+        st.unit = 0;
+        if (++st.head >= x.K) {
+          st.head = 0;
+          do {
+            if (++st.seq >= b.n_seqs) break;
+            sq = paged_seq(b, st.seq);
+          } while (sq.n <= 0);
+        }
+      }
+    }
+    return true;
+  }
+};
+
+// Called by the whole block: this block's share of the axis.
+__device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long long* s_warp, Start* s_start) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = (b.n_seqs + kThreads - 1) / kThreads;
+  const int s0 = min(b.n_seqs, (int)threadIdx.x * per), s1 = min(b.n_seqs, s0 + per);
+  unsigned long long mine = 0;
+  for (int s = s0; s < s1; ++s) mine += (unsigned long long)head_tiles(x, paged_seq(b, s)) * x.K;
+  unsigned long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) s_warp[warp] = incl;
+  if (threadIdx.x == 0) s_start->left = 0;
+  __syncthreads();
+  unsigned long long before = incl - mine, total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += s_warp[w];
+    total += s_warp[w];
+  }
+  if (!total) return;
+  const long long most = (long long)(total + kMinTiles - 1) / kMinTiles;
+  const int blocks = (int)(most < gridDim.x ? most : gridDim.x);
+  const int c = blockIdx.x;
+  if (c >= blocks) return;
+  const unsigned long long begin = block_begin(total, blocks, c), end = block_begin(total, blocks, c + 1);
+  if (begin < before || begin >= before + mine) return;
+  // this thread's sequences hold the block's first tile
+  unsigned long long rem = begin - before;
+  for (int s = s0; s < s1; ++s) {
+    const PagedSeq q = paged_seq(b, s);
+    const unsigned per_head = head_tiles(x, q);
+    const unsigned long long all = (unsigned long long)per_head * x.K;
+    if (rem >= all) {
+      rem -= all;
+      continue;
+    }
+    Start st;
+    st.seq = s;
+    st.head = (int)(rem / per_head);
+    const unsigned in_head = (unsigned)(rem % per_head);
+    int lo = 0, hi = n_units(x, q);  // units_before(lo) <= in_head < units_before(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (units_before(x, q, mid) <= in_head) lo = mid; else hi = mid;
+    }
+    st.unit = lo;
+    st.off = (int)(in_head - units_before(x, q, lo));
+    st.left = (int)(end - begin);
+    st.begin = (long long)begin;
+    st.total = (long long)total;
+    st.blocks = blocks;
+    *s_start = st;
+    return;
+  }
+}
+
+// -------------------------------------------------------------------------------------------- numerics
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// bits [lo, hi) of a 32-bit word, lo and hi clipped to [0, 32]
+__device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
+  lo = min(max(lo, 0), 32);
+  hi = min(max(hi, 0), 32);
+  if (lo >= hi) return 0u;
+  return (0xffffffffu >> (32 - (hi - lo))) << lo;
+}
+
+// Workspace: [0] status word, [64 ..] counters, then per block and slot (0: a unit begun by an earlier block, 1:
+// one that a later block goes on with) 2 x 256 floats (m, l) and 256 rows of HD floats.
+constexpr size_t kHeadBytes = 256 + kMaxGrid * 4;
+template <int HD>
+constexpr size_t rec_floats() { return 2 * 256 + 256 * (size_t)HD; }
 
 }  // namespace
 
-size_t paged_attention_scratch(int head_dim, int n_sms) { return 256; }
+struct PagedAttnParams {
+  PagedBatch b;
+  Axis x;
+  void* out;
+  long long out_stride;
+  float c;  // scale * log2(e)
+  int gq;   // query heads per kv head
+  int oob;  // a row outside the page pool's tensor maps
+  unsigned* head;
+  float* recs;
+};
 
-cudaError_t paged_attention(const PagedAttnArgs& a, int head_dim, int type, cudaStream_t s) {
-  const void* fn = head_dim == 128 ? (type == 1 ? reinterpret_cast<const void*>(&paged_attn_kernel<128, __half>)
-                                                : reinterpret_cast<const void*>(&paged_attn_kernel<128, __nv_bfloat16>))
-                                   : (type == 1 ? reinterpret_cast<const void*>(&paged_attn_kernel<64, __half>)
-                                                : reinterpret_cast<const void*>(&paged_attn_kernel<64, __nv_bfloat16>));
-  void* args[] = {const_cast<PagedAttnArgs*>(&a)};
-  return cudaLaunchKernel(fn, dim3(a.b.n_tokens, (a.b.n_heads + 3) / 4), dim3(128), args, 0, s);
+template <int HD, typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                      const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PagedAttnParams a) {
+  using C = Cfg<HD>;
+  constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+  constexpr uint32_t kIdS = kBf16 ? umma_idesc_bf16(kRows, kKT, 0, 0) : umma_idesc_f16(kRows, kKT, 0, 0);
+  constexpr uint32_t kIdO = kBf16 ? umma_idesc_bf16(kRows, HD, 0, 1) : umma_idesc_f16(kRows, HD, 0, 1);
+  constexpr float kBias = kBf16 ? 0.f : 7.f;
+  constexpr uint32_t kColO = 2 * kKT;  // tensor memory: S0, S1, O0, O1
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t sb = smem_u32(smem), ring = sb + 2 * C::kTile;
+  float* s_ml = reinterpret_cast<float*>(smem + (2 + C::kStages) * C::kTile);  // [2][128]
+  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], q_full, q_empty, s_full[2], p_full[2],
+      o_done[2], o_free, ml_ready, ml_free, rec_done, rec_last;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort, s_last;
+  __shared__ unsigned long long s_scan[kThreads / 32];
+  __shared__ Start s_start;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PagedBatch& b = a.b;
+  find_start(b, a.x, s_scan, &s_start);
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&q_full, 1);
+    mbar_init(&q_empty, 1);
+    for (int p = 0; p < 2; ++p) {
+      mbar_init(&s_full[p], 1);
+      mbar_init(&p_full[p], 4);
+      mbar_init(&o_done[p], 1);
+    }
+    mbar_init(&o_free, 8);
+    mbar_init(&ml_ready, 4);
+    mbar_init(&ml_free, 4);
+    mbar_init(&rec_done, 8);
+    mbar_init(&rec_last, 1);
+    mbar_fence_init();
+  }
+  __syncthreads();
+  if (s_start.left <= 0) return;
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  volatile int* abort_flag = &s_abort;
+  unsigned* status = a.head;
+  const int QB = kRows / a.gq;
+  Walk walk(b, s_start);
+  Piece pc;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------------------- loads
+    const int lg = b.ps_log2, ps = 1 << lg;
+    const int boxes = ps >= kKT ? 1 : kKT >> lg;  // pages per key tile
+    const uint32_t box_bytes = (uint32_t)min(ps, kKT) * 128u;
+    unsigned it = 0, pieces = 0;
+    bool ok = true;
+    while (ok && !*abort_flag && walk.next(b, a.x, pc)) {
+      if (pc.u.none) continue;
+      const bool two = pc.u.nq > QB;
+      // Q, once the products of the piece before have read theirs
+      if (pieces && !(ok = mbar_wait(&q_empty, (pieces - 1) & 1, status))) break;
+      ++pieces;
+      if (lane == 0) {
+        const uint32_t bytes = (uint32_t)(QB * a.gq) * 128u;
+        mbar_arrive_expect_tx(&q_full, bytes * C::kHalves * (two ? 2 : 1));
+        for (int t = 0; t < (two ? 2 : 1); ++t)
+          for (int h = 0; h < C::kHalves; ++h)
+            tma_load_3d_s(sb + t * C::kTile + h * kBlk, &qmap, 64 * h, pc.head * a.gq, pc.sq.row0 + pc.u.q0 + t * QB,
+                          smem_u32(&q_full));
+      }
+      const int* table = b.page_table + (size_t)pc.seq * b.max_pages;
+      // row of the page pool where this lane's page of a key tile starts (outside it: zeros)
+      auto row_of = [&](int tile) {
+        const int slot = (tile << 7) + (lane << lg);
+        if (lane >= boxes || slot >= pc.sq.kv) return a.oob;
+        const int id = __ldg(table + (slot >> lg));
+        if (id < 0 || id >= b.n_pages) return a.oob;
+        return ((id * a.x.K + pc.head) << lg) + (slot & (ps - 1));
+      };
+      auto load = [&](const CUtensorMap* map, int row) {
+        const int s = it % C::kStages;
+        if (it >= C::kStages && !mbar_wait(&empty[s], (it / C::kStages - 1) & 1, status)) return false;
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], C::kTile);
+        __syncwarp();
+        if (lane < boxes)
+          for (int h = 0; h < C::kHalves; ++h)
+            tma_load_2d_s(ring + s * C::kTile + h * kBlk + lane * box_bytes, map, 64 * h, row, smem_u32(&full[s]));
+        ++it;
+        return true;
+      };
+      // in the order of the products: K of steps 0 and 1, then V of step i and K of step i + 2
+      const int first = pc.u.tile0 + pc.t0, n = pc.t1 - pc.t0, ahead = two ? 1 : 2;
+      int next_row = row_of(first);
+      for (int j = 0; j < n + ahead && ok; ++j) {
+        if (j >= ahead) ok = load(&vmap, row_of(first + j - ahead));
+        if (ok && j < n) {
+          const int row = next_row;
+          if (j + 1 < n) next_row = row_of(first + j + 1);
+          ok = load(&kmap, row);
+        }
+      }
+    }
+    if (!ok) *abort_flag = 1;
+    // never leave while a copy issued here may still be landing
+    for (unsigned i = it > C::kStages ? it - C::kStages : 0; i < it; ++i)
+      mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1, status);
+    if (pieces) mbar_wait(&q_full, (pieces - 1) & 1, status);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------------------- products
+    unsigned it = 0, pieces = 0, steps[2] = {0, 0};
+    bool ok = true;
+    while (ok && !*abort_flag && walk.next(b, a.x, pc)) {
+      if (pc.u.none) continue;
+      const bool two = pc.u.nq > QB;
+      const int first = pc.u.tile0 + pc.t0, nk = pc.t1 - pc.t0, n = two ? 2 * nk : nk;
+      if (!(ok = mbar_wait(&q_full, pieces & 1, status))) break;
+      int kslot = 0, vslot = 0;
+      auto qk = [&](int i) {
+        if (!two || !(i & 1)) {
+          kslot = it % C::kStages;
+          if (!mbar_wait(&full[kslot], (it / C::kStages) & 1, status)) return false;
+          ++it;
+        }
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t q = sb + (two && (i & 1) ? C::kTile : 0u), k = ring + kslot * C::kTile;
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint32_t off = (uint32_t)(kk / 4) * kBlk + (uint32_t)(kk % 4) * 32u;
+            umma_f16(tmem + (uint32_t)(i & 1) * kKT, umma_desc_k_sw128(q + off), umma_desc_k_sw128(k + off), kIdS, kk ? 1u : 0u);
+          }
+          umma_commit(&s_full[i & 1]);
+          if (!two || (i & 1)) umma_commit(&empty[kslot]);
+          if (i == n - 1) umma_commit(&q_empty);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto pv = [&](int i) {
+        const int p = i & 1;
+        if (!two || !p) {
+          vslot = it % C::kStages;
+          if (!mbar_wait(&full[vslot], (it / C::kStages) & 1, status)) return false;
+          ++it;
+          // slots behind the sequence's last one, in its last page, may hold anything: their weight is 0, and
+          // 0 * v has to be 0
+          const int rem = pc.sq.kv - (first + (two ? i >> 1 : i)) * kKT;
+          const int end = min(kKT, ((rem + (1 << b.ps_log2) - 1) >> b.ps_log2) << b.ps_log2);
+          if (rem < end) {
+            const uint32_t v = ring + vslot * C::kTile;
+            for (int e = lane; e < (end - rem) * 8 * C::kHalves; e += 32) {
+              const int h = e / ((end - rem) * 8), r = e % ((end - rem) * 8);
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * kBlk + (rem * 8 + r) * 16u), "r"(0u)
+                           : "memory");
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        if (i < 2 && pieces && !mbar_wait(&o_free, (pieces - 1) & 1, status)) return false;
+        if (!mbar_wait(&p_full[p], steps[p] & 1, status)) return false;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t v = ring + vslot * C::kTile;
+#pragma unroll
+          for (int kk = 0; kk < kKT / 16; ++kk)
+            umma_f16_ta(tmem + kColO + (uint32_t)p * HD, tmem + (uint32_t)p * kKT + kk * 8,
+                        umma_desc_sw128(v + kk * 2048u, kBlk, 1024), kIdO, (i >= 2 || kk) ? 1u : 0u);
+          umma_commit(&o_done[p]);
+          if (!two || p) umma_commit(&empty[vslot]);
+        }
+        __syncwarp();
+        ++steps[p];
+        return true;
+      };
+      ok = qk(0) && (n < 2 || qk(1));
+      for (int i = 0; i < n && ok && !*abort_flag; ++i) {
+        ok = pv(i);
+        if (ok && i + 2 < n) ok = qk(i + 2);
+      }
+      ++pieces;
+    }
+    if (!ok) *abort_flag = 1;
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------------------- softmax
+    const int p = (warp - 4) >> 2, quad = warp & 3;  // pipeline, tensor-memory lane quadrant
+    const int r = quad * 32 + lane;                  // row of the row tile
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const uint32_t ts = tmem + lanes + (uint32_t)p * kKT, to = tmem + lanes + kColO;
+    const int qi = r / a.gq, h = r % a.gq;
+    unsigned steps[2] = {0, 0};  // steps of either pipeline in the pieces before
+    unsigned pieces = 0, singles = 0, cuts = 0;
+    bool ok = true;
+    while (ok && !*abort_flag && walk.next(b, a.x, pc)) {
+      const bool two = pc.u.nq > QB;
+      const int nk = pc.u.none ? 0 : pc.t1 - pc.t0;
+      const int tile = two ? p : 0;  // row tile
+      const int q = tile * QB + qi;  // query of the unit
+      const bool valid = r < QB * a.gq && q < pc.u.nq;
+      const bool live = quad * 32 < min(QB, pc.u.nq - tile * QB) * a.gq;  // any row of the warp
+      const int pos = pc.sq.kv - pc.sq.n + pc.u.q0 + q;
+      const int* table = b.page_table + (size_t)pc.seq * b.max_pages;
+      const int first = pc.u.tile0 + pc.t0;
+      const int mine = two ? nk : (nk + 1 - p) / 2, inc = two ? 1 : 2, off = two ? 0 : p;
+      // whether the 16 slots of lane i < 8 are on a page that is there
+      auto there = [&](int t) {
+        const int slot = (t << 7) + lane * 16;
+        int id = -1;
+        if (lane < 8 && slot < pc.sq.kv) id = __ldg(table + (slot >> b.ps_log2));
+        return lane < 8 && id >= 0 && id < b.n_pages;
+      };
+      float m = -INFINITY, l = 0.f;
+      bool nx = mine > 0 && there(first + off);
+      for (int i = 0; i < mine; ++i) {
+        const int t = first + off + i * inc;
+        const uint32_t pages = __ballot_sync(0xffffffffu, nx) & 0xffu;
+        if (i + 1 < mine) nx = there(t + inc);
+        if (*abort_flag || !(ok = mbar_wait(&s_full[p], (steps[p] + i) & 1, status))) break;
+        tc_fence_after();
+        if (live) {
+          const int k0 = t * kKT;
+          const int lo = valid ? pos - a.x.window + 1 - k0 : kKT, hi = valid ? pos + 1 - k0 : 0;
+          const bool all = lo <= 0 && hi >= kKT && pages == 0xffu;
+          uint32_t msk[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t pg = ((pages >> (2 * w)) & 1u ? 0xffffu : 0u) | ((pages >> (2 * w + 1)) & 1u ? 0xffff0000u : 0u);
+            msk[w] = bit_range(lo - 32 * w, hi - 32 * w) & pg;
+          }
+          float mx = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            float s[32];
+            tmem_ld32(ts + 32 * w, s);
+            if (all) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) mx = fmaxf(mx, s[k]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) mx = fmaxf(mx, (msk[w] >> k) & 1u ? s[k] : -INFINITY);
+            }
+          }
+          mx *= a.c;
+          const bool need = mx > m + 8.0f;  // the first slots seen, or a maximum grown by over 2^8
+          const float mn = need ? mx : m;
+          const float alpha = need ? ex2(m - mn) : 1.f;  // 0 while m is -inf
+          if (i > 0 && __any_sync(0xffffffffu, need)) {
+            if (!(ok = mbar_wait(&o_done[p], (steps[p] + i - 1) & 1, status))) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c0 = 0; c0 < HD; c0 += 32) {
+              float v[32];
+              tmem_ld32(to + p * HD + c0, v);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[k] *= alpha;
+              tmem_st32(to + p * HD + c0, v);
+            }
+          }
+          m = mn;
+          const float shift = m == -INFINITY ? 0.f : m - kBias;
+          float sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            float s[32];
+            tmem_ld32(ts + 32 * w, s);
+            uint32_t pk[16];
+            if (all) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) s[k] = ex2(fmaf(s[k], a.c, -shift));
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) s[k] = (msk[w] >> k) & 1u ? ex2(fmaf(s[k], a.c, -shift)) : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              sum += s[2 * k] + s[2 * k + 1];
+              pk[k] = pack2<T>(s[2 * k], s[2 * k + 1]);
+            }
+            tmem_st16_u32(ts + 16 * w, pk);
+          }
+          l = l * alpha + sum;
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[p]);
+      }
+      if (!ok || *abort_flag) break;
+
+      // ---- the piece's rows: o * w0 (+ o of pipeline 1 * w1)
+      const int other = two ? 0 : nk / 2;  // steps of pipeline 1 that pipeline 0 merges
+      float w0 = 1.f, w1 = 0.f;
+      if (mine > 0) {
+        if (!(ok = mbar_wait(&o_done[p], (steps[p] + mine - 1) & 1, status))) break;
+      }
+      if (!two && nk > 0) {
+        if (p == 1) {
+          // pipeline 0 is through with the piece before (it may be slower than a pipeline without steps)
+          if (singles && !(ok = mbar_wait(&ml_free, (singles - 1) & 1, status))) break;
+          s_ml[r] = m;
+          s_ml[kRows + r] = l;
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&ml_ready);
+            mbar_arrive(&o_free);  // pipeline 0 reads the outputs
+          }
+        } else {
+          if (!(ok = mbar_wait(&ml_ready, singles & 1, status))) break;
+          if (other > 0) {
+            if (!(ok = mbar_wait(&o_done[1], (steps[1] + other - 1) & 1, status))) break;
+            const float m1 = s_ml[r], l1 = s_ml[kRows + r], mm = fmaxf(m, m1);
+            w0 = m == -INFINITY ? 0.f : ex2(m - mm);
+            w1 = m1 == -INFINITY ? 0.f : ex2(m1 - mm);
+            l = l * w0 + l1 * w1;
+            m = mm;
+          }
+        }
+        ++singles;
+      }
+      tc_fence_after();
+      const bool whole = pc.t0 == 0 && pc.t1 == pc.u.cost;
+      const int slot = pc.t0 == 0 ? 1 : 0;
+      float* rec = a.recs + ((size_t)blockIdx.x * 2 + slot) * rec_floats<HD>();
+      const size_t token = (size_t)pc.sq.row0 + pc.u.q0 + q;
+      T* out = static_cast<T*>(a.out) + token * a.out_stride + (size_t)(pc.head * a.gq + h) * HD;
+      if (two || p == 0) {
+        const float inv = whole ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
+        w0 *= inv;
+        w1 *= inv;
+        if (live) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < HD; c0 += 32) {
+            float v[32];
+            if (nk > 0) {
+              tmem_ld32(to + p * HD + c0, v);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[k] = l != 0.f ? v[k] * w0 : 0.f;
+              if (other > 0) {
+                float v1[32];
+                tmem_ld32(to + HD + c0, v1);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) v[k] = l != 0.f ? fmaf(v1[k], w1, v[k]) : 0.f;
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[k] = 0.f;
+            }
+            if (!valid) continue;
+            if (whole) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                reinterpret_cast<uint4*>(out + c0)[k] =
+                    make_uint4(pack2<T>(v[8 * k], v[8 * k + 1]), pack2<T>(v[8 * k + 2], v[8 * k + 3]),
+                               pack2<T>(v[8 * k + 4], v[8 * k + 5]), pack2<T>(v[8 * k + 6], v[8 * k + 7]));
+            } else {
+              float4* o = reinterpret_cast<float4*>(rec + 512 + (size_t)(tile * kRows + r) * HD + c0);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) o[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+            }
+          }
+        }
+        if (!whole && valid) {
+          rec[tile * kRows + r] = m;
+          rec[256 + tile * kRows + r] = l;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (nk > 0 && lane == 0) {
+          mbar_arrive(&o_free);
+          if (!two) mbar_arrive(&ml_free);
+        }
+      }
+      if (!whole) {
+        // ---- a cut unit: the block that counts last merges every block's record
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&rec_done);
+        const long long begin = s_start.begin + (s_start.left - walk.st.left) - pc.t1;  // the unit's first tile
+        const int c0 = block_of(s_start.total, s_start.blocks, begin);
+        const int c1 = block_of(s_start.total, s_start.blocks, begin + pc.u.cost - 1);
+        if (threadIdx.x == 128) {
+          int last = 0;
+          if (mbar_wait(&rec_done, cuts & 1, status)) {
+            last = atom_add_acq_rel_gpu(a.head + 64 + c0, 1u) == (unsigned)(c1 - c0);
+            if (last) a.head[64 + c0] = 0u;
+          }
+          s_last = last;
+          mbar_arrive(&rec_last);
+        }
+        __syncwarp();
+        if (!(ok = mbar_wait(&rec_last, cuts & 1, status))) break;
+        ++cuts;
+        if (s_last) {
+          const int tid = threadIdx.x - 128;
+          const float* base = a.recs;
+          auto part = [&](int c) { return base + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * rec_floats<HD>(); };
+          const int n0 = min(QB, pc.u.nq) * a.gq, n1 = (pc.u.nq - min(QB, pc.u.nq)) * a.gq;
+          for (int e = tid; e < (n0 + n1) * (HD / 4); e += 256) {
+            const int er = e / (HD / 4), ec = e % (HD / 4) * 4;
+            const int rr = er < n0 ? er : kRows + er - n0;
+            float mm = -INFINITY;
+            for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, __ldcg(part(c) + rr));
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float ll = 0.f;
+            for (int c = c0; c <= c1; ++c) {
+              const float* pr = part(c);
+              const float mc = __ldcg(pr + rr), lc = __ldcg(pr + 256 + rr);
+              const float4 o = __ldcg(reinterpret_cast<const float4*>(pr + 512 + (size_t)rr * HD + ec));
+              const float w = mc == -INFINITY ? 0.f : ex2(mc - mm);
+              ll = fmaf(lc, w, ll);
+              acc.x = fmaf(o.x, w, acc.x);
+              acc.y = fmaf(o.y, w, acc.y);
+              acc.z = fmaf(o.z, w, acc.z);
+              acc.w = fmaf(o.w, w, acc.w);
+            }
+            const float inv = ll != 0.f ? 1.f / ll : 0.f;
+            const int eq = er / a.gq, eh = er % a.gq;
+            T* eo = static_cast<T*>(a.out) + ((size_t)pc.sq.row0 + pc.u.q0 + eq) * a.out_stride +
+                    (size_t)(pc.head * a.gq + eh) * HD + ec;
+            *reinterpret_cast<uint2*>(eo) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+          }
+        }
+      }
+      steps[0] += two ? nk : (nk + 1) / 2;
+      steps[1] += two ? nk : nk / 2;
+      ++pieces;
+    }
+    if (!ok) *abort_flag = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+size_t paged_attention_scratch(int head_dim, int n_sms) {
+  const int grid = n_sms < kMaxGrid ? n_sms : kMaxGrid;
+  return kHeadBytes + (size_t)grid * 2 * (head_dim == 128 ? rec_floats<128>() : rec_floats<64>()) * 4;
+}
+
+namespace {
+template <int HD, typename T>
+cudaError_t launch(const PagedAttnArgs& a, int grid, bool bf16, cudaStream_t s) {
+  const int K = a.b.n_kv_heads, ps = 1 << a.b.ps_log2, gq = a.b.n_heads / K, qb = kRows / gq;
+  const long long rows = (long long)a.b.n_pages * K * ps;
+  CUtensorMap qm, km, vm;
+  const int box = ps < kKT ? ps : kKT;
+  if (!tmap_16_3d_sw128(&qm, a.q, bf16, {HD, a.b.n_heads, a.b.n_tokens}, {HD, a.q_stride}, {64, gq, qb}) ||
+      !tmap_f16_2d_sw128(&km, static_cast<const __half*>(a.k_pages), rows, HD, 64, box) ||
+      !tmap_f16_2d_sw128(&vm, static_cast<const __half*>(a.v_pages), rows, HD, 64, box))
+    return cudaErrorInvalidValue;
+  PagedAttnParams p;
+  p.b = a.b;
+  p.x = Axis{2 * qb, a.window < (1 << 22) ? a.window : 1 << 22, K};
+  p.out = a.out;
+  p.out_stride = a.out_stride;
+  p.c = a.scale * 1.4426950408889634f;
+  p.gq = gq;
+  p.oob = (int)rows;
+  p.head = static_cast<unsigned*>(a.scratch);
+  p.recs = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kHeadBytes);
+  const void* fn = reinterpret_cast<const void*>(&paged_attn_kernel<HD, T>);
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::kSmem);
+  if (e != cudaSuccess) return e;
+  void* args[] = {&qm, &km, &vm, &p};
+  return cudaLaunchKernel(fn, dim3(grid), dim3(kThreads), args, Cfg<HD>::kSmem, s);
+}
+}  // namespace
+
+cudaError_t paged_attention(const PagedAttnArgs& a, int head_dim, int type, int n_sms, cudaStream_t s) {
+  const int grid = n_sms < kMaxGrid ? n_sms : kMaxGrid;
+  if (head_dim == 128)
+    return type == 1 ? launch<128, __half>(a, grid, false, s) : launch<128, __nv_bfloat16>(a, grid, true, s);
+  return type == 1 ? launch<64, __half>(a, grid, false, s) : launch<64, __nv_bfloat16>(a, grid, true, s);
 }
 
 }  // namespace yb

@@ -158,6 +158,6 @@ extern "C" int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long l
   a.scale = scale;
   a.window = window ? window : INT_MAX;
   a.scratch = scratch_dev;
-  YB_CK(paged_attention(a, b->head_dim, b->dtype, static_cast<cudaStream_t>(stream)));
+  YB_CK(paged_attention(a, b->head_dim, b->dtype, device_sms(), static_cast<cudaStream_t>(stream)));
   return 0;
 }

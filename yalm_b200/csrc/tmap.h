@@ -39,4 +39,20 @@ inline bool tmap_f16_2d_sw128(CUtensorMap* m, const __half* base, long long rows
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// 3-D fp16 or bf16 tensor, dims and box innermost first (box[0] * 2 <= 128 bytes, 128-byte swizzle),
+// strides in elements of the two outer dimensions; elements outside read as zeros.
+inline bool tmap_16_3d_sw128(CUtensorMap* m, const void* base, bool bf16, const long long (&dim)[3],
+                             const long long (&stride)[2], const int (&box)[3]) {
+  EncodeTiledFn enc = tmap_encode_fn();
+  if (!enc || box[0] * 2 > 128) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)dim[0], (cuuint64_t)dim[1], (cuuint64_t)dim[2]};
+  const cuuint64_t strides[2] = {(cuuint64_t)stride[0] * 2, (cuuint64_t)stride[1] * 2};
+  const cuuint32_t b[3] = {(cuuint32_t)box[0], (cuuint32_t)box[1], (cuuint32_t)box[2]};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+             const_cast<void*>(base), dims, strides, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace yb
