@@ -136,6 +136,9 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
   tma_load_2d_s(smem_u32(dst), map, x, y, smem_u32(bar));
 }
 
+__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 __device__ __forceinline__ void tma_load_3d_s(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -312,6 +315,11 @@ __device__ __forceinline__ float2 bits_f2(unsigned long long u) {
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   unsigned long long d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
+  return bits_f2(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(f2_bits(a)), "l"(f2_bits(b)));
   return bits_f2(d);
 }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {

@@ -19,7 +19,7 @@
 //   warp 0       loads Q (a 3-D box of queries x heads) and the ring of K and V tiles, one lane a page
 //   warp 1       issues the products: S[p] = Q . K^T into tensor memory, then O[p] += P . V with P read from
 //                tensor memory, where it took the place of S
-//   warps 4-7, 8-11   softmax of pipeline 0 / 1, a row per thread
+//   warps 4-7, 8-11   softmax of pipeline 0 / 1, a row per thread (they take over registers of warps 0-3)
 // A unit of two row tiles runs them as the pipelines over the same key tiles.  A unit of one row tile (single
 // tokens, short chunks) gives the pipelines alternate key tiles, and merges the two at its end.
 //
@@ -46,8 +46,8 @@ namespace {
 constexpr int kKT = 128;       // slots per key tile
 constexpr int kRows = 128;     // rows per row tile = tensor-memory lanes
 constexpr int kThreads = 384;
+constexpr int kRegsFew = 56, kRegsMany = 224;  // 128 * 56 + 256 * 224 <= 384 * 168, the registers at launch
 constexpr int kMaxGrid = 256;  // blocks the workspace has counters for
-constexpr int kMinTiles = 1;   // key tiles a block takes at least
 constexpr uint32_t kBlk = kRows * 128;  // bytes of 128 rows x 64 elements
 
 template <int HD>
@@ -120,18 +120,28 @@ __device__ __forceinline__ unsigned head_tiles(const Axis& x, const PagedSeq& q)
   return units_before(x, q, nu - 1) + (unsigned)unit_of(x, q, nu - 1).cost;
 }
 
-// Where a block starts, and its share.
+// Where a block starts, and its share.  Of `total` key tiles every block takes `share`, the first `more`
+// blocks one more.
 struct Start {
+  PagedSeq sq;
   int seq, head, unit, off;
-  int left;          // key tiles of this block
-  long long begin;   // first key tile on the axis
-  long long total;
-  int blocks;        // blocks that have work
+  int left;                  // key tiles of this block
+  unsigned long long begin;  // first key tile on the axis
+  unsigned long long share;
+  int more;
 };
-// begin of block c, and the block that holds tile x
-__device__ __forceinline__ long long block_begin(long long total, int blocks, int c) { return total * c / blocks; }
-__device__ __forceinline__ int block_of(long long total, int blocks, long long x) {
-  return (int)(((x + 1) * blocks + total - 1) / total) - 1;
+// a / b: in 32 bits where both fit, as they nearly always do
+__device__ __forceinline__ unsigned long long quot(unsigned long long a, unsigned long long b) {
+  if (!((a | b) >> 32)) return (unsigned)a / (unsigned)b;
+  return a / b;
+}
+__device__ __forceinline__ unsigned long long block_begin(unsigned long long share, int more, int c) {
+  return share * c + min(c, more);
+}
+// the block that holds tile x
+__device__ __forceinline__ int block_of(unsigned long long share, int more, unsigned long long x) {
+  const unsigned long long cut = (share + 1) * more;
+  return x < cut ? (int)quot(x, share + 1) : more + (int)quot(x - cut, share);
 }
 
 // The next piece of this block's share: tiles [t0, t1) of a unit.
@@ -144,9 +154,7 @@ struct Piece {
 struct Walk {
   Start st;
   PagedSeq sq;
-  __device__ __forceinline__ Walk(const PagedBatch& b, const Start& s) : st(s) {
-    if (st.left > 0) sq = paged_seq(b, st.seq);
-  }
+  __device__ __forceinline__ explicit Walk(const Start& s) : st(s), sq(s.sq) {}
   __device__ __forceinline__ bool next(const PagedBatch& b, const Axis& x, Piece& p) {
     if (st.left <= 0 || st.seq >= b.n_seqs) return false;
     p.sq = sq;
@@ -196,12 +204,11 @@ __device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long lon
     total += s_warp[w];
   }
   if (!total) return;
-  const long long most = (long long)(total + kMinTiles - 1) / kMinTiles;
-  const int blocks = (int)(most < gridDim.x ? most : gridDim.x);
   const int c = blockIdx.x;
-  if (c >= blocks) return;
-  const unsigned long long begin = block_begin(total, blocks, c), end = block_begin(total, blocks, c + 1);
-  if (begin < before || begin >= before + mine) return;
+  const unsigned long long share = quot(total, gridDim.x);
+  const int more = (int)(total - share * gridDim.x);
+  const unsigned long long begin = block_begin(share, more, c), end = block_begin(share, more, c + 1);
+  if (end <= begin || begin < before || begin >= before + mine) return;
   // this thread's sequences hold the block's first tile
   unsigned long long rem = begin - before;
   for (int s = s0; s < s1; ++s) {
@@ -214,8 +221,8 @@ __device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long lon
     }
     Start st;
     st.seq = s;
-    st.head = (int)(rem / per_head);
-    const unsigned in_head = (unsigned)(rem % per_head);
+    st.head = (int)quot(rem, per_head);
+    const unsigned in_head = (unsigned)(rem - (unsigned long long)st.head * per_head);
     int lo = 0, hi = n_units(x, q);  // units_before(lo) <= in_head < units_before(hi)
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
@@ -224,9 +231,10 @@ __device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long lon
     st.unit = lo;
     st.off = (int)(in_head - units_before(x, q, lo));
     st.left = (int)(end - begin);
-    st.begin = (long long)begin;
-    st.total = (long long)total;
-    st.blocks = blocks;
+    st.sq = q;
+    st.begin = begin;
+    st.share = share;
+    st.more = more;
     *s_start = st;
     return;
   }
@@ -236,6 +244,28 @@ __device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long lon
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^x of a pair on the multiply-add pipe, for a share of the weights: the special-function unit alone would
+// take as long as a tile's products.  x = n + f with n whole and |f| <= 1/2 (Cody and Waite's reduction; adding
+// 1.5 * 2^23 rounds to whole numbers and leaves n in the low bits), 2^f by the polynomial of degree 4 with the
+// least relative error on that range (2.6e-6, fitted by reweighted least squares), n added to the exponent.
+// Below 2^-125 the value does not matter.
+constexpr int kPolyPairs = 2;  // of 8 pairs
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  x.x = fmaxf(x.x, -125.f);
+  x.y = fmaxf(x.y, -125.f);
+  const float2 big = make_float2(12582912.f, 12582912.f), nbig = make_float2(-12582912.f, -12582912.f);
+  const float2 t = add2(x, big);
+  const float2 n = add2(t, nbig);
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+  float2 y = fma2(f, make_float2(0.009570102207362652f, 0.009570102207362652f),
+                  make_float2(0.05591786280274391f, 0.05591786280274391f));
+  y = fma2(y, f, make_float2(0.240247443318367f, 0.240247443318367f));
+  y = fma2(y, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+  y = fma2(y, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+  y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23));
+  y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23));
   return y;
 }
 template <typename T>
@@ -302,8 +332,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedBatch& b = a.b;
-  find_start(b, a.x, s_scan, &s_start);
-  if (threadIdx.x == 0) {
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (threadIdx.x == 64) {
     s_abort = 0;
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&full[s], 1);
@@ -322,14 +355,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&rec_done, 8);
     mbar_init(&rec_last, 1);
     mbar_fence_init();
+    tma_prefetch_map(&qmap);
+    tma_prefetch_map(&kmap);
+    tma_prefetch_map(&vmap);
   }
-  __syncthreads();
-  if (s_start.left <= 0) return;
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  find_start(b, a.x, s_scan, &s_start);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -337,144 +367,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = &s_abort;
   unsigned* status = a.head;
   const int QB = kRows / a.gq;
-  Walk walk(b, s_start);
+  Walk walk(s_start);
   Piece pc;
-
-  if (warp == 0) {
-    // ------------------------------------------------------------------------------- loads
-    const int lg = b.ps_log2, ps = 1 << lg;
-    const int boxes = ps >= kKT ? 1 : kKT >> lg;  // pages per key tile
-    const uint32_t box_bytes = (uint32_t)min(ps, kKT) * 128u;
-    unsigned it = 0, pieces = 0;
-    bool ok = true;
-    while (ok && !*abort_flag && walk.next(b, a.x, pc)) {
-      if (pc.u.none) continue;
-      const bool two = pc.u.nq > QB;
-      // Q, once the products of the piece before have read theirs
-      if (pieces && !(ok = mbar_wait(&q_empty, (pieces - 1) & 1, status))) break;
-      ++pieces;
-      if (lane == 0) {
-        const uint32_t bytes = (uint32_t)(QB * a.gq) * 128u;
-        mbar_arrive_expect_tx(&q_full, bytes * C::kHalves * (two ? 2 : 1));
-        for (int t = 0; t < (two ? 2 : 1); ++t)
-          for (int h = 0; h < C::kHalves; ++h)
-            tma_load_3d_s(sb + t * C::kTile + h * kBlk, &qmap, 64 * h, pc.head * a.gq, pc.sq.row0 + pc.u.q0 + t * QB,
-                          smem_u32(&q_full));
-      }
-      const int* table = b.page_table + (size_t)pc.seq * b.max_pages;
-      // row of the page pool where this lane's page of a key tile starts (outside it: zeros)
-      auto row_of = [&](int tile) {
-        const int slot = (tile << 7) + (lane << lg);
-        if (lane >= boxes || slot >= pc.sq.kv) return a.oob;
-        const int id = __ldg(table + (slot >> lg));
-        if (id < 0 || id >= b.n_pages) return a.oob;
-        return ((id * a.x.K + pc.head) << lg) + (slot & (ps - 1));
-      };
-      auto load = [&](const CUtensorMap* map, int row) {
-        const int s = it % C::kStages;
-        if (it >= C::kStages && !mbar_wait(&empty[s], (it / C::kStages - 1) & 1, status)) return false;
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], C::kTile);
-        __syncwarp();
-        if (lane < boxes)
-          for (int h = 0; h < C::kHalves; ++h)
-            tma_load_2d_s(ring + s * C::kTile + h * kBlk + lane * box_bytes, map, 64 * h, row, smem_u32(&full[s]));
-        ++it;
-        return true;
-      };
-      // in the order of the products: K of steps 0 and 1, then V of step i and K of step i + 2
-      const int first = pc.u.tile0 + pc.t0, n = pc.t1 - pc.t0, ahead = two ? 1 : 2;
-      int next_row = row_of(first);
-      for (int j = 0; j < n + ahead && ok; ++j) {
-        if (j >= ahead) ok = load(&vmap, row_of(first + j - ahead));
-        if (ok && j < n) {
-          const int row = next_row;
-          if (j + 1 < n) next_row = row_of(first + j + 1);
-          ok = load(&kmap, row);
-        }
-      }
-    }
-    if (!ok) *abort_flag = 1;
-    // never leave while a copy issued here may still be landing
-    for (unsigned i = it > C::kStages ? it - C::kStages : 0; i < it; ++i)
-      mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1, status);
-    if (pieces) mbar_wait(&q_full, (pieces - 1) & 1, status);
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------------------- products
-    unsigned it = 0, pieces = 0, steps[2] = {0, 0};
-    bool ok = true;
-    while (ok && !*abort_flag && walk.next(b, a.x, pc)) {
-      if (pc.u.none) continue;
-      const bool two = pc.u.nq > QB;
-      const int first = pc.u.tile0 + pc.t0, nk = pc.t1 - pc.t0, n = two ? 2 * nk : nk;
-      if (!(ok = mbar_wait(&q_full, pieces & 1, status))) break;
-      int kslot = 0, vslot = 0;
-      auto qk = [&](int i) {
-        if (!two || !(i & 1)) {
-          kslot = it % C::kStages;
-          if (!mbar_wait(&full[kslot], (it / C::kStages) & 1, status)) return false;
-          ++it;
-        }
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t q = sb + (two && (i & 1) ? C::kTile : 0u), k = ring + kslot * C::kTile;
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t off = (uint32_t)(kk / 4) * kBlk + (uint32_t)(kk % 4) * 32u;
-            umma_f16(tmem + (uint32_t)(i & 1) * kKT, umma_desc_k_sw128(q + off), umma_desc_k_sw128(k + off), kIdS, kk ? 1u : 0u);
-          }
-          umma_commit(&s_full[i & 1]);
-          if (!two || (i & 1)) umma_commit(&empty[kslot]);
-          if (i == n - 1) umma_commit(&q_empty);
-        }
-        __syncwarp();
-        return true;
-      };
-      auto pv = [&](int i) {
-        const int p = i & 1;
-        if (!two || !p) {
-          vslot = it % C::kStages;
-          if (!mbar_wait(&full[vslot], (it / C::kStages) & 1, status)) return false;
-          ++it;
-          // slots behind the sequence's last one, in its last page, may hold anything: their weight is 0, and
-          // 0 * v has to be 0
-          const int rem = pc.sq.kv - (first + (two ? i >> 1 : i)) * kKT;
-          const int end = min(kKT, ((rem + (1 << b.ps_log2) - 1) >> b.ps_log2) << b.ps_log2);
-          if (rem < end) {
-            const uint32_t v = ring + vslot * C::kTile;
-            for (int e = lane; e < (end - rem) * 8 * C::kHalves; e += 32) {
-              const int h = e / ((end - rem) * 8), r = e % ((end - rem) * 8);
-              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * kBlk + (rem * 8 + r) * 16u), "r"(0u)
-                           : "memory");
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
-        }
-        if (i < 2 && pieces && !mbar_wait(&o_free, (pieces - 1) & 1, status)) return false;
-        if (!mbar_wait(&p_full[p], steps[p] & 1, status)) return false;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t v = ring + vslot * C::kTile;
-#pragma unroll
-          for (int kk = 0; kk < kKT / 16; ++kk)
-            umma_f16_ta(tmem + kColO + (uint32_t)p * HD, tmem + (uint32_t)p * kKT + kk * 8,
-                        umma_desc_sw128(v + kk * 2048u, kBlk, 1024), kIdO, (i >= 2 || kk) ? 1u : 0u);
-          umma_commit(&o_done[p]);
-          if (!two || p) umma_commit(&empty[vslot]);
-        }
-        __syncwarp();
-        ++steps[p];
-        return true;
-      };
-      ok = qk(0) && (n < 2 || qk(1));
-      for (int i = 0; i < n && ok && !*abort_flag; ++i) {
-        ok = pv(i);
-        if (ok && i + 2 < n) ok = qk(i + 2);
-      }
-      ++pieces;
-    }
-    if (!ok) *abort_flag = 1;
-  } else if (warp >= 4) {
+  if (warp >= 4) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
     // ------------------------------------------------------------------------------- softmax
     const int p = (warp - 4) >> 2, quad = warp & 3;  // pipeline, tensor-memory lane quadrant
     const int r = quad * 32 + lane;                  // row of the row tile
@@ -513,65 +409,72 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (live) {
           const int k0 = t * kKT;
           const int lo = valid ? pos - a.x.window + 1 - k0 : kKT, hi = valid ? pos + 1 - k0 : 0;
-          const bool all = lo <= 0 && hi >= kKT && pages == 0xffu;
-          uint32_t msk[4];
+          float s[kKT];
+          tmem_ld128(ts, s);
+          // rows behind the unit's last one compute with what lies in their lanes; nothing reads them
+          const bool all = __all_sync(0xffffffffu, !valid || (lo <= 0 && hi >= kKT && pages == 0xffu));
+          if (!all) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t pg = ((pages >> (2 * w)) & 1u ? 0xffffu : 0u) | ((pages >> (2 * w + 1)) & 1u ? 0xffff0000u : 0u);
-            msk[w] = bit_range(lo - 32 * w, hi - 32 * w) & pg;
-          }
-          float mx = -INFINITY;
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t pg = ((pages >> (2 * w)) & 1u ? 0xffffu : 0u) | ((pages >> (2 * w + 1)) & 1u ? 0xffff0000u : 0u);
+              const uint32_t msk = bit_range(lo - 32 * w, hi - 32 * w) & pg;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            float s[32];
-            tmem_ld32(ts + 32 * w, s);
-            if (all) {
-#pragma unroll
-              for (int k = 0; k < 32; ++k) mx = fmaxf(mx, s[k]);
-            } else {
-#pragma unroll
-              for (int k = 0; k < 32; ++k) mx = fmaxf(mx, (msk[w] >> k) & 1u ? s[k] : -INFINITY);
+              for (int k = 0; k < 32; ++k) s[32 * w + k] = (msk >> k) & 1u ? s[32 * w + k] : -INFINITY;
             }
           }
-          mx *= a.c;
-          const bool need = mx > m + 8.0f;  // the first slots seen, or a maximum grown by over 2^8
+          float mx;
+          {
+            float c4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int k = 4; k < kKT - 4; k += 8)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) c4[e] = fmaxf(fmaxf(c4[e], s[k + e]), s[k + 4 + e]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c4[e] = fmaxf(c4[e], s[kKT - 4 + e]);
+            mx = fmaxf(fmaxf(c4[0], c4[1]), fmaxf(c4[2], c4[3])) * a.c;
+          }
+          const bool need = valid && mx > m + 8.0f;  // the first slots seen, or a maximum grown by over 2^8
           const float mn = need ? mx : m;
           const float alpha = need ? ex2(m - mn) : 1.f;  // 0 while m is -inf
           if (i > 0 && __any_sync(0xffffffffu, need)) {
             if (!(ok = mbar_wait(&o_done[p], (steps[p] + i - 1) & 1, status))) break;
             tc_fence_after();
 #pragma unroll 1
-            for (int c0 = 0; c0 < HD; c0 += 32) {
-              float v[32];
-              tmem_ld32(to + p * HD + c0, v);
+            for (int c0 = 0; c0 < HD; c0 += 16) {
+              float v[16];
+              tmem_ld16(to + p * HD + c0, v);
+              uint32_t u[16];
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[k] *= alpha;
-              tmem_st32(to + p * HD + c0, v);
+              for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(v[k] * alpha);
+              tmem_st16_u32(to + p * HD + c0, u);
             }
           }
           m = mn;
           const float shift = m == -INFINITY ? 0.f : m - kBias;
-          float sum = 0.f;
+          const float2 cc = make_float2(a.c, a.c), sh = make_float2(-shift, -shift);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          auto weights = [&](auto masked) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            float s[32];
-            tmem_ld32(ts + 32 * w, s);
-            uint32_t pk[16];
-            if (all) {
+            for (int w = 0; w < 8; ++w) {
+              uint32_t pk[8];
 #pragma unroll
-              for (int k = 0; k < 32; ++k) s[k] = ex2(fmaf(s[k], a.c, -shift));
-            } else {
-#pragma unroll
-              for (int k = 0; k < 32; ++k) s[k] = (msk[w] >> k) & 1u ? ex2(fmaf(s[k], a.c, -shift)) : 0.f;
+              for (int k = 0; k < 8; ++k) {
+                const int e = 16 * w + 2 * k;
+                float2 t = fma2(make_float2(s[e], s[e + 1]), cc, sh);
+                if (!masked.value && k >= 8 - kPolyPairs) {
+                  t = ex2_poly(t);
+                } else {
+                  t.x = ex2(t.x);
+                  t.y = ex2(t.y);
+                }
+                sum[k & 1] = add2(sum[k & 1], t);
+                pk[k] = pack2<T>(t.x, t.y);
+              }
+              tmem_st8_u32(ts + 8 * w, pk);
             }
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              sum += s[2 * k] + s[2 * k + 1];
-              pk[k] = pack2<T>(s[2 * k], s[2 * k + 1]);
-            }
-            tmem_st16_u32(ts + 16 * w, pk);
-          }
-          l = l * alpha + sum;
+          };
+          if (all) weights(std::false_type{}); else weights(std::true_type{});
+          l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
           tmem_st_wait();
         }
         tc_fence_before();
@@ -668,9 +571,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         __threadfence();
         __syncwarp();
         if (lane == 0) mbar_arrive(&rec_done);
-        const long long begin = s_start.begin + (s_start.left - walk.st.left) - pc.t1;  // the unit's first tile
-        const int c0 = block_of(s_start.total, s_start.blocks, begin);
-        const int c1 = block_of(s_start.total, s_start.blocks, begin + pc.u.cost - 1);
+        const unsigned long long begin = s_start.begin + (s_start.left - walk.st.left) - pc.t1;  // the unit's first tile
+        const int c0 = block_of(s_start.share, s_start.more, begin);
+        const int c1 = block_of(s_start.share, s_start.more, begin + pc.u.cost - 1);
         if (threadIdx.x == 128) {
           int last = 0;
           if (mbar_wait(&rec_done, cuts & 1, status)) {
@@ -719,6 +622,139 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++pieces;
     }
     if (!ok) *abort_flag = 1;
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
+  if (warp == 0) {
+    // ------------------------------------------------------------------------------- loads
+    const int lg = b.ps_log2, ps = 1 << lg;
+    const int boxes = ps >= kKT ? 1 : kKT >> lg;  // pages per key tile
+    const uint32_t box_bytes = (uint32_t)min(ps, kKT) * 128u;
+    unsigned it = 0, pieces = 0;
+    bool ok = true;
+    while (ok && !*abort_flag && walk.next(b, a.x, pc)) {
+      if (pc.u.none) continue;
+      const bool two = pc.u.nq > QB;
+      // Q, once the products of the piece before have read theirs
+      if (pieces && !(ok = mbar_wait(&q_empty, (pieces - 1) & 1, status))) break;
+      ++pieces;
+      if (lane == 0) {
+        const uint32_t bytes = (uint32_t)(QB * a.gq) * 128u;
+        mbar_arrive_expect_tx(&q_full, bytes * C::kHalves * (two ? 2 : 1));
+        for (int t = 0; t < (two ? 2 : 1); ++t)
+          for (int h = 0; h < C::kHalves; ++h)
+            tma_load_3d_s(sb + t * C::kTile + h * kBlk, &qmap, 64 * h, pc.head * a.gq, pc.sq.row0 + pc.u.q0 + t * QB,
+                          smem_u32(&q_full));
+      }
+      const int* table = b.page_table + (size_t)pc.seq * b.max_pages;
+      // row of the page pool where this lane's page of a key tile starts (outside it: zeros)
+      auto row_of = [&](int tile) {
+        const int slot = (tile << 7) + (lane << lg);
+        if (lane >= boxes || slot >= pc.sq.kv) return a.oob;
+        const int id = __ldg(table + (slot >> lg));
+        if (id < 0 || id >= b.n_pages) return a.oob;
+        return ((id * a.x.K + pc.head) << lg) + (slot & (ps - 1));
+      };
+      auto load = [&](const CUtensorMap* map, int row) {
+        const int s = it % C::kStages;
+        if (it >= C::kStages && !mbar_wait(&empty[s], (it / C::kStages - 1) & 1, status)) return false;
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], C::kTile);
+        __syncwarp();
+        if (lane < boxes)
+          for (int h = 0; h < C::kHalves; ++h)
+            tma_load_2d_s(ring + s * C::kTile + h * kBlk + lane * box_bytes, map, 64 * h, row, smem_u32(&full[s]));
+        ++it;
+        return true;
+      };
+      // in the order of the products: K of steps 0 and 1, then V of step i and K of step i + 2
+      const int first = pc.u.tile0 + pc.t0, n = pc.t1 - pc.t0, ahead = two ? 1 : 2;
+      int next_row = row_of(first);
+      for (int j = 0; j < n + ahead && ok; ++j) {
+        if (j >= ahead) ok = load(&vmap, row_of(first + j - ahead));
+        if (ok && j < n) {
+          const int row = next_row;
+          if (j + 1 < n) next_row = row_of(first + j + 1);
+          ok = load(&kmap, row);
+        }
+      }
+    }
+    if (!ok) *abort_flag = 1;
+    // never leave while a copy issued here may still be landing
+    for (unsigned i = it > C::kStages ? it - C::kStages : 0; i < it; ++i)
+      mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1, status);
+    if (pieces) mbar_wait(&q_full, (pieces - 1) & 1, status);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------------------- products
+    unsigned slot = 0, phase = 0, pieces = 0, steps[2] = {0, 0};
+    const uint32_t e = elect_lane();
+    bool ok = true;
+    while (ok && !*abort_flag && walk.next(b, a.x, pc)) {
+      if (pc.u.none) continue;
+      const bool two = pc.u.nq > QB;
+      const int first = pc.u.tile0 + pc.t0, nk = pc.t1 - pc.t0, n = two ? 2 * nk : nk;
+      if (!(ok = mbar_wait(&q_full, pieces & 1, status))) break;
+      unsigned kslot = 0, vslot = 0;
+      auto take = [&](unsigned& at) {
+        at = slot;
+        if (!mbar_wait(&full[slot], phase, status)) return false;
+        if (++slot == C::kStages) slot = 0, phase ^= 1;
+        return true;
+      };
+      auto qk = [&](int i) {
+        if ((!two || !(i & 1)) && !take(kslot)) return false;
+        tc_fence_after();
+        const uint32_t q = sb + (two && (i & 1) ? C::kTile : 0u), k = ring + kslot * C::kTile;
+        const uint64_t dq = umma_desc_k_sw128(q), dk = umma_desc_k_sw128(k);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t off = ((kk / 4) * kBlk + (kk % 4) * 32u) >> 4;
+          umma_f16_if(e, tmem + (uint32_t)(i & 1) * kKT, dq + off, dk + off, kIdS, kk ? 1u : 0u);
+        }
+        umma_commit_if(e, &s_full[i & 1]);
+        if (!two || (i & 1)) umma_commit_if(e, &empty[kslot]);
+        if (i == n - 1) umma_commit_if(e, &q_empty);
+        return true;
+      };
+      auto pv = [&](int i) {
+        const int p = i & 1;
+        if (!two || !p) {
+          if (!take(vslot)) return false;
+          // slots behind the sequence's last one, in its last page, may hold anything: their weight is 0, and
+          // 0 * v has to be 0
+          const int rem = pc.sq.kv - (first + (two ? i >> 1 : i)) * kKT;
+          if (rem < kKT) {
+            const int end = min(kKT, ((rem + (1 << b.ps_log2) - 1) >> b.ps_log2) << b.ps_log2);
+            const uint32_t v = ring + vslot * C::kTile;
+            for (int x = lane; x < (end - rem) * 8 * C::kHalves; x += 32) {
+              const int h = x / ((end - rem) * 8), r = x % ((end - rem) * 8);
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * kBlk + (rem * 8 + r) * 16u), "r"(0u)
+                           : "memory");
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        if (i < 2 && pieces && !mbar_wait(&o_free, (pieces - 1) & 1, status)) return false;
+        if (!mbar_wait(&p_full[p], steps[p] & 1, status)) return false;
+        tc_fence_after();
+        const uint64_t dv = umma_desc_sw128(ring + vslot * C::kTile, kBlk, 1024);
+#pragma unroll
+        for (int kk = 0; kk < kKT / 16; ++kk)
+          umma_f16_ta_if(e, tmem + kColO + (uint32_t)p * HD, tmem + (uint32_t)p * kKT + kk * 8, dv + ((kk * 2048u) >> 4), kIdO,
+                         (i >= 2 || kk) ? 1u : 0u);
+        umma_commit_if(e, &o_done[p]);
+        if (!two || p) umma_commit_if(e, &empty[vslot]);
+        ++steps[p];
+        return true;
+      };
+      ok = qk(0) && (n < 2 || qk(1));
+      for (int i = 0; i < n && ok && !*abort_flag; ++i) {
+        ok = pv(i);
+        if (ok && i + 2 < n) ok = qk(i + 2);
+      }
+      ++pieces;
+    }
+    if (!ok) *abort_flag = 1;
+  }
   }
   tc_fence_before();
   __syncthreads();
