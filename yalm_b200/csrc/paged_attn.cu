@@ -12,8 +12,9 @@
 // evenly: a long cache of few rows is cut over many blocks, and ragged lengths balance themselves.
 // The cuts follow from the lengths on the device, by a closed form for a sequence's tiles (floor
 // sums), so there is no plan to be made on the host and a captured launch follows new lengths.  A unit
-// that is cut leaves (o, m, l) records in the workspace; the block that finishes it last merges them in
-// the order of the slots, so results do not depend on timing.
+// that is cut leaves (o, m, l) records in the workspace, which a second kernel, launched as the dependent of
+// the first, merges in the order of the slots, spread over the whole GPU: results do not depend on timing,
+// and no block waits for another.
 //
 // Block.  Two pipelines of 128 rows share the tensor cores, one's softmax under the other's products:
 //   warp 0       loads Q (a 3-D box of queries x heads) and the ring of K and V tiles, one lane a page
@@ -111,6 +112,7 @@ __device__ __forceinline__ Unit unit_of(const Axis& x, const PagedSeq& q, int i)
 __device__ __forceinline__ int n_units(const Axis& x, const PagedSeq& q) { return (q.n + x.U - 1) / x.U; }
 // key tiles of the first m units of a (sequence, kv head), m < n_units: unit i ends at slot p0 + (i + 1) U
 __device__ __forceinline__ unsigned units_before(const Axis& x, const PagedSeq& q, int m) {
+  if (m == 0) return 0;
   const int p0 = q.kv - q.n;
   return (unsigned)m + ramp(m, p0 + x.U - 1, x.U) - ramp(m, p0 - x.window + 1, x.U);
 }
@@ -185,10 +187,16 @@ struct Walk {
 // Called by the whole block: this block's share of the axis.
 __device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long long* s_warp, Start* s_start) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per = (b.n_seqs + kThreads - 1) / kThreads;
+  const int per = (b.n_seqs + kThreads - 1) / kThreads;  // sequences of a thread
   const int s0 = min(b.n_seqs, (int)threadIdx.x * per), s1 = min(b.n_seqs, s0 + per);
   unsigned long long mine = 0;
-  for (int s = s0; s < s1; ++s) mine += (unsigned long long)head_tiles(x, paged_seq(b, s)) * x.K;
+  PagedSeq q{0, 0, 0};
+  unsigned per_head = 0;
+  for (int s = s0; s < s1; ++s) {
+    q = paged_seq(b, s);
+    per_head = head_tiles(x, q);
+    mine += (unsigned long long)per_head * x.K;
+  }
   unsigned long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -199,45 +207,47 @@ __device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long lon
   if (threadIdx.x == 0) s_start->left = 0;
   __syncthreads();
   unsigned long long before = incl - mine, total = 0;
+#pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += s_warp[w];
-    total += s_warp[w];
+    const unsigned long long v = s_warp[w];
+    if (w < warp) before += v;
+    total += v;
   }
-  if (!total) return;
-  const int c = blockIdx.x;
+  if (!mine) return;
   const unsigned long long share = quot(total, gridDim.x);
-  const int more = (int)(total - share * gridDim.x);
-  const unsigned long long begin = block_begin(share, more, c), end = block_begin(share, more, c + 1);
-  if (end <= begin || begin < before || begin >= before + mine) return;
+  const int more = (int)(total - share * gridDim.x), c = blockIdx.x;
+  const unsigned long long begin = block_begin(share, more, c);
+  const int left = (int)share + (c < more ? 1 : 0);
+  if (!left || begin < before || begin >= before + mine) return;
   // this thread's sequences hold the block's first tile
   unsigned long long rem = begin - before;
-  for (int s = s0; s < s1; ++s) {
-    const PagedSeq q = paged_seq(b, s);
-    const unsigned per_head = head_tiles(x, q);
-    const unsigned long long all = (unsigned long long)per_head * x.K;
-    if (rem >= all) {
+  int s = s1 - 1;
+  if (per > 1) {
+    for (s = s0;; ++s) {
+      q = paged_seq(b, s);
+      per_head = head_tiles(x, q);
+      const unsigned long long all = (unsigned long long)per_head * x.K;
+      if (rem < all) break;
       rem -= all;
-      continue;
     }
-    Start st;
-    st.seq = s;
-    st.head = (int)quot(rem, per_head);
-    const unsigned in_head = (unsigned)(rem - (unsigned long long)st.head * per_head);
-    int lo = 0, hi = n_units(x, q);  // units_before(lo) <= in_head < units_before(hi)
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (units_before(x, q, mid) <= in_head) lo = mid; else hi = mid;
-    }
-    st.unit = lo;
-    st.off = (int)(in_head - units_before(x, q, lo));
-    st.left = (int)(end - begin);
-    st.sq = q;
-    st.begin = begin;
-    st.share = share;
-    st.more = more;
-    *s_start = st;
-    return;
   }
+  Start st;
+  st.sq = q;
+  st.seq = s;
+  st.head = (int)quot(rem, per_head);
+  const unsigned in_head = (unsigned)(rem - (unsigned long long)st.head * per_head);
+  int lo = 0, hi = n_units(x, q);  // units_before(lo) <= in_head < units_before(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (units_before(x, q, mid) <= in_head) lo = mid; else hi = mid;
+  }
+  st.unit = lo;
+  st.off = (int)(in_head - units_before(x, q, lo));
+  st.left = left;
+  st.begin = begin;
+  st.share = share;
+  st.more = more;
+  *s_start = st;
 }
 
 // -------------------------------------------------------------------------------------------- numerics
@@ -289,11 +299,19 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
   return (0xffffffffu >> (32 - (hi - lo))) << lo;
 }
 
-// Workspace: [0] status word, [64 ..] counters, then per block and slot (0: a unit begun by an earlier block, 1:
-// one that a later block goes on with) 2 x 256 floats (m, l) and 256 rows of HD floats.
-constexpr size_t kHeadBytes = 256 + kMaxGrid * 4;
+// Workspace: [0] status word; from byte 256 a Cut per block, the unit that the block begins and later blocks
+// go on with; then two records per block: 0 for a unit begun by an earlier block, 1 for the one it leaves to
+// later ones.  A record holds o as [HD / 4][rows] groups of 4 floats (a warp's rows side by side), then m and
+// l, [rows] each.
+struct __align__(16) Cut {
+  int token;  // first row of the token-major buffers
+  int nq;     // queries
+  int head;   // kv head
+  int parts;  // blocks that hold a record of it, this one first; 0: no unit
+};
+constexpr size_t kHeadBytes = 256 + kMaxGrid * sizeof(Cut);
 template <int HD>
-constexpr size_t rec_floats() { return 2 * 256 + 256 * (size_t)HD; }
+constexpr size_t rec_floats() { return 256 * (size_t)(HD + 2); }
 
 }  // namespace
 
@@ -305,7 +323,8 @@ struct PagedAttnParams {
   float c;  // scale * log2(e)
   int gq;   // query heads per kv head
   int oob;  // a row outside the page pool's tensor maps
-  unsigned* head;
+  unsigned* status;
+  Cut* cuts;
   float* recs;
 };
 
@@ -323,15 +342,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sb = smem_u32(smem), ring = sb + 2 * C::kTile;
   float* s_ml = reinterpret_cast<float*>(smem + (2 + C::kStages) * C::kTile);  // [2][128]
-  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], q_full, q_empty, s_full[2], p_full[2],
-      o_done[2], o_free, ml_ready, ml_free, rec_done, rec_last;
+  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], q_full[2], q_empty[2], s_full[2], p_full[2][2],
+      o_done[2], o_free, ml_ready, ml_free;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_last;
+  __shared__ int s_abort;
   __shared__ unsigned long long s_scan[kThreads / 32];
   __shared__ Start s_start;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedBatch& b = a.b;
+  pdl_trigger();  // the merge may be set up; it waits for this kernel's end
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
                  : "memory");
@@ -342,18 +362,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(&q_full, 1);
-    mbar_init(&q_empty, 1);
     for (int p = 0; p < 2; ++p) {
+      mbar_init(&q_full[p], 1);
+      mbar_init(&q_empty[p], 1);
       mbar_init(&s_full[p], 1);
-      mbar_init(&p_full[p], 4);
+      mbar_init(&p_full[p][0], 4);
+      mbar_init(&p_full[p][1], 4);
       mbar_init(&o_done[p], 1);
     }
     mbar_init(&o_free, 8);
     mbar_init(&ml_ready, 4);
     mbar_init(&ml_free, 4);
-    mbar_init(&rec_done, 8);
-    mbar_init(&rec_last, 1);
     mbar_fence_init();
     tma_prefetch_map(&qmap);
     tma_prefetch_map(&kmap);
@@ -365,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   volatile int* abort_flag = &s_abort;
-  unsigned* status = a.head;
+  unsigned* status = a.status;
   const int QB = kRows / a.gq;
   Walk walk(s_start);
   Piece pc;
@@ -378,7 +397,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ts = tmem + lanes + (uint32_t)p * kKT, to = tmem + lanes + kColO;
     const int qi = r / a.gq, h = r % a.gq;
     unsigned steps[2] = {0, 0};  // steps of either pipeline in the pieces before
-    unsigned pieces = 0, singles = 0, cuts = 0;
+    unsigned singles = 0;
+    if (threadIdx.x == 128) a.cuts[blockIdx.x].parts = 0;  // the same thread's later store tells otherwise
     bool ok = true;
     while (ok && !*abort_flag && walk.next(b, a.x, pc)) {
       const bool two = pc.u.nq > QB;
@@ -471,15 +491,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                 pk[k] = pack2<T>(t.x, t.y);
               }
               tmem_st8_u32(ts + 8 * w, pk);
+              if (w == 3) {  // the first half's product may begin
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[p][0]);
+              }
             }
           };
           if (all) weights(std::false_type{}); else weights(std::true_type{});
           l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
           tmem_st_wait();
+        } else if (lane == 0) {
+          mbar_arrive(&p_full[p][0]);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[p]);
+        if (lane == 0) mbar_arrive(&p_full[p][1]);
       }
       if (!ok || *abort_flag) break;
 
@@ -515,10 +543,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_after();
       const bool whole = pc.t0 == 0 && pc.t1 == pc.u.cost;
-      const int slot = pc.t0 == 0 ? 1 : 0;
-      float* rec = a.recs + ((size_t)blockIdx.x * 2 + slot) * rec_floats<HD>();
-      const size_t token = (size_t)pc.sq.row0 + pc.u.q0 + q;
-      T* out = static_cast<T*>(a.out) + token * a.out_stride + (size_t)(pc.head * a.gq + h) * HD;
+      const int rows = pc.u.nq * a.gq, row = tile * QB * a.gq + r;
+      const int token = pc.sq.row0 + pc.u.q0;
+      float* rec = a.recs + ((size_t)blockIdx.x * 2 + (pc.t0 == 0 ? 1 : 0)) * rec_floats<HD>();
+      T* out = static_cast<T*>(a.out) + (size_t)(token + q) * a.out_stride + (size_t)(pc.head * a.gq + h) * HD;
       if (two || p == 0) {
         const float inv = whole ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
         w0 *= inv;
@@ -549,15 +577,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     make_uint4(pack2<T>(v[8 * k], v[8 * k + 1]), pack2<T>(v[8 * k + 2], v[8 * k + 3]),
                                pack2<T>(v[8 * k + 4], v[8 * k + 5]), pack2<T>(v[8 * k + 6], v[8 * k + 7]));
             } else {
-              float4* o = reinterpret_cast<float4*>(rec + 512 + (size_t)(tile * kRows + r) * HD + c0);
+              float4* o = reinterpret_cast<float4*>(rec) + (size_t)(c0 / 4) * rows + row;
 #pragma unroll
-              for (int k = 0; k < 8; ++k) o[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+              for (int k = 0; k < 8; ++k) o[(size_t)k * rows] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
             }
           }
         }
         if (!whole && valid) {
-          rec[tile * kRows + r] = m;
-          rec[256 + tile * kRows + r] = l;
+          rec[HD * rows + row] = m;
+          rec[(HD + 1) * rows + row] = l;
         }
         tc_fence_before();
         __syncwarp();
@@ -566,60 +594,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!two) mbar_arrive(&ml_free);
         }
       }
-      if (!whole) {
-        // ---- a cut unit: the block that counts last merges every block's record
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&rec_done);
+      if (!whole && pc.t0 == 0 && threadIdx.x == 128) {
         const unsigned long long begin = s_start.begin + (s_start.left - walk.st.left) - pc.t1;  // the unit's first tile
-        const int c0 = block_of(s_start.share, s_start.more, begin);
-        const int c1 = block_of(s_start.share, s_start.more, begin + pc.u.cost - 1);
-        if (threadIdx.x == 128) {
-          int last = 0;
-          if (mbar_wait(&rec_done, cuts & 1, status)) {
-            last = atom_add_acq_rel_gpu(a.head + 64 + c0, 1u) == (unsigned)(c1 - c0);
-            if (last) a.head[64 + c0] = 0u;
-          }
-          s_last = last;
-          mbar_arrive(&rec_last);
-        }
-        __syncwarp();
-        if (!(ok = mbar_wait(&rec_last, cuts & 1, status))) break;
-        ++cuts;
-        if (s_last) {
-          const int tid = threadIdx.x - 128;
-          const float* base = a.recs;
-          auto part = [&](int c) { return base + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * rec_floats<HD>(); };
-          const int n0 = min(QB, pc.u.nq) * a.gq, n1 = (pc.u.nq - min(QB, pc.u.nq)) * a.gq;
-          for (int e = tid; e < (n0 + n1) * (HD / 4); e += 256) {
-            const int er = e / (HD / 4), ec = e % (HD / 4) * 4;
-            const int rr = er < n0 ? er : kRows + er - n0;
-            float mm = -INFINITY;
-            for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, __ldcg(part(c) + rr));
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            float ll = 0.f;
-            for (int c = c0; c <= c1; ++c) {
-              const float* pr = part(c);
-              const float mc = __ldcg(pr + rr), lc = __ldcg(pr + 256 + rr);
-              const float4 o = __ldcg(reinterpret_cast<const float4*>(pr + 512 + (size_t)rr * HD + ec));
-              const float w = mc == -INFINITY ? 0.f : ex2(mc - mm);
-              ll = fmaf(lc, w, ll);
-              acc.x = fmaf(o.x, w, acc.x);
-              acc.y = fmaf(o.y, w, acc.y);
-              acc.z = fmaf(o.z, w, acc.z);
-              acc.w = fmaf(o.w, w, acc.w);
-            }
-            const float inv = ll != 0.f ? 1.f / ll : 0.f;
-            const int eq = er / a.gq, eh = er % a.gq;
-            T* eo = static_cast<T*>(a.out) + ((size_t)pc.sq.row0 + pc.u.q0 + eq) * a.out_stride +
-                    (size_t)(pc.head * a.gq + eh) * HD + ec;
-            *reinterpret_cast<uint2*>(eo) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-          }
-        }
+        const int last = block_of(s_start.share, s_start.more, begin + pc.u.cost - 1);
+        a.cuts[blockIdx.x] = Cut{token, pc.u.nq, pc.head, last - (int)blockIdx.x + 1};
       }
       steps[0] += two ? nk : (nk + 1) / 2;
       steps[1] += two ? nk : nk / 2;
-      ++pieces;
     }
     if (!ok) *abort_flag = 1;
   } else {
@@ -629,40 +610,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int lg = b.ps_log2, ps = 1 << lg;
     const int boxes = ps >= kKT ? 1 : kKT >> lg;  // pages per key tile
     const uint32_t box_bytes = (uint32_t)min(ps, kKT) * 128u;
-    unsigned it = 0, pieces = 0;
+    unsigned slot = 0, phase = 1, issued = 0, uses[2] = {0, 0};
+    int buf = 0;  // buffer of the next unit of one row tile
     bool ok = true;
     while (ok && !*abort_flag && walk.next(b, a.x, pc)) {
       if (pc.u.none) continue;
       const bool two = pc.u.nq > QB;
-      // Q, once the products of the piece before have read theirs
-      if (pieces && !(ok = mbar_wait(&q_empty, (pieces - 1) & 1, status))) break;
-      ++pieces;
-      if (lane == 0) {
-        const uint32_t bytes = (uint32_t)(QB * a.gq) * 128u;
-        mbar_arrive_expect_tx(&q_full, bytes * C::kHalves * (two ? 2 : 1));
-        for (int t = 0; t < (two ? 2 : 1); ++t)
-          for (int h = 0; h < C::kHalves; ++h)
-            tma_load_3d_s(sb + t * C::kTile + h * kBlk, &qmap, 64 * h, pc.head * a.gq, pc.sq.row0 + pc.u.q0 + t * QB,
-                          smem_u32(&q_full));
-      }
       const int* table = b.page_table + (size_t)pc.seq * b.max_pages;
       // row of the page pool where this lane's page of a key tile starts (outside it: zeros)
       auto row_of = [&](int tile) {
-        const int slot = (tile << 7) + (lane << lg);
-        if (lane >= boxes || slot >= pc.sq.kv) return a.oob;
-        const int id = __ldg(table + (slot >> lg));
+        const int at = (tile << 7) + (lane << lg);
+        if (lane >= boxes || at >= pc.sq.kv) return a.oob;
+        const int id = __ldg(table + (at >> lg));
         if (id < 0 || id >= b.n_pages) return a.oob;
-        return ((id * a.x.K + pc.head) << lg) + (slot & (ps - 1));
+        return ((id * a.x.K + pc.head) << lg) + (at & (ps - 1));
       };
       auto load = [&](const CUtensorMap* map, int row) {
-        const int s = it % C::kStages;
-        if (it >= C::kStages && !mbar_wait(&empty[s], (it / C::kStages - 1) & 1, status)) return false;
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], C::kTile);
+        if (issued >= C::kStages && !mbar_wait(&empty[slot], phase, status)) return false;
+        if (lane == 0) mbar_arrive_expect_tx(&full[slot], C::kTile);
         __syncwarp();
         if (lane < boxes)
           for (int h = 0; h < C::kHalves; ++h)
-            tma_load_2d_s(ring + s * C::kTile + h * kBlk + lane * box_bytes, map, 64 * h, row, smem_u32(&full[s]));
-        ++it;
+            tma_load_2d_s(ring + slot * C::kTile + h * kBlk + lane * box_bytes, map, 64 * h, row, smem_u32(&full[slot]));
+        ++issued;
+        if (++slot == C::kStages) slot = 0, phase ^= 1;
+        return true;
+      };
+      // a row tile of queries, once the products of the unit before have read its buffer
+      auto load_q = [&](int to, int tile) {
+        if (uses[to] && !mbar_wait(&q_empty[to], (uses[to] - 1) & 1, status)) return false;
+        ++uses[to];
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&q_full[to], (uint32_t)(QB * a.gq) * 128u * C::kHalves);
+          for (int h = 0; h < C::kHalves; ++h)
+            tma_load_3d_s(sb + to * C::kTile + h * kBlk, &qmap, 64 * h, pc.head * a.gq, pc.sq.row0 + pc.u.q0 + tile * QB,
+                          smem_u32(&q_full[to]));
+        }
         return true;
       };
       // in the order of the products: K of steps 0 and 1, then V of step i and K of step i + 2
@@ -675,23 +658,36 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j + 1 < n) next_row = row_of(first + j + 1);
           ok = load(&kmap, row);
         }
+        if (ok && j == 0) {
+          if (two) {
+            ok = load_q(0, 0) && load_q(1, 1);
+          } else {
+            ok = load_q(buf, 0);
+            buf ^= 1;
+          }
+        }
       }
     }
     if (!ok) *abort_flag = 1;
-    // never leave while a copy issued here may still be landing
-    for (unsigned i = it > C::kStages ? it - C::kStages : 0; i < it; ++i)
+    // never leave while a copy issued here may still be landing: the last one into each slot and buffer
+    for (unsigned i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
       mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1, status);
-    if (pieces) mbar_wait(&q_full, (pieces - 1) & 1, status);
+    for (int t = 0; t < 2; ++t)
+      if (uses[t]) mbar_wait(&q_full[t], (uses[t] - 1) & 1, status);
   } else if (warp == 1) {
     // ------------------------------------------------------------------------------- products
-    unsigned slot = 0, phase = 0, pieces = 0, steps[2] = {0, 0};
+    unsigned slot = 0, phase = 0, pieces = 0, steps[2] = {0, 0}, uses[2] = {0, 0};
+    int buf = 0;
     const uint32_t e = elect_lane();
     bool ok = true;
     while (ok && !*abort_flag && walk.next(b, a.x, pc)) {
       if (pc.u.none) continue;
       const bool two = pc.u.nq > QB;
       const int first = pc.u.tile0 + pc.t0, nk = pc.t1 - pc.t0, n = two ? 2 * nk : nk;
-      if (!(ok = mbar_wait(&q_full, pieces & 1, status))) break;
+      for (int t = two ? 0 : buf; t <= (two ? 1 : buf) && ok; ++t) ok = mbar_wait(&q_full[t], uses[t]++ & 1, status);
+      if (!ok) break;
+      const int qbuf = buf;
+      if (!two) buf ^= 1;
       unsigned kslot = 0, vslot = 0;
       auto take = [&](unsigned& at) {
         at = slot;
@@ -702,7 +698,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto qk = [&](int i) {
         if ((!two || !(i & 1)) && !take(kslot)) return false;
         tc_fence_after();
-        const uint32_t q = sb + (two && (i & 1) ? C::kTile : 0u), k = ring + kslot * C::kTile;
+        const int qb = two ? i & 1 : qbuf;
+        const uint32_t q = sb + qb * C::kTile, k = ring + kslot * C::kTile;
         const uint64_t dq = umma_desc_k_sw128(q), dk = umma_desc_k_sw128(k);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
@@ -711,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         umma_commit_if(e, &s_full[i & 1]);
         if (!two || (i & 1)) umma_commit_if(e, &empty[kslot]);
-        if (i == n - 1) umma_commit_if(e, &q_empty);
+        if (i >= n - (two ? 2 : 1)) umma_commit_if(e, &q_empty[qb]);
         return true;
       };
       auto pv = [&](int i) {
@@ -734,13 +731,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (i < 2 && pieces && !mbar_wait(&o_free, (pieces - 1) & 1, status)) return false;
-        if (!mbar_wait(&p_full[p], steps[p] & 1, status)) return false;
-        tc_fence_after();
         const uint64_t dv = umma_desc_sw128(ring + vslot * C::kTile, kBlk, 1024);
 #pragma unroll
-        for (int kk = 0; kk < kKT / 16; ++kk)
-          umma_f16_ta_if(e, tmem + kColO + (uint32_t)p * HD, tmem + (uint32_t)p * kKT + kk * 8, dv + ((kk * 2048u) >> 4), kIdO,
-                         (i >= 2 || kk) ? 1u : 0u);
+        for (int half = 0; half < 2; ++half) {
+          if (!mbar_wait(&p_full[p][half], steps[p] & 1, status)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+            umma_f16_ta_if(e, tmem + kColO + (uint32_t)p * HD, tmem + (uint32_t)p * kKT + kk * 8, dv + ((kk * 2048u) >> 4),
+                           kIdO, (i >= 2 || kk) ? 1u : 0u);
+        }
         umma_commit_if(e, &o_done[p]);
         if (!two || p) umma_commit_if(e, &empty[vslot]);
         ++steps[p];
@@ -761,6 +761,56 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+// The units that were cut: out = sum_parts 2^(m - M) o / sum_parts 2^(m - M) l, over the parts in the order of
+// the slots.  Block x looks after the unit that attention block x began; a thread takes 8 elements of a row,
+// and loads several parts at once, since each is a trip to L2.
+constexpr int kMergeThreads = 128, kMergeSlices = 8, kMergeParts = 4;
+template <int HD, typename T>
+__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid_constant__ PagedAttnParams a) {
+  pdl_wait();
+  const int4 d = __ldcg(reinterpret_cast<const int4*>(a.cuts + blockIdx.x));  // token, nq, head, parts
+  if (!d.w) return;
+  const int rows = d.y * a.gq;
+  for (int e = blockIdx.y * kMergeThreads + threadIdx.x; e < rows * (HD / 8); e += kMergeSlices * kMergeThreads) {
+    const int row = e % rows, c8 = e / rows;
+    float mm = -INFINITY, ll = 0.f, acc[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+    for (int k0 = 0; k0 < d.w; k0 += kMergeParts) {
+      float m[kMergeParts], l[kMergeParts];
+      float4 o[kMergeParts][2];
+#pragma unroll
+      for (int k = 0; k < kMergeParts; ++k) {
+        m[k] = -INFINITY;
+        l[k] = 0.f;
+        o[k][0] = o[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k0 + k < d.w) {
+          const float* rec = a.recs + ((size_t)(blockIdx.x + k0 + k) * 2 + (k0 + k == 0 ? 1 : 0)) * rec_floats<HD>();
+          const float4* ro = reinterpret_cast<const float4*>(rec) + (size_t)(2 * c8) * rows + row;
+          o[k][0] = __ldcg(ro);
+          o[k][1] = __ldcg(ro + rows);
+          m[k] = __ldcg(rec + HD * rows + row);
+          l[k] = __ldcg(rec + (HD + 1) * rows + row);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kMergeParts; ++k) {
+        const float mn = fmaxf(mm, m[k]);
+        const float old = mm == -INFINITY ? 0.f : ex2(mm - mn), w = m[k] == -INFINITY ? 0.f : ex2(m[k] - mn);
+        const float v[8] = {o[k][0].x, o[k][0].y, o[k][0].z, o[k][0].w, o[k][1].x, o[k][1].y, o[k][1].z, o[k][1].w};
+        mm = mn;
+        ll = ll * old + l[k] * w;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = acc[j] * old + v[j] * w;
+      }
+    }
+    const float inv = ll != 0.f ? 1.f / ll : 0.f;
+    T* out = static_cast<T*>(a.out) + (size_t)(d.x + row / a.gq) * a.out_stride + (size_t)(d.z * a.gq + row % a.gq) * HD + 8 * c8;
+    *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv),
+                                                pack2<T>(acc[4] * inv, acc[5] * inv), pack2<T>(acc[6] * inv, acc[7] * inv));
   }
 }
 
@@ -788,13 +838,17 @@ cudaError_t launch(const PagedAttnArgs& a, int grid, bool bf16, cudaStream_t s) 
   p.c = a.scale * 1.4426950408889634f;
   p.gq = gq;
   p.oob = (int)rows;
-  p.head = static_cast<unsigned*>(a.scratch);
+  p.status = static_cast<unsigned*>(a.scratch);
+  p.cuts = reinterpret_cast<Cut*>(static_cast<char*>(a.scratch) + 256);
   p.recs = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kHeadBytes);
   const void* fn = reinterpret_cast<const void*>(&paged_attn_kernel<HD, T>);
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::kSmem);
   if (e != cudaSuccess) return e;
   void* args[] = {&qm, &km, &vm, &p};
-  return cudaLaunchKernel(fn, dim3(grid), dim3(kThreads), args, Cfg<HD>::kSmem, s);
+  if ((e = cudaLaunchKernel(fn, dim3(grid), dim3(kThreads), args, Cfg<HD>::kSmem, s)) != cudaSuccess) return e;
+  if (a.b.max_pages * ps <= kKT) return cudaSuccess;  // every unit is one key tile: nothing is cut
+  return launch_kernel(reinterpret_cast<const void*>(&paged_merge_kernel<HD, T>), dim3(grid, kMergeSlices),
+                       dim3(kMergeThreads), 0, s, true, &p);
 }
 }  // namespace
 
