@@ -84,6 +84,6 @@ struct PagedAttnArgs {
   void* scratch;
 };
 size_t paged_attention_scratch(int head_dim, int n_sms);
-cudaError_t paged_attention(const PagedAttnArgs& a, int head_dim, int type, int n_sms, cudaStream_t s);
+cudaError_t paged_attention(const PagedAttnArgs& a, int head_dim, int type, int device, int n_sms, cudaStream_t s);
 
 }  // namespace yb

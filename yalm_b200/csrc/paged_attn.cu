@@ -34,6 +34,7 @@
 #include <cuda_bf16.h>
 
 #include <math.h>
+#include <atomic>
 #include <type_traits>
 
 #include "launch.h"
@@ -251,31 +252,14 @@ __device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long lon
 }
 
 // -------------------------------------------------------------------------------------------- numerics
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// 2^x of a pair on the multiply-add pipe, for a share of the weights: the special-function unit alone would
-// take as long as a tile's products.  x = n + f with n whole and |f| <= 1/2 (Cody and Waite's reduction; adding
-// 1.5 * 2^23 rounds to whole numbers and leaves n in the low bits), 2^f by the polynomial of degree 4 with the
-// least relative error on that range (2.6e-6, fitted by reweighted least squares), n added to the exponent.
-// Below 2^-125 the value does not matter.
-constexpr int kPolyPairs = 2;  // of 8 pairs
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-  x.x = fmaxf(x.x, -125.f);
-  x.y = fmaxf(x.y, -125.f);
-  const float2 big = make_float2(12582912.f, 12582912.f), nbig = make_float2(-12582912.f, -12582912.f);
-  const float2 t = add2(x, big);
-  const float2 n = add2(t, nbig);
-  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
-  float2 y = fma2(f, make_float2(0.009570102207362652f, 0.009570102207362652f),
-                  make_float2(0.05591786280274391f, 0.05591786280274391f));
-  y = fma2(y, f, make_float2(0.240247443318367f, 0.240247443318367f));
-  y = fma2(y, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
-  y = fma2(y, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-  y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23));
-  y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23));
   return y;
 }
 template <typename T>
@@ -448,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 4; k < kKT - 4; k += 8)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) c4[e] = fmaxf(fmaxf(c4[e], s[k + e]), s[k + 4 + e]);
+                for (int e = 0; e < 4; ++e) c4[e] = max3(c4[e], s[k + e], s[k + 4 + e]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) c4[e] = fmaxf(c4[e], s[kKT - 4 + e]);
             mx = fmaxf(fmaxf(c4[0], c4[1]), fmaxf(c4[2], c4[3])) * a.c;
@@ -473,33 +457,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float shift = m == -INFINITY ? 0.f : m - kBias;
           const float2 cc = make_float2(a.c, a.c), sh = make_float2(-shift, -shift);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          auto weights = [&](auto masked) {
 #pragma unroll
-            for (int w = 0; w < 8; ++w) {
-              uint32_t pk[8];
+          for (int w = 0; w < 8; ++w) {
+            uint32_t pk[8];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const int e = 16 * w + 2 * k;
-                float2 t = fma2(make_float2(s[e], s[e + 1]), cc, sh);
-                if (!masked.value && k >= 8 - kPolyPairs) {
-                  t = ex2_poly(t);
-                } else {
-                  t.x = ex2(t.x);
-                  t.y = ex2(t.y);
-                }
-                sum[k & 1] = add2(sum[k & 1], t);
-                pk[k] = pack2<T>(t.x, t.y);
-              }
-              tmem_st8_u32(ts + 8 * w, pk);
-              if (w == 3) {  // the first half's product may begin
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[p][0]);
-              }
+            for (int k = 0; k < 8; ++k) {
+              const int e = 16 * w + 2 * k;
+              float2 t = fma2(make_float2(s[e], s[e + 1]), cc, sh);
+              t.x = ex2(t.x);
+              t.y = ex2(t.y);
+              sum[k & 1] = add2(sum[k & 1], t);
+              pk[k] = pack2<T>(t.x, t.y);
             }
-          };
-          if (all) weights(std::false_type{}); else weights(std::true_type{});
+            tmem_st8_u32(ts + 8 * w, pk);
+            if (w == 3) {  // the first half's product may begin
+              tmem_st_wait();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_full[p][0]);
+            }
+          }
           l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
           tmem_st_wait();
         } else if (lane == 0) {
@@ -695,12 +672,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (++slot == C::kStages) slot = 0, phase ^= 1;
         return true;
       };
+      // the tiles of step i's products, taken in the order of the ring ahead of the waits for the weights
+      auto take_k = [&](int i) { return (two && (i & 1)) || take(kslot); };
+      auto take_v = [&](int i) {
+        if (two && (i & 1)) return true;
+        if (!take(vslot)) return false;
+        // slots behind the sequence's last one, in its last page, may hold anything: their weight is 0, and
+        // 0 * v has to be 0
+        const int rem = pc.sq.kv - (first + (two ? i >> 1 : i)) * kKT;
+        if (rem < kKT) {
+          const int end = min(kKT, ((rem + (1 << b.ps_log2) - 1) >> b.ps_log2) << b.ps_log2);
+          const uint32_t v = ring + vslot * C::kTile;
+          for (int x = lane; x < (end - rem) * 8 * C::kHalves; x += 32) {
+            const int h = x / ((end - rem) * 8), r = x % ((end - rem) * 8);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * kBlk + (rem * 8 + r) * 16u), "r"(0u)
+                         : "memory");
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        return true;
+      };
       auto qk = [&](int i) {
-        if ((!two || !(i & 1)) && !take(kslot)) return false;
-        tc_fence_after();
         const int qb = two ? i & 1 : qbuf;
-        const uint32_t q = sb + qb * C::kTile, k = ring + kslot * C::kTile;
-        const uint64_t dq = umma_desc_k_sw128(q), dk = umma_desc_k_sw128(k);
+        const uint64_t dq = umma_desc_k_sw128(sb + qb * C::kTile), dk = umma_desc_k_sw128(ring + kslot * C::kTile);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           const uint32_t off = ((kk / 4) * kBlk + (kk % 4) * 32u) >> 4;
@@ -709,47 +704,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         umma_commit_if(e, &s_full[i & 1]);
         if (!two || (i & 1)) umma_commit_if(e, &empty[kslot]);
         if (i >= n - (two ? 2 : 1)) umma_commit_if(e, &q_empty[qb]);
-        return true;
       };
-      auto pv = [&](int i) {
+      if ((ok = take_k(0))) {
+        tc_fence_after();
+        qk(0);
+      }
+      if (ok && n > 1 && (ok = take_k(1))) {
+        tc_fence_after();
+        qk(1);
+      }
+      for (int i = 0; i < n && ok; ++i) {
         const int p = i & 1;
-        if (!two || !p) {
-          if (!take(vslot)) return false;
-          // slots behind the sequence's last one, in its last page, may hold anything: their weight is 0, and
-          // 0 * v has to be 0
-          const int rem = pc.sq.kv - (first + (two ? i >> 1 : i)) * kKT;
-          if (rem < kKT) {
-            const int end = min(kKT, ((rem + (1 << b.ps_log2) - 1) >> b.ps_log2) << b.ps_log2);
-            const uint32_t v = ring + vslot * C::kTile;
-            for (int x = lane; x < (end - rem) * 8 * C::kHalves; x += 32) {
-              const int h = x / ((end - rem) * 8), r = x % ((end - rem) * 8);
-              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * kBlk + (rem * 8 + r) * 16u), "r"(0u)
-                           : "memory");
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
-        }
-        if (i < 2 && pieces && !mbar_wait(&o_free, (pieces - 1) & 1, status)) return false;
+        if (!(ok = take_v(i) && (i + 2 >= n || take_k(i + 2)))) break;
+        if (i < 2 && pieces && !(ok = mbar_wait(&o_free, (pieces - 1) & 1, status))) break;
         const uint64_t dv = umma_desc_sw128(ring + vslot * C::kTile, kBlk, 1024);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          if (!mbar_wait(&p_full[p][half], steps[p] & 1, status)) return false;
+          if (!(ok = mbar_wait(&p_full[p][half], steps[p] & 1, status))) break;
           tc_fence_after();
 #pragma unroll
           for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
             umma_f16_ta_if(e, tmem + kColO + (uint32_t)p * HD, tmem + (uint32_t)p * kKT + kk * 8, dv + ((kk * 2048u) >> 4),
                            kIdO, (i >= 2 || kk) ? 1u : 0u);
         }
+        if (!ok) break;
         umma_commit_if(e, &o_done[p]);
         if (!two || p) umma_commit_if(e, &empty[vslot]);
         ++steps[p];
-        return true;
-      };
-      ok = qk(0) && (n < 2 || qk(1));
-      for (int i = 0; i < n && ok && !*abort_flag; ++i) {
-        ok = pv(i);
-        if (ok && i + 2 < n) ok = qk(i + 2);
+        if (i + 2 < n) qk(i + 2);
       }
       ++pieces;
     }
@@ -821,7 +803,7 @@ size_t paged_attention_scratch(int head_dim, int n_sms) {
 
 namespace {
 template <int HD, typename T>
-cudaError_t launch(const PagedAttnArgs& a, int grid, bool bf16, cudaStream_t s) {
+cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cudaStream_t s) {
   const int K = a.b.n_kv_heads, ps = 1 << a.b.ps_log2, gq = a.b.n_heads / K, qb = kRows / gq;
   const long long rows = (long long)a.b.n_pages * K * ps;
   CUtensorMap qm, km, vm;
@@ -842,8 +824,14 @@ cudaError_t launch(const PagedAttnArgs& a, int grid, bool bf16, cudaStream_t s) 
   p.cuts = reinterpret_cast<Cut*>(static_cast<char*>(a.scratch) + 256);
   p.recs = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kHeadBytes);
   const void* fn = reinterpret_cast<const void*>(&paged_attn_kernel<HD, T>);
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::kSmem);
-  if (e != cudaSuccess) return e;
+  static std::atomic<unsigned long long> raised{0};  // devices (by bit) whose shared-memory cap is set
+  const unsigned long long bit = 1ull << (device & 63);
+  cudaError_t e;
+  if (device >= 64 || !(raised.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::kSmem);
+    if (e != cudaSuccess) return e;
+    if (device < 64) raised.fetch_or(bit, std::memory_order_release);
+  }
   void* args[] = {&qm, &km, &vm, &p};
   if ((e = cudaLaunchKernel(fn, dim3(grid), dim3(kThreads), args, Cfg<HD>::kSmem, s)) != cudaSuccess) return e;
   if (a.b.max_pages * ps <= kKT) return cudaSuccess;  // every unit is one key tile: nothing is cut
@@ -852,11 +840,11 @@ cudaError_t launch(const PagedAttnArgs& a, int grid, bool bf16, cudaStream_t s) 
 }
 }  // namespace
 
-cudaError_t paged_attention(const PagedAttnArgs& a, int head_dim, int type, int n_sms, cudaStream_t s) {
+cudaError_t paged_attention(const PagedAttnArgs& a, int head_dim, int type, int device, int n_sms, cudaStream_t s) {
   const int grid = n_sms < kMaxGrid ? n_sms : kMaxGrid;
   if (head_dim == 128)
-    return type == 1 ? launch<128, __half>(a, grid, false, s) : launch<128, __nv_bfloat16>(a, grid, true, s);
-  return type == 1 ? launch<64, __half>(a, grid, false, s) : launch<64, __nv_bfloat16>(a, grid, true, s);
+    return type == 1 ? launch<128, __half>(a, device, grid, false, s) : launch<128, __nv_bfloat16>(a, device, grid, true, s);
+  return type == 1 ? launch<64, __half>(a, device, grid, false, s) : launch<64, __nv_bfloat16>(a, device, grid, true, s);
 }
 
 }  // namespace yb

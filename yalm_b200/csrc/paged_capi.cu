@@ -2,6 +2,7 @@
 #include "engine.h"
 #include "paged.cuh"
 
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <initializer_list>
@@ -59,11 +60,9 @@ int check_rows(const char* name, const void* p, long long stride, long long widt
   return 0;
 }
 
-// Every buffer must be memory that the current device can read: a host pointer or another device's
+// Every buffer must be memory that the current device `dev` can read: a host pointer or another device's
 // memory is refused here instead of faulting in the kernel.
-int check_device(std::initializer_list<std::pair<const char*, const void*>> bufs) {
-  int dev = 0;
-  YB_CK(cudaGetDevice(&dev));
+int check_device(int dev, std::initializer_list<std::pair<const char*, const void*>> bufs) {
   for (const auto& b : bufs) {
     if (!b.second) continue;
     cudaPointerAttributes at;
@@ -74,13 +73,19 @@ int check_device(std::initializer_list<std::pair<const char*, const void*>> bufs
   return 0;
 }
 
-int device_sms() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+// SMs of a device, asked for once (148 without one, so that sizes can be computed anywhere)
+int device_sms(int dev) {
+  static std::atomic<int> known[64];
+  if (dev >= 0 && dev < 64) {
+    const int n = known[dev].load(std::memory_order_relaxed);
+    if (n) return n;
+  }
+  int n = 0;
+  if (dev < 0 || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
     cudaGetLastError();
     return 148;
   }
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 
@@ -103,7 +108,9 @@ extern "C" int yb_paged_append_dev(const yb_paged_batch* b, void* q_out, long lo
   if (rotary_dim && !inv_freq_dev) return set_error(YB_E_INVALID, "null inv_freq_dev");
   if (!(eps >= 0.f) || !(qkv_clip > 0.f)) return set_error(YB_E_INVALID, "eps must be >= 0 and qkv_clip > 0");
   if (empty) return 0;
-  rc = check_device({{"q_out", q_out}, {"qkv", qkv}, {"q_start_dev", b->q_start_dev}, {"kv_len_dev", b->kv_len_dev},
+  int dev = 0;
+  YB_CK(cudaGetDevice(&dev));
+  rc = check_device(dev, {{"q_out", q_out}, {"qkv", qkv}, {"q_start_dev", b->q_start_dev}, {"kv_len_dev", b->kv_len_dev},
                      {"page_table_dev", b->page_table_dev}, {"k_pages", b->k_pages}, {"v_pages", b->v_pages},
                      {"q_norm_dev", q_norm_dev}, {"k_norm_dev", k_norm_dev}, {"inv_freq_dev", inv_freq_dev},
                      {"pos_dev", pos_dev}});
@@ -130,7 +137,12 @@ extern "C" size_t yb_paged_attention_scratch_bytes(const yb_paged_batch* b) {
   PagedBatch p;
   bool empty;
   if (check_batch(b, &p, &empty)) return 0;
-  return paged_attention_scratch(b->head_dim, device_sms());
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    dev = -1;
+  }
+  return paged_attention_scratch(b->head_dim, device_sms(dev));
 }
 
 extern "C" int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long long out_stride, const void* q,
@@ -145,7 +157,9 @@ extern "C" int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long l
   if (window < 0) return set_error(YB_E_INVALID, "negative window");
   if (!scratch_dev || !aligned16(scratch_dev)) return set_error(YB_E_INVALID, "scratch_dev must be 16-byte aligned memory");
   if (empty) return 0;
-  rc = check_device({{"out", out}, {"q", q}, {"q_start_dev", b->q_start_dev}, {"kv_len_dev", b->kv_len_dev},
+  int dev = 0;
+  YB_CK(cudaGetDevice(&dev));
+  rc = check_device(dev, {{"out", out}, {"q", q}, {"q_start_dev", b->q_start_dev}, {"kv_len_dev", b->kv_len_dev},
                      {"page_table_dev", b->page_table_dev}, {"k_pages", b->k_pages}, {"v_pages", b->v_pages},
                      {"scratch_dev", scratch_dev}});
   if (rc) return rc;
@@ -158,6 +172,6 @@ extern "C" int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long l
   a.scale = scale;
   a.window = window ? window : INT_MAX;
   a.scratch = scratch_dev;
-  YB_CK(paged_attention(a, b->head_dim, b->dtype, device_sms(), static_cast<cudaStream_t>(stream)));
+  YB_CK(paged_attention(a, b->head_dim, b->dtype, dev, device_sms(dev), static_cast<cudaStream_t>(stream)));
   return 0;
 }

@@ -53,39 +53,50 @@ class PagedBatch:
             kv_len_dev=kv_len.data_ptr(), page_table_dev=page_table.data_ptr(), k_pages=k_pages.data_ptr(),
             v_pages=v_pages.data_ptr())
         self._ref = ctypes.byref(self.c)
-        self._q_width = self.n_heads * self.head_dim
+        self._append, self._attend = _lib.lib().yb_paged_append_dev, _lib.lib().yb_paged_attention_dev
         self._scratch = 0
-        self._qkv_width = (self.n_heads + 2 * self.n_kv_heads) * self.head_dim
+        self._scale = 1.0 / math.sqrt(self.head_dim)
+        self._codes = {}
+        self._index = k_pages.get_device()
+        import torch  # the caller's tensors are torch's; the package itself does not need it
+        self._f32, self._i32 = torch.float32, torch.int32
+        self._q_shape = (self.n_tokens, self.n_heads * self.head_dim)
+        self._qkv_shape = (self.n_tokens, (self.n_heads + 2 * self.n_kv_heads) * self.head_dim)
 
-    def _rows(self, t, name: str, width: int) -> int:
+    def _rows(self, t, name: str, shape) -> int:
         """Checks a token-major tensor and returns its row stride in elements."""
-        if tuple(t.shape) != (self.n_tokens, width) or t.stride(1) != 1 or t.device != self.device:
-            raise ValueError(f"{name} must be [{self.n_tokens}][{width}] with unit column stride on {self.device}")
-        return t.stride(0) if self.n_tokens > 1 else max(t.stride(0), width)
+        row, col = t.stride()
+        if t.shape != shape or col != 1 or t.get_device() != self._index:
+            raise ValueError(f"{name} must be [{shape[0]}][{shape[1]}] with unit column stride on {self.device}")
+        return row if self.n_tokens > 1 else shape[1]
+
+    def _vector(self, t, name: str, n: int, dtype):
+        """Checks an optional vector and returns its address."""
+        if t is None:
+            return None
+        if t.dtype is not dtype or t.numel() < n or t.get_device() != self._index or not t.is_contiguous():
+            raise ValueError(f"{name} must hold {n} contiguous {dtype} values on {self.device}")
+        return t.data_ptr()
 
     def append(self, qkv, q_out, inv_freq, rotary_dim: int, *, q_norm=None, k_norm=None, eps: float = 1e-5,
                half: bool = False, pos=None, clip: float = FLT_MAX, stream: int = 0) -> None:
         """yb_paged_append_dev: clip, norm and rotate qkv [n_tokens][(n_heads + 2 n_kv_heads) head_dim], queries to
         q_out, keys and values into their pages."""
-        src = _dtype(qkv, "qkv")
-        s_in, s_out = self._rows(qkv, "qkv", self._qkv_width), self._rows(q_out, "q_out", self._q_width)
+        src = self._codes.get(qkv.dtype)
+        if src is None:
+            src = self._codes[qkv.dtype] = _dtype(qkv, "qkv")
+        s_in, s_out = self._rows(qkv, "qkv", self._qkv_shape), self._rows(q_out, "q_out", self._q_shape)
         if q_out.dtype != self._dtype:
             raise ValueError("q_out must have the caches' type")
-        for name, t, n, d in (("q_norm", q_norm, self.head_dim, "torch.float32"),
-                              ("k_norm", k_norm, self.head_dim, "torch.float32"),
-                              ("inv_freq", inv_freq if rotary_dim else None, rotary_dim // 2, "torch.float32"),
-                              ("pos", pos, self.n_tokens, "torch.int32")):
-            if t is not None and (t.numel() < n or not t.is_contiguous() or str(t.dtype) != d
-                                  or t.device != self.device):
-                raise ValueError(f"{name} must hold {n} contiguous {d} values on {self.device}")
-        _lib.call("yb_paged_append_dev", self._ref, q_out.data_ptr(), s_out, qkv.data_ptr(), s_in, src,
-                  q_norm.data_ptr() if q_norm is not None else None,
-                  k_norm.data_ptr() if k_norm is not None else None, eps,
-                  inv_freq.data_ptr() if inv_freq is not None else None, rotary_dim, 1 if half else 0,
-                  pos.data_ptr() if pos is not None else None, clip, stream)
+        _lib.check(self._append(
+            self._ref, q_out.data_ptr(), s_out, qkv.data_ptr(), s_in, src,
+            self._vector(q_norm, "q_norm", self.head_dim, self._f32),
+            self._vector(k_norm, "k_norm", self.head_dim, self._f32), eps,
+            self._vector(inv_freq if rotary_dim else None, "inv_freq", rotary_dim // 2, self._f32), rotary_dim,
+            1 if half else 0, self._vector(pos, "pos", self.n_tokens, self._i32), clip, stream))
 
     def scratch_bytes(self) -> int:
-        """Size of attend's workspace: zero-filled before its first use, one per stream of calls."""
+        """Size of attend's workspace: one for each stream of calls, its contents of no meaning between calls."""
         if not self._scratch:
             self._scratch = _lib.lib().yb_paged_attention_scratch_bytes(self._ref)
             if not self._scratch:
@@ -94,11 +105,11 @@ class PagedBatch:
 
     def attend(self, q, out, scratch, *, scale: float | None = None, window: int = 0, stream: int = 0) -> None:
         """yb_paged_attention_dev: causal attention of q [n_tokens][n_heads * head_dim] over the caches."""
-        s_q, s_out = self._rows(q, "q", self._q_width), self._rows(out, "out", self._q_width)
+        s_q, s_out = self._rows(q, "q", self._q_shape), self._rows(out, "out", self._q_shape)
         if q.dtype != self._dtype or out.dtype != self._dtype:
             raise ValueError("q and out must have the caches' type")
-        if scratch.device != self.device or not scratch.is_contiguous() or \
-                scratch.numel() * scratch.element_size() < self.scratch_bytes():
+        if scratch.get_device() != self._index or not scratch.is_contiguous() or \
+                scratch.numel() * scratch.element_size() < (self._scratch or self.scratch_bytes()):
             raise ValueError("scratch must hold scratch_bytes() contiguous bytes")
-        _lib.call("yb_paged_attention_dev", self._ref, out.data_ptr(), s_out, q.data_ptr(), s_q,
-                  1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, scratch.data_ptr(), stream)
+        _lib.check(self._attend(self._ref, out.data_ptr(), s_out, q.data_ptr(), s_q,
+                                self._scale if scale is None else scale, window, scratch.data_ptr(), stream))
