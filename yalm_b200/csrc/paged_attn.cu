@@ -18,11 +18,16 @@
 //
 // Block.  Two pipelines of 128 rows share the tensor cores, one's softmax under the other's products:
 //   warp 0       loads Q (a 3-D box of queries x heads) and the ring of K and V tiles, one lane a page
-//   warp 1       issues the products: S[p] = Q . K^T into tensor memory, then O[p] += P . V with P read from
-//                tensor memory, where it took the place of S
-//   warps 4-7, 8-11   softmax of pipeline 0 / 1, a row per thread (they take over registers of warps 0-3)
-// A unit of two row tiles runs them as the pipelines over the same key tiles.  A unit of one row tile (single
-// tokens, short chunks) gives the pipelines alternate key tiles, and merges the two at its end.
+//   warps 1, 2   issue the products of pipeline 0 / 1, 64 slots a step: S = Q . K^T into tensor memory, then
+//                O += P . V with P read from tensor memory, where it took the place of S (one warp for both
+//                pipelines was the bottleneck: 1300 clocks a step, of which the products are 650).  S has two buffers, so the
+//                scores of a step are there before the softmax of the step before is done.  (Steps of 128
+//                slots leave no room for that: 512 columns hold two outputs and two such S.  A pipeline then
+//                waits a third of its time for its scores.  The 64-column products run at 0.75 of the
+//                rate of the 128-column ones and still win: profiles/paged_attention.md.)
+//   warps 4-7, 8-11   softmax of pipeline 0 / 1, a row per thread
+// A unit of two row tiles runs them as the pipelines over the same slots.  A unit of one row tile (single
+// tokens, short chunks) gives each pipeline half of every key tile, and merges the two at its end.
 //
 // P is rounded to the caches' type for the tensor cores (the weights' rounding error is that of the
 // output's rounding, and averages over the slots); scores, maxima, sums and outputs are fp32.  The output is
@@ -46,9 +51,9 @@ namespace yb {
 namespace {
 
 constexpr int kKT = 128;       // slots per key tile
+constexpr int kST = 64;        // slots per step
 constexpr int kRows = 128;     // rows per row tile = tensor-memory lanes
 constexpr int kThreads = 384;
-constexpr int kRegsFew = 56, kRegsMany = 224;  // 128 * 56 + 256 * 224 <= 384 * 168, the registers at launch
 constexpr int kMaxGrid = 256;  // blocks the workspace has counters for
 constexpr uint32_t kBlk = kRows * 128;  // bytes of 128 rows x 64 elements
 
@@ -318,16 +323,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                       const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PagedAttnParams a) {
   using C = Cfg<HD>;
   constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
-  constexpr uint32_t kIdS = kBf16 ? umma_idesc_bf16(kRows, kKT, 0, 0) : umma_idesc_f16(kRows, kKT, 0, 0);
+  constexpr uint32_t kIdS = kBf16 ? umma_idesc_bf16(kRows, kST, 0, 0) : umma_idesc_f16(kRows, kST, 0, 0);
   constexpr uint32_t kIdO = kBf16 ? umma_idesc_bf16(kRows, HD, 0, 1) : umma_idesc_f16(kRows, HD, 0, 1);
   constexpr float kBias = kBf16 ? 0.f : 7.f;
-  constexpr uint32_t kColO = 2 * kKT;  // tensor memory: S0, S1, O0, O1
+  constexpr uint32_t kColO = 4 * kST;  // tensor memory: two buffers of S0, of S1, then O0, O1
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sb = smem_u32(smem), ring = sb + 2 * C::kTile;
   float* s_ml = reinterpret_cast<float*>(smem + (2 + C::kStages) * C::kTile);  // [2][128]
-  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], q_full[2], q_empty[2], s_full[2], p_full[2][2],
-      o_done[2], o_free, ml_ready, ml_free;
+  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], q_full[2], q_empty[2], s_full[2][2],
+      p_full[2][2], o_done[2][2], o_free, ml_ready;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ unsigned long long s_scan[kThreads / 32];
@@ -340,23 +345,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  } else if (threadIdx.x == 64) {
+  } else if (threadIdx.x == 96) {
     s_abort = 0;
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], 2);
     }
     for (int p = 0; p < 2; ++p) {
       mbar_init(&q_full[p], 1);
-      mbar_init(&q_empty[p], 1);
-      mbar_init(&s_full[p], 1);
-      mbar_init(&p_full[p][0], 4);
-      mbar_init(&p_full[p][1], 4);
-      mbar_init(&o_done[p], 1);
+      mbar_init(&q_empty[p], 2);
+      for (int u = 0; u < 2; ++u) {
+        mbar_init(&s_full[p][u], 1);
+        mbar_init(&p_full[p][u], 4);
+        mbar_init(&o_done[p][u], 1);
+      }
     }
     mbar_init(&o_free, 8);
     mbar_init(&ml_ready, 4);
-    mbar_init(&ml_free, 4);
     mbar_fence_init();
     tma_prefetch_map(&qmap);
     tma_prefetch_map(&kmap);
@@ -373,20 +378,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   Walk walk(s_start);
   Piece pc;
   if (warp >= 4) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
     // ------------------------------------------------------------------------------- softmax
     const int p = (warp - 4) >> 2, quad = warp & 3;  // pipeline, tensor-memory lane quadrant
     const int r = quad * 32 + lane;                  // row of the row tile
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    const uint32_t ts = tmem + lanes + (uint32_t)p * kKT, to = tmem + lanes + kColO;
+    const uint32_t ts = tmem + lanes + (uint32_t)p * 2 * kST, to = tmem + lanes + kColO;
     const int qi = r / a.gq, h = r % a.gq;
-    unsigned steps[2] = {0, 0};  // steps of either pipeline in the pieces before
-    unsigned singles = 0;
+    unsigned steps = 0, singles = 0;  // a pipeline's steps in the pieces before; pieces of one row tile
     if (threadIdx.x == 128) a.cuts[blockIdx.x].parts = 0;  // the same thread's later store tells otherwise
     bool ok = true;
     while (ok && !*abort_flag && walk.next(b, a.x, pc)) {
       const bool two = pc.u.nq > QB;
-      const int nk = pc.u.none ? 0 : pc.t1 - pc.t0;
+      const int nk = pc.u.none ? 0 : pc.t1 - pc.t0, n = two ? 2 * nk : nk;  // key tiles, steps
       const int tile = two ? p : 0;  // row tile
       const int q = tile * QB + qi;  // query of the unit
       const bool valid = r < QB * a.gq && q < pc.u.nq;
@@ -394,7 +397,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int pos = pc.sq.kv - pc.sq.n + pc.u.q0 + q;
       const int* table = b.page_table + (size_t)pc.seq * b.max_pages;
       const int first = pc.u.tile0 + pc.t0;
-      const int mine = two ? nk : (nk + 1 - p) / 2, inc = two ? 1 : 2, off = two ? 0 : p;
       // whether the 16 slots of lane i < 8 are on a page that is there
       auto there = [&](int t) {
         const int slot = (t << 7) + lane * 16;
@@ -403,24 +405,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         return lane < 8 && id >= 0 && id < b.n_pages;
       };
       float m = -INFINITY, l = 0.f;
-      bool nx = mine > 0 && there(first + off);
-      for (int i = 0; i < mine; ++i) {
-        const int t = first + off + i * inc;
-        const uint32_t pages = __ballot_sync(0xffffffffu, nx) & 0xffu;
-        if (i + 1 < mine) nx = there(t + inc);
-        if (*abort_flag || !(ok = mbar_wait(&s_full[p], (steps[p] + i) & 1, status))) break;
+      bool nx = nk > 0 && there(first);
+      uint32_t pages = 0;
+      for (int i = 0; i < n; ++i) {
+        const int t = two ? i >> 1 : i, half = two ? i & 1 : p;
+        if (!two || !half) {
+          pages = __ballot_sync(0xffffffffu, nx);
+          if (t + 1 < nk) nx = there(first + t + 1);
+        }
+        const unsigned step = steps + i, buf = step & 1;
+        if (!(ok = mbar_wait(&s_full[p][buf], (step >> 1) & 1, status))) break;
         tc_fence_after();
         if (live) {
-          const int k0 = t * kKT;
-          const int lo = valid ? pos - a.x.window + 1 - k0 : kKT, hi = valid ? pos + 1 - k0 : 0;
-          float s[kKT];
-          tmem_ld128(ts, s);
+          const int k0 = (first + t) * kKT + half * kST;
+          const int lo = valid ? pos - a.x.window + 1 - k0 : kST, hi = valid ? pos + 1 - k0 : 0;
+          const uint32_t here = (pages >> (4 * half)) & 0xfu;
+          float s[kST];
+          tmem_ld64(ts + buf * kST, s);
           // rows behind the unit's last one compute with what lies in their lanes; nothing reads them
-          const bool all = __all_sync(0xffffffffu, !valid || (lo <= 0 && hi >= kKT && pages == 0xffu));
-          if (!all) {
+          if (!__all_sync(0xffffffffu, !valid || (lo <= 0 && hi >= kST && here == 0xfu))) {
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const uint32_t pg = ((pages >> (2 * w)) & 1u ? 0xffffu : 0u) | ((pages >> (2 * w + 1)) & 1u ? 0xffff0000u : 0u);
+            for (int w = 0; w < 2; ++w) {
+              const uint32_t pg = ((here >> (2 * w)) & 1u ? 0xffffu : 0u) | ((here >> (2 * w + 1)) & 1u ? 0xffff0000u : 0u);
               const uint32_t msk = bit_range(lo - 32 * w, hi - 32 * w) & pg;
 #pragma unroll
               for (int k = 0; k < 32; ++k) s[32 * w + k] = (msk >> k) & 1u ? s[32 * w + k] : -INFINITY;
@@ -430,76 +436,72 @@ __global__ void __launch_bounds__(kThreads, 1)
           {
             float c4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int k = 4; k < kKT - 4; k += 8)
+            for (int k = 4; k < kST - 4; k += 8)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) c4[e] = max3(c4[e], s[k + e], s[k + 4 + e]);
+              for (int e = 0; e < 4; ++e) c4[e] = max3(c4[e], s[k + e], s[k + 4 + e]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) c4[e] = fmaxf(c4[e], s[kKT - 4 + e]);
-            mx = fmaxf(fmaxf(c4[0], c4[1]), fmaxf(c4[2], c4[3])) * a.c;
+            for (int e = 0; e < 4; ++e) c4[e] = fmaxf(c4[e], s[kST - 4 + e]);
+            mx = fmaxf(max3(c4[0], c4[1], c4[2]), c4[3]) * a.c;
           }
           const bool need = valid && mx > m + 8.0f;  // the first slots seen, or a maximum grown by over 2^8
-          const float mn = need ? mx : m;
-          const float alpha = need ? ex2(m - mn) : 1.f;  // 0 while m is -inf
-          if (i > 0 && __any_sync(0xffffffffu, need)) {
-            if (!(ok = mbar_wait(&o_done[p], (steps[p] + i - 1) & 1, status))) break;
-            tc_fence_after();
+          float alpha = 1.f;
+          if (__any_sync(0xffffffffu, need)) {
+            const float mn = need ? mx : m;
+            alpha = need ? ex2(m - mn) : 1.f;  // 0 while m is -inf
+            m = mn;
+            if (i > 0) {
+              if (!(ok = mbar_wait(&o_done[p][buf ^ 1], ((step - 1) >> 1) & 1, status))) break;
+              tc_fence_after();
 #pragma unroll 1
-            for (int c0 = 0; c0 < HD; c0 += 16) {
-              float v[16];
-              tmem_ld16(to + p * HD + c0, v);
-              uint32_t u[16];
+              for (int c0 = 0; c0 < HD; c0 += 16) {
+                float v[16];
+                tmem_ld16(to + p * HD + c0, v);
+                uint32_t u[16];
 #pragma unroll
-              for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(v[k] * alpha);
-              tmem_st16_u32(to + p * HD + c0, u);
+                for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(v[k] * alpha);
+                tmem_st16_u32(to + p * HD + c0, u);
+              }
             }
           }
-          m = mn;
           const float shift = m == -INFINITY ? 0.f : m - kBias;
           const float2 cc = make_float2(a.c, a.c), sh = make_float2(-shift, -shift);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-          for (int w = 0; w < 8; ++w) {
+          for (int w = 0; w < kST / 16; ++w) {
             uint32_t pk[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const int e = 16 * w + 2 * k;
-              float2 t = fma2(make_float2(s[e], s[e + 1]), cc, sh);
-              t.x = ex2(t.x);
-              t.y = ex2(t.y);
-              sum[k & 1] = add2(sum[k & 1], t);
-              pk[k] = pack2<T>(t.x, t.y);
+              float2 t2 = fma2(make_float2(s[e], s[e + 1]), cc, sh);
+              t2.x = ex2(t2.x);
+              t2.y = ex2(t2.y);
+              sum[k & 1] = add2(sum[k & 1], t2);
+              pk[k] = pack2<T>(t2.x, t2.y);
             }
-            tmem_st8_u32(ts + 8 * w, pk);
-            if (w == 3) {  // the first half's product may begin
-              tmem_st_wait();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&p_full[p][0]);
-            }
+            tmem_st8_u32(ts + buf * kST + 8 * w, pk);
           }
           l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
           tmem_st_wait();
-        } else if (lane == 0) {
-          mbar_arrive(&p_full[p][0]);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[p][1]);
+        if (lane == 0) mbar_arrive(&p_full[p][buf]);
       }
       if (!ok || *abort_flag) break;
 
       // ---- the piece's rows: o * w0 (+ o of pipeline 1 * w1)
-      const int other = two ? 0 : nk / 2;  // steps of pipeline 1 that pipeline 0 merges
+      const bool other = !two && nk > 0;  // pipeline 0 takes pipeline 1's rows in
       float w0 = 1.f, w1 = 0.f;
-      if (mine > 0) {
-        if (!(ok = mbar_wait(&o_done[p], (steps[p] + mine - 1) & 1, status))) break;
-      }
-      if (!two && nk > 0) {
+      // (a barrier for each buffer: its phase before the awaited one is over, since the scores that came into the
+      // buffer later followed the product of that phase)
+      if (n > 0) ok = mbar_wait(&o_done[p][(steps + n - 1) & 1], ((steps + n - 1) >> 1) & 1, status);
+      if (!ok) break;
+      if (other) {
         if (p == 1) {
-          // pipeline 0 is through with the piece before (it may be slower than a pipeline without steps)
-          if (singles && !(ok = mbar_wait(&ml_free, (singles - 1) & 1, status))) break;
           s_ml[r] = m;
           s_ml[kRows + r] = l;
+          tc_fence_after();
+          tc_fence_before();
           __syncwarp();
           if (lane == 0) {
             mbar_arrive(&ml_ready);
@@ -507,14 +509,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
           if (!(ok = mbar_wait(&ml_ready, singles & 1, status))) break;
-          if (other > 0) {
-            if (!(ok = mbar_wait(&o_done[1], (steps[1] + other - 1) & 1, status))) break;
-            const float m1 = s_ml[r], l1 = s_ml[kRows + r], mm = fmaxf(m, m1);
-            w0 = m == -INFINITY ? 0.f : ex2(m - mm);
-            w1 = m1 == -INFINITY ? 0.f : ex2(m1 - mm);
-            l = l * w0 + l1 * w1;
-            m = mm;
-          }
+          const float m1 = s_ml[r], l1 = s_ml[kRows + r], mm = fmaxf(m, m1);
+          w0 = m == -INFINITY ? 0.f : ex2(m - mm);
+          w1 = m1 == -INFINITY ? 0.f : ex2(m1 - mm);
+          l = l * w0 + l1 * w1;
+          m = mm;
         }
         ++singles;
       }
@@ -536,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_ld32(to + p * HD + c0, v);
 #pragma unroll
               for (int k = 0; k < 32; ++k) v[k] = l != 0.f ? v[k] * w0 : 0.f;
-              if (other > 0) {
+              if (other) {
                 float v1[32];
                 tmem_ld32(to + HD + c0, v1);
 #pragma unroll
@@ -566,22 +565,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (nk > 0 && lane == 0) {
-          mbar_arrive(&o_free);
-          if (!two) mbar_arrive(&ml_free);
-        }
+        if (nk > 0 && lane == 0) mbar_arrive(&o_free);
       }
       if (!whole && pc.t0 == 0 && threadIdx.x == 128) {
         const unsigned long long begin = s_start.begin + (s_start.left - walk.st.left) - pc.t1;  // the unit's first tile
         const int last = block_of(s_start.share, s_start.more, begin + pc.u.cost - 1);
         a.cuts[blockIdx.x] = Cut{token, pc.u.nq, pc.head, last - (int)blockIdx.x + 1};
       }
-      steps[0] += two ? nk : (nk + 1) / 2;
-      steps[1] += two ? nk : nk / 2;
+      steps += n;
     }
     if (!ok) *abort_flag = 1;
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
   if (warp == 0) {
     // ------------------------------------------------------------------------------- loads
     const int lg = b.ps_log2, ps = 1 << lg;
@@ -625,7 +619,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         return true;
       };
-      // in the order of the products: K of steps 0 and 1, then V of step i and K of step i + 2
+      // in the order of the products, whose scores are two steps ahead of the weights: one key tile with two row
+      // tiles, two with one
       const int first = pc.u.tile0 + pc.t0, n = pc.t1 - pc.t0, ahead = two ? 1 : 2;
       int next_row = row_of(first);
       for (int j = 0; j < n + ahead && ok; ++j) {
@@ -651,9 +646,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1, status);
     for (int t = 0; t < 2; ++t)
       if (uses[t]) mbar_wait(&q_full[t], (uses[t] - 1) & 1, status);
-  } else if (warp == 1) {
+  } else if (warp < 3) {
     // ------------------------------------------------------------------------------- products
-    unsigned slot = 0, phase = 0, pieces = 0, steps[2] = {0, 0}, uses[2] = {0, 0};
+    const int p = warp - 1;
+    const uint32_t ts = tmem + (uint32_t)p * 2 * kST, to = tmem + kColO + (uint32_t)p * HD;
+    unsigned slot = 0, phase = 0, pieces = 0, steps = 0, uses[2] = {0, 0};
     int buf = 0;
     const uint32_t e = elect_lane();
     bool ok = true;
@@ -661,10 +658,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (pc.u.none) continue;
       const bool two = pc.u.nq > QB;
       const int first = pc.u.tile0 + pc.t0, nk = pc.t1 - pc.t0, n = two ? 2 * nk : nk;
-      for (int t = two ? 0 : buf; t <= (two ? 1 : buf) && ok; ++t) ok = mbar_wait(&q_full[t], uses[t]++ & 1, status);
+      const int qb = two ? p : buf;
+      // each pipeline's warp keeps count of both buffers, whichever it reads
+      for (int t = two ? 0 : buf; t <= (two ? 1 : buf); ++t) {
+        if (t == qb) ok = mbar_wait(&q_full[t], uses[t] & 1, status);
+        ++uses[t];
+      }
       if (!ok) break;
-      const int qbuf = buf;
-      if (!two) buf ^= 1;
       unsigned kslot = 0, vslot = 0;
       auto take = [&](unsigned& at) {
         at = slot;
@@ -672,13 +672,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (++slot == C::kStages) slot = 0, phase ^= 1;
         return true;
       };
-      // the tiles of step i's products, taken in the order of the ring ahead of the waits for the weights
-      auto take_k = [&](int i) { return (two && (i & 1)) || take(kslot); };
+      // a key tile serves two steps of a unit of two row tiles, else one, on this pipeline's half
+      auto begins = [&](int i) { return !two || !(i & 1); };
+      auto ends = [&](int i) { return !two || (i & 1); };
+      auto half_of = [&](int i) { return (uint32_t)(two ? i & 1 : p) * (kST * 128u); };  // bytes into the blocks
+      auto take_k = [&](int i) { return !begins(i) || take(kslot); };
       auto take_v = [&](int i) {
-        if (two && (i & 1)) return true;
+        if (!begins(i)) return true;
         if (!take(vslot)) return false;
         // slots behind the sequence's last one, in its last page, may hold anything: their weight is 0, and
-        // 0 * v has to be 0
+        // 0 * v has to be 0 (both warps write the same zeros)
         const int rem = pc.sq.kv - (first + (two ? i >> 1 : i)) * kKT;
         if (rem < kKT) {
           const int end = min(kKT, ((rem + (1 << b.ps_log2) - 1) >> b.ps_log2) << b.ps_log2);
@@ -693,47 +696,44 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         return true;
       };
+      const uint64_t dq = umma_desc_k_sw128(sb + qb * C::kTile);
       auto qk = [&](int i) {
-        const int qb = two ? i & 1 : qbuf;
-        const uint64_t dq = umma_desc_k_sw128(sb + qb * C::kTile), dk = umma_desc_k_sw128(ring + kslot * C::kTile);
+        const unsigned u = (steps + i) & 1;
+        const uint64_t dk = umma_desc_k_sw128(ring + kslot * C::kTile + half_of(i));
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           const uint32_t off = ((kk / 4) * kBlk + (kk % 4) * 32u) >> 4;
-          umma_f16_if(e, tmem + (uint32_t)(i & 1) * kKT, dq + off, dk + off, kIdS, kk ? 1u : 0u);
+          umma_f16_if(e, ts + u * kST, dq + off, dk + off, kIdS, kk ? 1u : 0u);
         }
-        umma_commit_if(e, &s_full[i & 1]);
-        if (!two || (i & 1)) umma_commit_if(e, &empty[kslot]);
-        if (i >= n - (two ? 2 : 1)) umma_commit_if(e, &q_empty[qb]);
+        umma_commit_if(e, &s_full[p][u]);
+        if (ends(i)) umma_commit_if(e, &empty[kslot]);
+        if (i == n - 1) {
+          umma_commit_if(e, &q_empty[two ? 0 : qb]);
+          if (two) umma_commit_if(e, &q_empty[1]);
+        }
       };
-      if ((ok = take_k(0))) {
+      // a buffer of S is free again once the product that reads P from it is issued: they execute in order
+      for (int i = 0; i < min(n, 2) && (ok = take_k(i)); ++i) {
         tc_fence_after();
-        qk(0);
-      }
-      if (ok && n > 1 && (ok = take_k(1))) {
-        tc_fence_after();
-        qk(1);
+        qk(i);
       }
       for (int i = 0; i < n && ok; ++i) {
-        const int p = i & 1;
+        const unsigned step = steps + i, u = step & 1;
         if (!(ok = take_v(i) && (i + 2 >= n || take_k(i + 2)))) break;
-        if (i < 2 && pieces && !(ok = mbar_wait(&o_free, (pieces - 1) & 1, status))) break;
-        const uint64_t dv = umma_desc_sw128(ring + vslot * C::kTile, kBlk, 1024);
+        if (i == 0 && pieces && !(ok = mbar_wait(&o_free, (pieces - 1) & 1, status))) break;
+        const uint64_t dv = umma_desc_sw128(ring + vslot * C::kTile + half_of(i), kBlk, 1024);
+        if (!(ok = mbar_wait(&p_full[p][u], (step >> 1) & 1, status))) break;
+        tc_fence_after();
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (!(ok = mbar_wait(&p_full[p][half], steps[p] & 1, status))) break;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-            umma_f16_ta_if(e, tmem + kColO + (uint32_t)p * HD, tmem + (uint32_t)p * kKT + kk * 8, dv + ((kk * 2048u) >> 4),
-                           kIdO, (i >= 2 || kk) ? 1u : 0u);
-        }
-        if (!ok) break;
-        umma_commit_if(e, &o_done[p]);
-        if (!two || p) umma_commit_if(e, &empty[vslot]);
-        ++steps[p];
+        for (int kk = 0; kk < kST / 16; ++kk)
+          umma_f16_ta_if(e, to, ts + u * kST + kk * 8, dv + ((kk * 2048u) >> 4), kIdO, (i || kk) ? 1u : 0u);
+        umma_commit_if(e, &o_done[p][u]);
+        if (ends(i)) umma_commit_if(e, &empty[vslot]);
         if (i + 2 < n) qk(i + 2);
       }
+      steps += n;
       ++pieces;
+      if (!two) buf ^= 1;
     }
     if (!ok) *abort_flag = 1;
   }
