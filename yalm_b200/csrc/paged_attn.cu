@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t sb = smem_u32(smem), ring = sb + 2 * C::kTile;
   float* s_ml = reinterpret_cast<float*>(smem + (2 + C::kStages) * C::kTile);  // [2][128]
   __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], q_full[2], q_empty[2], s_full[2][2],
-      p_full[2][2], o_done[2][2], o_free, ml_ready;
+      p_full[2][2], o_done[2][2], turn[2][4], o_free, ml_ready;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ unsigned long long s_scan[kThreads / 32];
@@ -360,6 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&o_done[p][u], 1);
       }
     }
+    for (int w = 0; w < 8; ++w) mbar_init(&turn[w & 1][w >> 1], 1);
     mbar_init(&o_free, 8);
     mbar_init(&ml_ready, 4);
     mbar_fence_init();
@@ -403,6 +404,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         int id = -1;
         if (lane < 8 && slot < pc.sq.kv) id = __ldg(table + (slot >> b.ps_log2));
         return lane < 8 && id >= 0 && id < b.n_pages;
+      };
+      // The two warps of a quadrant share a scheduler and its special-function unit: they take their exponentials
+      // in turns, one's under the other's loads, maxima and waits.  Left alone they fall into step.
+      auto my_turn = [&](unsigned step) {
+        return p == 0 ? step == 0 || mbar_wait(&turn[1][quad], (step - 1) & 1, status) : mbar_wait(&turn[0][quad], step & 1, status);
       };
       float m = -INFINITY, l = 0.f;
       bool nx = nk > 0 && there(first);
@@ -463,6 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
+          if (!(ok = my_turn(step))) break;
           const float shift = m == -INFINITY ? 0.f : m - kBias;
           const float2 cc = make_float2(a.c, a.c), sh = make_float2(-shift, -shift);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -478,10 +485,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               sum[k & 1] = add2(sum[k & 1], t2);
               pk[k] = pack2<T>(t2.x, t2.y);
             }
+            if (w == kST / 16 - 1 && lane == 0) mbar_arrive(&turn[p][quad]);
             tmem_st8_u32(ts + buf * kST + 8 * w, pk);
           }
           l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
           tmem_st_wait();
+        } else {
+          if (!(ok = my_turn(step))) break;
+          if (lane == 0) mbar_arrive(&turn[p][quad]);
         }
         tc_fence_before();
         __syncwarp();
