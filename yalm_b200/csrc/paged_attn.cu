@@ -12,9 +12,8 @@
 // evenly: a long cache of few rows is cut over many blocks, and ragged lengths balance themselves.
 // The cuts follow from the lengths on the device, by a closed form for a sequence's tiles (floor
 // sums), so there is no plan to be made on the host and a captured launch follows new lengths.  A unit
-// that is cut leaves (o, m, l) records in the workspace, which a second kernel, launched as the dependent of
-// the first, merges in the order of the slots, spread over the whole GPU: results do not depend on timing,
-// and no block waits for another.
+// that is cut leaves (o, m, l) records in the workspace, which a second kernel merges, spread over the whole
+// GPU: results do not depend on timing, and no block waits for another.
 //
 // Block.  Two pipelines of 128 rows share the tensor cores, one's softmax under the other's products:
 //   warp 0       loads Q (a 3-D box of queries x heads) and the ring of K and V tiles, one lane a page
@@ -66,33 +65,45 @@ struct Cfg {
 };
 
 // -------------------------------------------------------------------------------------- the work axis
-// sum_{i < n} floor((a i + b) / m), a, b >= 0: each round takes the whole parts out and swaps the roles of the
-// axes, as Euclid's algorithm does.  The arguments here keep every product below 2^32.
-__device__ __forceinline__ unsigned floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
-  unsigned s = 0;
+// sum_{i < n} floor((a i + b) / 128), a, b >= 0: each round takes the whole parts out and swaps the roles of the
+// axes, as Euclid's algorithm does.  Where a is a power of two (one, two, four ... query heads per kv head) two
+// rounds of shifts end it.  The arguments here keep every product below 2^32.
+__device__ __forceinline__ unsigned floor_sum(unsigned n, unsigned a, unsigned b) {
+  unsigned s = (a >> 7) * (n * (n - 1) / 2) + (b >> 7) * n;
+  a &= 127u;
+  b &= 127u;
+  unsigned y = a * n + b, m = a;
+  n = y >> 7;
+  b = y & 127u;
+  if (!(m & (m - 1))) {
+    if (!m) return s;
+    const int sh = 31 - __clz(m);
+    return s + (128u >> sh) * (n * (n - 1) / 2) + (b >> sh) * n;
+  }
+  a = 128u;
   while (n) {
     s += (a / m) * (n * (n - 1) / 2) + (b / m) * n;
     a %= m;
     b %= m;
-    const unsigned y = a * n + b;
+    if (!a) break;
+    y = a * n + b;
     n = y / m;
     b = y % m;
     const unsigned t = m;
     m = a;
     a = t;
-    if (!m) break;
   }
   return s;
 }
 // sum_{i < n} floor(max(0, a + i u) / 128)
 __device__ __forceinline__ unsigned ramp(int n, int a, int u) {
   if (a < 0) {
+    if (a + (n - 1) * u < 128) return 0;
     const int skip = (-a + u - 1) / u;
-    if (skip >= n) return 0;
     n -= skip;
     a += skip * u;
   }
-  return n > 0 ? floor_sum((unsigned)n, kKT, (unsigned)u, (unsigned)a) : 0u;
+  return n > 0 ? floor_sum((unsigned)n, (unsigned)u, (unsigned)a) : 0u;
 }
 
 struct Unit {
@@ -110,12 +121,12 @@ __device__ __forceinline__ Unit unit_of(const Axis& x, const PagedSeq& q, int i)
   u.q0 = i * x.U;
   u.nq = min(x.U, q.n - u.q0);
   const int end = p0 + u.q0 + u.nq;
-  u.tile0 = max(0, p0 + u.q0 - x.window + 1) / kKT;
+  u.tile0 = max(0, p0 + u.q0 - x.window + 1) >> 7;
   u.none = end <= 0;
-  u.cost = max(1, (end + kKT - 1) / kKT - u.tile0);
+  u.cost = max(1, ((end + kKT - 1) >> 7) - u.tile0);
   return u;
 }
-__device__ __forceinline__ int n_units(const Axis& x, const PagedSeq& q) { return (q.n + x.U - 1) / x.U; }
+__device__ __forceinline__ int n_units(const Axis& x, const PagedSeq& q) { return q.n <= x.U ? 1 : (q.n + x.U - 1) / x.U; }
 // key tiles of the first m units of a (sequence, kv head), m < n_units: unit i ends at slot p0 + (i + 1) U
 __device__ __forceinline__ unsigned units_before(const Axis& x, const PagedSeq& q, int m) {
   if (m == 0) return 0;
@@ -340,7 +351,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedBatch& b = a.b;
-  pdl_trigger();  // the merge may be set up; it waits for this kernel's end
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
                  : "memory");
@@ -757,22 +767,32 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// The units that were cut: out = sum_parts 2^(m - M) o / sum_parts 2^(m - M) l, over the parts in the order of
-// the slots.  Block x looks after the unit that attention block x began; a thread takes 8 elements of a row,
-// and loads several parts at once, since each is a trip to L2.
-constexpr int kMergeThreads = 128, kMergeSlices = 8, kMergeParts = 4;
+// The units that were cut: out = sum_parts 2^(m - M) o / sum_parts 2^(m - M) l.  Blocks x look after the unit that
+// attention block x began; 8 elements of a row are a thread's for up to 4 parts (a prompt's unit over two or
+// three blocks, 4096 such groups), else the work of 8 lanes that share out the parts and join them by
+// shuffles (a single token's unit over 18 blocks, 64 groups), so that every load is under way at once.  The
+// order of the sum depends on the number of parts alone.
+constexpr int kMergeThreads = 128, kMergeSlices = 16, kMergeParts = 4;
 template <int HD, typename T>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid_constant__ PagedAttnParams a) {
-  pdl_wait();
   const int4 d = __ldcg(reinterpret_cast<const int4*>(a.cuts + blockIdx.x));  // token, nq, head, parts
-  if (!d.w) return;
-  const int rows = d.y * a.gq;
-  for (int e = blockIdx.y * kMergeThreads + threadIdx.x; e < rows * (HD / 8); e += kMergeSlices * kMergeThreads) {
+  const int rows = d.y * a.gq, lanes = d.w > kMergeParts ? 8 : 1;
+  const int lane = threadIdx.x & 31, items = d.w ? rows * (HD / 8) * lanes : 0;
+  for (int w0 = blockIdx.y * kMergeThreads + (threadIdx.x & ~31); w0 < items; w0 += kMergeSlices * kMergeThreads) {
+    const int item = min(w0 + lane, items - 1), e = item / lanes, sub = item % lanes;
     const int row = e % rows, c8 = e / rows;
     float mm = -INFINITY, ll = 0.f, acc[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[k] = 0.f;
-    for (int k0 = 0; k0 < d.w; k0 += kMergeParts) {
+    auto join = [&](float m, float l, const float (&v)[8]) {
+      const float mn = fmaxf(mm, m);
+      const float old = mm == -INFINITY ? 0.f : ex2(mm - mn), w = m == -INFINITY ? 0.f : ex2(m - mn);
+      mm = mn;
+      ll = ll * old + l * w;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = acc[j] * old + v[j] * w;
+    };
+    for (int k0 = sub; k0 < d.w; k0 += kMergeParts * lanes) {
       float m[kMergeParts], l[kMergeParts];
       float4 o[kMergeParts][2];
 #pragma unroll
@@ -780,8 +800,9 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
         m[k] = -INFINITY;
         l[k] = 0.f;
         o[k][0] = o[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (k0 + k < d.w) {
-          const float* rec = a.recs + ((size_t)(blockIdx.x + k0 + k) * 2 + (k0 + k == 0 ? 1 : 0)) * rec_floats<HD>();
+        const int part = k0 + k * lanes;
+        if (part < d.w) {
+          const float* rec = a.recs + ((size_t)(blockIdx.x + part) * 2 + (part == 0 ? 1 : 0)) * rec_floats<HD>();
           const float4* ro = reinterpret_cast<const float4*>(rec) + (size_t)(2 * c8) * rows + row;
           o[k][0] = __ldcg(ro);
           o[k][1] = __ldcg(ro + rows);
@@ -791,15 +812,18 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
       }
 #pragma unroll
       for (int k = 0; k < kMergeParts; ++k) {
-        const float mn = fmaxf(mm, m[k]);
-        const float old = mm == -INFINITY ? 0.f : ex2(mm - mn), w = m[k] == -INFINITY ? 0.f : ex2(m[k] - mn);
         const float v[8] = {o[k][0].x, o[k][0].y, o[k][0].z, o[k][0].w, o[k][1].x, o[k][1].y, o[k][1].z, o[k][1].w};
-        mm = mn;
-        ll = ll * old + l[k] * w;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = acc[j] * old + v[j] * w;
+        join(m[k], l[k], v);
       }
     }
+    for (int x = 1; x < lanes; x <<= 1) {
+      float v[8];
+      const float m = __shfl_xor_sync(0xffffffffu, mm, x), l = __shfl_xor_sync(0xffffffffu, ll, x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = __shfl_xor_sync(0xffffffffu, acc[k], x);
+      join(m, l, v);
+    }
+    if (sub || w0 + lane >= items) continue;
     const float inv = ll != 0.f ? 1.f / ll : 0.f;
     T* out = static_cast<T*>(a.out) + (size_t)(d.x + row / a.gq) * a.out_stride + (size_t)(d.z * a.gq + row % a.gq) * HD + 8 * c8;
     *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv),
@@ -847,7 +871,7 @@ cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cuda
   if ((e = cudaLaunchKernel(fn, dim3(grid), dim3(kThreads), args, Cfg<HD>::kSmem, s)) != cudaSuccess) return e;
   if (a.b.max_pages * ps <= kKT) return cudaSuccess;  // every unit is one key tile: nothing is cut
   return launch_kernel(reinterpret_cast<const void*>(&paged_merge_kernel<HD, T>), dim3(grid, kMergeSlices),
-                       dim3(kMergeThreads), 0, s, true, &p);
+                       dim3(kMergeThreads), 0, s, false, &p);
 }
 }  // namespace
 
