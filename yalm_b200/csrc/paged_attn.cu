@@ -16,7 +16,8 @@
 // GPU: results do not depend on timing, and no block waits for another.
 //
 // Block.  Two pipelines of 128 rows share the tensor cores, one's softmax under the other's products:
-//   warp 0       loads Q (a 3-D box of queries x heads) and the ring of K and V tiles, one lane a page
+//   warps 0, 3   load the K tiles and Q (a 3-D box of queries x heads), and the V tiles, into one ring, one lane a
+//                page (with pages of 16 slots a tile is 16 copies, which keep one warp busier than the memory)
 //   warps 1, 2   issue the products of pipeline 0 / 1, 64 slots a step: S = Q . K^T into tensor memory, then
 //                O += P . V with P read from tensor memory, where it took the place of S (one warp for both
 //                pipelines was the bottleneck: 1300 clocks a step, of which the products are 650).  S has two buffers, so the
@@ -597,8 +598,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!ok) *abort_flag = 1;
   } else {
-  if (warp == 0) {
+  if (warp == 0 || warp == 3) {
     // ------------------------------------------------------------------------------- loads
+    const bool keys = warp == 0;
     const int lg = b.ps_log2, ps = 1 << lg;
     const int boxes = ps >= kKT ? 1 : kKT >> lg;  // pages per key tile
     const uint32_t box_bytes = (uint32_t)min(ps, kKT) * 128u;
@@ -609,21 +611,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (pc.u.none) continue;
       const bool two = pc.u.nq > QB;
       const int* table = b.page_table + (size_t)pc.seq * b.max_pages;
-      // row of the page pool where this lane's page of a key tile starts (outside it: zeros)
-      auto row_of = [&](int tile) {
+      // this lane's page of a key tile, and the row of the page pool where it starts (outside the pool: zeros)
+      auto page_of = [&](int tile) {
         const int at = (tile << 7) + (lane << lg);
-        if (lane >= boxes || at >= pc.sq.kv) return a.oob;
-        const int id = __ldg(table + (at >> lg));
-        if (id < 0 || id >= b.n_pages) return a.oob;
-        return ((id * a.x.K + pc.head) << lg) + (at & (ps - 1));
+        return lane < boxes && at < pc.sq.kv ? __ldg(table + (at >> lg)) : -1;
       };
-      auto load = [&](const CUtensorMap* map, int row) {
-        if (issued >= C::kStages && !mbar_wait(&empty[slot], phase, status)) return false;
-        if (lane == 0) mbar_arrive_expect_tx(&full[slot], C::kTile);
-        __syncwarp();
-        if (lane < boxes)
-          for (int h = 0; h < C::kHalves; ++h)
-            tma_load_2d_s(ring + slot * C::kTile + h * kBlk + lane * box_bytes, map, 64 * h, row, smem_u32(&full[slot]));
+      auto row_of = [&](int tile, int page) {
+        if (page < 0 || page >= b.n_pages) return a.oob;
+        return ((page * a.x.K + pc.head) << lg) + (((tile << 7) + (lane << lg)) & (ps - 1));
+      };
+      auto load = [&](const CUtensorMap* map, int row, bool mine) {
+        if (mine) {
+          if (issued >= C::kStages && !mbar_wait(&empty[slot], phase, status)) return false;
+          if (lane == 0) mbar_arrive_expect_tx(&full[slot], C::kTile);
+          __syncwarp();
+          if (lane < boxes)
+            for (int h = 0; h < C::kHalves; ++h)
+              tma_load_2d_s(ring + slot * C::kTile + h * kBlk + lane * box_bytes, map, 64 * h, row, smem_u32(&full[slot]));
+        }
         ++issued;
         if (++slot == C::kStages) slot = 0, phase ^= 1;
         return true;
@@ -643,15 +648,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       // in the order of the products, whose scores are two steps ahead of the weights: one key tile with two row
       // tiles, two with one
       const int first = pc.u.tile0 + pc.t0, n = pc.t1 - pc.t0, ahead = two ? 1 : 2;
-      int next_row = row_of(first);
+      // the table is read a tile ahead: an entry is a trip to L2
+      const int lag = keys ? 0 : ahead;
+      int next = page_of(first);
       for (int j = 0; j < n + ahead && ok; ++j) {
-        if (j >= ahead) ok = load(&vmap, row_of(first + j - ahead));
-        if (ok && j < n) {
-          const int row = next_row;
-          if (j + 1 < n) next_row = row_of(first + j + 1);
-          ok = load(&kmap, row);
+        int row = a.oob;
+        if (j >= lag && j < n + lag) {
+          row = row_of(first + j - lag, next);
+          if (j + 1 < n + lag) next = page_of(first + j + 1 - lag);
         }
-        if (ok && j == 0) {
+        if (j >= ahead) ok = load(&vmap, row, !keys);
+        if (ok && j < n) ok = load(&kmap, row, keys);
+        if (ok && keys && j == 0) {
           if (two) {
             ok = load_q(0, 0) && load_q(1, 1);
           } else {
@@ -662,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (!ok) *abort_flag = 1;
-    // never leave while a copy issued here may still be landing: the last one into each slot and buffer
+    // never leave while a copy may still be landing: the last one into each slot and buffer
     for (unsigned i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
       mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1, status);
     for (int t = 0; t < 2; ++t)
