@@ -224,13 +224,15 @@ __device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long lon
   if (lane == 31) s_warp[warp] = incl;
   if (threadIdx.x == 0) s_start->left = 0;
   __syncthreads();
-  unsigned long long before = incl - mine, total = 0;
+  // the sums of the warps before this one, and of all, by the lanes of each warp
+  unsigned long long sums = lane < kThreads / 32 ? s_warp[lane] : 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    const unsigned long long v = s_warp[w];
-    if (w < warp) before += v;
-    total += v;
+  for (int o = 1; o < 16; o <<= 1) {
+    const unsigned long long v = __shfl_up_sync(0xffffffffu, sums, o);
+    if (lane >= o) sums += v;
   }
+  const unsigned long long total = __shfl_sync(0xffffffffu, sums, kThreads / 32 - 1);
+  const unsigned long long before = __shfl_sync(0xffffffffu, sums, warp) - s_warp[warp] + incl - mine;
   if (!mine) return;
   const unsigned long long share = quot(total, gridDim.x);
   const int more = (int)(total - share * gridDim.x), c = blockIdx.x;
@@ -253,19 +255,32 @@ __device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long lon
   st.sq = q;
   st.seq = s;
   st.head = (int)quot(rem, per_head);
-  const unsigned in_head = (unsigned)(rem - (unsigned long long)st.head * per_head);
-  int lo = 0, hi = n_units(x, q);  // units_before(lo) <= in_head < units_before(hi)
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (units_before(x, q, mid) <= in_head) lo = mid; else hi = mid;
-  }
-  st.unit = lo;
-  st.off = (int)(in_head - units_before(x, q, lo));
+  st.unit = 0;
+  st.off = (int)(rem - (unsigned long long)st.head * per_head);  // within the head: find_unit
   st.left = left;
   st.begin = begin;
   st.share = share;
   st.more = more;
   *s_start = st;
+}
+
+// Called by a whole warp: the unit in which tile st.off of the head lies, and the tile within it.  Unit u begins
+// at tile units_before(u); 32 guesses at a time.
+__device__ __forceinline__ void find_unit(const Axis& x, Start& st) {
+  int lo = 0, hi = n_units(x, st.sq);  // units_before(lo) <= off < units_before(hi)
+  if (hi == 1) return;
+  const int lane = threadIdx.x & 31;
+  unsigned begin = 0;  // units_before(lo)
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
+    const unsigned tiles = at < hi ? units_before(x, st.sq, at) : 0xffffffffu;
+    const int below = __popc(__ballot_sync(0xffffffffu, tiles <= (unsigned)st.off));
+    if (below) begin = __shfl_sync(0xffffffffu, tiles, below - 1);
+    lo += below * step;
+    hi = min(hi, lo + step);
+  }
+  st.off -= (int)begin;
+  st.unit = lo;
 }
 
 // -------------------------------------------------------------------------------------------- numerics
@@ -387,7 +402,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = &s_abort;
   unsigned* status = a.status;
   const int QB = kRows / a.gq;
-  Walk walk(s_start);
+  Start st0 = s_start;
+  if (st0.left > 0) find_unit(a.x, st0);
+  Walk walk(st0);
   Piece pc;
   if (warp >= 4) {
     // ------------------------------------------------------------------------------- softmax
