@@ -3,12 +3,25 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 
 #include "common.cuh"
 
 namespace yb {
+
+// Raises a kernel's dynamic shared-memory cap, once per device.
+struct SmemCap {
+  std::atomic<unsigned long long> done{0};  // devices, by bit
+  cudaError_t raise(const void* fn, int device, size_t bytes) {
+    const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
+};
 
 // The batch as the kernels see it (include/yalm_b200.h, yb_paged_batch).  The lengths and the table are
 // read on the device, so a captured launch follows them; every index made from them is clamped to

@@ -39,7 +39,6 @@
 #include <cuda_bf16.h>
 
 #include <math.h>
-#include <atomic>
 #include <type_traits>
 
 #include "launch.h"
@@ -884,14 +883,9 @@ cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cuda
   p.cuts = reinterpret_cast<Cut*>(static_cast<char*>(a.scratch) + 256);
   p.recs = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kHeadBytes);
   const void* fn = reinterpret_cast<const void*>(&paged_attn_kernel<HD, T>);
-  static std::atomic<unsigned long long> raised{0};  // devices (by bit) whose shared-memory cap is set
-  const unsigned long long bit = 1ull << (device & 63);
-  cudaError_t e;
-  if (device >= 64 || !(raised.load(std::memory_order_acquire) & bit)) {
-    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::kSmem);
-    if (e != cudaSuccess) return e;
-    if (device < 64) raised.fetch_or(bit, std::memory_order_release);
-  }
+  static SmemCap cap;
+  cudaError_t e = cap.raise(fn, device, Cfg<HD>::kSmem);
+  if (e != cudaSuccess) return e;
   void* args[] = {&qm, &km, &vm, &p};
   if ((e = cudaLaunchKernel(fn, dim3(grid), dim3(kThreads), args, Cfg<HD>::kSmem, s)) != cudaSuccess) return e;
   if (a.b.max_pages * ps <= kKT) return cudaSuccess;  // every unit is one key tile: nothing is cut
