@@ -74,8 +74,15 @@ __device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Where element e of a head lies in a row of shared memory: groups of four by the lanes that hold them, so that
+// neighbouring lanes read neighbouring groups (in the head's own order they would meet in the same banks).
+template <int HD>
+__device__ __forceinline__ int at(int e) {
+  return (((e / (HD / 2)) * 2 + ((e >> 2) & 1)) * (HD / 16) + (e % (HD / 2)) / 8) * 4 + (e & 3);
+}
+
 template <int HD, typename S, typename T, int P>
-__global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_constant__ PagedAppendArgs a, int shares,
+__global__ void __launch_bounds__(kThreads, 7) paged_append_kernel(const __grid_constant__ PagedAppendArgs a, int shares,
                                                                 int share_groups) {
   constexpr int kLanes = HD / 16;                   // lanes of a head
   constexpr int kHeads = 32 / kLanes;               // heads of a group, which a warp takes at a time
@@ -132,10 +139,10 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
     for (int k = 0; k < 2; ++k) {
       const float* w = k ? a.k_norm : a.q_norm;
       const float we = w ? __ldg(w + e) : 1.f, wf = w ? __ldg(w + f) : 1.f;
-      fac[k][0][e] = we * c;
-      fac[k][0][f] = wf * c;
-      fac[k][1][e] = -s * wf;
-      fac[k][1][f] = s * we;
+      fac[k][0][at<HD>(e)] = we * c;
+      fac[k][0][at<HD>(f)] = wf * c;
+      fac[k][1][at<HD>(e)] = -s * wf;
+      fac[k][1][at<HD>(f)] = s * we;
     }
   }
   __syncwarp();
@@ -179,7 +186,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
         __syncwarp();  // the lanes have read what they need of the group before
 #pragma unroll
         for (int m = 0; m < 16; m += 4)
-          *reinterpret_cast<float4*>(mine + (m >> 3) * (HD / 2) + 8 * l + (m & 7)) = make_float4(v[m], v[m + 1], v[m + 2], v[m + 3]);
+          *reinterpret_cast<float4*>(mine + at<HD>((m >> 3) * (HD / 2) + 8 * l + (m & 7))) = make_float4(v[m], v[m + 1], v[m + 2], v[m + 3]);
         __syncwarp();
       }
       const int h = head_of(g, kind);
@@ -198,7 +205,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
 #pragma unroll
             for (int j = 0; j < 8; j += 4) {  // d is a multiple of 4: four neighbours' partners are neighbours
               const int e = e0 + j, f = e < d ? e + d : e < R ? e - d : e;
-              const float4 o = *reinterpret_cast<const float4*>(mine + f);
+              const float4 o = *reinterpret_cast<const float4*>(mine + at<HD>(f));
               other[j] = o.x, other[j + 1] = o.y, other[j + 2] = o.z, other[j + 3] = o.w;
             }
           }
@@ -208,7 +215,8 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
           }
 #pragma unroll
           for (int j = 0; j < 8; j += 4) {
-            const float4 o = *reinterpret_cast<const float4*>(&fac[kind][0][e0 + j]), q = *reinterpret_cast<const float4*>(&fac[kind][1][e0 + j]);
+            const float4 o = *reinterpret_cast<const float4*>(&fac[kind][0][at<HD>(e0 + j)]),
+                         q = *reinterpret_cast<const float4*>(&fac[kind][1][at<HD>(e0 + j)]);
             y[j] = fmaf(other[j], q.x, v[8 * c + j] * o.x);
             y[j + 1] = fmaf(other[j + 1], q.y, v[8 * c + j + 1] * o.y);
             y[j + 2] = fmaf(other[j + 2], q.z, v[8 * c + j + 2] * o.z);
