@@ -80,9 +80,8 @@ inline cudaError_t raise_smem_cap(const void* fn) {
 // cudaLaunchKernelEx with the programmatic-stream-serialization attribute when `pdl` is set, so the
 // kernel may begin while the previous kernel in the stream is still running (it must call
 // griddepcontrol.wait before reading that kernel's results).
-template <typename Args>
-inline cudaError_t launch_kernel(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool pdl,
-                                 Args* args) {
+inline cudaError_t launch_kernel_params(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool pdl,
+                                        void** params) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -93,8 +92,13 @@ inline cudaError_t launch_kernel(const void* fn, dim3 grid, dim3 block, size_t s
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
-  void* params[] = {args};
   return cudaLaunchKernelExC(&cfg, fn, params);
+}
+template <typename Args>
+inline cudaError_t launch_kernel(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool pdl,
+                                 Args* args) {
+  void* params[] = {args};
+  return launch_kernel_params(fn, grid, block, smem, stream, pdl, params);
 }
 
 }  // namespace yb

@@ -20,6 +20,8 @@
 
 #include <math.h>
 
+#include "launch.h"
+
 namespace yb {
 
 namespace {
@@ -93,6 +95,7 @@ __global__ void __launch_bounds__(kThreads, 7) paged_append_kernel(const __grid_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int id = blockIdx.x * kWarps + warp, row = id / shares, share = id % shares;
   if (row >= a.b.n_tokens) return;
+  pdl_wait();
   const int l = lane % kLanes, sub = lane / kLanes;  // elements 8 l + j and HD / 2 + 8 l + j of a head, j < 8
   const int H = a.b.n_heads, K = a.b.n_kv_heads, R = a.rotary_dim;
   // groups: those of the query heads, then the key heads', then the value heads'
@@ -274,7 +277,7 @@ cudaError_t paged_append(const PagedAppendArgs& a, int head_dim, int src_type, i
   shares = (groups + share_groups - 1) / share_groups;
   const long long warps = (long long)a.b.n_tokens * shares;
   void* args[] = {const_cast<PagedAppendArgs*>(&a), &shares, &share_groups};
-  return cudaLaunchKernel(fn, dim3((unsigned)((warps + kWarps - 1) / kWarps)), dim3(kThreads), args, 0, s);
+  return launch_kernel_params(fn, dim3((unsigned)((warps + kWarps - 1) / kWarps)), dim3(kThreads), 0, s, true, args);
 }
 
 }  // namespace yb

