@@ -351,11 +351,16 @@ int yb_paged_append_dev(const yb_paged_batch* b, void* q_out, long long q_out_st
 
 /* Causal attention of the new tokens over their sequences' caches, which hold them already: the token of
  * slot p sees slots max(0, p - window + 1) .. p (window 0: 0 .. p), less those on pages that are not
- * there; out = sum softmax(scale * q.k) v, or zeros where it sees no slot.  Slots from kv_len on and
- * pages that are not there may hold anything, NaN included; the slots below kv_len hold finite values.
+ * there; out = sum softmax(scale * q.k) v, or zeros where it sees no slot.  Slots from kv_len on, those before
+ * the window of the sequence's first new token, and pages that are not there may hold anything, NaN
+ * included (pages that have left the window may be given to other sequences); the slots between hold
+ * finite values: one that does not may spoil the rows of tokens before it, too.
  * scratch_dev: yb_paged_attention_scratch_bytes(b) bytes (the same for every batch of this head_dim on a
- * device), zero-filled before its first use and left ready by every call; calls that may run at the
- * same time, replayed graphs among them, each need their own. */
+ * device), 16-byte aligned; its contents have no meaning between calls.  Calls that may run at the same
+ * time, replayed graphs among them, each need their own.  Its first word takes status bits as yb_status
+ * has them when a bounded wait in the kernel runs out (set it to zero before to tell); the output is then
+ * not complete.  Results do not depend on timing, but on the number of SMs, which decides where a long
+ * cache is cut. */
 int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long long out_stride, const void* q,
                            long long q_stride, float scale, int window, void* scratch_dev, void* stream);
 size_t yb_paged_attention_scratch_bytes(const yb_paged_batch* b); /* 0 for a batch that is refused */

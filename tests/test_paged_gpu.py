@@ -175,6 +175,20 @@ def test_pages_that_are_not_there_are_masked(gpu, hd, ps, dtype):
     assert torch.isfinite(got).all()
 
 
+@pytest.mark.parametrize("new,kv,window,hd,ps", [([1], [1000], 100, 128, 16), ([90, 1], [700, 333], 130, 64, 64),
+                                                 ([200], [2000], 7, 128, 256)])
+def test_slots_before_the_first_window_may_hold_anything(gpu, new, kv, window, hd, ps):
+    import torch
+    s = Step(new, kv, 8, 2, hd, ps, "f16", seed=63)
+    ref, tol = s.attend64(window)
+    for row, (n, m) in enumerate(zip(new, kv)):
+        for t in range(m - n - window + 1):
+            s.k[s.table[row][t // ps], :, t % ps] = math.nan
+            s.v[s.table[row][t // ps], :, t % ps] = math.inf if t % 2 else math.nan
+    got = s.attend(window).double()
+    assert ((got - ref).abs() <= tol).all()
+
+
 def test_large_scores_and_other_scales(gpu):
     """Scores of several hundred, where only the differences to the row's maximum matter; rising along the
     cache, so that the running maximum keeps growing; another scale."""
@@ -267,6 +281,96 @@ def test_lengths_out_of_range_stay_inside_the_buffers(gpu):
     s.kv_len.copy_(torch.tensor([40, 10 ** 9, 48]))
     s.attend(out=out)
     assert (guard[: s.n] == 7).all() and (guard[2 * s.n:] == 7).all()
+
+
+def test_rows_do_not_touch_each_other(gpu):
+    """A query that is not finite spoils its own head's row alone."""
+    import torch
+    s = Step([70, 1], [300, 200], 8, 2, 128, 16, "f16", seed=55)
+    clean = s.attend()
+    s.q[5, 3 * 128] = math.nan
+    s.q[69, 0] = math.inf
+    s.q[70, 7 * 128 + 5] = -math.inf
+    got = s.attend().view(s.n, 8, 128)
+    bad = torch.zeros(s.n, 8, dtype=torch.bool, device="cuda")
+    bad[5, 3] = bad[69, 0] = bad[70, 7] = True
+    assert got[5, 3].isnan().all()
+    assert torch.equal(got[~bad], clean.view(s.n, 8, 128)[~bad])
+
+
+def test_sequences_share_a_prefix(gpu):
+    """Two sequences whose first pages are the same ones."""
+    s = Step([40, 3], [500, 300], 8, 2, 64, 32, "bf16", seed=56)
+    for i in range(8):
+        s.table[1][i] = s.table[0][i]
+    s.page_table[1, :8] = s.page_table[0, :8]
+    s.check()
+    s.check(window=77)
+
+
+def test_many_sequences(gpu):
+    """More sequences than a block has threads, most of them without new tokens."""
+    n = 3000
+    new = [1 if i % 7 == 0 else 0 for i in range(n)]
+    new[1234] = 150
+    kv = [1 + (i * 13) % 40 for i in range(n)]
+    kv[1234] = 400
+    Step(new, kv, 4, 2, 64, 16, "f16", seed=57).check()
+
+
+def test_pools_past_32_bit_offsets(gpu):
+    """Pages whose elements lie past 2^31 and whose bytes lie past 2^32, for the reads and the stores."""
+    import torch
+    nh, nkv, hd, ps, n_pages = 16, 8, 128, 256, 11000  # 2.9e9 elements in either cache
+    k = torch.empty(n_pages, nkv, ps, hd, dtype=torch.float16, device="cuda")
+    v = torch.empty_like(k)
+    assert k.numel() > 2 ** 31
+    s = Step([3, 80], [600, 300], nh, nkv, hd, ps, "f16", seed=58)
+    old, far = [list(t) for t in s.table], [10999, 8192, 8193, 10500, 2]
+    for row in range(2):
+        for i, page in enumerate(old[row]):
+            if page >= 0:
+                to = far.pop()
+                k[to], v[to] = s.k[page], s.v[page]
+                s.table[row][i] = to
+    s.k, s.v, s.n_pages = k, v, n_pages
+    s.page_table.copy_(torch.tensor(s.table))
+    s.check()
+    qkv = torch.randn(s.n, (nh + 2 * nkv) * hd, device="cuda")
+    out = torch.empty_like(s.q)
+    s.batch().append(qkv, out, None, 0, stream=torch.cuda.current_stream().cuda_stream)
+    for at, (row, slot) in enumerate([(0, t) for t in (597, 598, 599)] + [(1, t) for t in range(220, 300)]):
+        page, r = s.table[row][slot // ps], slot % ps
+        want = qkv[at].half().view(nh + 2 * nkv, hd)
+        assert torch.equal(k[page, :, r], want[nh: nh + nkv]) and torch.equal(v[page, :, r], want[nh + nkv:])
+    assert torch.equal(out, qkv[:, : nh * hd].half())
+
+
+def test_two_streams_at_once(gpu):
+    """Calls on two streams, each with its own workspace."""
+    import torch
+    a = Step([1] * 5, [3000] * 5, 32, 8, 128, 16, "f16", seed=59)
+    b = Step([300], [1200], 8, 2, 64, 64, "bf16", seed=60)
+    want = [x.attend() for x in (a, b)]
+    runs = []
+    for x in (a, b):
+        batch = x.batch()
+        runs.append((x, batch, torch.zeros(batch.scratch_bytes(), dtype=torch.uint8, device="cuda"),
+                     [torch.full_like(want[len(runs)], 7.0) for _ in range(20)], torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for i in range(20):
+        for x, batch, scratch, outs, stream in runs:
+            batch.attend(x.q, outs[i], scratch, stream=stream.cuda_stream)
+    torch.cuda.synchronize()
+    for w, run in zip(want, runs):
+        assert all(torch.equal(w, o) for o in run[3])
+
+
+def test_workspace_needs_no_initial_value(gpu):
+    import torch
+    s = Step([1, 130], [4000, 900], 32, 8, 128, 32, "f16", seed=62)
+    b = s.batch()
+    s.check(scratch=torch.full((b.scratch_bytes(),), 0xFF, dtype=torch.uint8, device="cuda"), batch=b)
 
 
 def test_host_memory_is_refused(gpu):

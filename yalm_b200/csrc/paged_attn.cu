@@ -726,20 +726,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto take_v = [&](int i) {
         if (!begins(i)) return true;
         if (!take(vslot)) return false;
-        // slots behind the sequence's last one, in its last page, may hold anything: their weight is 0, and
-        // 0 * v has to be 0 (both warps write the same zeros)
-        const int rem = pc.sq.kv - (first + (two ? i >> 1 : i)) * kKT;
-        if (rem < kKT) {
-          const int end = min(kKT, ((rem + (1 << b.ps_log2) - 1) >> b.ps_log2) << b.ps_log2);
-          const uint32_t v = ring + vslot * C::kTile;
-          for (int x = lane; x < (end - rem) * 8 * C::kHalves; x += 32) {
-            const int h = x / ((end - rem) * 8), r = x % ((end - rem) * 8);
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * kBlk + (rem * 8 + r) * 16u), "r"(0u)
+        // Slots before the first token's window, and behind the sequence's last one in its last page, may hold
+        // anything: their weight is 0, and 0 * v has to be 0 (both warps write the same zeros).
+        const int k0 = (first + (two ? i >> 1 : i)) * kKT;
+        const uint32_t v = ring + vslot * C::kTile;
+        auto zero = [&](int from, int to) {
+          if (from >= to) return;
+          for (int x = lane; x < (to - from) * 8 * C::kHalves; x += 32) {
+            const int h = x / ((to - from) * 8), r = x % ((to - from) * 8);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * kBlk + (from * 8 + r) * 16u), "r"(0u)
                          : "memory");
           }
           fence_proxy_async_smem();
           __syncwarp();
-        }
+        };
+        const int rem = pc.sq.kv - k0, seen = pc.sq.kv - pc.sq.n + pc.u.q0 - a.x.window + 1 - k0;
+        if (rem < kKT) zero(rem, min(kKT, ((rem + (1 << b.ps_log2) - 1) >> b.ps_log2) << b.ps_log2));
+        if (seen > 0) zero(0, seen);
         return true;
       };
       const uint64_t dq = umma_desc_k_sw128(sb + qb * C::kTile);
