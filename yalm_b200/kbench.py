@@ -1,7 +1,8 @@
 """Isolated decode-kernel benchmark (benchmark config 4; the counterpart of yalm's
 `build/test -bk {matmul,matmul-wide,mha,ffn}`, src/test.cpp:339-405).
 
-    python -m yalm_b200.kbench [--kernel gemv|gateup|qkv|attention|prefill_attention|prefill_gemm|prefill|all]
+    python -m yalm_b200.kbench [--kernel gemv|gateup|qkv|attention|prefill_attention|prefill_gemm|prefill|
+                               paged_append|paged_attention|all]
                                [--iters N] [--warm W] [--quick]
 
 Each launch goes through the C ABI (yb_gemv_dev, yb_gateup_dev, yb_qkv_dev, yb_attention_dev) on
@@ -201,6 +202,62 @@ def bench_prefill_attention(nh, nkv, hd, T, iters, seed=0):
             "us": round(ms * 1000, 2), "tflops": round(flop / (ms / 1000) / 1e12, 1), **_LAST_SPREAD}
 
 
+def _paged(new, kv, nh, nkv, hd, ps, dtype, seed):
+    """A batch of sequences with `new` new tokens over kv slots each, in pages handed out in random order."""
+    import torch
+    from .paged import PagedBatch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    need = [-(-m // ps) for m in kv]
+    k, v = (torch.randn(sum(need), nkv, ps, hd, device="cuda", generator=g).to(dtype) for _ in range(2))
+    order = iter(torch.randperm(sum(need), device="cuda", generator=g).tolist())
+    table = [[next(order) for _ in range(n)] + [-1] * (max(need) - n) for n in need]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    starts = np.concatenate([[0], np.cumsum(new)]).tolist()
+    return PagedBatch(k, v, torch.tensor(table, **i32), torch.tensor(starts, **i32), torch.tensor(kv, **i32), nh,
+                      sum(new))
+
+
+def bench_paged_append(new, kv, nh, nkv, hd, ps, iters, seed=0):
+    """Norm, rotation and append of the new tokens (yb_paged_append_dev), fp16 projections and cache."""
+    import torch
+    T, width = sum(new), (nh + 2 * nkv) * hd
+    n = min(16, _copies(4 * T * width))  # few tokens: not over 4 x L2, but a new pool for every launch
+    b = [_paged(new, kv, nh, nkv, hd, ps, torch.float16, seed + i) for i in range(n)]
+    qkv = [torch.randn(T, width, device="cuda").half() for _ in range(n)]
+    q = [torch.empty(T, nh * hd, dtype=torch.float16, device="cuda") for _ in range(n)]
+    w = torch.ones(hd, device="cuda")
+    inv = torch.tensor([1e6 ** (-2.0 * j / hd) for j in range(hd // 2)], device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def fn(i):
+        b[i % n].append(qkv[i % n], q[i % n], inv, hd, q_norm=w, k_norm=w, stream=stream)
+    ms = _time(fn, iters)
+    return {"kernel": "paged_append", "sequences": len(new), "tokens": T, "n_heads": nh, "n_kv_heads": nkv,
+            "head_dim": hd, "page": ps, "us": round(ms * 1000, 2),
+            "gbs": round(4 * T * width / (ms / 1000) / 1e9, 1), **_LAST_SPREAD}
+
+
+def bench_paged_attention(new, kv, nh, nkv, hd, ps, iters, seed=0):
+    """Attention of the new tokens over the paged cache (yb_paged_attention_dev), fp16."""
+    import torch
+    T = sum(new)
+    n = _copies(4 * sum(kv) * nkv * hd)
+    b = [_paged(new, kv, nh, nkv, hd, ps, torch.float16, seed + i) for i in range(n)]
+    q = torch.randn(T, nh * hd, device="cuda").half()
+    out = torch.empty_like(q)
+    scratch = torch.zeros(b[0].scratch_bytes(), dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def fn(i):
+        b[i % n].attend(q, out, scratch, stream=stream)
+    ms = _time(fn, iters)
+    pairs = sum(t * m - t * (t - 1) // 2 for t, m in zip(new, kv))
+    return {"kernel": "paged_attention", "sequences": len(new), "tokens": T, "slots": sum(kv), "n_heads": nh,
+            "n_kv_heads": nkv, "head_dim": hd, "page": ps, "us": round(ms * 1000, 2),
+            "gbs": round((4 * sum(kv) * nkv + 4 * T * nh) * hd / (ms / 1000) / 1e9, 1),
+            "tflops": round(4.0 * pairs * nh * hd / (ms / 1000) / 1e12, 2), **_LAST_SPREAD}
+
+
 def bench_prefill(tokens, iters, config="mistral-7b", seed=0):
     """The whole batched prompt pass (yb_prefill, every layer's GEMMs, norms, RoPE / KV append and
     attention, then the classifier) of the seeded synthetic checkpoint.  Per prompt length one
@@ -242,7 +299,7 @@ def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("--kernel", default="all",
                     choices=["gemv", "gateup", "qkv", "attention", "prefill_attention", "prefill_gemm", "prefill",
-                             "all"])
+                             "paged_append", "paged_attention", "all"])
     ap.add_argument("--iters", type=int, default=200)
     ap.add_argument("--quick", action="store_true", help="one shape per kernel (for profiler captures)")
     ap.add_argument("--kv-lens", default="", help="attention: comma-separated kv_len values")
@@ -278,6 +335,14 @@ def main(argv=None):
         lens = [int(v) for v in args.tokens.split(",")] if args.tokens else ([1024] if args.quick else [1024, 3202])
         for t in lens:
             rows.append(bench_prefill_attention(32, 8, 128, t, max(3, args.iters // 20)))
+    if args.kernel in ("paged_append", "all"):
+        for new, kv in [([512], [512])] if args.quick else [([1] * 64, [256] * 64), ([512], [512]), ([8192], [8192])]:
+            rows.append(bench_paged_append(new, kv, 32, 8, 128, 16, args.iters))
+    if args.kernel in ("paged_attention", "all"):
+        cases = [([512], [3202])] if args.quick else [([1], [4096]), ([1], [32768]), ([1] * 64, [4096] * 64),
+                                                      ([512], [3202]), ([2048], [16384])]
+        for new, kv in cases:
+            rows.append(bench_paged_attention(new, kv, 32, 8, 128, 16, max(3, args.iters // (20 if sum(new) > 64 else 1))))
     if args.kernel == "prefill_gemm":
         T = int(args.tokens.split(",")[0]) if args.tokens else 3202
         for planes in (1, 2):
