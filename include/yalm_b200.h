@@ -314,7 +314,7 @@ int yb_prefill_attention_dev(uint16_t* out, const float* q, const uint16_t* k_ca
  * [0, n_pages) stands for a page that is not there (nothing is stored in it, its slots are masked).
  * Two sequences may read the same page; a page that tokens are appended to belongs to one sequence. */
 typedef struct yb_paged_batch {
-  int n_seqs;     /* up to 65536; 0 is an empty batch */
+  int n_seqs;     /* up to 65536; without sequences or tokens nothing is done, buffers without elements may be NULL */
   int n_tokens;   /* rows of the token-major buffers, up to 2^20 */
   int n_heads;
   int n_kv_heads; /* n_heads / n_kv_heads: a whole number from 1 to 16 */
@@ -322,7 +322,8 @@ typedef struct yb_paged_batch {
   int dtype;      /* of the caches, q and out: YB_DTYPE_F16 or YB_DTYPE_BF16 */
   int page_size;  /* 16, 32, 64, 128 or 256 */
   int n_pages;    /* pages in each cache */
-  int max_pages;  /* row length of page_table; max_pages * page_size up to 2^21 */
+  int max_pages;  /* row length of page_table; max_pages * page_size up to 2^21 (less for more than
+                     2^16 sequences times 64 kv heads, whose key tiles would overflow a count) */
   const int* q_start_dev;    /* [n_seqs + 1] */
   const int* kv_len_dev;     /* [n_seqs] */
   const int* page_table_dev; /* [n_seqs][max_pages] */

@@ -94,6 +94,28 @@ def test_empty_batches_need_no_gpu():
         assert _attend(_batch(**kw)) == 0
 
 
+def test_empty_tensors_need_no_gpu():
+    """Tensors without elements have no address; their batch is empty, not refused."""
+    import torch
+
+    from yalm_b200 import PagedBatch
+    k, i32 = torch.zeros(3, 2, 16, 64, dtype=torch.float16), dict(dtype=torch.int32)
+    for n_seqs, n_tokens in ((0, 0), (2, 0), (0, 4)):
+        b = PagedBatch(k, k.clone(), torch.zeros(n_seqs, 4, **i32), torch.zeros(n_seqs + 1, **i32),
+                       torch.zeros(n_seqs, **i32), 8, n_tokens)
+        q = torch.zeros(n_tokens, 512, dtype=torch.float16)
+        b.append(torch.zeros(n_tokens, 768), q, torch.zeros(32), 64)
+        b.attend(q, q.clone(), torch.zeros(b.scratch_bytes(), dtype=torch.uint8))
+
+
+def test_more_key_tiles_than_a_block_can_count_are_refused():
+    big = dict(n_seqs=65536, n_tokens=65536, n_heads=512, n_kv_heads=512, max_pages=(1 << 21) // 16)
+    assert _attend(_batch(**big), out_stride=512 * 64, q_stride=512 * 64) == _lib.YB_E_UNSUPPORTED
+    assert "too many slots" in _lib.last_error()
+    big["n_seqs"], big["n_tokens"] = 4096, 0  # the same table for fewer sequences
+    assert _attend(_batch(**big), out_stride=512 * 64, q_stride=512 * 64) == 0
+
+
 def test_descriptor_matches_the_header():
     """The ctypes structure has the header's fields in the header's order."""
     import re

@@ -33,7 +33,12 @@ int check_batch(const yb_paged_batch* b, PagedBatch* out, bool* empty) {
     return set_error(YB_E_UNSUPPORTED, "at most 65536 sequences, 2^20 new tokens and 2^21 slots per sequence");
   if (((long long)b->n_pages * b->n_kv_heads << lg) > INT_MAX - 256)
     return set_error(YB_E_UNSUPPORTED, "the page pool has too many rows (n_pages * n_kv_heads * page_size)");
-  if (!b->q_start_dev || !b->kv_len_dev || !b->page_table_dev || !b->k_pages || !b->v_pages)
+  // the key tiles of 128 slots that one of 64 or more blocks may have to walk are counted in 32 bits
+  const long long units = b->n_tokens / (2 * (128 / (b->n_heads / b->n_kv_heads))) + (b->n_seqs < b->n_tokens ? b->n_seqs : b->n_tokens);
+  if (units * b->n_kv_heads * ((((long long)b->max_pages << lg) >> 7) + 1) > (1ll << 37))
+    return set_error(YB_E_UNSUPPORTED, "the batch may have too many slots to attend to (n_seqs * n_kv_heads * max_pages * page_size)");
+  *empty = b->n_seqs == 0 || b->n_tokens == 0;  // its buffers of no elements may be null
+  if (!b->k_pages || !b->v_pages || (!*empty && (!b->q_start_dev || !b->kv_len_dev || !b->page_table_dev)))
     return set_error(YB_E_INVALID, "null buffer in the batch");
   if (!aligned16(b->k_pages) || !aligned16(b->v_pages))
     return set_error(YB_E_INVALID, "k_pages and v_pages must be 16-byte aligned");
@@ -47,13 +52,12 @@ int check_batch(const yb_paged_batch* b, PagedBatch* out, bool* empty) {
   out->n_pages = b->n_pages;
   out->max_pages = b->max_pages;
   out->ps_log2 = lg;
-  *empty = b->n_seqs == 0 || b->n_tokens == 0;
   return 0;
 }
 
 // Rows of `width` elements of `size` bytes, `stride` elements apart: 16-byte aligned, not overlapping.
-int check_rows(const char* name, const void* p, long long stride, long long width, int size) {
-  if (!p) return set_error(YB_E_INVALID, std::string("null ") + name);
+int check_rows(const char* name, const void* p, long long stride, long long width, int size, bool empty) {
+  if (!p && !empty) return set_error(YB_E_INVALID, std::string("null ") + name);
   if (!aligned16(p) || stride < width || stride > (1ll << 31) || stride * size % 16)
     return set_error(YB_E_INVALID, std::string(name) + ": rows must be 16-byte aligned and at least " +
                                        std::to_string(width) + " elements apart");
@@ -101,8 +105,8 @@ extern "C" int yb_paged_append_dev(const yb_paged_batch* b, void* q_out, long lo
   if (rc) return rc;
   if (qkv_dtype < 0 || qkv_dtype > 2) return set_error(YB_E_UNSUPPORTED, "qkv must be fp32, fp16 or bf16 (dtype 0, 1, 2)");
   const long long hd = b->head_dim;
-  if ((rc = check_rows("q_out", q_out, q_out_stride, b->n_heads * hd, 2))) return rc;
-  if ((rc = check_rows("qkv", qkv, qkv_stride, (b->n_heads + 2ll * b->n_kv_heads) * hd, qkv_dtype ? 2 : 4))) return rc;
+  if ((rc = check_rows("q_out", q_out, q_out_stride, b->n_heads * hd, 2, empty))) return rc;
+  if ((rc = check_rows("qkv", qkv, qkv_stride, (b->n_heads + 2ll * b->n_kv_heads) * hd, qkv_dtype ? 2 : 4, empty))) return rc;
   if (rotary_dim < 0 || rotary_dim > hd || rotary_dim % 2 || (rope_half && rotary_dim % 8))
     return set_error(YB_E_INVALID, "rotary_dim must be even and <= head_dim (a multiple of 8 for half-split pairs)");
   if (rotary_dim && !inv_freq_dev) return set_error(YB_E_INVALID, "null inv_freq_dev");
@@ -152,7 +156,7 @@ extern "C" int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long l
   int rc = check_batch(b, &a.b, &empty);
   if (rc) return rc;
   const long long width = (long long)b->n_heads * b->head_dim;
-  if ((rc = check_rows("out", out, out_stride, width, 2)) || (rc = check_rows("q", q, q_stride, width, 2))) return rc;
+  if ((rc = check_rows("out", out, out_stride, width, 2, empty)) || (rc = check_rows("q", q, q_stride, width, 2, empty))) return rc;
   if (!(scale > 0.f) || !std::isfinite(scale)) return set_error(YB_E_INVALID, "scale must be positive and finite");
   if (window < 0) return set_error(YB_E_INVALID, "negative window");
   if (!scratch_dev || !aligned16(scratch_dev)) return set_error(YB_E_INVALID, "scratch_dev must be 16-byte aligned memory");

@@ -26,7 +26,7 @@ def _dtype(t, name: str) -> int:
 class PagedBatch:
     """k_pages, v_pages [n_pages][n_kv_heads][page_size][head_dim] fp16 or bf16; page_table [n_seqs][max_pages],
     q_start [n_seqs + 1] and kv_len [n_seqs] int32; n_tokens: rows of the token-major tensors.  All on one
-    GPU, contiguous."""
+    GPU, contiguous.  The calls launch on `stream`, a cudaStream_t as an integer (0: the default stream)."""
 
     def __init__(self, k_pages, v_pages, page_table, q_start, kv_len, n_heads: int, n_tokens: int):
         if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
