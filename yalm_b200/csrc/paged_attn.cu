@@ -19,12 +19,12 @@
 //   warps 0, 3   load the K tiles and Q (a 3-D box of queries x heads), and the V tiles, into one ring, one lane a
 //                page (with pages of 16 slots a tile is 16 copies, which keep one warp busier than the memory)
 //   warps 1, 2   issue the products of pipeline 0 / 1, 64 slots a step: S = Q . K^T into tensor memory, then
-//                O += P . V with P read from tensor memory, where it took the place of S (one warp for both
-//                pipelines was the bottleneck: 1300 clocks a step, of which the products are 650).  S has two buffers, so the
-//                scores of a step are there before the softmax of the step before is done.  (Steps of 128
+//                O += P . V with P read from tensor memory, where it took the place of S.  S has two buffers, so
+//                the scores of a step are there before the softmax of the step before is done.  (Steps of 128
 //                slots leave no room for that: 512 columns hold two outputs and two such S.  A pipeline then
-//                waits a third of its time for its scores.  The 64-column products run at 0.75 of the
-//                rate of the 128-column ones and still win: profiles/paged_attention.md.)
+//                waits a third of its time for its scores.  The 64-column scores' products run at 0.67 of the rate
+//                of 128-column ones, 388 clocks for eight and not 259, and still win.  2048 tokens over 16384 slots: 504 us
+//                with 128 slots a step, 495 with 64; 606 with one warp for both pipelines' products.)
 //   warps 4-7, 8-11   softmax of pipeline 0 / 1, a row per thread
 // A unit of two row tiles runs them as the pipelines over the same slots.  A unit of one row tile (single
 // tokens, short chunks) gives each pipeline half of every key tile, and merges the two at its end.
@@ -34,6 +34,12 @@
 // rescaled only when a row's maximum grew by more than 2^8: until then the old maximum serves, and every
 // weight stays below 2^8.  fp16 weights carry a factor 2^7, which keeps the small ones above 2^-32 of the
 // largest out of the subnormal range.
+//
+// What bounds it.  Prompts and chunks: the exponentials and the passes over S and P through registers beside the
+// products.  2048 tokens over 16384 slots, 32 heads of 128 on 8 kv heads, take 495 us at sustained power (1040
+// TFLOP/s; 446 us, 1155 TFLOP/s, before the clock falls), with the tensor and the special-function units each busy 39 %
+// of the time in a chunk of 1024.  Single tokens: the cache's bytes, 64 x 4096 slots 174 us = 6.2 TB/s; one
+// of 32767 slots 33 us = 4.1 TB/s, of which 8 are the launch, the first loads, the last tile's softmax and the merge.
 #include "paged.cuh"
 
 #include <cuda_bf16.h>
