@@ -367,8 +367,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sb = smem_u32(smem), ring = sb + 2 * C::kTile;
   float* s_ml = reinterpret_cast<float*>(smem + (2 + C::kStages) * C::kTile);  // [2][128]
-  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], q_full[2], q_empty[2], s_full[2][2],
-      p_full[2][2], o_done[2][2], turn[2][4], o_free, ml_ready;
+  struct Bars {
+    uint64_t one[C::kStages + 2 + 4 + 4 + 8];  // one arrival a phase: full, q_full, s_full, o_done, turn
+    uint64_t two[C::kStages + 2];              // two: empty, q_empty
+    uint64_t four[4 + 1];                      // four: p_full, ml_ready
+    uint64_t o_free;                           // eight
+  };
+  __shared__ __align__(8) Bars bars;
+  uint64_t* const full = bars.one;
+  uint64_t* const q_full = full + C::kStages;
+  uint64_t (*const s_full)[2] = reinterpret_cast<uint64_t (*)[2]>(q_full + 2);
+  uint64_t (*const o_done)[2] = s_full + 2;
+  uint64_t (*const turn)[4] = reinterpret_cast<uint64_t (*)[4]>(o_done + 2);
+  uint64_t* const empty = bars.two;
+  uint64_t* const q_empty = empty + C::kStages;
+  uint64_t (*const p_full)[2] = reinterpret_cast<uint64_t (*)[2]>(bars.four);
+  uint64_t& ml_ready = bars.four[4];
+  uint64_t& o_free = bars.o_free;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ unsigned long long s_scan[kThreads / 32];
@@ -380,28 +395,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  } else if (threadIdx.x == 96) {
-    s_abort = 0;
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 2);
-    }
-    for (int p = 0; p < 2; ++p) {
-      mbar_init(&q_full[p], 1);
-      mbar_init(&q_empty[p], 2);
-      for (int u = 0; u < 2; ++u) {
-        mbar_init(&s_full[p][u], 1);
-        mbar_init(&p_full[p][u], 4);
-        mbar_init(&o_done[p][u], 1);
-      }
-    }
-    for (int w = 0; w < 8; ++w) mbar_init(&turn[w & 1][w >> 1], 1);
-    mbar_init(&o_free, 8);
-    mbar_init(&ml_ready, 4);
+  } else if (warp == 3) {
+    constexpr int kOne = sizeof(bars.one) / 8, kTwo = kOne + sizeof(bars.two) / 8, kFour = kTwo + sizeof(bars.four) / 8;
+    for (int i = lane; i < (int)sizeof(Bars) / 8; i += 32)
+      mbar_init(reinterpret_cast<uint64_t*>(&bars) + i, i < kOne ? 1 : i < kTwo ? 2 : i < kFour ? 4 : 8);
     mbar_fence_init();
-    tma_prefetch_map(&qmap);
-    tma_prefetch_map(&kmap);
-    tma_prefetch_map(&vmap);
+    if (lane == 0) {
+      s_abort = 0;
+      tma_prefetch_map(&qmap);
+      tma_prefetch_map(&kmap);
+      tma_prefetch_map(&vmap);
+    }
   }
   pdl_wait();  // up to here nothing of what earlier kernels write was touched
   find_start(b, a.x, s_scan, &s_start);
@@ -426,7 +430,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     unsigned steps = 0, singles = 0;  // a pipeline's steps in the pieces before; pieces of one row tile
     if (threadIdx.x == 128) a.cuts[blockIdx.x].parts = 0;  // the same thread's later store tells otherwise
     bool ok = true;
-    while (ok && !*abort_flag && walk.next(b, a.x, pc)) {
+    // whether the 16 slots of lane i < 8 in key tile t of a piece are on a page that is there
+    auto there = [&](const Piece& c, int t) {
+      const int slot = ((c.u.tile0 + c.t0 + t) << 7) + lane * 16;
+      int id = -1;
+      if (lane < 8 && slot < c.sq.kv) id = __ldg(b.page_table + (size_t)c.seq * b.max_pages + (slot >> b.ps_log2));
+      return id >= 0 && id < b.n_pages;
+    };
+    bool more = walk.next(b, a.x, pc), nx = more && there(pc, 0);  // (a unit without a slot has one empty tile)
+    while (ok && !*abort_flag && more) {
       const bool two = pc.u.nq > QB;
       const int nk = pc.u.none ? 0 : pc.t1 - pc.t0, n = two ? 2 * nk : nk;  // key tiles, steps
       const int tile = two ? p : 0;  // row tile
@@ -434,28 +446,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool valid = r < QB * a.gq && q < pc.u.nq;
       const bool live = quad * 32 < min(QB, pc.u.nq - tile * QB) * a.gq;  // any row of the warp
       const int pos = pc.sq.kv - pc.sq.n + pc.u.q0 + q;
-      const int* table = b.page_table + (size_t)pc.seq * b.max_pages;
       const int first = pc.u.tile0 + pc.t0;
-      // whether the 16 slots of lane i < 8 are on a page that is there
-      auto there = [&](int t) {
-        const int slot = (t << 7) + lane * 16;
-        int id = -1;
-        if (lane < 8 && slot < pc.sq.kv) id = __ldg(table + (slot >> b.ps_log2));
-        return lane < 8 && id >= 0 && id < b.n_pages;
-      };
       // The two warps of a quadrant share a scheduler and its special-function unit: they take their exponentials
       // in turns, one's under the other's loads, maxima and waits.  Left alone they fall into step.
       auto my_turn = [&](unsigned step) {
         return p == 0 ? step == 0 || mbar_wait(&turn[1][quad], (step - 1) & 1, status) : mbar_wait(&turn[0][quad], step & 1, status);
       };
       float m = -INFINITY, l = 0.f;
-      bool nx = nk > 0 && there(first);
       uint32_t pages = 0;
       for (int i = 0; i < n; ++i) {
         const int t = two ? i >> 1 : i, half = two ? i & 1 : p;
         if (!two || !half) {
           pages = __ballot_sync(0xffffffffu, nx);
-          if (t + 1 < nk) nx = there(first + t + 1);
+          if (t + 1 < nk) nx = there(pc, t + 1);
         }
         const unsigned step = steps + i, buf = step & 1;
         if (!(ok = mbar_wait(&s_full[p][buf], (step >> 1) & 1, status))) break;
@@ -538,6 +541,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok || *abort_flag) break;
 
+      // the piece after this one is looked up under the last product and the stores
+      const int left = walk.st.left;
+      Piece after;
+      more = walk.next(b, a.x, after);
+      nx = more && there(after, 0);
       // ---- the piece's rows: o * w0 (+ o of pipeline 1 * w1)
       const bool other = !two && nk > 0;  // pipeline 0 takes pipeline 1's rows in
       float w0 = 1.f, w1 = 0.f;
@@ -582,13 +590,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             float v[32];
             if (nk > 0) {
               tmem_ld32(to + p * HD + c0, v);
+              if (other || whole) {  // a row that has seen no slot has zeros there: its weights were all 0
+                const float2 w00 = make_float2(w0, w0);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[k] = l != 0.f ? v[k] * w0 : 0.f;
+                for (int k = 0; k < 32; k += 2) {
+                  const float2 t2 = mul2(make_float2(v[k], v[k + 1]), w00);
+                  v[k] = t2.x, v[k + 1] = t2.y;
+                }
+              }
               if (other) {
+                const float2 w11 = make_float2(w1, w1);
                 float v1[32];
                 tmem_ld32(to + HD + c0, v1);
 #pragma unroll
-                for (int k = 0; k < 32; ++k) v[k] = l != 0.f ? fmaf(v1[k], w1, v[k]) : 0.f;
+                for (int k = 0; k < 32; k += 2) {
+                  const float2 t2 = fma2(make_float2(v1[k], v1[k + 1]), w11, make_float2(v[k], v[k + 1]));
+                  v[k] = t2.x, v[k + 1] = t2.y;
+                }
               }
             } else {
 #pragma unroll
@@ -617,11 +635,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (nk > 0 && lane == 0) mbar_arrive(&o_free);
       }
       if (!whole && pc.t0 == 0 && threadIdx.x == 128) {
-        const unsigned long long begin = s_start.begin + (s_start.left - walk.st.left) - pc.t1;  // the unit's first tile
+        const unsigned long long begin = s_start.begin + (s_start.left - left) - pc.t1;  // the unit's first tile
         const int last = block_of(s_start.share, s_start.more, begin + pc.u.cost - 1);
         a.cuts[blockIdx.x] = Cut{token, pc.u.nq, pc.head, last - (int)blockIdx.x + 1};
       }
       steps += n;
+      pc = after;
     }
     if (!ok) *abort_flag = 1;
   } else {
