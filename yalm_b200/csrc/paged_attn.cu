@@ -584,7 +584,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float inv = whole ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
         w0 *= inv;
         w1 *= inv;
-        if (live) {
+        if (live && two && whole && nk > 0) {
+          // Whole outputs of many rows: of 32 columns a lane holds its row's four groups of 16 bytes.  Two lanes exchange
+          // two of theirs, so that a store writes whole sectors of 32 bytes of every second row.
+          const bool up = lane & 1;
+          T* to_row[2];
+          bool has[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int from = (lane & ~1) + k;
+            to_row[k] = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), from)) + 8 * (lane & 1);
+            has[k] = __shfl_sync(0xffffffffu, (int)valid, from);
+          }
+#pragma unroll 1
+          for (int c0 = 0; c0 < HD; c0 += 32) {
+            float v[32];
+            tmem_ld32(to + p * HD + c0, v);
+#pragma unroll
+            for (int k = 0; k < 4; k += 2) {
+              uint32_t w[2][4];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float2 t2 = mul2(make_float2(v[8 * k + 2 * e], v[8 * k + 2 * e + 1]), make_float2(w0, w0));
+                w[e / 4][e % 4] = pack2<T>(t2.x, t2.y);
+              }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? w[0][e] : w[1][e], 1);
+                if (up) w[0][e] = got; else w[1][e] = got;
+              }
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+                if (has[x]) *reinterpret_cast<uint4*>(to_row[x] + c0 + 8 * k) = make_uint4(w[x][0], w[x][1], w[x][2], w[x][3]);
+            }
+          }
+        } else if (live) {
 #pragma unroll 1
           for (int c0 = 0; c0 < HD; c0 += 32) {
             float v[32];
