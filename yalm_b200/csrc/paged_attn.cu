@@ -61,6 +61,7 @@ constexpr int kRows = 128;     // rows per row tile = tensor-memory lanes
 constexpr int kThreads = 384;
 constexpr int kMaxGrid = 256;  // blocks the workspace has room for
 constexpr int kFewTiles = 4;   // shares below this are all the same
+constexpr int kUnitTiles = 2;  // a unit's start and end, in key tiles
 constexpr uint32_t kBlk = kRows * 128;  // bytes of 128 rows x 64 elements
 
 template <int HD>
@@ -116,7 +117,7 @@ __device__ __forceinline__ unsigned ramp(int n, int a, int u) {
 struct Unit {
   int q0, nq;      // queries [q0, q0 + nq) of the sequence
   int tile0;       // first key tile
-  int cost;        // key tiles, at least 1
+  int cost;        // key tiles, at least 1; kUnitTiles more on the axis
   bool none;       // no slot is seen: zeros
 };
 struct Axis {
@@ -134,20 +135,23 @@ __device__ __forceinline__ Unit unit_of(const Axis& x, const PagedSeq& q, int i)
   return u;
 }
 __device__ __forceinline__ int n_units(const Axis& x, const PagedSeq& q) { return q.n <= x.U ? 1 : (q.n + x.U - 1) / x.U; }
-// key tiles of the first m units of a (sequence, kv head), m < n_units: unit i ends at slot p0 + (i + 1) U
+// length on the axis of the first m units of a (sequence, kv head), m < n_units: unit i ends at slot p0 + (i + 1) U
 __device__ __forceinline__ unsigned units_before(const Axis& x, const PagedSeq& q, int m) {
   if (m == 0) return 0;
   const int p0 = q.kv - q.n;
-  return (unsigned)m + ramp(m, p0 + x.U - 1, x.U) - ramp(m, p0 - x.window + 1, x.U);
+  return (unsigned)m * (1 + kUnitTiles) + ramp(m, p0 + x.U - 1, x.U) - ramp(m, p0 - x.window + 1, x.U);
 }
+// ... of all units of a (sequence, kv head)
 __device__ __forceinline__ unsigned head_tiles(const Axis& x, const PagedSeq& q) {
   if (q.n <= 0) return 0;
   const int nu = n_units(x, q);
-  return units_before(x, q, nu - 1) + (unsigned)unit_of(x, q, nu - 1).cost;
+  return units_before(x, q, nu - 1) + (unsigned)unit_of(x, q, nu - 1).cost + kUnitTiles;
 }
 
-// Where a block starts, and its share.  Of all key tiles every block takes `share`, the first `more` blocks one
-// more.  Shares of a few tiles are all the same instead, and the last blocks have none: they end no later, and
+// Where a block starts, and its share.  Of the axis, key tiles and kUnitTiles a unit, every block takes `share`, the
+// first `more` blocks one more.  A unit's start and end (the last product, the outputs, the next first scores) take
+// 5500 clocks beside 2000 to 3300 for a tile, so blocks of many short units would be the last by far: without
+// them on the axis five prompts of head_dim 64 took 26.1 us, not 22.4, and 64 single tokens 110, not 105.5.  Shares of a few tiles are all the same instead, and the last blocks have none: they end no later, and
 // cut less (one token over 4096 slots 16.2 -> 14.9 us; with shares of 12 tiles a mixed step took 55.5 us, not 51).
 struct Start {
   PagedSeq sq;
@@ -183,28 +187,31 @@ struct Walk {
   PagedSeq sq;
   __device__ __forceinline__ explicit Walk(const Start& s) : st(s), sq(s.sq) {}
   __device__ __forceinline__ bool next(const PagedBatch& b, const Axis& x, Piece& p) {
-    if (st.left <= 0 || st.seq >= b.n_seqs) return false;
-    p.sq = sq;
-    p.seq = st.seq;
-    p.head = st.head;
-    p.u = unit_of(x, sq, st.unit);
-    p.t0 = st.off;
-    p.t1 = min(p.u.cost, st.off + st.left);
-    st.left -= p.t1 - p.t0;
-    st.off = p.t1;
-    if (st.off == p.u.cost && st.left > 0) {
-      st.off = 0;
-      if (++st.unit >= n_units(x, sq)) {
-        st.unit = 0;
-        if (++st.head >= x.K) {
-          st.head = 0;
-          do {
-            if (++st.seq >= b.n_seqs) break;
-            sq = paged_seq(b, st.seq);
-          } while (sq.n <= 0);
+    do {
+      if (st.left <= 0 || st.seq >= b.n_seqs) return false;
+      p.sq = sq;
+      p.seq = st.seq;
+      p.head = st.head;
+      p.u = unit_of(x, sq, st.unit);
+      const int all = p.u.cost + kUnitTiles, end = min(all, st.off + st.left);
+      p.t0 = st.off;
+      p.t1 = min(p.u.cost, end);
+      st.left -= end - st.off;
+      st.off = end;
+      if (end == all && st.left > 0) {
+        st.off = 0;
+        if (++st.unit >= n_units(x, sq)) {
+          st.unit = 0;
+          if (++st.head >= x.K) {
+            st.head = 0;
+            do {
+              if (++st.seq >= b.n_seqs) break;
+              sq = paged_seq(b, st.seq);
+            } while (sq.n <= 0);
+          }
         }
       }
-    }
+    } while (p.t0 >= p.t1);  // no tile, only the rest of a unit's length
     return true;
   }
 };
@@ -863,7 +870,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // three blocks, 4096 such groups), else the work of 8 lanes that share out the parts and join them by
 // shuffles (a single token's unit over 18 blocks, 64 groups), so that every load is under way at once.  The
 // order of the sum depends on the number of parts alone.
-constexpr int kMergeThreads = 128, kMergeSlices = 16, kMergeParts = 4;
+constexpr int kMergeThreads = 128, kMergeSlices = 24, kMergeParts = 4;
 template <int HD, typename T>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid_constant__ PagedAttnParams a) {
   pdl_wait();

@@ -35,7 +35,7 @@ int check_batch(const yb_paged_batch* b, PagedBatch* out, bool* empty) {
     return set_error(YB_E_UNSUPPORTED, "the page pool has too many rows (n_pages * n_kv_heads * page_size)");
   // the key tiles of 128 slots that one of 64 or more blocks may have to walk are counted in 32 bits
   const long long units = b->n_tokens / (2 * (128 / (b->n_heads / b->n_kv_heads))) + (b->n_seqs < b->n_tokens ? b->n_seqs : b->n_tokens);
-  if (units * b->n_kv_heads * ((((long long)b->max_pages << lg) >> 7) + 1) > (1ll << 37))
+  if (units * b->n_kv_heads * ((((long long)b->max_pages << lg) >> 7) + 3) > (1ll << 37))
     return set_error(YB_E_UNSUPPORTED, "the batch may have too many slots to attend to (n_seqs * n_kv_heads * max_pages * page_size)");
   *empty = b->n_seqs == 0 || b->n_tokens == 0;  // its buffers of no elements may be null
   if (!b->k_pages || !b->v_pages || (!*empty && (!b->q_start_dev || !b->kv_len_dev || !b->page_table_dev)))
