@@ -7,10 +7,10 @@
 //
 // Work.  A unit is (sequence, kv head, block of up to 2 QB queries), QB = 128 / (query heads per kv head):
 // its rows are (query, head of the group) pairs, in two row tiles of 128, so every K and V tile that is
-// loaded serves all query heads of its group.  A unit's cost is its number of 128-slot key tiles.  The
-// units of the whole batch in order make one axis of key tiles, which the blocks (one per SM) share out
+// loaded serves all query heads of its group.  A unit's cost is that of its 128-slot key tiles and of its start
+// and end.  The units of the whole batch in order make one axis, which the blocks (one per SM) share out
 // evenly: a long cache of few rows is cut over many blocks, and ragged lengths balance themselves.
-// The cuts follow from the lengths on the device, by a closed form for a sequence's tiles (floor
+// The cuts follow from the lengths on the device, by a closed form for a sequence's units (floor
 // sums), so there is no plan to be made on the host and a captured launch follows new lengths.  A unit
 // that is cut leaves (o, m, l) records in the workspace, which a second kernel merges, spread over the whole
 // GPU: results do not depend on timing, and no block waits for another.
@@ -61,7 +61,7 @@ constexpr int kRows = 128;     // rows per row tile = tensor-memory lanes
 constexpr int kThreads = 384;
 constexpr int kMaxGrid = 256;  // blocks the workspace has room for
 constexpr int kFewTiles = 4;   // shares below this are all the same
-constexpr int kUnitTiles = 2;  // a unit's start and end, in key tiles
+constexpr int kUnitTiles = 2;  // what a unit's start and end cost, in key tiles
 constexpr uint32_t kBlk = kRows * 128;  // bytes of 128 rows x 64 elements
 
 template <int HD>
@@ -150,14 +150,17 @@ __device__ __forceinline__ unsigned head_tiles(const Axis& x, const PagedSeq& q)
 
 // Where a block starts, and its share.  Of the axis, key tiles and kUnitTiles a unit, every block takes `share`, the
 // first `more` blocks one more.  A unit's start and end (the last product, the outputs, the next first scores) take
-// 5500 clocks beside 2000 to 3300 for a tile, so blocks of many short units would be the last by far: without
-// them on the axis five prompts of head_dim 64 took 26.1 us, not 22.4, and 64 single tokens 110, not 105.5.  Shares of a few tiles are all the same instead, and the last blocks have none: they end no later, and
-// cut less (one token over 4096 slots 16.2 -> 14.9 us; with shares of 12 tiles a mixed step took 55.5 us, not 51).
+// 4000 to 5500 clocks beside 2000 (one row tile) to 3300 (two) for a key tile, so blocks of many short units would be
+// the last by far: without them on the axis five prompts of head_dim 64 took 26.1 us, not 22.4, and 64 single tokens
+// 110, not 105.5.  (Tiles weighted 2 : 3 by their row tiles: a mixed step 43.6 us, not 45.6, the prompts 24.2, not
+// 22.5, three hundred other batches in a model of it 0.3 % less.)
+// Shares of a few tiles are all the same instead, and the last blocks have none: they end no later, and cut less
+// (one token over 4096 slots 16.2 -> 14.9 us; with shares of 12 tiles a mixed step took 55.5 us, not 51).
 struct Start {
   PagedSeq sq;
   int seq, head, unit, off;
-  int left;                  // key tiles of this block
-  unsigned long long begin;  // first key tile on the axis
+  int left;                  // length of this block's part of the axis
+  unsigned long long begin;  // where it begins
   unsigned long long share;
   int more;
 };
@@ -169,7 +172,7 @@ __device__ __forceinline__ unsigned long long quot(unsigned long long a, unsigne
 __device__ __forceinline__ unsigned long long block_begin(unsigned long long share, int more, int c) {
   return share * c + min(c, more);
 }
-// the block that holds tile x
+// the block that holds position x
 __device__ __forceinline__ int block_of(unsigned long long share, int more, unsigned long long x) {
   const unsigned long long cut = (share + 1) * more;
   return x < cut ? (int)quot(x, share + 1) : more + (int)quot(x - cut, share);
@@ -255,7 +258,7 @@ __device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long lon
   const unsigned long long begin = block_begin(share, more, c);
   if (begin < before || begin >= before + mine) return;
   const int left = (int)min(share + (c < more ? 1 : 0), total - begin);
-  // this thread's sequences hold the block's first tile
+  // this thread's sequences hold the block's first position
   unsigned long long rem = begin - before;
   int s = s1 - 1;
   if (per > 1) {
@@ -280,8 +283,8 @@ __device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long lon
   *s_start = st;
 }
 
-// Called by a whole warp: the unit in which tile st.off of the head lies, and the tile within it.  Unit u begins
-// at tile units_before(u); 32 guesses at a time.
+// Called by a whole warp: the unit in which position st.off of the head lies, and the position within it.  Unit u
+// begins at units_before(u); 32 guesses at a time.
 __device__ __forceinline__ void find_unit(const Axis& x, Start& st) {
   int lo = 0, hi = n_units(x, st.sq);  // units_before(lo) <= off < units_before(hi)
   if (hi == 1) return;
