@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kThreads, 7) paged_append_kernel(const __grid_
   constexpr int kAhead = sizeof(S) == 4 ? 1 : 2;    // groups loaded ahead
   constexpr bool kNear = P == kNeighbours || P == kPartNeighbours, kPart = P == kPartNeighbours || P == kPartHalves;
   __shared__ __align__(16) float s_fac[kWarps][2][2][HD];  // queries, keys: the factors of v_e and v_f
-  __shared__ __align__(16) float s_head[P == kPartHalves ? kWarps : 1][P == kPartHalves ? 512 : 4];
+  __shared__ __align__(16) float s_head[P == kPartHalves ? kWarps : 1][P == kPartHalves ? 512 + 4 : 4];  // heads, four zeros
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int id = blockIdx.x * kWarps + warp, row = id / shares, share = id % shares;
   if (row >= a.b.n_tokens) return;
@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(kThreads, 7) paged_append_kernel(const __grid_
       fac[k][1][at<HD>(f)] = s * we;
     }
   }
+  if (P == kPartHalves && lane < 4) s_head[warp][512 + lane] = 0.f;
   __syncwarp();
 
   const bool clipped = a.clip < 3.4028234e38f;
@@ -208,12 +209,12 @@ __global__ void __launch_bounds__(kThreads, 7) paged_append_kernel(const __grid_
           if (P == kPartHalves) {
 #pragma unroll
             for (int j = 0; j < 8; j += 4) {  // d is a multiple of 4: four neighbours' partners are neighbours
-              const int e = e0 + j, f = e < d ? e + d : e < R ? e - d : e;
-              const float4 o = *reinterpret_cast<const float4*>(mine + at<HD>(f));
+              const int e = e0 + j, f = e < d ? e + d : e - d;
+              const float4 o = *reinterpret_cast<const float4*>(e < R ? mine + at<HD>(f) : &s_head[warp][512]);
               other[j] = o.x, other[j + 1] = o.y, other[j + 2] = o.z, other[j + 3] = o.w;
             }
           }
-          if (kPart) {  // an element that is not rotated takes nothing from another, not even 0 * inf
+          if (P == kPartNeighbours) {  // an element that is not rotated takes nothing from another, not even 0 * inf
 #pragma unroll
             for (int j = 0; j < 8; ++j) other[j] = e0 + j < R ? other[j] : 0.f;
           }
