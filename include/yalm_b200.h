@@ -366,6 +366,10 @@ int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long long out_str
                            long long q_stride, float scale, int window, void* scratch_dev, void* stream);
 size_t yb_paged_attention_scratch_bytes(const yb_paged_batch* b); /* 0 for a batch that is refused */
 
+/* Diagnostics: the SM clocks that a wait in the kernel of later yb_paged_attention_dev calls of this process may take
+ * before it gives up (0: the default of 4e9, about 2 s, which is also the most).  A healthy wait takes microseconds. */
+int yb_paged_attention_wait_budget(long long clocks);
+
 /* Number of streaming multiprocessors the kernels size their grids for (device 0 if none set). */
 int yb_num_sms(void);
 

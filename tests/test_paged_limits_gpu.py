@@ -1,0 +1,48 @@
+"""The paged-cache operators where they end: waits that run out, streams, sequences far longer than a block's share,
+values that are not finite.  Plain implementations and tolerances are those of test_paged_gpu.py where nothing else is
+said."""
+import math
+
+import pytest
+
+from test_paged_gpu import Step
+from yalm_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def wait_budget():
+    """Sets the clocks that a wait may take; the default comes back at the end."""
+    def use(clocks):
+        _lib.check(_lib.lib().yb_paged_attention_wait_budget(clocks))
+    yield use
+    use(0)
+
+
+@pytest.mark.parametrize("clocks", [1, 500, 2000, 6000, 20000])
+@pytest.mark.parametrize("new,kv,nh,nkv,hd,ps,dtype", [
+    ([1, 1, 260, 300], [4000, 900, 1500, 700], 32, 8, 128, 16, "f16"),
+    ([1] * 30, [700] * 30, 8, 2, 64, 64, "bf16"),
+])
+def test_a_wait_that_runs_out_ends_the_call(gpu, wait_budget, new, kv, nh, nkv, hd, ps, dtype, clocks):
+    """The kernel gives up, says so in the workspace's first word and returns, with nothing in flight: the next call in
+    the same workspace is right.  A budget of one clock always runs out: the first queries are a trip to memory away."""
+    import torch
+    s = Step(new, kv, nh, nkv, hd, ps, dtype, seed=91)
+    b = s.batch()
+    scratch = torch.zeros(b.scratch_bytes(), dtype=torch.uint8, device="cuda")
+    word = scratch[:4].view(torch.int32)
+    want = s.check(scratch=scratch, batch=b)
+    assert int(word) == 0
+    for _ in range(5):
+        wait_budget(clocks)
+        got = s.attend(scratch=scratch, batch=b).double()
+        bits = int(word)
+        assert bits in ((1,) if clocks == 1 else (0, 1))
+        if not bits:
+            assert torch.equal(got, want)
+        wait_budget(0)
+        word.zero_()
+        assert torch.equal(s.attend(scratch=scratch, batch=b).double(), want)
+        assert int(word) == 0

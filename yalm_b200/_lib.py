@@ -92,6 +92,7 @@ _SIGS = {
     "yb_paged_append_dev": (_I, [_P, _P, _LL, _P, _LL, _I, _P, _P, _F, _P, _I, _I, _P, _F, _P]),
     "yb_paged_attention_dev": (_I, [_P, _P, _LL, _P, _LL, _F, _I, _P, _P]),
     "yb_paged_attention_scratch_bytes": (_S, [_P]),
+    "yb_paged_attention_wait_budget": (_I, [_LL]),
     "yb_num_sms": (_I, []),
     "yb_profile_kernel": (_I, [_P, _I, _I, ctypes.POINTER(_F)]),
 }

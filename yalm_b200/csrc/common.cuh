@@ -68,6 +68,18 @@ __device__ __forceinline__ bool mbar_try_wait_s(uint32_t bar, unsigned parity) {
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, unsigned parity) {
   return mbar_try_wait_s(smem_u32(bar), parity);
 }
+// The same without the time for which try_wait may suspend the thread.
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, unsigned parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Waits for the barrier phase with the given parity.  Returns false (and records kStatusMbarTimeout)
 // when the cycle budget runs out.
 __device__ __forceinline__ bool mbar_wait_s(uint32_t bar, unsigned parity, unsigned* status) {

@@ -94,6 +94,7 @@ struct PagedAttnArgs {
   long long q_stride, out_stride;
   float scale;
   int window;  // slots a token sees, itself counted; INT_MAX: all of them
+  long long wait_budget;  // clocks after which a wait in the kernel gives up
   void* scratch;
 };
 size_t paged_attention_scratch(int head_dim, int n_sms);

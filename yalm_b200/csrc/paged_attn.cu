@@ -348,6 +348,13 @@ constexpr size_t kHeadBytes = 256 + kMaxGrid * sizeof(Cut);
 template <int HD>
 constexpr size_t rec_floats() { return 256 * (size_t)(HD + 2); }
 
+// SM clocks that a wait may take.  Less than the default: without try_wait, which may suspend a warp for longer.
+struct Budget {
+  long long clocks;
+  unsigned nap;
+};
+inline Budget budget_of(long long clocks) { return {clocks, clocks < kWaitBudgetCycles ? 0u : 1u}; }
+
 }  // namespace
 
 struct PagedAttnParams {
@@ -355,13 +362,30 @@ struct PagedAttnParams {
   Axis x;
   void* out;
   long long out_stride;
-  float c;  // scale * log2(e)
-  int gq;   // query heads per kv head
-  int oob;  // a row outside the page pool's tensor maps
+  Budget budget, full;  // of the waits, and of those for what is in flight at the end
+  float c;              // scale * log2(e)
+  int gq;               // query heads per kv head
+  int oob;              // a row outside the page pool's tensor maps
   unsigned* status;
   Cut* cuts;
   float* recs;
 };
+
+// Waits for the phase, or until the budget has run out, here or in another warp of the block, which *mark then tells.
+// It returns to the same place either way: a warp votes on the mark before it leaves a loop (lanes that left by
+// themselves would be waited for without end at the next vote of the others).
+__device__ __forceinline__ void bounded_wait(uint64_t* bar, unsigned parity, const Budget& budget, volatile int* mark,
+                                             unsigned* status) {
+  if (mbar_test_wait(bar, parity)) return;
+  const long long t0 = clock64();
+  while (!*mark && !(budget.nap ? mbar_try_wait(bar, parity) : mbar_test_wait(bar, parity))) {
+    if (clock64() - t0 > budget.clocks) {
+      *mark = 1;
+      atomicOr(status, kStatusMbarTimeout);
+      return;
+    }
+  }
+}
 
 template <int HD, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -378,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t sb = smem_u32(smem), ring = sb + 2 * C::kTile;
   float* s_ml = reinterpret_cast<float*>(smem + (2 + C::kStages) * C::kTile);  // [2][128]
   struct Bars {
-    uint64_t one[C::kStages + 2 + 4 + 4 + 8];  // one arrival a phase: full, q_full, s_full, o_done, turn
+    uint64_t one[C::kStages + 2 + 4 + 4 + 8 + 2];  // one arrival a phase: full, q_full, s_full, o_done, turn, idle
     uint64_t two[C::kStages + 2];              // two: empty, q_empty
     uint64_t four[4 + 1];                      // four: p_full, ml_ready
     uint64_t o_free;                           // eight
@@ -389,13 +413,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t (*const s_full)[2] = reinterpret_cast<uint64_t (*)[2]>(q_full + 2);
   uint64_t (*const o_done)[2] = s_full + 2;
   uint64_t (*const turn)[4] = reinterpret_cast<uint64_t (*)[4]>(o_done + 2);
+  uint64_t* const idle = reinterpret_cast<uint64_t*>(turn + 2);
   uint64_t* const empty = bars.two;
   uint64_t* const q_empty = empty + C::kStages;
   uint64_t (*const p_full)[2] = reinterpret_cast<uint64_t (*)[2]>(bars.four);
   uint64_t& ml_ready = bars.four[4];
   uint64_t& o_free = bars.o_free;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort;
+  __shared__ int s_abort, s_late;  // a wait has run out; one for what is in flight at the end
+  __shared__ unsigned s_issued[2][2];  // keys, values: the slots that copies were issued into, and whose count is odd
   __shared__ unsigned long long s_scan[kThreads / 32];
   __shared__ Start s_start;
 
@@ -411,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(reinterpret_cast<uint64_t*>(&bars) + i, i < kOne ? 1 : i < kTwo ? 2 : i < kFour ? 4 : 8);
     mbar_fence_init();
     if (lane == 0) {
-      s_abort = 0;
+      s_abort = s_late = 0;
       tma_prefetch_map(&qmap);
       tma_prefetch_map(&kmap);
       tma_prefetch_map(&vmap);
@@ -423,8 +449,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  volatile int* abort_flag = &s_abort;
-  unsigned* status = a.status;
+  // Once a wait has run out, here or there, no wait of the block lasts: every warp goes on to the end of its piece with
+  // whatever lies in its buffers, and leaves.  (A look at the mark in every step cost 3 %.)  Barriers may be arrived at
+  // early, but a copy must not be announced to one where another is landing, so the loaders look before each copy.
+  // Nobody leaves the block before its copies and products have ended.
+  auto wait = [&](uint64_t* bar, unsigned parity) { bounded_wait(bar, parity, a.budget, &s_abort, a.status); };
+  auto aborted = [&] { return __any_sync(0xffffffffu, *static_cast<volatile int*>(&s_abort)) != 0; };
   const int QB = kRows / a.gq;
   Start st0 = s_start;
   if (st0.left > 0) find_unit(a.x, st0);
@@ -439,7 +469,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int qi = r / a.gq, h = r % a.gq;
     unsigned steps = 0, singles = 0;  // a pipeline's steps in the pieces before; pieces of one row tile
     if (threadIdx.x == 128) a.cuts[blockIdx.x].parts = 0;  // the same thread's later store tells otherwise
-    bool ok = true;
     // whether the 16 slots of lane i < 8 in key tile t of a piece are on a page that is there
     auto there = [&](const Piece& c, int t) {
       const int slot = ((c.u.tile0 + c.t0 + t) << 7) + lane * 16;
@@ -448,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       return id >= 0 && id < b.n_pages;
     };
     bool more = walk.next(b, a.x, pc), nx = more && there(pc, 0);  // (a unit without a slot has one empty tile)
-    while (ok && !*abort_flag && more) {
+    while (more && !aborted()) {
       const bool two = pc.u.nq > QB;
       const int nk = pc.u.none ? 0 : pc.t1 - pc.t0, n = two ? 2 * nk : nk;  // key tiles, steps
       const int tile = two ? p : 0;  // row tile
@@ -460,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // The two warps of a quadrant share a scheduler and its special-function unit: they take their exponentials
       // in turns, one's under the other's loads, maxima and waits.  Left alone they fall into step.
       auto my_turn = [&](unsigned step) {
-        return p == 0 ? step == 0 || mbar_wait(&turn[1][quad], (step - 1) & 1, status) : mbar_wait(&turn[0][quad], step & 1, status);
+        if (p || step) wait(&turn[p ^ 1][quad], (p ? step : step - 1) & 1);
       };
       float m = -INFINITY, l = 0.f;
       uint32_t pages = 0;
@@ -471,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (t + 1 < nk) nx = there(pc, t + 1);
         }
         const unsigned step = steps + i, buf = step & 1;
-        if (!(ok = mbar_wait(&s_full[p][buf], (step >> 1) & 1, status))) break;
+        wait(&s_full[p][buf], (step >> 1) & 1);
         tc_fence_after();
         if (live) {
           const int k0 = (first + t) * kKT + half * kST;
@@ -507,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             alpha = need ? ex2(m - mn) : 1.f;  // 0 while m is -inf
             m = mn;
             if (i > 0) {
-              if (!(ok = mbar_wait(&o_done[p][buf ^ 1], ((step - 1) >> 1) & 1, status))) break;
+              wait(&o_done[p][buf ^ 1], ((step - 1) >> 1) & 1);
               tc_fence_after();
 #pragma unroll 1
               for (int c0 = 0; c0 < HD; c0 += 16) {
@@ -520,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
-          if (!(ok = my_turn(step))) break;
+          my_turn(step);
           const float shift = m == -INFINITY ? 0.f : m - kBias;
           const float2 cc = make_float2(a.c, a.c), sh = make_float2(-shift, -shift);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -542,14 +571,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
           tmem_st_wait();
         } else {
-          if (!(ok = my_turn(step))) break;
+          my_turn(step);
           if (lane == 0) mbar_arrive(&turn[p][quad]);
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[p][buf]);
       }
-      if (!ok || *abort_flag) break;
+      if (aborted()) break;
 
       // the piece after this one is looked up under the last product and the stores
       const int left = walk.st.left;
@@ -561,8 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float w0 = 1.f, w1 = 0.f;
       // (a barrier for each buffer: its phase before the awaited one is over, since the scores that came into the
       // buffer later followed the product of that phase)
-      if (n > 0) ok = mbar_wait(&o_done[p][(steps + n - 1) & 1], ((steps + n - 1) >> 1) & 1, status);
-      if (!ok) break;
+      if (n > 0) wait(&o_done[p][(steps + n - 1) & 1], ((steps + n - 1) >> 1) & 1);
       if (other) {
         if (p == 1) {
           s_ml[r] = m;
@@ -575,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_arrive(&o_free);  // pipeline 0 reads the outputs
           }
         } else {
-          if (!(ok = mbar_wait(&ml_ready, singles & 1, status))) break;
+          wait(&ml_ready, singles & 1);
           const float m1 = s_ml[r], l1 = s_ml[kRows + r], mm = fmaxf(m, m1);
           w0 = m == -INFINITY ? 0.f : ex2(m - mm);
           w1 = m1 == -INFINITY ? 0.f : ex2(m1 - mm);
@@ -686,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       steps += n;
       pc = after;
     }
-    if (!ok) *abort_flag = 1;
+    tmem_st_wait();
   } else {
   if (warp == 0 || warp == 3) {
     // ------------------------------------------------------------------------------- loads
@@ -695,9 +723,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int boxes = ps >= kKT ? 1 : kKT >> lg;  // pages per key tile
     const uint32_t box_bytes = (uint32_t)min(ps, kKT) * 128u;
     unsigned slot = 0, phase = 1, issued = 0, uses[2] = {0, 0};
+    unsigned mine_into = 0, mine_odd = 0;  // the slots that this warp's copies went into, and whose count is odd
     int buf = 0;  // buffer of the next unit of one row tile
     bool ok = true;
-    while (ok && !*abort_flag && walk.next(b, a.x, pc)) {
+    while (ok && walk.next(b, a.x, pc)) {
       if (pc.u.none) continue;
       const bool two = pc.u.nq > QB;
       const int* table = b.page_table + (size_t)pc.seq * b.max_pages;
@@ -712,7 +741,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto load = [&](const CUtensorMap* map, int row, bool mine) {
         if (mine) {
-          if (issued >= C::kStages && !mbar_wait(&empty[slot], phase, status)) return false;
+          if (issued >= C::kStages) wait(&empty[slot], phase);
+          if (aborted()) return false;
+          mine_into |= 1u << slot;
+          mine_odd ^= 1u << slot;
           if (lane == 0) mbar_arrive_expect_tx(&full[slot], C::kTile);
           __syncwarp();
           if (lane < boxes)
@@ -725,7 +757,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       // a row tile of queries, once the products of the unit before have read its buffer
       auto load_q = [&](int to, int tile) {
-        if (uses[to] && !mbar_wait(&q_empty[to], (uses[to] - 1) & 1, status)) return false;
+        if (uses[to]) wait(&q_empty[to], (uses[to] - 1) & 1);
+        if (aborted()) return false;
         ++uses[to];
         if (lane == 0) {
           mbar_arrive_expect_tx(&q_full[to], (uint32_t)(QB * a.gq) * 128u * C::kHalves);
@@ -759,12 +792,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (!ok) *abort_flag = 1;
-    // never leave while a copy may still be landing: the last one into each slot and buffer
-    for (unsigned i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
-      mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1, status);
-    for (int t = 0; t < 2; ++t)
-      if (uses[t]) mbar_wait(&q_full[t], (uses[t] - 1) & 1, status);
+    // never leave while a copy may still be landing: the last one into each slot, whichever of the two warps issued it
+    // (they may have stopped at different tiles), and into each query buffer
+    if (lane == 0) {
+      s_issued[keys ? 0 : 1][0] = mine_into;
+      s_issued[keys ? 0 : 1][1] = mine_odd;
+    }
+    asm volatile("bar.sync 1, 64;" ::: "memory");
+    if (keys) {
+      const unsigned into = s_issued[0][0] | s_issued[1][0], odd = s_issued[0][1] ^ s_issued[1][1];
+      for (int i = 0; i < C::kStages; ++i)
+        if ((into >> i) & 1u) bounded_wait(&full[i], ((odd >> i) & 1u) ^ 1u, a.full, &s_late, a.status);
+      for (int t = 0; t < 2; ++t)
+        if (uses[t]) bounded_wait(&q_full[t], (uses[t] - 1) & 1, a.full, &s_late, a.status);
+    }
   } else if (warp < 3) {
     // ------------------------------------------------------------------------------- products
     const int p = warp - 1;
@@ -772,33 +813,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     unsigned slot = 0, phase = 0, pieces = 0, steps = 0, uses[2] = {0, 0};
     int buf = 0;
     const uint32_t e = elect_lane();
-    bool ok = true;
-    while (ok && !*abort_flag && walk.next(b, a.x, pc)) {
+    bool any = false;
+    while (!aborted() && walk.next(b, a.x, pc)) {
       if (pc.u.none) continue;
       const bool two = pc.u.nq > QB;
       const int first = pc.u.tile0 + pc.t0, nk = pc.t1 - pc.t0, n = two ? 2 * nk : nk;
       const int qb = two ? p : buf;
       // each pipeline's warp keeps count of both buffers, whichever it reads
       for (int t = two ? 0 : buf; t <= (two ? 1 : buf); ++t) {
-        if (t == qb) ok = mbar_wait(&q_full[t], uses[t] & 1, status);
+        if (t == qb) wait(&q_full[t], uses[t] & 1);
         ++uses[t];
       }
-      if (!ok) break;
       unsigned kslot = 0, vslot = 0;
       auto take = [&](unsigned& at) {
         at = slot;
-        if (!mbar_wait(&full[slot], phase, status)) return false;
+        wait(&full[slot], phase);
         if (++slot == C::kStages) slot = 0, phase ^= 1;
-        return true;
       };
       // a key tile serves two steps of a unit of two row tiles, else one, on this pipeline's half
       auto begins = [&](int i) { return !two || !(i & 1); };
       auto ends = [&](int i) { return !two || (i & 1); };
       auto half_of = [&](int i) { return (uint32_t)(two ? i & 1 : p) * (kST * 128u); };  // bytes into the blocks
-      auto take_k = [&](int i) { return !begins(i) || take(kslot); };
+      auto take_k = [&](int i) {
+        if (begins(i)) take(kslot);
+      };
       auto take_v = [&](int i) {
-        if (!begins(i)) return true;
-        if (!take(vslot)) return false;
+        if (!begins(i)) return;
+        take(vslot);
         // Slots before the first token's window, and behind the sequence's last one in its last page, may hold
         // anything: their weight is 0, and 0 * v has to be 0 (both warps write the same zeros).
         const int k0 = (first + (two ? i >> 1 : i)) * kKT;
@@ -816,10 +857,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int rem = pc.sq.kv - k0, seen = pc.sq.kv - pc.sq.n + pc.u.q0 - a.x.window + 1 - k0;
         if (rem < kKT) zero(rem, min(kKT, ((rem + (1 << b.ps_log2) - 1) >> b.ps_log2) << b.ps_log2));
         if (seen > 0) zero(0, seen);
-        return true;
       };
       const uint64_t dq = umma_desc_k_sw128(sb + qb * C::kTile);
       auto qk = [&](int i) {
+        any = true;
         const unsigned u = (steps + i) & 1;
         const uint64_t dk = umma_desc_k_sw128(ring + kslot * C::kTile + half_of(i));
 #pragma unroll
@@ -835,16 +876,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       // a buffer of S is free again once the product that reads P from it is issued: they execute in order
-      for (int i = 0; i < min(n, 2) && (ok = take_k(i)); ++i) {
+      for (int i = 0; i < min(n, 2); ++i) {
+        take_k(i);
         tc_fence_after();
         qk(i);
       }
-      for (int i = 0; i < n && ok; ++i) {
+      for (int i = 0; i < n; ++i) {
         const unsigned step = steps + i, u = step & 1;
-        if (!(ok = take_v(i) && (i + 2 >= n || take_k(i + 2)))) break;
-        if (i == 0 && pieces && !(ok = mbar_wait(&o_free, (pieces - 1) & 1, status))) break;
+        take_v(i);
+        if (i + 2 < n) take_k(i + 2);
+        if (i == 0 && pieces) wait(&o_free, (pieces - 1) & 1);
         const uint64_t dv = umma_desc_sw128(ring + vslot * C::kTile + half_of(i), kBlk, 1024);
-        if (!(ok = mbar_wait(&p_full[p][u], (step >> 1) & 1, status))) break;
+        wait(&p_full[p][u], (step >> 1) & 1);
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < kST / 16; ++kk)
@@ -857,7 +900,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++pieces;
       if (!two) buf ^= 1;
     }
-    if (!ok) *abort_flag = 1;
+    if (any) {  // nor while a product may still be reading
+      umma_commit_if(e, &idle[p]);
+      bounded_wait(&idle[p], 0, a.full, &s_late, a.status);
+    }
   }
   }
   tc_fence_before();
@@ -955,6 +1001,8 @@ cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cuda
   p.x = Axis{2 * qb, a.window < (1 << 22) ? a.window : 1 << 22, K};
   p.out = a.out;
   p.out_stride = a.out_stride;
+  p.budget = budget_of(a.wait_budget);
+  p.full = budget_of(kWaitBudgetCycles);
   p.c = a.scale * 1.4426950408889634f;
   p.gq = gq;
   p.oob = (int)rows;

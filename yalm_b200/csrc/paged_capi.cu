@@ -93,6 +93,8 @@ int device_sms(int dev) {
   return n;
 }
 
+std::atomic<long long> wait_budget{kWaitBudgetCycles};
+
 }  // namespace
 
 extern "C" int yb_paged_append_dev(const yb_paged_batch* b, void* q_out, long long q_out_stride, const void* qkv,
@@ -149,6 +151,13 @@ extern "C" size_t yb_paged_attention_scratch_bytes(const yb_paged_batch* b) {
   return paged_attention_scratch(b->head_dim, device_sms(dev));
 }
 
+extern "C" int yb_paged_attention_wait_budget(long long clocks) {
+  if (clocks < 0 || clocks > kWaitBudgetCycles) return set_error(YB_E_INVALID, "the wait budget must be 0 (the default) to " +
+                                                                                   std::to_string(kWaitBudgetCycles) + " clocks");
+  wait_budget.store(clocks ? clocks : kWaitBudgetCycles, std::memory_order_relaxed);
+  return 0;
+}
+
 extern "C" int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long long out_stride, const void* q,
                                       long long q_stride, float scale, int window, void* scratch_dev, void* stream) {
   PagedAttnArgs a{};
@@ -176,6 +185,7 @@ extern "C" int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long l
   a.scale = scale;
   a.window = window ? window : INT_MAX;
   a.scratch = scratch_dev;
+  a.wait_budget = wait_budget.load(std::memory_order_relaxed);
   YB_CK(paged_attention(a, b->head_dim, b->dtype, dev, device_sms(dev), static_cast<cudaStream_t>(stream)));
   return 0;
 }
