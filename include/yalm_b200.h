@@ -358,9 +358,9 @@ int yb_paged_append_dev(const yb_paged_batch* b, void* q_out, long long q_out_st
  * finite values: one that does not may spoil the rows of tokens before it, too.
  * scratch_dev: yb_paged_attention_scratch_bytes(b) bytes (the same for every batch of this head_dim on a
  * device), 16-byte aligned; its contents have no meaning between calls.  Calls that may run at the same
- * time, replayed graphs among them, each need their own.  Its first word takes status bits as yb_status
- * has them when a bounded wait in the kernel runs out (set it to zero before to tell); the output is then
- * not complete.  Results do not depend on timing, but on the number of SMs, which decides where a long
+ * time, replayed graphs among them, each need their own.  Its first word collects status bits as yb_status
+ * has them when a bounded wait in the kernel runs out (set it to zero once, and after it was seen set, to tell); the
+ * call's output is then not complete, and the next call in the same workspace is as good as any.  Results do not depend on timing, but on the number of SMs, which decides where a long
  * cache is cut. */
 int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long long out_stride, const void* q,
                            long long q_stride, float scale, int window, void* scratch_dev, void* stream);

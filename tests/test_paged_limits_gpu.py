@@ -46,3 +46,29 @@ def test_a_wait_that_runs_out_ends_the_call(gpu, wait_budget, new, kv, nh, nkv, 
         word.zero_()
         assert torch.equal(s.attend(scratch=scratch, batch=b).double(), want)
         assert int(word) == 0
+
+
+def test_status_tells_of_a_wait_that_ran_out(gpu, wait_budget):
+    """Of any of the calls since the last look, on any stream, captured ones too."""
+    import torch
+    s = Step([40, 1], [300, 200], 8, 2, 64, 32, "f16", seed=92)
+    b = s.batch()
+    scratch = torch.zeros(b.scratch_bytes(), dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(s.q)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    wait_budget(1)
+    b.attend(s.q, out, scratch, stream=side.cuda_stream)
+    wait_budget(0)
+    b.attend(s.q, out, scratch, stream=side.cuda_stream)
+    assert b.status(scratch) == 1
+    assert b.status(scratch) == 0
+    wait_budget(1)
+    with torch.cuda.graph(graph):
+        b.attend(s.q, out, scratch, stream=torch.cuda.current_stream().cuda_stream)
+    wait_budget(0)
+    assert b.status(scratch) == 0
+    graph.replay()
+    assert b.status(scratch) == 1
+    s.check(scratch=scratch, batch=b)
+    assert b.status(scratch) == 0

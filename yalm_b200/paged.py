@@ -96,20 +96,41 @@ class PagedBatch:
             1 if half else 0, self._vector(pos, "pos", self.n_tokens, self._i32), clip, stream))
 
     def scratch_bytes(self) -> int:
-        """Size of attend's workspace: one for each stream of calls, its contents of no meaning between calls."""
+        """Size of attend's workspace: one for each stream of calls.  Its first word collects status bits, so it is
+        to start as zeros; the rest has no meaning between calls."""
         if not self._scratch:
             self._scratch = _lib.lib().yb_paged_attention_scratch_bytes(self._ref)
             if not self._scratch:
                 raise _lib.YalmB200Error(_lib.YB_E_INVALID, _lib.last_error())
         return self._scratch
 
-    def attend(self, q, out, scratch, *, scale: float | None = None, window: int = 0, stream: int = 0) -> None:
-        """yb_paged_attention_dev: causal attention of q [n_tokens][n_heads * head_dim] over the caches."""
-        s_q, s_out = self._rows(q, "q", self._q_shape), self._rows(out, "out", self._q_shape)
-        if q.dtype != self._dtype or out.dtype != self._dtype:
-            raise ValueError("q and out must have the caches' type")
+    def _check_scratch(self, scratch) -> None:
         if scratch.get_device() != self._index or not scratch.is_contiguous() or \
                 scratch.numel() * scratch.element_size() < (self._scratch or self.scratch_bytes()):
             raise ValueError("scratch must hold scratch_bytes() contiguous bytes")
+
+    def status(self, scratch) -> int:
+        """Waits for the device and returns the status bits (as Model.status) of the attend calls in this workspace
+        since the last look, or since it was made of zeros: 0, or their outputs are not complete.  Clears them.  Not
+        for a stream that is being captured."""
+        import torch
+        self._check_scratch(scratch)
+        if scratch.is_cuda:
+            torch.cuda.synchronize(scratch.device)
+        word = scratch.view(-1).view(torch.uint8)[:4].view(torch.int32)
+        bits = int(word.item()) & 0xFFFFFFFF
+        if bits:
+            word.zero_()
+            if scratch.is_cuda:  # before a call on any stream
+                torch.cuda.synchronize(scratch.device)
+        return bits
+
+    def attend(self, q, out, scratch, *, scale: float | None = None, window: int = 0, stream: int = 0) -> None:
+        """yb_paged_attention_dev: causal attention of q [n_tokens][n_heads * head_dim] over the caches.  The launch
+        is not waited for; a wait inside it that runs out is told by status()."""
+        s_q, s_out = self._rows(q, "q", self._q_shape), self._rows(out, "out", self._q_shape)
+        if q.dtype != self._dtype or out.dtype != self._dtype:
+            raise ValueError("q and out must have the caches' type")
+        self._check_scratch(scratch)
         _lib.check(self._attend(self._ref, out.data_ptr(), s_out, q.data_ptr(), s_q,
                                 self._scale if scale is None else scale, window, scratch.data_ptr(), stream))
