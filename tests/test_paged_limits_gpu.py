@@ -72,3 +72,37 @@ def test_status_tells_of_a_wait_that_ran_out(gpu, wait_budget):
     assert b.status(scratch) == 1
     s.check(scratch=scratch, batch=b)
     assert b.status(scratch) == 0
+
+
+def test_calls_without_a_stream_run_on_torchs_current_one(gpu):
+    """Inside torch.cuda.stream() and inside a capture; a long kernel before them holds their inputs back."""
+    import torch
+    s = Step([40, 1], [300, 200], 8, 2, 64, 32, "f16", seed=93)
+    b, want = s.batch(), s.check()
+    scratch = torch.zeros(b.scratch_bytes(), dtype=torch.uint8, device="cuda")
+    q, out = torch.zeros_like(s.q), torch.empty_like(s.q)
+    qkv, rows = torch.zeros(s.n, 768, device="cuda"), torch.randn(s.n, 768, device="cuda")
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        q.copy_(s.q)
+        b.attend(q, out, scratch)
+        side.synchronize()
+        assert torch.equal(out.double(), want)
+        torch.cuda._sleep(50_000_000)
+        qkv.copy_(rows)
+        b.append(qkv, out, None, 0)
+        side.synchronize()
+        assert torch.equal(out, rows[:, :512].half())
+    out.zero_()
+    with torch.cuda.graph(graph):
+        b.append(qkv, q, None, 0)
+        b.attend(q, out, scratch)
+    torch.cuda.synchronize()
+    assert not out.any()
+    graph.replay()
+    torch.cuda.synchronize()
+    s.q = q
+    ref, tol = s.attend64()
+    assert ((out.double() - ref).abs() <= tol).all()

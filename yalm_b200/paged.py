@@ -26,7 +26,8 @@ def _dtype(t, name: str) -> int:
 class PagedBatch:
     """k_pages, v_pages [n_pages][n_kv_heads][page_size][head_dim] fp16 or bf16; page_table [n_seqs][max_pages],
     q_start [n_seqs + 1] and kv_len [n_seqs] int32; n_tokens: rows of the token-major tensors.  All on one
-    GPU, contiguous.  The calls launch on `stream`, a cudaStream_t as an integer (0: the default stream)."""
+    GPU, contiguous.  The calls launch on `stream`, a cudaStream_t as an integer (0: the legacy default stream), or
+    without it on torch's current stream of that GPU."""
 
     def __init__(self, k_pages, v_pages, page_table, q_start, kv_len, n_heads: int, n_tokens: int):
         if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
@@ -60,6 +61,7 @@ class PagedBatch:
         self._index = k_pages.get_device()
         import torch  # the caller's tensors are torch's; the package itself does not need it
         self._f32, self._i32 = torch.float32, torch.int32
+        self._current = torch.cuda.current_stream
         self._q_shape = (self.n_tokens, self.n_heads * self.head_dim)
         self._qkv_shape = (self.n_tokens, (self.n_heads + 2 * self.n_kv_heads) * self.head_dim)
 
@@ -70,6 +72,9 @@ class PagedBatch:
             raise ValueError(f"{name} must be [{shape[0]}][{shape[1]}] with unit column stride on {self.device}")
         return row if self.n_tokens > 1 else shape[1]
 
+    def _stream(self) -> int:
+        return self._current(self._index).cuda_stream if self._index >= 0 else 0
+
     def _vector(self, t, name: str, n: int, dtype):
         """Checks an optional vector and returns its address."""
         if t is None:
@@ -79,7 +84,7 @@ class PagedBatch:
         return t.data_ptr()
 
     def append(self, qkv, q_out, inv_freq, rotary_dim: int, *, q_norm=None, k_norm=None, eps: float = 1e-5,
-               half: bool = False, pos=None, clip: float = FLT_MAX, stream: int = 0) -> None:
+               half: bool = False, pos=None, clip: float = FLT_MAX, stream: int | None = None) -> None:
         """yb_paged_append_dev: clip, norm and rotate qkv [n_tokens][(n_heads + 2 n_kv_heads) head_dim], queries to
         q_out, keys and values into their pages."""
         src = self._codes.get(qkv.dtype)
@@ -93,7 +98,8 @@ class PagedBatch:
             self._vector(q_norm, "q_norm", self.head_dim, self._f32),
             self._vector(k_norm, "k_norm", self.head_dim, self._f32), eps,
             self._vector(inv_freq if rotary_dim else None, "inv_freq", rotary_dim // 2, self._f32), rotary_dim,
-            1 if half else 0, self._vector(pos, "pos", self.n_tokens, self._i32), clip, stream))
+            1 if half else 0, self._vector(pos, "pos", self.n_tokens, self._i32), clip,
+            self._stream() if stream is None else stream))
 
     def scratch_bytes(self) -> int:
         """Size of attend's workspace: one for each stream of calls.  Its first word collects status bits, so it is
@@ -125,7 +131,8 @@ class PagedBatch:
                 torch.cuda.synchronize(scratch.device)
         return bits
 
-    def attend(self, q, out, scratch, *, scale: float | None = None, window: int = 0, stream: int = 0) -> None:
+    def attend(self, q, out, scratch, *, scale: float | None = None, window: int = 0,
+               stream: int | None = None) -> None:
         """yb_paged_attention_dev: causal attention of q [n_tokens][n_heads * head_dim] over the caches.  The launch
         is not waited for; a wait inside it that runs out is told by status()."""
         s_q, s_out = self._rows(q, "q", self._q_shape), self._rows(out, "out", self._q_shape)
@@ -133,4 +140,5 @@ class PagedBatch:
             raise ValueError("q and out must have the caches' type")
         self._check_scratch(scratch)
         _lib.check(self._attend(self._ref, out.data_ptr(), s_out, q.data_ptr(), s_q,
-                                self._scale if scale is None else scale, window, scratch.data_ptr(), stream))
+                                self._scale if scale is None else scale, window, scratch.data_ptr(),
+                                self._stream() if stream is None else stream))
