@@ -322,8 +322,7 @@ typedef struct yb_paged_batch {
   int dtype;      /* of the caches, q and out: YB_DTYPE_F16 or YB_DTYPE_BF16 */
   int page_size;  /* 16, 32, 64, 128 or 256 */
   int n_pages;    /* pages in each cache */
-  int max_pages;  /* row length of page_table; max_pages * page_size up to 2^21 (less for more than
-                     2^16 sequences times 64 kv heads, whose key tiles would overflow a count) */
+  int max_pages;  /* row length of page_table; max_pages * page_size up to 2^21 */
   const int* q_start_dev;    /* [n_seqs + 1] */
   const int* kv_len_dev;     /* [n_seqs] */
   const int* page_table_dev; /* [n_seqs][max_pages] */
@@ -361,7 +360,9 @@ int yb_paged_append_dev(const yb_paged_batch* b, void* q_out, long long q_out_st
  * time, replayed graphs among them, each need their own.  Its first word collects status bits as yb_status
  * has them when a bounded wait in the kernel runs out (set it to zero once, and after it was seen set, to tell); the
  * call's output is then not complete, and the next call in the same workspace is as good as any.  Results do not depend on timing, but on the number of SMs, which decides where a long
- * cache is cut. */
+ * cache is cut.  Refused (YB_E_UNSUPPORTED) is a batch whose share of work for one SM may not be counted in 31 bits: with
+ * U = 2 * floor(128 * n_kv_heads / n_heads) queries a unit, (n_tokens / U + min(n_seqs, n_tokens)) * n_kv_heads *
+ * (max_pages * page_size / 128 + 3) from 2^31 - 1 times the SMs on. */
 int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long long out_stride, const void* q,
                            long long q_stride, float scale, int window, void* scratch_dev, void* stream);
 size_t yb_paged_attention_scratch_bytes(const yb_paged_batch* b); /* 0 for a batch that is refused */

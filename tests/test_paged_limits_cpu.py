@@ -1,4 +1,6 @@
 """Refusals of the paged-cache entry points beyond those of test_paged_cpu.py, and what the class hands to them; no GPU."""
+import ctypes
+
 from yalm_b200 import _lib
 
 
@@ -31,3 +33,46 @@ def test_status_reads_and_clears_the_workspaces_first_word():
         assert (scratch.view(-1).view(torch.uint8)[4:8] == 255).all()  # the word alone
     with pytest.raises(ValueError):
         b.status(torch.zeros(b.scratch_bytes() - 1, dtype=torch.uint8))
+
+
+P = 4096  # an aligned address that nothing reads
+
+
+def _descriptor(**kw):
+    c = dict(n_seqs=2, n_tokens=5, n_heads=8, n_kv_heads=2, head_dim=64, dtype=1, page_size=16, n_pages=9, max_pages=4,
+             q_start_dev=P, kv_len_dev=P, page_table_dev=P, k_pages=P, v_pages=P)
+    c.update(kw)
+    return _lib.yb_paged_batch(**c)
+
+
+def _append(b, width, **kw):
+    c = dict(q_out=P, q_out_stride=width, qkv=P, qkv_stride=3 * width, qkv_dtype=0, q_norm=None, k_norm=None, eps=1e-5,
+             inv_freq=P, rotary_dim=64, half=0, pos=None, clip=3e38)
+    c.update(kw)
+    return _lib.lib().yb_paged_append_dev(ctypes.byref(b), *c.values(), None)
+
+
+def _attend(b, width, **kw):
+    c = dict(out=P, out_stride=width, q=P, q_stride=width, scale=0.125, window=0, scratch=P)
+    c.update(kw)
+    return _lib.lib().yb_paged_attention_dev(ctypes.byref(b), *c.values(), None)
+
+
+def test_the_attentions_limit_of_work_is_the_documented_one_and_its_own():
+    """At the limit the call passes on to the buffers' check (these are no device memory), one unit more is refused.
+    The append has no such limit."""
+    L = _lib.lib()
+    sms = L.yb_num_sms() or 148
+    H = 512  # a kv head a query head: units of 256 queries
+    tiles = (1 << 21) // 128 + 3
+    last = (sms * (2 ** 31 - 1) - 1) // (H * tiles)  # units
+    for units, refused in ((last, False), (last + 1, True), (60000, True)):
+        n = next(n for n in range(units, 0, -1) if n // 256 + n <= units)  # as many sequences as tokens
+        rest = units - n // 256 - n
+        b = _descriptor(n_seqs=n + rest, n_tokens=n + rest, n_heads=H, n_kv_heads=H, max_pages=(1 << 21) // 16)
+        assert (n + rest) // 256 + n + rest == units
+        rc = _attend(b, H * 64)
+        assert (rc == _lib.YB_E_UNSUPPORTED) == refused and rc != 0
+        assert ("too many slots" in _lib.last_error()) == refused
+        assert (L.yb_paged_attention_scratch_bytes(ctypes.byref(b)) == 0) == refused
+        assert _append(b, H * 64) not in (0, _lib.YB_E_UNSUPPORTED)

@@ -97,6 +97,7 @@ struct PagedAttnArgs {
   long long wait_budget;  // clocks after which a wait in the kernel gives up
   void* scratch;
 };
+int paged_attention_grid(int n_sms);  // blocks
 size_t paged_attention_scratch(int head_dim, int n_sms);
 cudaError_t paged_attention(const PagedAttnArgs& a, int head_dim, int type, int device, int n_sms, cudaStream_t s);
 

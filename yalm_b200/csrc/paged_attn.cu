@@ -980,8 +980,10 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
   }
 }
 
+int paged_attention_grid(int n_sms) { return n_sms < kMaxGrid ? n_sms : kMaxGrid; }
+
 size_t paged_attention_scratch(int head_dim, int n_sms) {
-  const int grid = n_sms < kMaxGrid ? n_sms : kMaxGrid;
+  const int grid = paged_attention_grid(n_sms);
   return kHeadBytes + (size_t)grid * 2 * (head_dim == 128 ? rec_floats<128>() : rec_floats<64>()) * 4;
 }
 
@@ -1024,7 +1026,7 @@ cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cuda
 }  // namespace
 
 cudaError_t paged_attention(const PagedAttnArgs& a, int head_dim, int type, int device, int n_sms, cudaStream_t s) {
-  const int grid = n_sms < kMaxGrid ? n_sms : kMaxGrid;
+  const int grid = paged_attention_grid(n_sms);
   if (head_dim == 128)
     return type == 1 ? launch<128, __half>(a, device, grid, false, s) : launch<128, __nv_bfloat16>(a, device, grid, true, s);
   return type == 1 ? launch<64, __half>(a, device, grid, false, s) : launch<64, __nv_bfloat16>(a, device, grid, true, s);

@@ -33,10 +33,6 @@ int check_batch(const yb_paged_batch* b, PagedBatch* out, bool* empty) {
     return set_error(YB_E_UNSUPPORTED, "at most 65536 sequences, 2^20 new tokens and 2^21 slots per sequence");
   if (((long long)b->n_pages * b->n_kv_heads << lg) > INT_MAX - 256)
     return set_error(YB_E_UNSUPPORTED, "the page pool has too many rows (n_pages * n_kv_heads * page_size)");
-  // the key tiles of 128 slots that one of 64 or more blocks may have to walk are counted in 32 bits
-  const long long units = b->n_tokens / (2 * (128 / (b->n_heads / b->n_kv_heads))) + (b->n_seqs < b->n_tokens ? b->n_seqs : b->n_tokens);
-  if (units * b->n_kv_heads * ((((long long)b->max_pages << lg) >> 7) + 3) > (1ll << 37))
-    return set_error(YB_E_UNSUPPORTED, "the batch may have too many slots to attend to (n_seqs * n_kv_heads * max_pages * page_size)");
   *empty = b->n_seqs == 0 || b->n_tokens == 0;  // its buffers of no elements may be null
   if (!b->k_pages || !b->v_pages || (!*empty && (!b->q_start_dev || !b->kv_len_dev || !b->page_table_dev)))
     return set_error(YB_E_INVALID, "null buffer in the batch");
@@ -93,6 +89,29 @@ int device_sms(int dev) {
   return n;
 }
 
+// What one of the attention's blocks may have to walk is counted in 31 bits: the units (blocks of up to 2 * (128 /
+// query heads per kv head) queries) of every sequence and kv head, with the key tiles of 128 slots of the longest cache
+// and 3 more each, shared out over the blocks.
+int check_share(const yb_paged_batch* b, const PagedBatch& p, int dev) {
+  const long long queries = 2 * (128 / (b->n_heads / b->n_kv_heads));
+  const long long units = b->n_tokens / queries + (b->n_seqs < b->n_tokens ? b->n_seqs : b->n_tokens);
+  const long long tiles = (((long long)b->max_pages << p.ps_log2) >> 7) + 3;
+  if (units * b->n_kv_heads * tiles / paged_attention_grid(device_sms(dev)) >= INT_MAX)
+    return set_error(YB_E_UNSUPPORTED, "the batch may have too many slots to attend to on this device "
+                                       "((n_tokens / queries of a unit + n_seqs) * n_kv_heads * max_pages * page_size)");
+  return 0;
+}
+
+// The current device, or -1 where there is none (sizes can be asked for without one).
+int current_device() {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  return dev;
+}
+
 std::atomic<long long> wait_budget{kWaitBudgetCycles};
 
 }  // namespace
@@ -143,11 +162,8 @@ extern "C" size_t yb_paged_attention_scratch_bytes(const yb_paged_batch* b) {
   PagedBatch p;
   bool empty;
   if (check_batch(b, &p, &empty)) return 0;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) {
-    cudaGetLastError();
-    dev = -1;
-  }
+  const int dev = current_device();
+  if (check_share(b, p, dev)) return 0;
   return paged_attention_scratch(b->head_dim, device_sms(dev));
 }
 
@@ -170,6 +186,7 @@ extern "C" int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long l
   if (window < 0) return set_error(YB_E_INVALID, "negative window");
   if (!scratch_dev || !aligned16(scratch_dev)) return set_error(YB_E_INVALID, "scratch_dev must be 16-byte aligned memory");
   if (empty) return 0;
+  if ((rc = check_share(b, a.b, current_device()))) return rc;
   int dev = 0;
   YB_CK(cudaGetDevice(&dev));
   rc = check_device(dev, {{"out", out}, {"q", q}, {"q_start_dev", b->q_start_dev}, {"kv_len_dev", b->kv_len_dev},
