@@ -332,7 +332,7 @@ typedef struct yb_paged_batch {
 
 /* Both entry points run on the current device and refuse (YB_E_INVALID) buffers that are not its memory.
  * Rows of q, q_out, out and qkv are given by their strides in elements; base addresses and row
- * strides must be multiples of 16 bytes.  No buffer that is written may overlap another one. */
+ * strides must be multiples of 16 bytes, the addresses of ints and floats of 4.  No buffer that is written may overlap another one. */
 
 /* One pass over the new tokens' projections, the epilogue that yb_qkv_dev has for one token: qkv rows
  * [n_heads query heads | n_kv_heads key heads | n_kv_heads value heads], of qkv_dtype (YB_DTYPE_*).

@@ -1,6 +1,8 @@
 """Refusals of the paged-cache entry points beyond those of test_paged_cpu.py, and what the class hands to them; no GPU."""
 import ctypes
 
+import pytest
+
 from yalm_b200 import _lib
 
 
@@ -22,7 +24,6 @@ def _batch():
 
 
 def test_status_reads_and_clears_the_workspaces_first_word():
-    import pytest
     import torch
     b = _batch()
     for scratch in (torch.zeros(b.scratch_bytes(), dtype=torch.uint8), torch.zeros(2, b.scratch_bytes(), dtype=torch.int32)):
@@ -76,3 +77,21 @@ def test_the_attentions_limit_of_work_is_the_documented_one_and_its_own():
         assert ("too many slots" in _lib.last_error()) == refused
         assert (L.yb_paged_attention_scratch_bytes(ctypes.byref(b)) == 0) == refused
         assert _append(b, H * 64) not in (0, _lib.YB_E_UNSUPPORTED)
+
+
+@pytest.mark.parametrize("name", ["q_start_dev", "kv_len_dev", "page_table_dev"])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_misaligned_lengths_and_tables_are_refused(name, off):
+    """A word read at such an address would end the context."""
+    b = _descriptor(**{name: P + off})
+    for call in (_append, _attend):
+        assert call(b, 512) == _lib.YB_E_INVALID
+        assert "4-byte aligned" in _lib.last_error()
+    assert _lib.lib().yb_paged_attention_scratch_bytes(ctypes.byref(b)) == 0
+
+
+@pytest.mark.parametrize("name", ["q_norm", "k_norm", "inv_freq", "pos"])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_misaligned_vectors_are_refused(name, off):
+    assert _append(_descriptor(), 512, **{name: P + off}) == _lib.YB_E_INVALID
+    assert "4-byte aligned" in _lib.last_error()

@@ -13,6 +13,7 @@ using namespace yb;
 namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
 // Shapes and NULLs, before any CUDA call.  *empty: nothing to do.
 int check_batch(const yb_paged_batch* b, PagedBatch* out, bool* empty) {
@@ -38,6 +39,8 @@ int check_batch(const yb_paged_batch* b, PagedBatch* out, bool* empty) {
     return set_error(YB_E_INVALID, "null buffer in the batch");
   if (!aligned16(b->k_pages) || !aligned16(b->v_pages))
     return set_error(YB_E_INVALID, "k_pages and v_pages must be 16-byte aligned");
+  if (!aligned4(b->q_start_dev) || !aligned4(b->kv_len_dev) || !aligned4(b->page_table_dev))
+    return set_error(YB_E_INVALID, "q_start_dev, kv_len_dev and page_table_dev must be 4-byte aligned");
   out->q_start = b->q_start_dev;
   out->kv_len = b->kv_len_dev;
   out->page_table = b->page_table_dev;
@@ -131,6 +134,8 @@ extern "C" int yb_paged_append_dev(const yb_paged_batch* b, void* q_out, long lo
   if (rotary_dim < 0 || rotary_dim > hd || rotary_dim % 2 || (rope_half && rotary_dim % 8))
     return set_error(YB_E_INVALID, "rotary_dim must be even and <= head_dim (a multiple of 8 for half-split pairs)");
   if (rotary_dim && !inv_freq_dev) return set_error(YB_E_INVALID, "null inv_freq_dev");
+  if (!aligned4(q_norm_dev) || !aligned4(k_norm_dev) || !aligned4(inv_freq_dev) || !aligned4(pos_dev))
+    return set_error(YB_E_INVALID, "q_norm_dev, k_norm_dev, inv_freq_dev and pos_dev must be 4-byte aligned");
   if (!(eps >= 0.f) || !(qkv_clip > 0.f)) return set_error(YB_E_INVALID, "eps must be >= 0 and qkv_clip > 0");
   if (empty) return 0;
   int dev = 0;
