@@ -355,6 +355,7 @@ int yb_paged_append_dev(const yb_paged_batch* b, void* q_out, long long q_out_st
  * the window of the sequence's first new token, and pages that are not there may hold anything, NaN
  * included (pages that have left the window may be given to other sequences); the slots between hold
  * finite values: one that does not may spoil the rows of tokens before it, too.
+ * scale is positive, and scale * log2(e) and its products with the sums q.k have to stay in fp32's range.
  * scratch_dev: yb_paged_attention_scratch_bytes(b) bytes (the same for every batch of this head_dim on a
  * device), 16-byte aligned; its contents have no meaning between calls.  Calls that may run at the same
  * time, replayed graphs among them, each need their own.  Its first word collects status bits as yb_status

@@ -95,3 +95,11 @@ def test_misaligned_lengths_and_tables_are_refused(name, off):
 def test_misaligned_vectors_are_refused(name, off):
     assert _append(_descriptor(), 512, **{name: P + off}) == _lib.YB_E_INVALID
     assert "4-byte aligned" in _lib.last_error()
+
+
+def test_scales_that_overflow_are_refused():
+    """The kernel's factor is scale * log2(e)."""
+    for scale in (3e38, 2.4e38):
+        assert _attend(_descriptor(), 512, scale=scale) == _lib.YB_E_INVALID
+        assert "scale" in _lib.last_error()
+    assert _attend(_descriptor(n_tokens=0), 512, scale=2.3e38) == 0

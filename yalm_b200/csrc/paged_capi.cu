@@ -187,7 +187,8 @@ extern "C" int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long l
   if (rc) return rc;
   const long long width = (long long)b->n_heads * b->head_dim;
   if ((rc = check_rows("out", out, out_stride, width, 2, empty)) || (rc = check_rows("q", q, q_stride, width, 2, empty))) return rc;
-  if (!(scale > 0.f) || !std::isfinite(scale)) return set_error(YB_E_INVALID, "scale must be positive and finite");
+  if (!(scale > 0.f) || !std::isfinite(scale * 1.4426950408889634f))
+    return set_error(YB_E_INVALID, "scale must be positive, and scale * log2(e) finite");
   if (window < 0) return set_error(YB_E_INVALID, "negative window");
   if (!scratch_dev || !aligned16(scratch_dev)) return set_error(YB_E_INVALID, "scratch_dev must be 16-byte aligned memory");
   if (empty) return 0;
