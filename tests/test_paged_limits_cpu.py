@@ -103,3 +103,25 @@ def test_scales_that_overflow_are_refused():
         assert _attend(_descriptor(), 512, scale=scale) == _lib.YB_E_INVALID
         assert "scale" in _lib.last_error()
     assert _attend(_descriptor(n_tokens=0), 512, scale=2.3e38) == 0
+
+
+@pytest.mark.parametrize("window,handed", [(0, 0), (5, 5), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 31, 2 ** 31 - 1),
+                                           (2 ** 32, 2 ** 31 - 1), (2 ** 32 + 5, 2 ** 31 - 1), (10 ** 30, 2 ** 31 - 1)])
+def test_windows_wider_than_an_int_see_everything(window, handed):
+    """A C int would take their low bits: 2^32 + 5 as a window of 5."""
+    import torch
+    b = _batch()
+    seen = []
+    b._attend = lambda *a: seen.append(ctypes.c_int(a[6]).value) or 0
+    q = torch.zeros(4, 512, dtype=torch.float16)
+    b.attend(q, q.clone(), torch.zeros(b.scratch_bytes(), dtype=torch.uint8), window=window)
+    assert seen == [handed]
+
+
+@pytest.mark.parametrize("window", [-1, -2 ** 31, -2 ** 32 + 5, -2 ** 32])
+def test_negative_windows_are_refused(window):
+    import torch
+    b = _batch()
+    q = torch.zeros(4, 512, dtype=torch.float16)
+    with pytest.raises(_lib.YalmB200Error):
+        b.attend(q, q.clone(), torch.zeros(b.scratch_bytes(), dtype=torch.uint8), window=window)

@@ -139,6 +139,7 @@ class PagedBatch:
         if q.dtype != self._dtype or out.dtype != self._dtype:
             raise ValueError("q and out must have the caches' type")
         self._check_scratch(scratch)
+        window = max(-1, min(window, 0x7FFFFFFF))  # a C int; what is wider than any cache sees all of it
         _lib.check(self._attend(self._ref, out.data_ptr(), s_out, q.data_ptr(), s_q,
                                 self._scale if scale is None else scale, window, scratch.data_ptr(),
                                 self._stream() if stream is None else stream))
