@@ -125,3 +125,14 @@ def test_negative_windows_are_refused(window):
     q = torch.zeros(4, 512, dtype=torch.float16)
     with pytest.raises(_lib.YalmB200Error):
         b.attend(q, q.clone(), torch.zeros(b.scratch_bytes(), dtype=torch.uint8), window=window)
+
+
+def test_inputs_are_read_by_coherent_loads():
+    """The kernels start while the one before them may still be writing lengths, tables and rows (programmatic launch);
+    non-coherent loads need memory that nothing writes while the kernel lives, wherever in the kernel they stand."""
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(_lib.__file__), "csrc")
+    for name in ("paged.cuh", "paged_append.cu", "paged_attn.cu"):
+        code = re.sub(r"//.*", "", open(os.path.join(csrc, name)).read())
+        assert not re.search(r"__ldg\b|ld\.global\.nc|__restrict__", code), name

@@ -106,3 +106,45 @@ def test_calls_without_a_stream_run_on_torchs_current_one(gpu):
     s.q = q
     ref, tol = s.attend64()
     assert ((out.double() - ref).abs() <= tol).all()
+
+
+def test_steps_whose_lengths_are_advanced_on_the_device(gpu):
+    """A captured step that begins by writing its own lengths and pages, replayed through page borders."""
+    import torch
+    nh, nkv, hd, ps, steps = 8, 2, 64, 16, 40
+    s = Step([0, 0, 0], [5, 47, 130], nh, nkv, hd, ps, "f16", seed=94, spare=12)
+    width = s.page_table.shape[1] + 4
+    used = {p for t in s.table for p in t}
+    free = [p for p in range(s.n_pages) if p not in used]
+    full = [[p for p in t if p >= 0] for t in s.table]
+    for t, m in zip(full, s.kv):
+        while len(t) < -(-(m + steps) // ps):
+            t.append(free.pop())
+    table = torch.tensor([t + [-1] * (width - len(t)) for t in full], dtype=torch.int32, device="cuda")
+    s.page_table = torch.full_like(table, -1)
+    s.n, s.new, s.starts = 3, [1, 1, 1], [0, 1, 2, 3]
+    s.q_start = torch.zeros(4, dtype=torch.int32, device="cuda")
+    b = s.batch()
+    qkv = torch.zeros(3, (nh + 2 * nkv) * hd, device="cuda")
+    s.q = torch.zeros(3, nh * hd, device="cuda").half()
+    out, scratch = torch.zeros_like(s.q), torch.zeros(b.scratch_bytes(), dtype=torch.uint8, device="cuda")
+    rows = torch.randn(steps, *qkv.shape, generator=s.g, device="cuda")
+    one, starts = torch.ones_like(s.kv_len), torch.arange(4, dtype=torch.int32, device="cuda")
+    at = torch.arange(width, device="cuda")[None] * ps
+    graph = torch.cuda.CUDAGraph()
+    kv = s.kv_len.clone()
+    with torch.cuda.graph(graph):
+        s.q_start.copy_(starts)
+        s.page_table.copy_(torch.where(at <= s.kv_len[:, None], table, -1))
+        s.kv_len.add_(one)
+        b.append(qkv, s.q, None, 0)
+        b.attend(s.q, out, scratch)
+    assert torch.equal(s.kv_len, kv)
+    for i in range(steps):
+        qkv.copy_(rows[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        s.kv = [m + 1 for m in s.kv]
+        ref, tol = s.attend64()
+        assert ((out.double() - ref).abs() <= tol).all(), i
+    assert b.status(scratch) == 0

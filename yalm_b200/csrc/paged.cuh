@@ -25,7 +25,9 @@ struct SmemCap {
 
 // The batch as the kernels see it (include/yalm_b200.h, yb_paged_batch).  The lengths and the table are
 // read on the device, so a captured launch follows them; every index made from them is clamped to
-// the buffers' bounds here, whatever they hold.
+// the buffers' bounds here, whatever they hold.  What the caller may have written just before is read by ordinary
+// loads (__ldca), after griddepcontrol.wait: the kernels may be resident while the one before them still writes, and
+// non-coherent loads (__ldg) are for what stays as it is as long as a kernel lives.
 struct PagedBatch {
   const int* q_start;     // [n_seqs + 1] first row of each sequence's new tokens
   const int* kv_len;      // [n_seqs] slots in the sequence's cache, the new tokens among them
@@ -43,9 +45,9 @@ struct PagedSeq {
 };
 __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int s) {
   PagedSeq r;
-  r.row0 = min(max(__ldg(b.q_start + s), 0), b.n_tokens);
-  r.n = min(max(__ldg(b.q_start + s + 1), r.row0), b.n_tokens) - r.row0;
-  r.kv = min(max(__ldg(b.kv_len + s), 0), b.max_pages << b.ps_log2);
+  r.row0 = min(max(__ldca(b.q_start + s), 0), b.n_tokens);
+  r.n = min(max(__ldca(b.q_start + s + 1), r.row0), b.n_tokens) - r.row0;
+  r.kv = min(max(__ldca(b.kv_len + s), 0), b.max_pages << b.ps_log2);
   return r;
 }
 
@@ -58,7 +60,7 @@ __device__ __forceinline__ int paged_find_seq(const PagedBatch& b, int row) {
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32;
     const int at = lo + (lane + 1) * step;  // 32 probes, ascending
-    const bool le = at < hi && __ldg(b.q_start + at) <= row;
+    const bool le = at < hi && __ldca(b.q_start + at) <= row;
     const int c = __popc(__ballot_sync(0xffffffffu, le));
     const int nlo = lo + c * step;
     hi = min(hi, nlo + step);

@@ -123,9 +123,9 @@ __global__ void __launch_bounds__(kThreads, 7) paged_append_kernel(const __grid_
   if (seq < 0) return;
   const PagedSeq sq = paged_seq(a.b, seq);
   if (row - sq.row0 >= sq.n) return;
-  const int slot = sq.kv - sq.n + row - sq.row0, pos = a.pos ? __ldg(a.pos + row) : slot;
+  const int slot = sq.kv - sq.n + row - sq.row0, pos = a.pos ? __ldca(a.pos + row) : slot;
   int page = -1;
-  if (slot >= 0) page = __ldg(a.b.page_table + (size_t)seq * a.b.max_pages + (slot >> a.b.ps_log2));
+  if (slot >= 0) page = __ldca(a.b.page_table + (size_t)seq * a.b.max_pages + (slot >> a.b.ps_log2));
   const bool there = page >= 0 && page < a.b.n_pages;
   const int d = kNear ? 1 : P == kHalves ? HD / 2 : R / 2;  // distance of a pair's elements
   float (&fac)[2][2][HD] = s_fac[warp];
@@ -136,13 +136,13 @@ __global__ void __launch_bounds__(kThreads, 7) paged_append_kernel(const __grid_
     if (!kPart || j < R / 2) {
       if (!kNear) e = j, f = j + d;
       // the angle in 64 bits, less whole turns: at a position of 10^5 its product in 32 bits would be off by 0.004
-      const double halves = (double)pos * (double)__ldg(a.inv_freq + j) * 0.3183098861837907;  // half turns
+      const double halves = (double)pos * (double)__ldca(a.inv_freq + j) * 0.3183098861837907;  // half turns
       sincospif((float)(halves - 2.0 * rint(0.5 * halves)), &s, &c);
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const float* w = k ? a.k_norm : a.q_norm;
-      const float we = w ? __ldg(w + e) : 1.f, wf = w ? __ldg(w + f) : 1.f;
+      const float we = w ? __ldca(w + e) : 1.f, wf = w ? __ldca(w + f) : 1.f;
       fac[k][0][at<HD>(e)] = we * c;
       fac[k][0][at<HD>(f)] = wf * c;
       fac[k][1][at<HD>(e)] = -s * wf;

@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto there = [&](const Piece& c, int t) {
       const int slot = ((c.u.tile0 + c.t0 + t) << 7) + lane * 16;
       int id = -1;
-      if (lane < 8 && slot < c.sq.kv) id = __ldg(b.page_table + (size_t)c.seq * b.max_pages + (slot >> b.ps_log2));
+      if (lane < 8 && slot < c.sq.kv) id = __ldca(b.page_table + (size_t)c.seq * b.max_pages + (slot >> b.ps_log2));
       return id >= 0 && id < b.n_pages;
     };
     bool more = walk.next(b, a.x, pc), nx = more && there(pc, 0);  // (a unit without a slot has one empty tile)
@@ -733,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // this lane's page of a key tile, and the row of the page pool where it starts (outside the pool: zeros)
       auto page_of = [&](int tile) {
         const int at = (tile << 7) + (lane << lg);
-        return lane < boxes && at < pc.sq.kv ? __ldg(table + (at >> lg)) : -1;
+        return lane < boxes && at < pc.sq.kv ? __ldca(table + (at >> lg)) : -1;
       };
       auto row_of = [&](int tile, int page) {
         if (page < 0 || page >= b.n_pages) return a.oob;
