@@ -136,3 +136,17 @@ def test_inputs_are_read_by_coherent_loads():
     for name in ("paged.cuh", "paged_append.cu", "paged_attn.cu"):
         code = re.sub(r"//.*", "", open(os.path.join(csrc, name)).read())
         assert not re.search(r"__ldg\b|ld\.global\.nc|__restrict__", code), name
+
+
+def test_work_axis_against_counting(tmp_path):
+    """The closed forms by which the attention's blocks share out the work (csrc/paged_axis.cuh), compiled for the
+    host: lengths up to the limits, every key tile walked once, every cut unit's parts where the merge looks."""
+    import os
+    import subprocess
+    here = os.path.dirname(os.path.abspath(__file__))
+    csrc = os.path.join(os.path.dirname(_lib.__file__), "csrc")
+    exe = str(tmp_path / "axis")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover", "-I" + csrc, "-o", exe,
+                    os.path.join(here, "paged_axis_check.cpp")], check=True, timeout=300)
+    r = subprocess.run([exe, "1500"], capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0 and r.stdout == "ok\n", r.stdout + r.stderr

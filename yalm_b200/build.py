@@ -27,7 +27,7 @@ NVCC_FLAGS = ARCH + [
 CU_SOURCES = ["gemv.cu", "attention.cu", "persistent.cu", "engine.cu", "capi.cu", "noalloc.cu", "sampler.cu", "loader.cu", "prefill_gemm.cu", "prefill.cu", "prefill_attn_tc.cu", "prefill_run.cu",
               "paged_append.cu", "paged_attn.cu", "paged_capi.cu"]
 HEADERS = ["common.cuh", "gemv.cuh", "attention.cuh", "persistent.cuh", "launch.h", "engine.h", "loader.h", "prefill.cuh",
-           "prefill_gemm.cuh", "sampler.cuh", "tmap.h", "umma.cuh", "paged.cuh"]
+           "prefill_gemm.cuh", "sampler.cuh", "tmap.h", "umma.cuh", "paged.cuh", "paged_axis.cuh"]
 
 
 def _newer(target: str, deps) -> bool:
