@@ -114,16 +114,22 @@ static void batch(const std::vector<PagedSeq>& seqs, int U, int window, int K, i
     Walk walk(st);
     Piece p;
     int begun = 0, ended = 0;  // records that the block leaves
+    int from = -1;
     while (walk.next(b, x, p)) {
       CHECK(w < want.size(), "a unit too many in block %d", c);
       const Want& u = want[w];
       CHECK(p.seq == u.seq && p.head == u.head && p.u.q0 == u.unit * U && p.t0 == done && p.t1 > p.t0 && p.t1 <= u.cost,
             "block %d: tiles %d to %d of unit %d of sequence %d", c, p.t0, p.t1, u.unit, u.seq);
-      if (p.t0 == 0) first_block = c, parts = 0;
-      ++parts;
+      const int most = p.u.nq > U / 2 ? kSumTiles : 2 * kSumTiles;
+      CHECK(p.t1 - p.t0 <= most && (p.last || p.t1 - p.t0 == most) && (from < 0 ? p.t0 : from) == p.from,
+            "block %d: tiles %d to %d, from %d", c, p.t0, p.t1, p.from);
       done = p.t1;
-      if (p.t0 != 0) CHECK(++begun == 1 && c == first_block + parts - 1, "block %d: records of a unit begun before", c);
-      if (p.t0 == 0 && p.t1 < u.cost) {
+      from = p.last ? -1 : p.from;
+      if (!p.last) continue;
+      if (p.from == 0) first_block = c, parts = 0;
+      ++parts;
+      if (p.from != 0) CHECK(++begun == 1 && c == first_block + parts - 1, "block %d: records of a unit begun before", c);
+      if (p.from == 0 && p.t1 < u.cost) {
         CHECK(++ended == 1, "block %d leaves two units", c);
         CHECK(block_of(share, more, u.begin + u.cost - 1) > c, "block %d", c);
       }
@@ -135,6 +141,7 @@ static void batch(const std::vector<PagedSeq>& seqs, int U, int window, int K, i
         ++w;
       }
     }
+    CHECK(from < 0, "block %d ends amid its pieces of a unit", c);
   }
   CHECK(w == want.size() && done == 0, "%zu of %zu units", w, want.size());
 }

@@ -148,3 +148,135 @@ def test_steps_whose_lengths_are_advanced_on_the_device(gpu):
         ref, tol = s.attend64()
         assert ((out.double() - ref).abs() <= tol).all(), i
     assert b.status(scratch) == 0
+
+
+# ------------------------------------------------------------------------------------- very long caches
+def _row64(q, k, v, scale, u):
+    """(output, tolerance) of one query head over k, v [slots][head_dim], in 64 bits.  Beside the terms of
+    test_paged_gpu.py: the tensor cores' additions need not round to nearest, so a sum is off by up to 2^-23 of it in each
+    of the 1024 additions (of 16 slots) after which it is joined to the rest, and by 2^-22 in each such join (a product
+    and a sum rounded to nearest); however long the cache."""
+    q, k, v = q.double(), k.double(), v.double()
+    sc = (k @ q) * scale
+    mag = float(((k.abs() @ q.abs()) * scale).max())
+    w = (sc - sc.max()).exp()
+    w /= w.sum()
+    o, size = w @ v, w @ v.abs()
+    joins = min(k.shape[0] // 16, 1024) + 2 * (k.shape[0] // 16384)
+    return o, u * o.abs() + (u + 2.0 ** -16 + 2 * 2.0 ** -20 * mag + joins * 2.0 ** -23) * size + 2.0 ** -25
+
+
+def _long(slots, nkv, hd, ps, dtype, seed):
+    """A cache of one sequence with values of one sign, so that a biased sum shows, in pages in random order; and its
+    keys and values in the order of the slots."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n = -(-slots // ps)
+    k = (torch.randn(n, nkv, ps, hd, generator=g, device="cuda") * 1.4).to(dtype)
+    v = (torch.rand(n, nkv, ps, hd, generator=g, device="cuda") + 0.5).to(dtype)
+    order = torch.randperm(n, generator=g, device="cuda")
+    table = order.to(torch.int32)[None].contiguous()
+
+    def slots_of(x, head, lo, hi):
+        a, b = lo // ps, -(-hi // ps)
+        return x[order[a:b], head].reshape(-1, hd)[lo - a * ps: hi - a * ps]
+    return g, k, v, table, slots_of
+
+
+@pytest.mark.parametrize("slots,new,window,nh,nkv,hd,ps,dtype", [
+    (200_003, 1, 0, 4, 1, 128, 16, "f16"),
+    (200_003, 1, 0, 8, 2, 64, 16, "bf16"),
+    (1 << 21, 1, 0, 4, 1, 128, 256, "f16"),  # the longest cache there is
+    (1 << 21, 1, 0, 1, 1, 64, 16, "f16"),
+    ((1 << 21) - 77, 2, 0, 16, 1, 64, 64, "bf16"),
+    (1_000_003, 3, 1000, 4, 1, 128, 16, "f16"),
+    (1_000_003, 3, 100_003, 4, 1, 128, 64, "f16"),
+    (1 << 21, 3, 1 << 20, 8, 1, 128, 32, "bf16"),
+    (1 << 21, 300, (1 << 21) - 100, 2, 2, 64, 256, "f16"),
+])
+def test_caches_up_to_the_longest(gpu, slots, new, window, nh, nkv, hd, ps, dtype):
+    import torch
+    from test_paged_gpu import U, _types
+    dt = _types()[dtype]
+    g, k, v, table, slots_of = _long(slots, nkv, hd, ps, dt, seed=slots % 1000 + new)
+    from yalm_b200 import PagedBatch
+    i32 = dict(dtype=torch.int32, device="cuda")
+    b = PagedBatch(k, v, table, torch.tensor([0, new], **i32), torch.tensor([slots], **i32), nh, new)
+    q = (torch.randn(new, nh * hd, generator=g, device="cuda") * 1.4).to(dt)
+    out, scratch = torch.full_like(q, 7.0), torch.zeros(b.scratch_bytes(), dtype=torch.uint8, device="cuda")
+    b.attend(q, out, scratch, window=window)
+    assert b.status(scratch) == 0
+    for i in sorted({0, new // 2, new - 1}):
+        for h in sorted({0, nh // 2, nh - 1}):
+            p = slots - new + i
+            lo = max(0, p - window + 1) if window else 0
+            o, tol = _row64(q[i, h * hd: (h + 1) * hd], slots_of(k, h * nkv // nh, lo, p + 1),
+                            slots_of(v, h * nkv // nh, lo, p + 1), 1 / math.sqrt(hd), U[dtype])
+            err = (out[i, h * hd: (h + 1) * hd].double() - o).abs()
+            assert (err <= tol).all(), (i, h, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("slots,hd,dtype", [(120_000, 128, "f16"), (120_000, 64, "bf16"), (1 << 20, 128, "bf16"),
+                                            (1 << 21, 64, "f16")])
+def test_long_units_that_no_cut_shortens(gpu, slots, hd, dtype):
+    """As many sequences as blocks over the same pages: each block carries one row's sums over the whole cache."""
+    import torch
+    from test_paged_gpu import U, _types
+    from yalm_b200 import PagedBatch
+    dt, n = _types()[dtype], _lib.lib().yb_num_sms()
+    g, k, v, table, slots_of = _long(slots, 1, hd, 64, dt, seed=hd)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    b = PagedBatch(k, v, table.expand(n, -1).contiguous(), torch.arange(n + 1, **i32),
+                   torch.full((n,), slots, **i32), 2, n)
+    q = (torch.randn(n, 2 * hd, generator=g, device="cuda") * 1.4).to(dt)
+    out, scratch = torch.full_like(q, 7.0), torch.zeros(b.scratch_bytes(), dtype=torch.uint8, device="cuda")
+    b.attend(q, out, scratch)
+    assert b.status(scratch) == 0
+    keys, values = slots_of(k, 0, 0, slots), slots_of(v, 0, 0, slots)
+    for i in (0, 1, n // 2, n - 1):
+        for h in range(2):
+            o, tol = _row64(q[i, h * hd: (h + 1) * hd], keys, values, 1 / math.sqrt(hd), U[dtype])
+            err = out[i, h * hd: (h + 1) * hd].double() - o
+            assert (err.abs() <= tol).all(), (i, h, float((err.abs() / tol).max()))
+
+
+@pytest.mark.parametrize("nh,window", [(1, 0), (16, 300)])
+def test_as_many_tokens_as_there_may_be(gpu, nh, window):
+    """A prompt of 2^20 tokens, appended and attended to: sampled rows."""
+    import torch
+    from test_paged_gpu import U
+    from yalm_b200 import PagedBatch
+    n, hd, ps = 1 << 20, 64, 256
+    i32 = dict(dtype=torch.int32, device="cuda")
+    g, k, v, table, slots_of = _long(n, 1, hd, ps, torch.float16, seed=nh)
+    k.zero_()
+    v.zero_()
+    b = PagedBatch(k, v, table, torch.tensor([0, n], **i32), torch.tensor([n], **i32), nh, n)
+    qkv = torch.randn(n, (nh + 2) * hd, generator=g, device="cuda", dtype=torch.float16)
+    qkv[:, (nh + 1) * hd:] = qkv[:, (nh + 1) * hd:].abs()
+    q = torch.empty(n, nh * hd, device="cuda", dtype=torch.float16)
+    inv = torch.tensor([1e6 ** (-2.0 * j / hd) for j in range(hd // 2)], device="cuda")
+    b.append(qkv, q, inv, hd, clip=3.0)
+    rows = sorted({0, 1, 255, 256, 65535, 65536, n // 2, n - 257, n - 1} |
+                  set(torch.randint(0, n, (12,), generator=g, device="cuda").tolist()))
+    at = torch.tensor(rows, device="cuda")
+    x = qkv[at].double().clamp(-3, 3).view(-1, nh + 2, hd)
+    a, c = x[:, : nh + 1, 0::2], x[:, : nh + 1, 1::2]
+    ang = at.double()[:, None, None] * inv.double()
+    want = torch.stack((a * ang.cos() - c * ang.sin(), a * ang.sin() + c * ang.cos()), -1).flatten(-2)
+    size = torch.stack((a.abs() + c.abs(),) * 2, -1).flatten(-2)
+    tol = U["f16"] * want.abs() + 2.0 ** -18 * size + 2.0 ** -25
+    assert ((q[at].double().view(-1, nh, hd) - want[:, :nh]).abs() <= tol[:, :nh]).all()
+    key, value = slots_of(k, 0, 0, n)[at].double(), slots_of(v, 0, 0, n)[at]
+    assert ((key - want[:, nh]).abs() <= tol[:, nh]).all()
+    assert torch.equal(value, qkv[at, (nh + 1) * hd:].clamp(-3, 3))
+    out, scratch = torch.full_like(q, 7.0), torch.zeros(b.scratch_bytes(), dtype=torch.uint8, device="cuda")
+    b.attend(q, out, scratch, window=window)
+    assert b.status(scratch) == 0
+    keys, values = slots_of(k, 0, 0, n), slots_of(v, 0, 0, n)
+    for p in rows:
+        lo = max(0, p - window + 1) if window else 0
+        for h in sorted({0, nh - 1}):
+            o, tol = _row64(q[p, h * hd: (h + 1) * hd], keys[lo: p + 1], values[lo: p + 1], 1 / math.sqrt(hd), U["f16"])
+            err = out[p, h * hd: (h + 1) * hd].double() - o
+            assert (err.abs() <= tol).all(), (p, h, float((err.abs() / tol).max()))

@@ -32,7 +32,8 @@
 // P is rounded to the caches' type for the tensor cores (the weights' rounding error is that of the
 // output's rounding, and averages over the slots); scores, maxima, sums and outputs are fp32.  The output is
 // rescaled only when a row's maximum grew by more than 2^8: until then the old maximum serves, and every
-// weight stays below 2^8.  fp16 weights carry a factor 2^7, which keeps the small ones above 2^-32 of the
+// weight stays below 2^8.  O is summed in tensor memory over 1024 additions at most, then joined to the sums before
+// (paged_axis.cuh, kSumTiles).  fp16 weights carry a factor 2^7, which keeps the small ones above 2^-32 of the
 // largest out of the subnormal range.
 //
 // What bounds it.  Prompts and chunks: the exponentials and the passes over S and P through registers beside the
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Piece after;
       more = walk.next(b, a.x, after);
       nx = more && there(after, 0);
-      // ---- the piece's rows: o * w0 (+ o of pipeline 1 * w1)
+      // ---- the piece's rows: o * w0 (+ o of pipeline 1 * w1) (+ o of the pieces before * w2)
       const bool other = !two && nk > 0;  // pipeline 0 takes pipeline 1's rows in
       float w0 = 1.f, w1 = 0.f;
       // (a barrier for each buffer: its phase before the awaited one is over, since the scores that came into the
@@ -464,16 +465,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++singles;
       }
       tc_fence_after();
-      const bool whole = pc.t0 == 0 && pc.t1 == pc.u.cost;
+      const bool whole = pc.from == 0 && pc.t1 == pc.u.cost, joins = pc.t0 > pc.from;
       const int rows = pc.u.nq * a.gq, row = tile * QB * a.gq + r;
       const int token = pc.sq.row0 + pc.u.q0;
-      float* rec = a.recs + ((size_t)blockIdx.x * 2 + (pc.t0 == 0 ? 1 : 0)) * rec_floats<HD>();
+      float* rec = a.recs + ((size_t)blockIdx.x * 2 + (pc.from == 0 ? 1 : 0)) * rec_floats<HD>();
       T* out = static_cast<T*>(a.out) + (size_t)(token + q) * a.out_stride + (size_t)(pc.head * a.gq + h) * HD;
       if (two || p == 0) {
+        float w2 = 0.f;
+        if (joins && valid) {  // the thread's own record
+          const float mm = fmaxf(m, rec[HD * rows + row]);
+          w2 = rec[HD * rows + row] == -INFINITY ? 0.f : ex2(rec[HD * rows + row] - mm);
+          const float f = m == -INFINITY ? 0.f : ex2(m - mm);
+          w0 *= f;
+          w1 *= f;
+          l = l * f + rec[(HD + 1) * rows + row] * w2;
+          m = mm;
+        }
         const float inv = whole ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
         w0 *= inv;
         w1 *= inv;
-        if (live && two && whole && nk > 0) {
+        w2 *= inv;
+        if (live && two && whole && !joins && nk > 0) {
           // Whole outputs of many rows: of 32 columns a lane holds its row's four groups of 16 bytes.  Two lanes exchange
           // two of theirs, so that a store writes whole sectors of 32 bytes of every second row.
           const bool up = lane & 1;
@@ -513,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float v[32];
             if (nk > 0) {
               tmem_ld32(to + p * HD + c0, v);
-              if (other || whole) {  // a row that has seen no slot has zeros there: its weights were all 0
+              if (other || whole || joins) {  // a row that has seen no slot has zeros there: its weights were all 0
                 const float2 w00 = make_float2(w0, w0);
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
@@ -536,6 +548,17 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int k = 0; k < 32; ++k) v[k] = 0.f;
             }
             if (!valid) continue;
+            if (joins) {
+              const float4* o = reinterpret_cast<const float4*>(rec) + (size_t)(c0 / 4) * rows + row;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float4 f = o[(size_t)k * rows];
+                v[4 * k] = fmaf(f.x, w2, v[4 * k]);
+                v[4 * k + 1] = fmaf(f.y, w2, v[4 * k + 1]);
+                v[4 * k + 2] = fmaf(f.z, w2, v[4 * k + 2]);
+                v[4 * k + 3] = fmaf(f.w, w2, v[4 * k + 3]);
+              }
+            }
             if (whole) {
 #pragma unroll
               for (int k = 0; k < 4; ++k)
@@ -557,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (nk > 0 && lane == 0) mbar_arrive(&o_free);
       }
-      if (!whole && pc.t0 == 0 && threadIdx.x == 128) {
+      if (!whole && pc.last && pc.from == 0 && threadIdx.x == 128) {
         const unsigned long long begin = s_start.begin + (s_start.left - left) - pc.t1;  // the unit's first tile
         const int last = block_of(s_start.share, s_start.more, begin + pc.u.cost - 1);
         a.cuts[blockIdx.x] = Cut{token, pc.u.nq, pc.head, last - (int)blockIdx.x + 1};

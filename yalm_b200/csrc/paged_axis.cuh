@@ -10,6 +10,13 @@ namespace {
 constexpr int kKT = 128;       // slots per key tile
 constexpr int kFewTiles = 4;   // shares below this are all the same
 constexpr int kUnitTiles = 2;  // what a unit's start and end cost, in key tiles
+// Key tiles whose products go into one sum of the tensor cores: of a unit of two row tiles, whose sums take a tile in
+// eight additions of 16 slots; twice as many of a unit of one, whose two sums have half of a tile each.  The additions
+// cut off what does not fit, half a last place each time on average, so a sum of values of one sign lost 3.3e-9 of itself
+// a slot, however many: as much as half an fp16 rounding (2^-12) after 75000 slots, 14 roundings after 2^21.  Sums of
+// 1024 additions lose a tenth of one at most; they are joined in fp32, rounded to nearest.  That costs 1 to 3 % of a call
+// whose blocks have several such sums of a unit (2048 tokens over 65536 slots 2330 -> 2377 us), and nothing below.
+constexpr int kSumTiles = 128;
 
 // sum_{i < n} floor((a i + b) / 128), a, b >= 0: each round takes the whole parts out and swaps the roles of the
 // axes, as Euclid's algorithm does.  Where a is a power of two (one, two, four ... query heads per kv head) two
@@ -121,17 +128,19 @@ __device__ __forceinline__ int block_of(unsigned long long share, int more, unsi
   return x < cut ? (int)quot(x, share + 1) : more + (int)quot(x - cut, share);
 }
 
-// The next piece of this block's share: tiles [t0, t1) of a unit.
+// The next piece of this block's share: tiles [t0, t1) of a unit, of which the block has those from `from` on.
 struct Piece {
   PagedSeq sq;
   int seq, head;
   Unit u;
-  int t0, t1;
+  int from, t0, t1;
+  bool last;  // of the block's pieces of the unit
 };
 struct Walk {
   Start st;
   PagedSeq sq;
-  __device__ __forceinline__ explicit Walk(const Start& s) : st(s), sq(s.sq) {}
+  int from;  // of the unit that a piece before this one began; -1: none
+  __device__ __forceinline__ explicit Walk(const Start& s) : st(s), sq(s.sq), from(-1) {}
   __device__ __forceinline__ bool next(const PagedBatch& b, const Axis& x, Piece& p) {
     do {
       if (st.left <= 0 || st.seq >= b.n_seqs) return false;
@@ -139,9 +148,15 @@ struct Walk {
       p.seq = st.seq;
       p.head = st.head;
       p.u = unit_of(x, sq, st.unit);
-      const int all = p.u.cost + kUnitTiles, end = min(all, st.off + st.left);
+      const int all = p.u.cost + kUnitTiles;
+      int end = min(all, st.off + st.left);
       p.t0 = st.off;
       p.t1 = min(p.u.cost, end);
+      p.from = from < 0 ? p.t0 : from;
+      const int most = p.u.nq > x.U / 2 ? kSumTiles : 2 * kSumTiles;
+      p.last = p.t1 - p.t0 <= most;
+      if (!p.last) p.t1 = end = p.t0 + most;
+      from = p.last ? -1 : p.from;
       st.left -= end - st.off;
       st.off = end;
       if (end == all && st.left > 0) {
