@@ -280,3 +280,41 @@ def test_as_many_tokens_as_there_may_be(gpu, nh, window):
             o, tol = _row64(q[p, h * hd: (h + 1) * hd], keys[lo: p + 1], values[lo: p + 1], 1 / math.sqrt(hd), U["f16"])
             err = out[p, h * hd: (h + 1) * hd].double() - o
             assert (err.abs() <= tol).all(), (p, h, float((err.abs() / tol).max()))
+
+
+@pytest.mark.parametrize("dtype,hd", [("f16", 64), ("f16", 128), ("bf16", 128)])
+@pytest.mark.parametrize("slots,top_at,second", [(1 << 20, 5, 0), (1 << 20, (1 << 20) - 3, 0), (300_000, 299_000, 7.9),
+                                                 (700, 3, 0)])
+def test_many_small_weights_beside_a_large_one(gpu, dtype, hd, slots, top_at, second):
+    """Weights of 2^-20 to 2^-33 of the largest, which together are up to a fifth of it; the largest comes first, last, or
+    after one (2^-7.9 of it) whose maximum then serves for the rest.  Tolerance: in fp16 a weight below 2^-21 of that maximum
+    is rounded by up to 2^-32 of it, which the other terms, relative to each weight, do not hold."""
+    import torch
+    from test_paged_gpu import U, _types
+    from yalm_b200 import PagedBatch
+    dt = _types()[dtype]
+    g, k, v, table, slots_of = _long(slots, 1, hd, 64, dt, seed=slots % 97 + hd)
+    score = torch.rand(slots, generator=g, device="cuda") * 13 + 20
+    if second:
+        score[: slots // 100] = 40.0
+        score[slots // 100] = second
+    score[top_at] = 0.0
+    k.zero_()
+    at = torch.arange(slots, device="cuda")
+    k[table[0].long()[at // 64], 0, at % 64, 0] = (score * -math.log(2)).to(dt)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    b = PagedBatch(k, v, table, torch.tensor([0, 1], **i32), torch.tensor([slots], **i32), 2, 1)
+    q = torch.zeros(1, 2 * hd, device="cuda", dtype=dt)
+    q[0, 0], q[0, hd] = 8.0, 16.0  # the second head: all weights squared
+    out, scratch = torch.full_like(q, 7.0), torch.zeros(b.scratch_bytes(), dtype=torch.uint8, device="cuda")
+    b.attend(q, out, scratch, scale=0.125)
+    assert b.status(scratch) == 0
+    keys, values = slots_of(k, 0, 0, slots), slots_of(v, 0, 0, slots)
+    for h in range(2):
+        qh = q[0, h * hd: (h + 1) * hd]
+        o, tol = _row64(qh, keys, values, 0.125, U[dtype])
+        if dtype == "f16":
+            s = (keys.double() @ qh.double()) * 0.125
+            tol = tol + slots * 2.0 ** -32 * float(values.max()) / float((s - s.max()).exp().sum())
+        err = (out[0, h * hd: (h + 1) * hd].double() - o).abs()
+        assert (err <= tol).all(), (h, float((err / tol).max()))

@@ -33,8 +33,8 @@
 // output's rounding, and averages over the slots); scores, maxima, sums and outputs are fp32.  The output is
 // rescaled only when a row's maximum grew by more than 2^8: until then the old maximum serves, and every
 // weight stays below 2^8.  O is summed in tensor memory over 1024 additions at most, then joined to the sums before
-// (paged_axis.cuh, kSumTiles).  fp16 weights carry a factor 2^7, which keeps the small ones above 2^-32 of the
-// largest out of the subnormal range.
+// (paged_axis.cuh, kSumTiles).  fp16 weights carry a factor 2^7, with which they are normal numbers from 2^-21 of
+// that maximum's weight on; smaller ones are rounded by up to 2^-32 of it each.
 //
 // What bounds it.  Prompts and chunks: the exponentials and the passes over S and P through registers beside the
 // products.  2048 tokens over 16384 slots, 32 heads of 128 on 8 kv heads, take 495 us at sustained power (1040
