@@ -318,3 +318,39 @@ def test_many_small_weights_beside_a_large_one(gpu, dtype, hd, slots, top_at, se
             tol = tol + slots * 2.0 ** -32 * float(values.max()) / float((s - s.max()).exp().sum())
         err = (out[0, h * hd: (h + 1) * hd].double() - o).abs()
         assert (err <= tol).all(), (h, float((err / tol).max()))
+
+
+# ---------------------------------------------------------------------------------------------- append
+@pytest.mark.parametrize("hd,R,half", [(128, 128, False), (128, 128, True), (128, 96, False), (128, 96, True), (64, 8, False),
+                                       (64, 8, True), (64, 62, False), (64, 0, False), (64, 0, True), (128, 0, True)])
+@pytest.mark.parametrize("src,dtype", [("f32", "f16"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("norms", ["", "q", "k", "qk"])
+def test_append_with_either_norm_and_values_that_are_not_finite(gpu, hd, R, half, src, dtype, norms):
+    """One norm without the other, half-split pairs over nothing; infinities and NaN spoil what the definition says
+    they do: without a norm their pair, or themselves alone where nothing is rotated, with one their head (an infinity
+    makes the finite ones 0)."""
+    import torch
+    from test_paged_gpu import _append64, _types
+    nh, nkv, ps, n = 6, 3, 16, 40
+    s = Step([n], [n + 70], nh, nkv, hd, ps, dtype, seed=hd + R)
+    g = s.g
+    qkv = (torch.randn(n, (nh + 2 * nkv) * hd, generator=g, device="cuda") * 2).to(_types()[src])
+    for bad in (math.inf, -math.inf, math.nan):
+        where = torch.randint(0, qkv.numel(), (24,), generator=g, device="cuda")
+        qkv.view(-1)[where] = bad
+    w = 1 + 0.3 * torch.randn(2, hd, generator=g, device="cuda")
+    qn, kn = (w[0].clone() if "q" in norms else None), (w[1].clone() if "k" in norms else None)
+    inv = torch.tensor([1e4 ** (-2.0 * j / max(R, 1)) for j in range(R // 2)] or [0.0], device="cuda")
+    pos = torch.randint(1, 5000, (n,), dtype=torch.int32, generator=g, device="cuda")
+    q = torch.empty_like(s.q)
+    s.batch().append(qkv, q, inv if R else None, R, q_norm=qn, k_norm=kn, eps=1e-6, half=half, pos=pos)
+    torch.cuda.synchronize()
+    ref, tol = _append64(s, qkv, qn, kn, 1e-6, inv, R, half, pos, math.inf)
+    slot = torch.arange(70, 70 + n, device="cuda")
+    page = s.page_table[0].long()[slot // ps]
+    got = torch.cat((q.view(n, nh, hd), s.k[page, :, slot % ps], s.v[page, :, slot % ps]), 1).double()
+    assert torch.equal(got.isnan(), ref.isnan())
+    assert torch.equal(got.isinf(), ref.isinf()) and torch.equal(got[got.isinf()], ref[ref.isinf()])
+    fine = ref.isfinite()
+    assert fine.float().mean() > 0.3 and not fine.all()
+    assert ((got - ref).abs()[fine] <= tol[fine]).all()
