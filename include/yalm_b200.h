@@ -342,28 +342,35 @@ typedef struct yb_paged_batch {
  * pairs (2j, 2j + 1) as yalm has them (src/infer.cpp:205), or (j, j + rotary_dim / 2) when rope_half != 0
  * (rotary_dim then a multiple of 8); queries go to q_out, keys and values to the token's slot.  The position
  * is the slot, or pos_dev[row] when pos_dev is not NULL.  A token whose slot is negative or on a
- * page that is not there is not stored; its query is written all the same.  Norms, angles (64 bits)
- * and rotation are computed before the one rounding to dtype. */
+ * page that is not there is not stored; its query is written all the same.  Norms (sums of squares in fp32, which
+ * elements from 1e18 on overflow), angles (64 bits) and rotation are computed before the one rounding to dtype. */
 int yb_paged_append_dev(const yb_paged_batch* b, void* q_out, long long q_out_stride, const void* qkv,
                         long long qkv_stride, int qkv_dtype, const float* q_norm_dev, const float* k_norm_dev,
                         float eps, const float* inv_freq_dev, int rotary_dim, int rope_half, const int* pos_dev,
                         float qkv_clip, void* stream);
 
 /* Causal attention of the new tokens over their sequences' caches, which hold them already: the token of
- * slot p sees slots max(0, p - window + 1) .. p (window 0: 0 .. p), less those on pages that are not
- * there; out = sum softmax(scale * q.k) v, or zeros where it sees no slot.  Slots from kv_len on, those before
- * the window of the sequence's first new token, and pages that are not there may hold anything, NaN
- * included (pages that have left the window may be given to other sequences); the slots between hold
- * finite values: one that does not may spoil the rows of tokens before it, too.
- * scale is positive, and scale * log2(e) and its products with the sums q.k have to stay in fp32's range.
+ * slot p sees slots max(0, p - window + 1) .. p (window 0: 0 .. p), less those on pages that are not there;
+ * out = sum softmax(scale * q.k) v, or zeros where it sees no slot.  Slots from kv_len on, those before the
+ * window of the sequence's first new token, and pages that are not there may hold anything, NaN included
+ * (pages that have left the window may be given to other sequences); the slots between hold finite values:
+ * one that does not may spoil the rows of tokens before it, too.  scale is positive, and scale * log2(e) and
+ * its products with the sums q.k have to stay in fp32's range.
+ * Numerics: scores, maxima, sums and outputs are held in fp32; q enters as it is and every softmax weight is
+ * rounded to dtype before its product with v (yb_prefill_attention_dev, of one sequence, keeps both to about
+ * 22 bits), which is off by as much as the output's own rounding, and averages over the slots.  Results do
+ * not depend on timing: the same batch on a device with as many SMs gives the same bits.  A sequence's
+ * output is not the same to the bit in another batch, since the lengths of all its sequences, their order,
+ * the heads and the window decide where the slots of each are split into sums.
  * scratch_dev: yb_paged_attention_scratch_bytes(b) bytes (the same for every batch of this head_dim on a
- * device), 16-byte aligned; its contents have no meaning between calls.  Calls that may run at the same
- * time, replayed graphs among them, each need their own.  Its first word collects status bits as yb_status
- * has them when a bounded wait in the kernel runs out (set it to zero once, and after it was seen set, to tell); the
- * call's output is then not complete, and the next call in the same workspace is as good as any.  Results do not depend on timing, but on the number of SMs, which decides where a long
- * cache is cut.  Refused (YB_E_UNSUPPORTED) is a batch whose share of work for one SM may not be counted in 31 bits: with
- * U = 2 * floor(128 * n_kv_heads / n_heads) queries a unit, (n_tokens / U + min(n_seqs, n_tokens)) * n_kv_heads *
- * (max_pages * page_size / 128 + 3) from 2^31 - 1 times the SMs on. */
+ * device), 16-byte aligned; its contents have no meaning between calls, but for the first word.  Calls that
+ * may run at the same time, replayed graphs among them, each need their own.  The first word collects status
+ * bits as yb_status has them when a bounded wait in the kernel runs out (set it to zero once, and after it
+ * was seen set, to tell); the call's output is then not complete, and the next call in the same workspace is
+ * as good as any.
+ * Refused (YB_E_UNSUPPORTED) is a batch whose share of work for one SM may not be counted in 31 bits: with U
+ * = 2 * floor(128 * n_kv_heads / n_heads) queries a unit, (n_tokens / U + min(n_seqs, n_tokens)) *
+ * n_kv_heads * (max_pages * page_size / 128 + 3) from 2^31 - 1 times the SMs on. */
 int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long long out_stride, const void* q,
                            long long q_stride, float scale, int window, void* scratch_dev, void* stream);
 size_t yb_paged_attention_scratch_bytes(const yb_paged_batch* b); /* 0 for a batch that is refused */
