@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = s_tmem;
   // Once a wait has run out, here or there, no wait of the block lasts: every warp goes on to the end of its piece with
   // whatever lies in its buffers, and leaves.  (A look at the mark in every step cost 3 %.)  Barriers may be arrived at
-  // early, but a copy must not be announced to one where another is landing, so the loaders look before each copy.
+  // early, but a copy must not be announced to one where another is landing, so the loaders look after each wait.
   // Nobody leaves the block before its copies and products have ended.
   auto wait = [&](uint64_t* bar, unsigned parity) { bounded_wait(bar, parity, a.budget, &s_abort, a.status); };
   auto aborted = [&] { return __any_sync(0xffffffffu, *static_cast<volatile int*>(&s_abort)) != 0; };
@@ -430,8 +430,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[p][buf]);
       }
-      if (aborted()) break;
-
       // the piece after this one is looked up under the last product and the stores
       const int left = walk.st.left;
       Piece after;
@@ -615,8 +613,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto load = [&](const CUtensorMap* map, int row, bool mine) {
         if (mine) {
-          if (issued >= C::kStages) wait(&empty[slot], phase);
-          if (aborted()) return false;
+          if (issued >= C::kStages) {
+            wait(&empty[slot], phase);
+            if (aborted()) return false;
+          }
           mine_into |= 1u << slot;
           mine_odd ^= 1u << slot;
           if (lane == 0) mbar_arrive_expect_tx(&full[slot], C::kTile);
@@ -631,8 +631,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       // a row tile of queries, once the products of the unit before have read its buffer
       auto load_q = [&](int to, int tile) {
-        if (uses[to]) wait(&q_empty[to], (uses[to] - 1) & 1);
-        if (aborted()) return false;
+        if (uses[to]) {
+          wait(&q_empty[to], (uses[to] - 1) & 1);
+          if (aborted()) return false;
+        }
         ++uses[to];
         if (lane == 0) {
           mbar_arrive_expect_tx(&q_full[to], (uint32_t)(QB * a.gq) * 128u * C::kHalves);
