@@ -202,6 +202,15 @@ def bench_prefill_attention(nh, nkv, hd, T, iters, seed=0):
             "us": round(ms * 1000, 2), "tflops": round(flop / (ms / 1000) / 1e12, 1), **_LAST_SPREAD}
 
 
+def _fresh():
+    """Memory of its own for the next case: in blocks that a case before it had freed, 512 tokens over 3202 slots took
+    55 us and not 42."""
+    import gc
+    import torch
+    gc.collect()
+    torch.cuda.empty_cache()
+
+
 def _paged(new, kv, nh, nkv, hd, ps, dtype, seed):
     """A batch of sequences with `new` new tokens over kv slots each, in pages handed out in random order."""
     import torch
@@ -220,6 +229,7 @@ def _paged(new, kv, nh, nkv, hd, ps, dtype, seed):
 def bench_paged_append(new, kv, nh, nkv, hd, ps, iters, seed=0):
     """Norm, rotation and append of the new tokens (yb_paged_append_dev), fp16 projections and cache."""
     import torch
+    _fresh()
     T, width = sum(new), (nh + 2 * nkv) * hd
     n = min(16, _copies(4 * T * width))  # few tokens: not over 4 x L2, but a new pool for every launch
     b = [_paged(new, kv, nh, nkv, hd, ps, torch.float16, seed + i) for i in range(n)]
@@ -240,6 +250,7 @@ def bench_paged_append(new, kv, nh, nkv, hd, ps, iters, seed=0):
 def bench_paged_attention(new, kv, nh, nkv, hd, ps, iters, seed=0):
     """Attention of the new tokens over the paged cache (yb_paged_attention_dev), fp16."""
     import torch
+    _fresh()
     T = sum(new)
     n = _copies(4 * sum(kv) * nkv * hd)
     b = [_paged(new, kv, nh, nkv, hd, ps, torch.float16, seed + i) for i in range(n)]
