@@ -6,12 +6,14 @@
 //
 // Memory-bound: every element is read once and written once, if the instructions stay few (a kernel that issued
 // 183 of a warp for every KB moved was bound by them, at a third of the bandwidth; this one issues 107).  8192
-// tokens of 32 + 2 x 8 heads of 128 take 35.5 us = 5.67 TB/s, 512 tokens 5.3 us, 64 tokens 2.8 us.  A warp has a
+// tokens of 32 + 2 x 8 heads of 128 take 35.7 us = 5.6 TB/s (50 us = 6.0 TB/s from fp32), 512 tokens 5.3 us, 64 tokens
+// 2.7 us.  A warp has a
 // row (token), or a share of its heads where there are few rows, and waits for no other.  A lane holds 16 elements
 // of a head, 8 neighbours in either half, so a head is 8 (head_dim 128) or 4 lanes and a warp has 4 or 8 heads at
 // a time; loads and stores are 16 bytes a lane and whole lines a head, the sum of squares is 3 or 2 shuffles, and
 // the other element of a rotation's pair lies in the same lane (where half-split pairs take a part of the head, it
-// comes by shared memory).  Norm weight and angle are one factor for each element of a pair, r (v_e w_e cos + v_f
+// comes by shared memory, for 170 instructions a KB and 8 to 12 spilled bytes a thread, which the seven blocks an SM are
+// worth: 1803 tokens of 64 + 2 x 8 heads 20.9 us, 16.7 with neighbouring pairs, 15.6 where whole heads are rotated).  Norm weight and angle are one factor for each element of a pair, r (v_e w_e cos + v_f
 // w_f (-+sin)), formed once a row and kept in shared memory: in registers they would halve the warps that an SM
 // holds.  The loads of the first heads are under way before the row's sequence, its page and the angles are looked
 // up, and each later one starts when its registers are free.

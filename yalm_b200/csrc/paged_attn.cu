@@ -37,10 +37,12 @@
 // that maximum's weight on; smaller ones are rounded by up to 2^-32 of it each.
 //
 // What bounds it.  Prompts and chunks: the exponentials and the passes over S and P through registers beside the
-// products.  2048 tokens over 16384 slots, 32 heads of 128 on 8 kv heads, take 495 us at sustained power (1040
-// TFLOP/s; 442 us, 1167 TFLOP/s, before the clock falls), with the tensor and the special-function units each busy 39 %
-// of the time in a chunk of 1024.  Single tokens: the cache's bytes, 64 x 4096 slots 171 us = 6.3 TB/s; one
-// of 32768 slots 32 us = 4.2 TB/s, of which 8 are the launch, the first loads, the last tile's softmax and the merge.
+// products.  2048 tokens over 16384 slots, 32 heads of 128 on 8 kv heads, take 510 us at sustained power (1010
+// TFLOP/s; 435 us, 1184 TFLOP/s, before the clock falls), with the tensor and the special-function units each busy 43 %
+// of the time in a chunk of 1024.  Single tokens: the cache's bytes, 64 x 4096 slots 171 us = 6.3 TB/s, one of 2^20
+// slots 605 us = 7.1 TB/s; one of 32768 slots 32 us = 4.2 TB/s, of which 8 are the launch, the first loads, the last
+// tile's softmax and the merge; with heads of 64 a step has half the bytes and the same latencies, 64 x 4096 slots 117 us
+// = 4.6 TB/s.
 #include "paged.cuh"
 
 #include <cuda_bf16.h>
