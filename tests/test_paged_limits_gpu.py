@@ -320,6 +320,43 @@ def test_many_small_weights_beside_a_large_one(gpu, dtype, hd, slots, top_at, se
         assert (err <= tol).all(), (h, float((err / tol).max()))
 
 
+@pytest.mark.parametrize("busy", [[0, 1, 40_000, 65_535], [65_535], None])
+def test_as_many_sequences_as_there_may_be(gpu, busy):
+    """2^16 sequences of up to 40 slots: a few with one new token (none in the rest), or all of them."""
+    import torch
+    from test_paged_gpu import U
+    from yalm_b200 import PagedBatch
+    n, nh, nkv, hd, ps = 1 << 16, 4, 2, 64, 16
+    g = torch.Generator(device="cuda").manual_seed(95)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    new = torch.ones(n, **i32) if busy is None else torch.zeros(n, **i32).index_fill_(0, torch.tensor(busy, device="cuda"), 1)
+    kv = torch.randint(1, 41, (n,), generator=g, **i32)
+    start = torch.cat((torch.zeros(1, **i32), new.cumsum(0, dtype=torch.int32)))
+    T = int(start[-1])
+    pages = 3 * n
+    table = torch.randperm(pages, generator=g, device="cuda").to(torch.int32).view(n, 3)
+    k, v = (torch.randn(pages, nkv, ps, hd, generator=g, device="cuda", dtype=torch.float16) for _ in range(2))
+    b = PagedBatch(k, v, table, start, kv, nh, T + 1)
+    qkv = torch.randn(T + 1, (nh + 2 * nkv) * hd, generator=g, device="cuda", dtype=torch.float16)
+    q = torch.full((T + 1, nh * hd), 7.0, device="cuda", dtype=torch.float16)
+    out, scratch = q.clone(), torch.zeros(b.scratch_bytes(), dtype=torch.uint8, device="cuda")
+    b.append(qkv, q, None, 0)
+    b.attend(q, out, scratch)
+    assert b.status(scratch) == 0
+    assert (out[T] == 7).all() and torch.equal(q[:T], qkv[:T, : nh * hd]) and (q[T] == 7).all()
+    seqs = new.nonzero().flatten()
+    seqs = seqs[torch.linspace(0, T - 1, min(T, 500), device="cuda").long()]
+    for s in seqs.tolist():
+        m, row = int(kv[s]), int(start[s])
+        own_k, own_v = (x[table[s].long()].transpose(1, 2).reshape(-1, nkv, hd)[:m] for x in (k, v))
+        assert torch.equal(own_k[m - 1].flatten(), qkv[row, nh * hd: (nh + nkv) * hd])
+        assert torch.equal(own_v[m - 1].flatten(), qkv[row, (nh + nkv) * hd:])
+        for h in range(nh):
+            o, tol = _row64(q[row, h * hd: (h + 1) * hd], own_k[:, h // 2], own_v[:, h // 2], 1 / math.sqrt(hd), U["f16"])
+            err = (out[row, h * hd: (h + 1) * hd].double() - o).abs()
+            assert (err <= tol).all(), (s, h, float((err / tol).max()))
+
+
 # ---------------------------------------------------------------------------------------------- append
 @pytest.mark.parametrize("hd,R,half", [(128, 128, False), (128, 128, True), (128, 96, False), (128, 96, True), (64, 8, False),
                                        (64, 8, True), (64, 62, False), (64, 0, False), (64, 0, True), (128, 0, True)])
