@@ -85,7 +85,7 @@ struct PagedAppendArgs {
   int half;  // pairs (j, j + rotary_dim / 2) instead of (2j, 2j + 1)
 };
 // src_type: element type of qkv, type: of q_out and the caches (0 fp32, 1 fp16, 2 bf16)
-cudaError_t paged_append(const PagedAppendArgs& a, int head_dim, int src_type, int type, cudaStream_t s);
+cudaError_t paged_append(const PagedAppendArgs& a, int head_dim, int src_type, int type, int n_sms, cudaStream_t s);
 
 struct PagedAttnArgs {
   PagedBatch b;

@@ -31,7 +31,7 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMostWarps = 148 * 32;  // rows are shared out among warps up to this many
+constexpr int kWarpsPerSm = 32;  // rows are shared out among warps up to this many an SM
 
 // how a rotation's pairs lie: (2j, 2j + 1) or (j, j + R / 2), over the whole head or a part of it
 enum Pairs { kNeighbours, kHalves, kPartNeighbours, kPartHalves };
@@ -268,14 +268,14 @@ const void* pick(int src, int type, int pairs) {
 
 }  // namespace
 
-cudaError_t paged_append(const PagedAppendArgs& a, int head_dim, int src_type, int type, cudaStream_t s) {
+cudaError_t paged_append(const PagedAppendArgs& a, int head_dim, int src_type, int type, int n_sms, cudaStream_t s) {
   const bool whole = a.rotary_dim == head_dim;
   const int pairs = a.half ? (whole ? kHalves : kPartHalves) : (whole ? kNeighbours : kPartNeighbours);
   const void* fn = head_dim == 128 ? pick<128>(src_type, type, pairs) : pick<64>(src_type, type, pairs);
   // few rows: a warp has a part of a row's groups of heads
   const int in_group = 512 / head_dim;
   const int groups = (a.b.n_heads + in_group - 1) / in_group + 2 * ((a.b.n_kv_heads + in_group - 1) / in_group);
-  int shares = kMostWarps / a.b.n_tokens;
+  int shares = kWarpsPerSm * n_sms / a.b.n_tokens;
   shares = shares < 1 ? 1 : shares > groups ? groups : shares;
   int share_groups = (groups + shares - 1) / shares;
   shares = (groups + share_groups - 1) / share_groups;

@@ -159,7 +159,7 @@ extern "C" int yb_paged_append_dev(const yb_paged_batch* b, void* q_out, long lo
   a.clip = qkv_clip;
   a.rotary_dim = rotary_dim;
   a.half = rope_half ? 1 : 0;
-  YB_CK(paged_append(a, b->head_dim, qkv_dtype, b->dtype, static_cast<cudaStream_t>(stream)));
+  YB_CK(paged_append(a, b->head_dim, qkv_dtype, b->dtype, device_sms(dev), static_cast<cudaStream_t>(stream)));
   return 0;
 }
 
