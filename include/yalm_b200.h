@@ -330,9 +330,33 @@ typedef struct yb_paged_batch {
   void* v_pages;
 } yb_paged_batch;
 
-/* Both entry points run on the current device and refuse (YB_E_INVALID) buffers that are not its memory.
+/* The entry points run on the current device and refuse (YB_E_INVALID) buffers that are not its memory.
  * Rows of q, q_out, out and qkv are given by their strides in elements; base addresses and row
  * strides must be multiples of 16 bytes, the addresses of ints and floats of 4.  No buffer that is written may overlap another one. */
+
+/* Plans a step: from the tokens that every sequence brings, the batch's row starts and lengths, the pages that they
+ * need, and each token's position and slot, all on the device, so a captured step follows new requests.  Writes the
+ * batch's q_start, kv_len and page_table, which the calls below read.  With P = page_size, for every sequence s:
+ *  - new_len_dev[s] = n >= 0: its cache of kv_before_dev[s] slots grows to kv_len[s] = kv_before + n; entries
+ *    ceil(kv_before / P) .. ceil(kv_len / P) - 1 of its row of the table are pages taken from the end of the list of
+ *    free ones, in the order of (sequence, page): free_pages[n_free - 1] first.  q_start[s + 1] = q_start[s] + n.
+ *  - new_len_dev[s] < 0: it ends and brings nothing, kv_len[s] = 0.  Pages max(0, kept_dev[s]) .. ceil(kv_before / P) - 1
+ *    of its row go to the end of the list before any are taken, in the same order (kept_dev: the first pages that
+ *    it shares with others, which stay; NULL: none); entries outside [0, n_pages) are passed over.  Its row of the
+ *    table stays as it is, and means nothing.
+ * free_pages_dev: [n_pages], of which the first *n_free are free; no page may be in it twice or in use.  kv_before_dev
+ * may be the batch's kv_len_dev and n_free_before_dev may be n_free_dev (values are read before they are written); with
+ * buffers of their own a step can be planned again from the same state, with the same result.  kv_before is taken as
+ * clamped to [0, max_pages * page_size], n_free to [0, n_pages].
+ * pos_dev (int32, or NULL) and slots_dev (64-bit, or NULL) are [n_tokens]: for the i-th new token of s at row q_start[s] + i
+ * the position kv_before + i, and the slot page_table[s][pos / P] * P + pos % P counted over the whole pool (-1 on a page
+ * that is not there).  Rows from q_start[n_seqs] on are left as they are.
+ * A step that does not fit brings no token at all: q_start is all 0, lengths stay, no page is taken (ended sequences
+ * have given theirs back all the same).  status_dev[4] tells: [0] is 0, or bits: 1 pages are short ([1]: how many), 2
+ * more tokens than n_tokens ([2]: how many), 4 a sequence longer than max_pages * page_size ([3]: the first, else -1). */
+int yb_paged_plan_dev(const yb_paged_batch* b, const int* new_len_dev, const int* kv_before_dev, const int* kept_dev,
+                      int* free_pages_dev, const int* n_free_before_dev, int* n_free_dev, int* pos_dev,
+                      long long* slots_dev, int* status_dev, void* stream);
 
 /* One pass over the new tokens' projections, the epilogue that yb_qkv_dev has for one token: qkv rows
  * [n_heads query heads | n_kv_heads key heads | n_kv_heads value heads], of qkv_dtype (YB_DTYPE_*).
@@ -378,6 +402,27 @@ size_t yb_paged_attention_scratch_bytes(const yb_paged_batch* b); /* 0 for a bat
 /* Diagnostics: the SM clocks that a wait in the kernel of later yb_paged_attention_dev calls of this process may take
  * before it gives up (0: the default of 4e9, about 2 s, which is also the most).  A healthy wait takes microseconds. */
 int yb_paged_attention_wait_budget(long long clocks);
+
+/* ---------------------------------------------------------------- a token for every row of logits
+ * yalm's Sampler (src/sampler.cpp:11-64) for the rows of a batch, each with settings of its own, and the usual limits:
+ * of a row l of `vocab` logits (dtype YB_DTYPE_*, rows logits_stride elements apart, any alignment to the type)
+ *   w_i = exp((l_i - max l) / temperature);
+ *   with top_k in 1 .. vocab - 1: the top_k first tokens, by l descending, then by index;
+ *   with top_p < 1: of those the fewest, in that order, whose weights sum to at least top_p times the sum of those;
+ *   with min_p > 0: of those the ones of w_i >= min_p (more than 1 counts as 1, so the first always stays);
+ * and of those, by index, the first whose running sum reaches coin times their sum (a coin up to 0 counts as the least
+ * there is, one from 1 on as 1).  temperature <= 0 or NaN: the first index of the maximum, whatever the other
+ * settings are.  A top_p <= 0 keeps the first token alone.  NaN logits are never drawn (they count as -infinity); where
+ * the maximum is +infinity, its tokens share the draw.  A row without a logit above -infinity gives token 0 and probability 0.
+ * coin_dev [rows]; temperature_dev, top_k_dev, top_p_dev, min_p_dev [rows], each may be NULL: 1, and no limit.  A NaN
+ * among coins counts as 0, among limits as none.  tokens_dev [rows] gets the tokens, prob_dev [rows] (or NULL) their
+ * probability among those that were kept (1 where temperature <= 0).
+ * Numerics: logarithms and weights in 64 bits, each weight then rounded to a multiple of 2^-43 of the largest (what
+ * is under 2^-44 of it is never drawn); sums of those are exact, so the token does not depend on the device or the
+ * split of the row.  Up to 65536 rows of 2^20 logits.  Nothing is allocated, no workspace is needed. */
+int yb_sample_rows_dev(int* tokens_dev, float* prob_dev, const void* logits, long long logits_stride, int dtype,
+                       int rows, int vocab, const float* coin_dev, const float* temperature_dev, const int* top_k_dev,
+                       const float* top_p_dev, const float* min_p_dev, void* stream);
 
 /* Number of streaming multiprocessors the kernels size their grids for (device 0 if none set). */
 int yb_num_sms(void);

@@ -89,10 +89,12 @@ _SIGS = {
     "yb_attention_scratch_bytes": (_S, [_I, _I, _I, _I]),
     "yb_attention_plan_info": (_I, [_I, _I, _I, _I, _P]),
     "yb_attention_dev_noalloc": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "yb_paged_plan_dev": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "yb_paged_append_dev": (_I, [_P, _P, _LL, _P, _LL, _I, _P, _P, _F, _P, _I, _I, _P, _F, _P]),
     "yb_paged_attention_dev": (_I, [_P, _P, _LL, _P, _LL, _F, _I, _P, _P]),
     "yb_paged_attention_scratch_bytes": (_S, [_P]),
     "yb_paged_attention_wait_budget": (_I, [_LL]),
+    "yb_sample_rows_dev": (_I, [_P, _P, _P, _LL, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
     "yb_num_sms": (_I, []),
     "yb_profile_kernel": (_I, [_P, _I, _I, ctypes.POINTER(_F)]),
 }

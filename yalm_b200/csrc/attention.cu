@@ -29,6 +29,7 @@
 //     on the kv head's counter merges them.  A cache of one portion goes to one CTA, which writes
 //     the outputs itself.
 #include "attention.cuh"
+#include "cluster.cuh"
 #include "launch.h"
 #include "tmap.h"
 
@@ -46,30 +47,6 @@ constexpr int kAttnCtaSlots = 128;    // slots per CTA before a kv head's cache 
 constexpr int kAttnMaxClusters = 32;  // clusters per kv head
 constexpr int kAttnClusterSlots = 1024;  // slots per CTA of one cluster before more clusters share a kv head
 constexpr int kAttnBox = 64 * 128;    // one 64-row x 128-byte swizzled box
-
-// ---------------------------------------------------------------- cluster helpers
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_nctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-// Every thread of every CTA of the cluster arrives (release: its shared-memory writes become
-// visible to the other CTAs) and waits for all others (acquire).
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-// Generic address of the same shared-memory variable in CTA `rank` of the cluster (distributed
-// shared memory): plain loads through it, which the compiler may batch, read the peer's copy.
-__device__ __forceinline__ const float* dsmem_ptr(const float* local, uint32_t rank) {
-  uint64_t r;
-  asm volatile("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"(local), "r"(rank));
-  return reinterpret_cast<const float*>(r);
-}
 
 // Shared-memory byte offset of 16-byte chunk q (0 .. HD / 8 - 1) of row i in a staged K or V block:
 // HD / 64 boxes of 64 rows x 128 bytes, each row's eight 16-byte chunks permuted by the 128-byte

@@ -77,6 +77,25 @@ inline cudaError_t raise_smem_cap(const void* fn) {
   return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, optin - (int)fa.sharedSizeBytes);
 }
 
+// Launch with the grid's CTAs in clusters of `cluster` along x (up to 8: no opt-in), programmatic as below.
+inline cudaError_t launch_cluster_params(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                         int cluster, bool pdl, void** params) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 2 : 1;
+  return cudaLaunchKernelExC(&cfg, fn, params);
+}
+
 // cudaLaunchKernelEx with the programmatic-stream-serialization attribute when `pdl` is set, so the
 // kernel may begin while the previous kernel in the stream is still running (it must call
 // griddepcontrol.wait before reading that kernel's results).

@@ -1,5 +1,5 @@
-// The paged KV cache of a batch of sequences: append (norm, rotation, store) and attention
-// (paged_append.cu, paged_attn.cu; entry points in paged_capi.cu).
+// The paged KV cache of a batch of sequences: the plan of a step, append (norm, rotation, store) and attention
+// (paged_plan.cu, paged_append.cu, paged_attn.cu; entry points in paged_capi.cu).
 #pragma once
 
 #include <cuda_runtime.h>
@@ -99,6 +99,34 @@ struct PagedAttnArgs {
   long long wait_budget;  // clocks after which a wait in the kernel gives up
   void* scratch;
 };
+// Why a step cannot be planned: status[0] of paged_plan, by bits.
+enum : int {
+  kPlanPages = 1,  // fewer free pages than its tokens need
+  kPlanRows = 2,   // more tokens than the batch has rows
+  kPlanTable = 4,  // a sequence would outgrow its row of the table
+};
+struct PagedPlanArgs {
+  const int* new_len;        // [n_seqs] tokens that a sequence brings, negative: it ends
+  const int* kv_before;      // [n_seqs] slots in its cache; may be kv_len
+  const int* kept;           // [n_seqs] first pages that an ended sequence does not give back, or null: none
+  const int* n_free_before;  // [1]; may be n_free
+  int* q_start;
+  int* kv_len;
+  int* page_table;
+  int* free_pages;  // [n_pages], of which the first n_free are free
+  int* n_free;
+  int* pos;          // [n_tokens] or null
+  long long* slots;  // [n_tokens] or null
+  int* status;       // [4]
+  int n_seqs, n_tokens, n_pages, max_pages, ps_log2;
+};
+// The slot of position p in the whole pool, or -1 where its page is not there.
+__device__ __forceinline__ long long paged_slot(const PagedPlanArgs& a, int p, int page) {
+  if (page < 0 || page >= a.n_pages) return -1;
+  return ((long long)page << a.ps_log2) + (p & ((1 << a.ps_log2) - 1));
+}
+cudaError_t paged_plan(const PagedPlanArgs& a, cudaStream_t s);
+
 int paged_attention_grid(int n_sms);  // blocks
 size_t paged_attention_scratch(int head_dim, int n_sms);
 cudaError_t paged_attention(const PagedAttnArgs& a, int head_dim, int type, int device, int n_sms, cudaStream_t s);

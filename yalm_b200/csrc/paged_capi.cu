@@ -1,19 +1,15 @@
 // C entry points of the paged KV cache: argument checks and launches.
+#include "checks.h"
 #include "engine.h"
 #include "paged.cuh"
 
 #include <atomic>
 #include <climits>
 #include <cmath>
-#include <initializer_list>
-#include <utility>
 
 using namespace yb;
 
 namespace {
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
 // Shapes and NULLs, before any CUDA call.  *empty: nothing to do.
 int check_batch(const yb_paged_batch* b, PagedBatch* out, bool* empty) {
@@ -60,19 +56,6 @@ int check_rows(const char* name, const void* p, long long stride, long long widt
   if (!aligned16(p) || stride < width || stride > (1ll << 31) || stride * size % 16)
     return set_error(YB_E_INVALID, std::string(name) + ": rows must be 16-byte aligned and at least " +
                                        std::to_string(width) + " elements apart");
-  return 0;
-}
-
-// Every buffer must be memory that the current device `dev` can read: a host pointer or another device's
-// memory is refused here instead of faulting in the kernel.
-int check_device(int dev, std::initializer_list<std::pair<const char*, const void*>> bufs) {
-  for (const auto& b : bufs) {
-    if (!b.second) continue;
-    cudaPointerAttributes at;
-    YB_CK(cudaPointerGetAttributes(&at, b.second));
-    if (at.type != cudaMemoryTypeManaged && (at.type != cudaMemoryTypeDevice || at.device != dev))
-      return set_error(YB_E_INVALID, std::string(b.first) + " is not memory of the current device");
-  }
   return 0;
 }
 
@@ -160,6 +143,52 @@ extern "C" int yb_paged_append_dev(const yb_paged_batch* b, void* q_out, long lo
   a.rotary_dim = rotary_dim;
   a.half = rope_half ? 1 : 0;
   YB_CK(paged_append(a, b->head_dim, qkv_dtype, b->dtype, device_sms(dev), static_cast<cudaStream_t>(stream)));
+  return 0;
+}
+
+extern "C" int yb_paged_plan_dev(const yb_paged_batch* b, const int* new_len_dev, const int* kv_before_dev,
+                                 const int* kept_dev, int* free_pages_dev, const int* n_free_before_dev,
+                                 int* n_free_dev, int* pos_dev, long long* slots_dev, int* status_dev, void* stream) {
+  PagedBatch p;
+  bool empty = false;
+  int rc = check_batch(b, &p, &empty);
+  if (rc) return rc;
+  if (!b->q_start_dev || !free_pages_dev || !n_free_before_dev || !n_free_dev || !status_dev ||
+      (b->n_seqs && (!b->kv_len_dev || !b->page_table_dev || !new_len_dev || !kv_before_dev)))
+    return set_error(YB_E_INVALID, "null buffer of the plan");
+  for (const void* v : {(const void*)b->q_start_dev, (const void*)b->kv_len_dev, (const void*)b->page_table_dev,
+                        (const void*)new_len_dev, (const void*)kv_before_dev, (const void*)kept_dev,
+                        (const void*)free_pages_dev, (const void*)n_free_before_dev, (const void*)n_free_dev,
+                        (const void*)pos_dev, (const void*)status_dev})
+    if (!aligned4(v)) return set_error(YB_E_INVALID, "the plan's buffers of ints must be 4-byte aligned");
+  if (reinterpret_cast<uintptr_t>(slots_dev) & 7) return set_error(YB_E_INVALID, "slots_dev must be 8-byte aligned");
+  int dev = 0;
+  YB_CK(cudaGetDevice(&dev));
+  rc = check_device(dev, {{"q_start_dev", b->q_start_dev}, {"kv_len_dev", b->kv_len_dev},
+                          {"page_table_dev", b->page_table_dev}, {"new_len_dev", new_len_dev},
+                          {"kv_before_dev", kv_before_dev}, {"kept_dev", kept_dev}, {"free_pages_dev", free_pages_dev},
+                          {"n_free_before_dev", n_free_before_dev}, {"n_free_dev", n_free_dev}, {"pos_dev", pos_dev},
+                          {"slots_dev", slots_dev}, {"status_dev", status_dev}});
+  if (rc) return rc;
+  PagedPlanArgs a{};
+  a.new_len = new_len_dev;
+  a.kv_before = kv_before_dev;
+  a.kept = kept_dev;
+  a.n_free_before = n_free_before_dev;
+  a.q_start = const_cast<int*>(b->q_start_dev);
+  a.kv_len = const_cast<int*>(b->kv_len_dev);
+  a.page_table = const_cast<int*>(b->page_table_dev);
+  a.free_pages = free_pages_dev;
+  a.n_free = n_free_dev;
+  a.pos = pos_dev;
+  a.slots = slots_dev;
+  a.status = status_dev;
+  a.n_seqs = b->n_seqs;
+  a.n_tokens = b->n_tokens;
+  a.n_pages = b->n_pages;
+  a.max_pages = b->max_pages;
+  a.ps_log2 = p.ps_log2;
+  YB_CK(paged_plan(a, static_cast<cudaStream_t>(stream)));
   return 0;
 }
 

@@ -1,7 +1,7 @@
 """The paged KV cache of a batch of sequences (include/yalm_b200.h, yb_paged_batch) on torch tensors.
 
 PagedBatch checks the tensors' types, shapes and strides once, keeps the batch descriptor, and launches
-the two kernels of a serving step: append (per-head norm, rotation, store) and attend.  The tensors
+the kernels of a serving step: plan (rows, lengths, pages), append (per-head norm, rotation, store) and attend.  The tensors
 stay the caller's: new lengths and page tables are written into them between steps, also between replays
 of a captured graph.  No counterpart in yalm, which runs one sequence over one contiguous cache.
 """
@@ -60,7 +60,7 @@ class PagedBatch:
         self._codes = {}
         self._index = k_pages.get_device()
         import torch  # the caller's tensors are torch's; the package itself does not need it
-        self._f32, self._i32 = torch.float32, torch.int32
+        self._f32, self._i32, self._i64 = torch.float32, torch.int32, torch.int64
         self._current = torch.cuda.current_stream
         self._q_shape = (self.n_tokens, self.n_heads * self.head_dim)
         self._qkv_shape = (self.n_tokens, (self.n_heads + 2 * self.n_kv_heads) * self.head_dim)
@@ -82,6 +82,22 @@ class PagedBatch:
         if t.dtype is not dtype or t.numel() < n or t.get_device() != self._index or not t.is_contiguous():
             raise ValueError(f"{name} must hold {n} contiguous {dtype} values on {self.device}")
         return t.data_ptr()
+
+    def plan(self, new_len, free_pages, n_free, status, *, kv_before=None, n_free_before=None, kept=None, pos=None,
+             slots=None, stream: int | None = None) -> None:
+        """yb_paged_plan_dev: from new_len [n_seqs] (tokens a sequence brings; negative: it ends) writes the batch's
+        q_start, kv_len and page_table, takes pages from free_pages [n_pages] and n_free [1], and fills pos [n_tokens]
+        (int32) and slots [n_tokens] (int64) where they are given.  kv_before and n_free_before: the state that it
+        starts from, else kv_len and n_free themselves.  status [4]: [0] is 0, or the step did not fit."""
+        n = int(self.c.n_seqs)
+        _lib.check(_lib.lib().yb_paged_plan_dev(
+            self._ref, self._vector(new_len, "new_len", n, self._i32),
+            self._vector(self._keep[4] if kv_before is None else kv_before, "kv_before", n, self._i32),
+            self._vector(kept, "kept", n, self._i32), self._vector(free_pages, "free_pages", self.c.n_pages, self._i32),
+            self._vector(n_free if n_free_before is None else n_free_before, "n_free_before", 1, self._i32),
+            self._vector(n_free, "n_free", 1, self._i32), self._vector(pos, "pos", self.n_tokens, self._i32),
+            self._vector(slots, "slots", self.n_tokens, self._i64), self._vector(status, "status", 4, self._i32),
+            self._stream() if stream is None else stream))
 
     def append(self, qkv, q_out, inv_freq, rotary_dim: int, *, q_norm=None, k_norm=None, eps: float = 1e-5,
                half: bool = False, pos=None, clip: float = FLT_MAX, stream: int | None = None) -> None:
