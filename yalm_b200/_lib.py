@@ -93,6 +93,8 @@ _SIGS = {
     "yb_paged_append_dev": (_I, [_P, _P, _LL, _P, _LL, _I, _P, _P, _F, _P, _I, _I, _P, _F, _P]),
     "yb_paged_attention_dev": (_I, [_P, _P, _LL, _P, _LL, _F, _I, _P, _P]),
     "yb_paged_attention_scratch_bytes": (_S, [_P]),
+    "yb_paged_attention_shared_dev": (_I, [_P, _I, _P, _P, _P, _LL, _P, _LL, _F, _P, _P]),
+    "yb_paged_attention_shared_scratch_bytes": (_S, [_P, _I]),
     "yb_paged_attention_wait_budget": (_I, [_LL]),
     "yb_sample_rows_dev": (_I, [_P, _P, _P, _LL, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
     "yb_num_sms": (_I, []),

@@ -98,6 +98,11 @@ struct PagedAttnArgs {
   int window;  // slots a token sees, itself counted; INT_MAX: all of them
   long long wait_budget;  // clocks after which a wait in the kernel gives up
   void* scratch;
+  // with shared prefixes (no window)
+  const int* group_start;
+  const int* prefix_len;
+  int n_groups;
+  int n_sms;
 };
 // Why a step cannot be planned: status[0] of paged_plan, by bits.
 enum : int {
@@ -130,5 +135,7 @@ cudaError_t paged_plan(const PagedPlanArgs& a, cudaStream_t s);
 int paged_attention_grid(int n_sms);  // blocks
 size_t paged_attention_scratch(int head_dim, int n_sms);
 cudaError_t paged_attention(const PagedAttnArgs& a, int head_dim, int type, int device, int n_sms, cudaStream_t s);
+size_t paged_shared_scratch(const PagedBatch& b, int n_groups, int head_dim, int n_sms);
+cudaError_t paged_attention_shared(const PagedAttnArgs& a, int head_dim, int type, int device, cudaStream_t s);
 
 }  // namespace yb

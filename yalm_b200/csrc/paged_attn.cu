@@ -51,7 +51,7 @@
 #include <type_traits>
 
 #include "launch.h"
-#include "paged_axis.cuh"
+#include "paged_shared.cuh"
 #include "tmap.h"
 #include "umma.cuh"
 
@@ -137,9 +137,45 @@ __device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long lon
   *s_start = st;
 }
 
+// The same from a plan in the workspace, by one warp.
+__device__ void find_start(const SharedBatch& b, const SharedHead* head, const Axis& x, StartOf<SharedSeq>* s_start) {
+  const int lane = threadIdx.x & 31, c = blockIdx.x;
+  const unsigned long long total = __ldca(&head->total), share = __ldca(&head->share);
+  const int more = __ldca(&head->more);
+  const unsigned long long begin = block_begin(share, more, c);
+  if (begin >= total) {
+    if (lane == 0) s_start->left = 0;
+    return;
+  }
+  // the last prefix or sequence that begins at or before the block: one that begins there and has no length comes earlier
+  int lo = 0, hi = b.n_seqs;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
+    const bool le = at < hi && __ldca(&b.seqs[at].begin) <= begin;
+    const int n = __popc(__ballot_sync(0xffffffffu, le));
+    lo += n * step;
+    hi = min(hi, lo + step);
+  }
+  if (lane) return;
+  StartOf<SharedSeq> st;
+  st.sq = paged_seq(b, lo);
+  st.seq = lo;
+  const unsigned long long rem = begin - st.sq.begin;
+  const unsigned per_head = head_tiles(x, st.sq);
+  st.head = (int)quot(rem, per_head);
+  st.unit = 0;
+  st.off = (int)(rem - (unsigned long long)st.head * per_head);
+  st.left = (int)min(share + (c < more ? 1 : 0), total - begin);
+  st.begin = begin;
+  st.share = share;
+  st.more = more;
+  *s_start = st;
+}
+
 // Called by a whole warp: the unit in which position st.off of the head lies, and the position within it.  Unit u
 // begins at units_before(u); 32 guesses at a time.
-__device__ __forceinline__ void find_unit(const Axis& x, Start& st) {
+template <typename Seq>
+__device__ __forceinline__ void find_unit(const Axis& x, StartOf<Seq>& st) {
   int lo = 0, hi = n_units(x, st.sq);  // units_before(lo) <= off < units_before(hi)
   if (hi == 1) return;
   const int lane = threadIdx.x & 31;
@@ -223,6 +259,12 @@ struct PagedAttnParams {
   unsigned* status;
   Cut* cuts;
   float* recs;
+  // with shared prefixes
+  SharedBatch shared;
+  const SharedHead* head;
+  int n_groups;
+  int part_rows;  // rows of a kv head in parts: of the tokens that have both
+  float* parts;   // [prefixes, sequences][kv heads], a record of part_rows rows each
 };
 
 // Waits for the phase, or until the budget has run out, here or in another warp of the block, which *mark then tells.
@@ -241,11 +283,14 @@ __device__ __forceinline__ void bounded_wait(uint64_t* bar, unsigned parity, con
   }
 }
 
-template <int HD, typename T>
+// kShared: the sequences are those of the plan in the workspace, the groups' prefixes among them.  A whole unit whose
+// tokens have another part goes to `parts`, as records do: paged_join_kernel puts all parts together.
+template <int HD, typename T, bool kShared>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PagedAttnParams a) {
   using C = Cfg<HD>;
+  using Seq = std::conditional_t<kShared, SharedSeq, PagedSeq>;
   constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
   constexpr uint32_t kIdS = kBf16 ? umma_idesc_bf16(kRows, kST, 0, 0) : umma_idesc_f16(kRows, kST, 0, 0);
   constexpr uint32_t kIdO = kBf16 ? umma_idesc_bf16(kRows, HD, 0, 1) : umma_idesc_f16(kRows, HD, 0, 1);
@@ -277,10 +322,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int s_abort, s_late;  // a wait has run out; one for what is in flight at the end
   __shared__ unsigned s_issued[2][2];  // keys, values: the slots that copies were issued into, and whose count is odd
   __shared__ unsigned long long s_scan[kThreads / 32];
-  __shared__ Start s_start;
+  __shared__ StartOf<Seq> s_start;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedBatch& b = a.b;
+  const auto& seqs = [&]() -> const auto& {
+    if constexpr (kShared) return a.shared;
+    else return a.b;
+  }();
+  auto table_of = [](const PieceOf<Seq>& c) {  // the piece's row of the page table
+    if constexpr (kShared) return c.sq.table;
+    else return c.seq;
+  };
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
                  : "memory");
@@ -298,7 +351,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   pdl_wait();  // up to here nothing of what earlier kernels write was touched
-  find_start(b, a.x, s_scan, &s_start);
+  if constexpr (kShared) {
+    if (warp == 0) find_start(a.shared, a.head, a.x, &s_start);
+  } else {
+    find_start(b, a.x, s_scan, &s_start);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -310,10 +367,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto wait = [&](uint64_t* bar, unsigned parity) { bounded_wait(bar, parity, a.budget, &s_abort, a.status); };
   auto aborted = [&] { return __any_sync(0xffffffffu, *static_cast<volatile int*>(&s_abort)) != 0; };
   const int QB = kRows / a.gq;
-  Start st0 = s_start;
+  StartOf<Seq> st0 = s_start;
   if (st0.left > 0) find_unit(a.x, st0);
-  Walk walk(st0);
-  Piece pc;
+  WalkOf<Seq> walk(st0);
+  PieceOf<Seq> pc;
   if (warp >= 4) {
     // ------------------------------------------------------------------------------- softmax
     const int p = (warp - 4) >> 2, quad = warp & 3;  // pipeline, tensor-memory lane quadrant
@@ -322,15 +379,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ts = tmem + lanes + (uint32_t)p * 2 * kST, to = tmem + lanes + kColO;
     const int qi = r / a.gq, h = r % a.gq;
     unsigned steps = 0, singles = 0;  // a pipeline's steps in the pieces before; pieces of one row tile
-    if (threadIdx.x == 128) a.cuts[blockIdx.x].parts = 0;  // the same thread's later store tells otherwise
+    if (!kShared && threadIdx.x == 128) a.cuts[blockIdx.x].parts = 0;  // the same thread's later store tells otherwise
     // whether the 16 slots of lane i < 8 in key tile t of a piece are on a page that is there
-    auto there = [&](const Piece& c, int t) {
+    auto there = [&](const PieceOf<Seq>& c, int t) {
       const int slot = ((c.u.tile0 + c.t0 + t) << 7) + lane * 16;
       int id = -1;
-      if (lane < 8 && slot < c.sq.kv) id = __ldca(b.page_table + (size_t)c.seq * b.max_pages + (slot >> b.ps_log2));
+      if (lane < 8 && slot < c.sq.kv) id = __ldca(b.page_table + (size_t)table_of(c) * b.max_pages + (slot >> b.ps_log2));
       return id >= 0 && id < b.n_pages;
     };
-    bool more = walk.next(b, a.x, pc), nx = more && there(pc, 0);  // (a unit without a slot has one empty tile)
+    bool more = walk.next(seqs, a.x, pc), nx = more && there(pc, 0);  // (a unit without a slot has one empty tile)
     while (more && !aborted()) {
       const bool two = pc.u.nq > QB;
       const int nk = pc.u.none ? 0 : pc.t1 - pc.t0, n = two ? 2 * nk : nk;  // key tiles, steps
@@ -338,7 +395,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int q = tile * QB + qi;  // query of the unit
       const bool valid = r < QB * a.gq && q < pc.u.nq;
       const bool live = quad * 32 < min(QB, pc.u.nq - tile * QB) * a.gq;  // any row of the warp
-      const int pos = pc.sq.kv - pc.sq.n + pc.u.q0 + q;
+      int pos = pc.sq.kv - pc.sq.n + pc.u.q0 + q;
+      if constexpr (kShared)
+        if (pc.sq.all) pos = pc.sq.kv - 1;
       const int first = pc.u.tile0 + pc.t0;
       // The two warps of a quadrant share a scheduler and its special-function unit: they take their exponentials
       // in turns, one's under the other's loads, maxima and waits.  Left alone they fall into step.
@@ -434,8 +493,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // the piece after this one is looked up under the last product and the stores
       const int left = walk.st.left;
-      Piece after;
-      more = walk.next(b, a.x, after);
+      PieceOf<Seq> after;
+      more = walk.next(seqs, a.x, after);
       nx = more && there(after, 0);
       // ---- the piece's rows: o * w0 (+ o of pipeline 1 * w1) (+ o of the pieces before * w2)
       const bool other = !two && nk > 0;  // pipeline 0 takes pipeline 1's rows in
@@ -469,6 +528,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int rows = pc.u.nq * a.gq, row = tile * QB * a.gq + r;
       const int token = pc.sq.row0 + pc.u.q0;
       float* rec = a.recs + ((size_t)blockIdx.x * 2 + (pc.from == 0 ? 1 : 0)) * rec_floats<HD>();
+      // the outputs themselves, or a record: the block's, or with shared prefixes that of the rows in their place
+      bool final = whole;
+      float* to_rec = rec;
+      int to_rows = rows, to_at = row;
+      if constexpr (kShared)
+        if (whole && pc.sq.part >= 0) {
+          final = false;
+          to_rows = a.part_rows;
+          to_at = (pc.sq.part + pc.u.q0) * a.gq + row;
+          to_rec = a.parts + (size_t)((pc.sq.all ? 0 : a.x.K) + pc.head) * (HD + 2) * a.part_rows;
+        }
       T* out = static_cast<T*>(a.out) + (size_t)(token + q) * a.out_stride + (size_t)(pc.head * a.gq + h) * HD;
       if (two || p == 0) {
         float w2 = 0.f;
@@ -481,11 +551,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           l = l * f + rec[(HD + 1) * rows + row] * w2;
           m = mm;
         }
-        const float inv = whole ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
+        const float inv = final ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
         w0 *= inv;
         w1 *= inv;
         w2 *= inv;
-        if (live && two && whole && !joins && nk > 0) {
+        if (live && two && final && !joins && nk > 0) {
           // Whole outputs of many rows: of 32 columns a lane holds its row's four groups of 16 bytes.  Two lanes exchange
           // two of theirs, so that a store writes whole sectors of 32 bytes of every second row.
           const bool up = lane & 1;
@@ -525,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float v[32];
             if (nk > 0) {
               tmem_ld32(to + p * HD + c0, v);
-              if (other || whole || joins) {  // a row that has seen no slot has zeros there: its weights were all 0
+              if (other || final || joins) {  // a row that has seen no slot has zeros there: its weights were all 0
                 const float2 w00 = make_float2(w0, w0);
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
@@ -559,28 +629,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 v[4 * k + 3] = fmaf(f.w, w2, v[4 * k + 3]);
               }
             }
-            if (whole) {
+            if (final) {
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 reinterpret_cast<uint4*>(out + c0)[k] =
                     make_uint4(pack2<T>(v[8 * k], v[8 * k + 1]), pack2<T>(v[8 * k + 2], v[8 * k + 3]),
                                pack2<T>(v[8 * k + 4], v[8 * k + 5]), pack2<T>(v[8 * k + 6], v[8 * k + 7]));
             } else {
-              float4* o = reinterpret_cast<float4*>(rec) + (size_t)(c0 / 4) * rows + row;
+              float4* o = reinterpret_cast<float4*>(to_rec) + (size_t)(c0 / 4) * to_rows + to_at;
 #pragma unroll
-              for (int k = 0; k < 8; ++k) o[(size_t)k * rows] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+              for (int k = 0; k < 8; ++k) o[(size_t)k * to_rows] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
             }
           }
         }
-        if (!whole && valid) {
-          rec[HD * rows + row] = m;
-          rec[(HD + 1) * rows + row] = l;
+        if (!final && valid) {
+          to_rec[(size_t)HD * to_rows + to_at] = m;
+          to_rec[(size_t)(HD + 1) * to_rows + to_at] = l;
         }
         tc_fence_before();
         __syncwarp();
         if (nk > 0 && lane == 0) mbar_arrive(&o_free);
       }
-      if (!whole && pc.last && pc.from == 0 && threadIdx.x == 128) {
+      if (!kShared && !whole && pc.last && pc.from == 0 && threadIdx.x == 128) {
         const unsigned long long begin = s_start.begin + (s_start.left - left) - pc.t1;  // the unit's first tile
         const int last = block_of(s_start.share, s_start.more, begin + pc.u.cost - 1);
         a.cuts[blockIdx.x] = Cut{token, pc.u.nq, pc.head, last - (int)blockIdx.x + 1};
@@ -600,10 +670,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     unsigned mine_into = 0, mine_odd = 0;  // the slots that this warp's copies went into, and whose count is odd
     int buf = 0;  // buffer of the next unit of one row tile
     bool ok = true;
-    while (ok && walk.next(b, a.x, pc)) {
+    while (ok && walk.next(seqs, a.x, pc)) {
       if (pc.u.none) continue;
       const bool two = pc.u.nq > QB;
-      const int* table = b.page_table + (size_t)pc.seq * b.max_pages;
+      const int* table = b.page_table + (size_t)table_of(pc) * b.max_pages;
       // this lane's page of a key tile, and the row of the page pool where it starts (outside the pool: zeros)
       auto page_of = [&](int tile) {
         const int at = (tile << 7) + (lane << lg);
@@ -692,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int buf = 0;
     const uint32_t e = elect_lane();
     bool any = false;
-    while (!aborted() && walk.next(b, a.x, pc)) {
+    while (!aborted() && walk.next(seqs, a.x, pc)) {
       if (pc.u.none) continue;
       const bool two = pc.u.nq > QB;
       const int first = pc.u.tile0 + pc.t0, nk = pc.t1 - pc.t0, n = two ? 2 * nk : nk;
@@ -858,6 +928,84 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
   }
 }
 
+// Shared prefixes: out = sum_parts 2^(m - M) o / sum_parts 2^(m - M) l over all parts of a row, those of its group's
+// prefix and those of its own slots, each a record in `parts` or, of a unit that was cut, several of the blocks'.  8
+// elements of a row are a thread's; neighbouring lanes have neighbouring rows, as the records hold them.
+constexpr int kJoinThreads = 128;
+template <int HD, typename T>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams a) {
+  pdl_wait();
+  const PagedBatch& b = a.b;
+  const long long item = (long long)blockIdx.x * kJoinThreads + threadIdx.x, rows = (long long)b.n_tokens * a.gq;
+  const int row = (int)(item % rows), token = row / a.gq, h = row % a.gq;
+  const long long rest = item / rows;
+  const int c8 = (int)(rest % (HD / 8)), head = (int)(rest / (HD / 8));
+  if (head >= a.x.K) return;
+  int lo = 0, hi = b.n_seqs;  // the last sequence that starts at or before the token
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (__ldca(b.q_start + mid) <= token) lo = mid;
+    else hi = mid;
+  }
+  const SharedSeq own = paged_seq(a.shared, a.n_groups + lo);
+  if (token < own.row0 || token >= own.row0 + own.n) return;
+  const unsigned long long share = __ldca(&a.head->share);
+  const int more = __ldca(&a.head->more);
+  float mm = -INFINITY, ll = 0.f, acc[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+  // a unit's parts: false if its outputs are in their place already
+  auto take = [&](const SharedSeq& q) {
+    const int at = token - q.row0, unit = at / a.x.U;
+    const Unit u = unit_of(a.x, q, unit);
+    const unsigned long long begin = q.begin + (unsigned long long)head_tiles(a.x, q) * head + units_before(a.x, q, unit);
+    const int first = block_of(share, more, begin), parts = block_of(share, more, begin + u.cost - 1) - first + 1;
+    if (parts == 1 && q.part < 0) return false;
+    int rs = u.nq * a.gq, r = (at - u.q0) * a.gq + h;
+    const float* whole = nullptr;
+    if (parts == 1) {
+      rs = a.part_rows;
+      r = (q.part + at) * a.gq + h;
+      whole = a.parts + (size_t)((q.all ? 0 : a.x.K) + head) * (HD + 2) * rs;
+    }
+    for (int p0 = 0; p0 < parts; p0 += kMergeParts) {
+      float m[kMergeParts], l[kMergeParts];
+      float4 o[kMergeParts][2];
+#pragma unroll
+      for (int k = 0; k < kMergeParts; ++k) {
+        m[k] = -INFINITY;
+        l[k] = 0.f;
+        o[k][0] = o[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p0 + k < parts) {
+          const float* rec = whole ? whole : a.recs + ((size_t)(first + p0 + k) * 2 + (p0 + k == 0 ? 1 : 0)) * rec_floats<HD>();
+          const float4* ro = reinterpret_cast<const float4*>(rec) + (size_t)(2 * c8) * rs + r;
+          o[k][0] = __ldcg(ro);
+          o[k][1] = __ldcg(ro + rs);
+          m[k] = __ldcg(rec + (size_t)HD * rs + r);
+          l[k] = __ldcg(rec + (size_t)(HD + 1) * rs + r);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kMergeParts; ++k) {
+        const float v[8] = {o[k][0].x, o[k][0].y, o[k][0].z, o[k][0].w, o[k][1].x, o[k][1].y, o[k][1].z, o[k][1].w};
+        const float mn = fmaxf(mm, m[k]);
+        const float old = mm == -INFINITY ? 0.f : ex2(mm - mn), w = m[k] == -INFINITY ? 0.f : ex2(m[k] - mn);
+        mm = mn;
+        ll = ll * old + l[k] * w;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = acc[j] * old + v[j] * w;
+      }
+    }
+    return true;
+  };
+  if (!take(own)) return;
+  if (own.part >= 0) take(paged_seq(a.shared, own.group));
+  const float inv = ll != 0.f ? 1.f / ll : 0.f;
+  T* out = static_cast<T*>(a.out) + (size_t)token * a.out_stride + (size_t)(head * a.gq + h) * HD + 8 * c8;
+  *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv),
+                                              pack2<T>(acc[4] * inv, acc[5] * inv), pack2<T>(acc[6] * inv, acc[7] * inv));
+}
+
 int paged_attention_grid(int n_sms) { return n_sms < kMaxGrid ? n_sms : kMaxGrid; }
 
 size_t paged_attention_scratch(int head_dim, int n_sms) {
@@ -865,8 +1013,24 @@ size_t paged_attention_scratch(int head_dim, int n_sms) {
   return kHeadBytes + (size_t)grid * 2 * (head_dim == 128 ? rec_floats<128>() : rec_floats<64>()) * 4;
 }
 
+// Rows (queries x query heads of a kv head) of the tokens that have a part in `parts`: of all, or of the most that groups
+// computed once may have, which is a unit's for every sequence (paged_shared.cu).
+static int part_tokens(const PagedBatch& b) {
+  const long long most = (long long)b.n_seqs * 2 * (kRows / (b.n_heads / b.n_kv_heads));
+  return (int)(b.n_tokens < most ? b.n_tokens : most);
+}
+static long long part_rows(const PagedBatch& b) { return ((long long)part_tokens(b) * (b.n_heads / b.n_kv_heads) + 3) / 4 * 4; }
+// Its workspace: that of a call without prefixes, the plan, the parts.
+static size_t shared_plan_at(int head_dim, int n_sms) { return (paged_attention_scratch(head_dim, n_sms) + 255) / 256 * 256; }
+static size_t shared_parts_at(const PagedBatch& b, int n_groups, int head_dim, int n_sms) {
+  return shared_plan_at(head_dim, n_sms) + 256 + ((size_t)n_groups + b.n_seqs) * sizeof(SharedSeq);
+}
+size_t paged_shared_scratch(const PagedBatch& b, int n_groups, int head_dim, int n_sms) {
+  return shared_parts_at(b, n_groups, head_dim, n_sms) + (size_t)2 * b.n_kv_heads * (head_dim + 2) * part_rows(b) * 4;
+}
+
 namespace {
-template <int HD, typename T>
+template <int HD, typename T, bool kShared>
 cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cudaStream_t s) {
   const int K = a.b.n_kv_heads, ps = 1 << a.b.ps_log2, gq = a.b.n_heads / K, qb = kRows / gq;
   const long long rows = (long long)a.b.n_pages * K * ps;
@@ -876,7 +1040,7 @@ cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cuda
       !tmap_f16_2d_sw128(&km, static_cast<const __half*>(a.k_pages), rows, HD, 64, box) ||
       !tmap_f16_2d_sw128(&vm, static_cast<const __half*>(a.v_pages), rows, HD, 64, box))
     return cudaErrorInvalidValue;
-  PagedAttnParams p;
+  PagedAttnParams p{};
   p.b = a.b;
   p.x = Axis{2 * qb, a.window < (1 << 22) ? a.window : 1 << 22, K};
   p.out = a.out;
@@ -889,25 +1053,50 @@ cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cuda
   p.status = static_cast<unsigned*>(a.scratch);
   p.cuts = reinterpret_cast<Cut*>(static_cast<char*>(a.scratch) + 256);
   p.recs = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kHeadBytes);
-  const void* fn = reinterpret_cast<const void*>(&paged_attn_kernel<HD, T>);
+  const void* fn = reinterpret_cast<const void*>(&paged_attn_kernel<HD, T, kShared>);
   static SmemCap cap;
   cudaError_t e = cap.raise(fn, device, Cfg<HD>::kSmem);
   if (e != cudaSuccess) return e;
+  if constexpr (kShared) {
+    char* const base = static_cast<char*>(a.scratch);
+    const size_t plan = shared_plan_at(HD, a.n_sms);
+    SharedPlanArgs sp{a.b, a.group_start, a.prefix_len, a.n_groups, p.x, grid, part_tokens(a.b), reinterpret_cast<SharedHead*>(base + plan),
+                      reinterpret_cast<SharedSeq*>(base + plan + 256)};
+    p.shared = SharedBatch{sp.seqs, a.n_groups + a.b.n_seqs};
+    p.head = sp.head;
+    p.n_groups = a.n_groups;
+    p.part_rows = (int)part_rows(a.b);
+    p.parts = reinterpret_cast<float*>(base + shared_parts_at(a.b, a.n_groups, HD, a.n_sms));
+    if ((e = paged_shared_plan(sp, s)) != cudaSuccess) return e;
+  }
   void* args[] = {&qm, &km, &vm, &p};
   // both kernels set up under the end of the one before (programmatic launch): 37.0 -> 33.1 us for one token over
   // 32767 slots, 47.8 -> 43.9 us for the chunk of 512
   if ((e = launch_kernel_params(fn, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, s, true, args)) != cudaSuccess) return e;
   if (a.b.max_pages * ps <= kKT) return cudaSuccess;  // every unit is one key tile: nothing is cut
+  if constexpr (kShared) {
+    const long long items = (long long)a.b.n_tokens * gq * K * (HD / 8);
+    return launch_kernel(reinterpret_cast<const void*>(&paged_join_kernel<HD, T>),
+                         dim3((unsigned)((items + kJoinThreads - 1) / kJoinThreads)), dim3(kJoinThreads), 0, s, true, &p);
+  }
   return launch_kernel(reinterpret_cast<const void*>(&paged_merge_kernel<HD, T>), dim3(grid, kMergeSlices),
                        dim3(kMergeThreads), 0, s, true, &p);
 }
 }  // namespace
 
-cudaError_t paged_attention(const PagedAttnArgs& a, int head_dim, int type, int device, int n_sms, cudaStream_t s) {
-  const int grid = paged_attention_grid(n_sms);
+template <bool kShared>
+static cudaError_t launch_any(const PagedAttnArgs& a, int head_dim, int type, int device, int grid, cudaStream_t s) {
   if (head_dim == 128)
-    return type == 1 ? launch<128, __half>(a, device, grid, false, s) : launch<128, __nv_bfloat16>(a, device, grid, true, s);
-  return type == 1 ? launch<64, __half>(a, device, grid, false, s) : launch<64, __nv_bfloat16>(a, device, grid, true, s);
+    return type == 1 ? launch<128, __half, kShared>(a, device, grid, false, s)
+                     : launch<128, __nv_bfloat16, kShared>(a, device, grid, true, s);
+  return type == 1 ? launch<64, __half, kShared>(a, device, grid, false, s)
+                   : launch<64, __nv_bfloat16, kShared>(a, device, grid, true, s);
+}
+cudaError_t paged_attention(const PagedAttnArgs& a, int head_dim, int type, int device, int n_sms, cudaStream_t s) {
+  return launch_any<false>(a, head_dim, type, device, paged_attention_grid(n_sms), s);
+}
+cudaError_t paged_attention_shared(const PagedAttnArgs& a, int head_dim, int type, int device, cudaStream_t s) {
+  return launch_any<true>(a, head_dim, type, device, paged_attention_grid(a.n_sms), s);
 }
 
 }  // namespace yb

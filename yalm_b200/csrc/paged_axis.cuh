@@ -101,14 +101,16 @@ __device__ __forceinline__ unsigned head_tiles(const Axis& x, const PagedSeq& q)
 // 22.5, three hundred other batches in a model of it 0.3 % less.)
 // Shares of a few tiles are all the same instead, and the last blocks have none: they end no later, and cut less
 // (one token over 4096 slots 16.2 -> 14.9 us; with shares of 12 tiles a mixed step took 55.5 us, not 51).
-struct Start {
-  PagedSeq sq;
+template <typename Seq>
+struct StartOf {
+  Seq sq;
   int seq, head, unit, off;
   int left;                  // length of this block's part of the axis
   unsigned long long begin;  // where it begins
   unsigned long long share;
   int more;
 };
+using Start = StartOf<PagedSeq>;
 // a / b: in 32 bits where both fit, as they nearly always do
 __device__ __forceinline__ unsigned long long quot(unsigned long long a, unsigned long long b) {
   if (!((a | b) >> 32)) return (unsigned)a / (unsigned)b;
@@ -129,19 +131,23 @@ __device__ __forceinline__ int block_of(unsigned long long share, int more, unsi
 }
 
 // The next piece of this block's share: tiles [t0, t1) of a unit, of which the block has those from `from` on.
-struct Piece {
-  PagedSeq sq;
+template <typename Seq>
+struct PieceOf {
+  Seq sq;
   int seq, head;
   Unit u;
   int from, t0, t1;
   bool last;  // of the block's pieces of the unit
 };
-struct Walk {
-  Start st;
-  PagedSeq sq;
+using Piece = PieceOf<PagedSeq>;
+template <typename Seq>
+struct WalkOf {
+  StartOf<Seq> st;
+  Seq sq;
   int from;  // of the unit that a piece before this one began; -1: none
-  __device__ __forceinline__ explicit Walk(const Start& s) : st(s), sq(s.sq), from(-1) {}
-  __device__ __forceinline__ bool next(const PagedBatch& b, const Axis& x, Piece& p) {
+  __device__ __forceinline__ explicit WalkOf(const StartOf<Seq>& s) : st(s), sq(s.sq), from(-1) {}
+  template <typename Batch>
+  __device__ __forceinline__ bool next(const Batch& b, const Axis& x, PieceOf<Seq>& p) {
     do {
       if (st.left <= 0 || st.seq >= b.n_seqs) return false;
       p.sq = sq;
@@ -176,6 +182,7 @@ struct Walk {
     return true;
   }
 };
+using Walk = WalkOf<PagedSeq>;
 
 }  // namespace
 

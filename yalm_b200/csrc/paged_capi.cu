@@ -1,7 +1,7 @@
 // C entry points of the paged KV cache: argument checks and launches.
 #include "checks.h"
 #include "engine.h"
-#include "paged.cuh"
+#include "paged_shared.cuh"
 
 #include <atomic>
 #include <climits>
@@ -78,9 +78,11 @@ int device_sms(int dev) {
 // What one of the attention's blocks may have to walk is counted in 31 bits: the units (blocks of up to 2 * (128 /
 // query heads per kv head) queries) of every sequence and kv head, with the key tiles of 128 slots of the longest cache
 // and 3 more each, shared out over the blocks.
-int check_share(const yb_paged_batch* b, const PagedBatch& p, int dev) {
+// With `groups` > 0 shared prefixes, which are units of their own.
+int check_share(const yb_paged_batch* b, const PagedBatch& p, int dev, int groups = 0) {
   const long long queries = 2 * (128 / (b->n_heads / b->n_kv_heads));
-  const long long units = b->n_tokens / queries + (b->n_seqs < b->n_tokens ? b->n_seqs : b->n_tokens);
+  long long units = b->n_tokens / queries + (b->n_seqs < b->n_tokens ? b->n_seqs : b->n_tokens);
+  if (groups) units += b->n_tokens / queries + groups;
   const long long tiles = (((long long)b->max_pages << p.ps_log2) >> 7) + 3;
   if (units * b->n_kv_heads * tiles / paged_attention_grid(device_sms(dev)) >= INT_MAX)
     return set_error(YB_E_UNSUPPORTED, "the batch may have too many slots to attend to on this device "
@@ -208,36 +210,89 @@ extern "C" int yb_paged_attention_wait_budget(long long clocks) {
   return 0;
 }
 
+// What both forms of the attention check before any CUDA call; fills in what they have in common.
+static int check_attention(const yb_paged_batch* b, PagedAttnArgs* a, bool* empty, void* out, long long out_stride,
+                           const void* q, long long q_stride, float scale, void* scratch_dev) {
+  int rc = check_batch(b, &a->b, empty);
+  if (rc) return rc;
+  const long long width = (long long)b->n_heads * b->head_dim;
+  if ((rc = check_rows("out", out, out_stride, width, 2, *empty)) || (rc = check_rows("q", q, q_stride, width, 2, *empty))) return rc;
+  if (!(scale > 0.f) || !std::isfinite(scale * 1.4426950408889634f))
+    return set_error(YB_E_INVALID, "scale must be positive, and scale * log2(e) finite");
+  if (!scratch_dev || !aligned16(scratch_dev)) return set_error(YB_E_INVALID, "scratch_dev must be 16-byte aligned memory");
+  a->q = q;
+  a->out = out;
+  a->k_pages = b->k_pages;
+  a->v_pages = b->v_pages;
+  a->q_stride = q_stride;
+  a->out_stride = out_stride;
+  a->scale = scale;
+  a->scratch = scratch_dev;
+  a->wait_budget = wait_budget.load(std::memory_order_relaxed);
+  return 0;
+}
+static int check_attention_device(int dev, const yb_paged_batch* b, const void* out, const void* q, const void* scratch_dev) {
+  return check_device(dev, {{"out", out}, {"q", q}, {"q_start_dev", b->q_start_dev}, {"kv_len_dev", b->kv_len_dev},
+                     {"page_table_dev", b->page_table_dev}, {"k_pages", b->k_pages}, {"v_pages", b->v_pages},
+                     {"scratch_dev", scratch_dev}});
+}
+
 extern "C" int yb_paged_attention_dev(const yb_paged_batch* b, void* out, long long out_stride, const void* q,
                                       long long q_stride, float scale, int window, void* scratch_dev, void* stream) {
   PagedAttnArgs a{};
   bool empty = false;
-  int rc = check_batch(b, &a.b, &empty);
+  int rc = check_attention(b, &a, &empty, out, out_stride, q, q_stride, scale, scratch_dev);
   if (rc) return rc;
-  const long long width = (long long)b->n_heads * b->head_dim;
-  if ((rc = check_rows("out", out, out_stride, width, 2, empty)) || (rc = check_rows("q", q, q_stride, width, 2, empty))) return rc;
-  if (!(scale > 0.f) || !std::isfinite(scale * 1.4426950408889634f))
-    return set_error(YB_E_INVALID, "scale must be positive, and scale * log2(e) finite");
   if (window < 0) return set_error(YB_E_INVALID, "negative window");
-  if (!scratch_dev || !aligned16(scratch_dev)) return set_error(YB_E_INVALID, "scratch_dev must be 16-byte aligned memory");
   if (empty) return 0;
   if ((rc = check_share(b, a.b, current_device()))) return rc;
   int dev = 0;
   YB_CK(cudaGetDevice(&dev));
-  rc = check_device(dev, {{"out", out}, {"q", q}, {"q_start_dev", b->q_start_dev}, {"kv_len_dev", b->kv_len_dev},
-                     {"page_table_dev", b->page_table_dev}, {"k_pages", b->k_pages}, {"v_pages", b->v_pages},
-                     {"scratch_dev", scratch_dev}});
-  if (rc) return rc;
-  a.q = q;
-  a.out = out;
-  a.k_pages = b->k_pages;
-  a.v_pages = b->v_pages;
-  a.q_stride = q_stride;
-  a.out_stride = out_stride;
-  a.scale = scale;
+  if ((rc = check_attention_device(dev, b, out, q, scratch_dev))) return rc;
   a.window = window ? window : INT_MAX;
-  a.scratch = scratch_dev;
-  a.wait_budget = wait_budget.load(std::memory_order_relaxed);
   YB_CK(paged_attention(a, b->head_dim, b->dtype, dev, device_sms(dev), static_cast<cudaStream_t>(stream)));
+  return 0;
+}
+
+static int check_groups(int n_groups) {
+  if (n_groups < 0) return set_error(YB_E_INVALID, "negative n_groups");
+  if (n_groups > kMaxGroups) return set_error(YB_E_UNSUPPORTED, "at most 2048 groups with a shared prefix");
+  return 0;
+}
+
+extern "C" size_t yb_paged_attention_shared_scratch_bytes(const yb_paged_batch* b, int n_groups) {
+  PagedBatch p;
+  bool empty;
+  if (check_batch(b, &p, &empty) || check_groups(n_groups)) return 0;
+  const int dev = current_device();
+  if (check_share(b, p, dev, n_groups)) return 0;
+  return paged_shared_scratch(p, n_groups, b->head_dim, device_sms(dev));
+}
+
+extern "C" int yb_paged_attention_shared_dev(const yb_paged_batch* b, int n_groups, const int* group_start_dev,
+                                             const int* prefix_len_dev, void* out, long long out_stride, const void* q,
+                                             long long q_stride, float scale, void* scratch_dev, void* stream) {
+  int rc = check_groups(n_groups);
+  if (rc) return rc;
+  if (n_groups == 0)  // nothing is shared
+    return yb_paged_attention_dev(b, out, out_stride, q, q_stride, scale, 0, scratch_dev, stream);
+  PagedAttnArgs a{};
+  bool empty = false;
+  if ((rc = check_attention(b, &a, &empty, out, out_stride, q, q_stride, scale, scratch_dev))) return rc;
+  if (!group_start_dev || !prefix_len_dev || !aligned4(group_start_dev) || !aligned4(prefix_len_dev))
+    return set_error(YB_E_INVALID, "group_start_dev and prefix_len_dev must be 4-byte aligned buffers");
+  if (empty) return 0;
+  if ((rc = check_share(b, a.b, current_device(), n_groups))) return rc;
+  int dev = 0;
+  YB_CK(cudaGetDevice(&dev));
+  if ((rc = check_attention_device(dev, b, out, q, scratch_dev)) ||
+      (rc = check_device(dev, {{"group_start_dev", group_start_dev}, {"prefix_len_dev", prefix_len_dev}})))
+    return rc;
+  a.window = INT_MAX;
+  a.group_start = group_start_dev;
+  a.prefix_len = prefix_len_dev;
+  a.n_groups = n_groups;
+  a.n_sms = device_sms(dev);
+  YB_CK(paged_attention_shared(a, b->head_dim, b->dtype, dev, static_cast<cudaStream_t>(stream)));
   return 0;
 }

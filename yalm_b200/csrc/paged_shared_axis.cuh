@@ -1,0 +1,49 @@
+// The axis of the paged attention's work (paged_axis.cuh) for a batch in which groups of sequences share a prefix: before
+// the sequences come the groups' prefixes, as sequences of their own, whose tokens are those of the whole group, and
+// a sequence of a group begins behind the prefix.  Integer arithmetic alone; tests compile it for the host.
+#pragma once
+
+#include "paged_axis.cuh"
+
+namespace yb {
+
+// A group's prefix or a sequence, as the kernel that plans a call (paged_shared.cu) leaves it in the workspace.
+struct __align__(16) SharedSeq {
+  int row0, n;   // tokens; of a prefix those of all its sequences
+  int kv;        // slots, the prefix's among them
+  int lo;        // first key tile: 0, or the tiles of the prefix that others look after
+  int table;     // row of the page table
+  int part;      // where its tokens' parts lie in the workspace; -1: there is no other part of them
+  int group;     // of a sequence with a part: its prefix
+  int all;       // a prefix: every token sees all of its slots
+  unsigned long long begin;  // where its units begin on the axis
+  unsigned long long pad;
+};
+struct SharedBatch {
+  const SharedSeq* seqs;
+  int n_seqs;  // with the prefixes
+};
+
+__device__ __forceinline__ Unit unit_of(const Axis& x, const SharedSeq& q, int i) {
+  Unit u;
+  u.q0 = i * x.U;
+  u.nq = min(x.U, q.n - u.q0);
+  u.tile0 = q.lo;
+  const int end = q.all ? q.kv : q.kv - q.n + u.q0 + u.nq;
+  u.none = end <= 0;
+  u.cost = max(1, ((end + kKT - 1) >> 7) - q.lo);
+  return u;
+}
+__device__ __forceinline__ int n_units(const Axis& x, const SharedSeq& q) { return q.n <= x.U ? 1 : (q.n + x.U - 1) / x.U; }
+__device__ __forceinline__ unsigned units_before(const Axis& x, const SharedSeq& q, int m) {
+  if (m == 0) return 0;
+  if (q.all) return (unsigned)m * ((unsigned)(q.kv >> 7) + kUnitTiles);
+  return (unsigned)m * (1 + kUnitTiles) + ramp(m, q.kv - q.n + x.U - 1, x.U) - (unsigned)m * q.lo;
+}
+__device__ __forceinline__ unsigned head_tiles(const Axis& x, const SharedSeq& q) {
+  if (q.n <= 0) return 0;
+  const int nu = n_units(x, q);
+  return units_before(x, q, nu - 1) + (unsigned)unit_of(x, q, nu - 1).cost + kUnitTiles;
+}
+
+}  // namespace yb

@@ -55,7 +55,8 @@ class PagedBatch:
             v_pages=v_pages.data_ptr())
         self._ref = ctypes.byref(self.c)
         self._append, self._attend = _lib.lib().yb_paged_append_dev, _lib.lib().yb_paged_attention_dev
-        self._scratch = 0
+        self._attend_shared, self._plan = _lib.lib().yb_paged_attention_shared_dev, _lib.lib().yb_paged_plan_dev
+        self._scratch, self._shared = 0, {}
         self._scale = 1.0 / math.sqrt(self.head_dim)
         self._codes = {}
         self._index = k_pages.get_device()
@@ -90,7 +91,7 @@ class PagedBatch:
         (int32) and slots [n_tokens] (int64) where they are given.  kv_before and n_free_before: the state that it
         starts from, else kv_len and n_free themselves.  status [4]: [0] is 0, or the step did not fit."""
         n = int(self.c.n_seqs)
-        _lib.check(_lib.lib().yb_paged_plan_dev(
+        _lib.check(self._plan(
             self._ref, self._vector(new_len, "new_len", n, self._i32),
             self._vector(self._keep[4] if kv_before is None else kv_before, "kv_before", n, self._i32),
             self._vector(kept, "kept", n, self._i32), self._vector(free_pages, "free_pages", self.c.n_pages, self._i32),
@@ -126,10 +127,19 @@ class PagedBatch:
                 raise _lib.YalmB200Error(_lib.YB_E_INVALID, _lib.last_error())
         return self._scratch
 
-    def _check_scratch(self, scratch) -> None:
+    def shared_scratch_bytes(self, n_groups: int) -> int:
+        """Size of attend_shared's workspace for so many groups; attend takes it too."""
+        if n_groups not in self._shared:
+            size = _lib.lib().yb_paged_attention_shared_scratch_bytes(self._ref, n_groups)
+            if not size:
+                raise _lib.YalmB200Error(_lib.YB_E_INVALID, _lib.last_error())
+            self._shared[n_groups] = size
+        return self._shared[n_groups]
+
+    def _check_scratch(self, scratch, size: int = 0) -> None:
         if scratch.get_device() != self._index or not scratch.is_contiguous() or \
-                scratch.numel() * scratch.element_size() < (self._scratch or self.scratch_bytes()):
-            raise ValueError("scratch must hold scratch_bytes() contiguous bytes")
+                scratch.numel() * scratch.element_size() < (size or self._scratch or self.scratch_bytes()):
+            raise ValueError("scratch must hold scratch_bytes() (attend_shared: shared_scratch_bytes()) contiguous bytes")
 
     def status(self, scratch) -> int:
         """Waits for the device and returns the status bits (as Model.status) of the attend calls in this workspace
@@ -159,3 +169,18 @@ class PagedBatch:
         _lib.check(self._attend(self._ref, out.data_ptr(), s_out, q.data_ptr(), s_q,
                                 self._scale if scale is None else scale, window, scratch.data_ptr(),
                                 self._stream() if stream is None else stream))
+
+    def attend_shared(self, q, out, scratch, group_start, prefix_len, *, scale: float | None = None,
+                      stream: int | None = None) -> None:
+        """yb_paged_attention_shared_dev: attend for a batch in which groups of sequences begin with the same pages.
+        group_start [n_groups + 1] int32: the groups' first sequences, prefix_len [n_groups] int32: how many slots
+        a group's sequences share.  scratch: shared_scratch_bytes(n_groups) bytes, as attend's."""
+        n = int(prefix_len.shape[0])
+        s_q, s_out = self._rows(q, "q", self._q_shape), self._rows(out, "out", self._q_shape)
+        if q.dtype != self._dtype or out.dtype != self._dtype:
+            raise ValueError("q and out must have the caches' type")
+        self._check_scratch(scratch, self.shared_scratch_bytes(n))
+        _lib.check(self._attend_shared(
+            self._ref, n, self._vector(group_start, "group_start", n + 1, self._i32),
+            self._vector(prefix_len, "prefix_len", n, self._i32), out.data_ptr(), s_out, q.data_ptr(), s_q,
+            self._scale if scale is None else scale, scratch.data_ptr(), self._stream() if stream is None else stream))
