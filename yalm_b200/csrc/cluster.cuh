@@ -20,6 +20,9 @@ __device__ __forceinline__ uint32_t cluster_nctarank() {
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// The same in two parts: a CTA that has arrived may go on with what the others do not read.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // Generic address of the same shared-memory variable in CTA `rank` of the cluster (distributed
 // shared memory): plain loads through it, which the compiler may batch, read the peer's copy.
 template <typename T>

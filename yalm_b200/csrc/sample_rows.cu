@@ -9,16 +9,18 @@
 // rounds to none of them (under 2^-44) is out of the draw.
 //
 // A cluster of blocks has a row, each block a stretch of it, which is read once into shared memory (rows too long for
-// that are read again, from L2); every later pass reads that.  The limits are found on a histogram of the weights'
-// logarithms, 16 bins an octave, whose bins are stretches of the sorted order (counts and sums, merged over the
-// cluster by its first block).  Where the limit's bin and all before it hold at most kList tokens, as a usual
-// top-k or top-p has, they are gathered in the first block, sorted, and the rest happens there.  Else the limit's
-// place is narrowed down by histograms of the range (value, then place in the row, as one 64-bit number) until
-// at most kList tokens are in it, and the draw is one more pass over the row in its order.
+// that are read again, from L2); every later pass reads that.  The limits are found on a histogram of the distance
+// to the maximum, 16 bins an octave of the weight, whose bins are stretches of the sorted order: of counts for top-k,
+// which needs no weights, of counts and sums for top-p alone.  The cluster's first block merges the blocks' bins.
+// Where the limit's bin and all before it hold at most kList tokens, as a usual top-k or top-p has, they are gathered
+// in the first block, sorted, and the rest happens there.  Else the limit's place is narrowed down by histograms of
+// the range (value, then place in the row, as one 64-bit number) until at most kList tokens are in it, and the draw
+// is one more pass over the row in its order.
 #include "sample_rows.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <float.h>
 #include <math.h>
 
 #include "cluster.cuh"
@@ -33,14 +35,36 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kOctaves = 44, kPerOctave = 16, kBins = kOctaves * kPerOctave;
-constexpr int kList = 2048;
-constexpr double kOne = 8796093022208.0;      // 2^43
-constexpr size_t kMaxStage = 160 * 1024;      // bytes of a row's stretch that shared memory takes
+constexpr int kEach = 4, kList = kThreads * kEach;  // tokens of a list: 4 a thread
+constexpr u64 kOne = 1ull << 43;                    // the largest weight
+constexpr float kLeastTemperature = 0x1p-60f;
+constexpr size_t kMaxStage = 160 * 1024;            // bytes of a row's stretch that shared memory takes
 constexpr int kMaxCluster = 8;
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// 16 bytes of logits
+template <typename T>
+struct Chunk {
+  static constexpr int kN = 16 / sizeof(T);
+  union {
+    uint4 raw;
+    T v[kN];
+  };
+  __device__ __forceinline__ Chunk() {}
+  __device__ __forceinline__ explicit Chunk(uint4 r) : raw(r) {}
+  __device__ __forceinline__ float operator[](int j) const { return to_float(v[j]); }
+};
+template <typename T>
+__device__ __forceinline__ T minus_infinity();
+template <>
+__device__ __forceinline__ float minus_infinity() { return -INFINITY; }
+template <>
+__device__ __forceinline__ __half minus_infinity() { return __ushort_as_half(0xfc00); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 minus_infinity() { return __ushort_as_bfloat16(0xff80); }
 
 // Numbers in the order of the values (no NaN comes here; -0 counts as 0), and back.
 __device__ __forceinline__ unsigned key_of(float l) {
@@ -51,20 +75,59 @@ __device__ __forceinline__ float value_of(unsigned k) { return __uint_as_float(k
 // In the order of the limits: the larger value first, then the smaller index.
 __device__ __forceinline__ u64 place_of(float l, int i) { return ((u64)key_of(l) << 32) | (unsigned)~i; }
 
-// The row's weights.
+// A finite fp32 number in 64 bits, by its bits: the conversion unit takes 16 a clock at most, and was what the weights
+// waited for.  Zeros and numbers below 2^-126 come out wrong by up to 2^-126, which no temperature here sees.
+__device__ __forceinline__ double widen(float l) {
+  const unsigned u = __float_as_uint(l);
+  return __hiloint2double((int)((u & 0x80000000u) | (((u & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(u << 29));
+}
+constexpr double kUnits = 4503599627370496.0;  // 2^52: added, it leaves a whole number of units in the low bits
+
+// The row's weights, by all lanes of a warp at once: 2^t = 2^(k / 32) 2^r with k the nearest whole number to 32 t; lane
+// j holds 2^(j / 32), and 2^r, |r| <= 1/64, is its Taylor series up to r^5 (2^-48.7 relative).  The last product adds
+// 2^52, which rounds to whole units.  11 operations in 64 bits, where exp2 takes about 25.
 struct Weights {
-  double max, c;  // log2(e) / T
-  float maxf;
+  double max, c, root;  // the maximum, log2(e) / T, 2^(lane / 32 + 43)
+  float maxf, cut;      // what lies below cut has no weight
+  float per_bin;        // bins a unit of l
   bool flat;  // all that equal the maximum weigh the same, all else nothing (T is 0, or the maximum infinite)
-  // the weight's logarithm; NaN or far below -kOctaves for what has none
-  __device__ __forceinline__ double log2_of(float l) const {
-    if (flat) return l == maxf ? 0.0 : -1e30;
-    return ((double)l - max) * c;
+  __device__ __forceinline__ void init(float m, float temp) {
+    maxf = m;
+    max = widen(m);
+    flat = !(temp > 0.f) || m == INFINITY;
+    c = 1.4426950408889634 / (double)fmaxf(temp, kLeastTemperature);
+    cut = flat ? m : fmaxf((float)((double)m - kOctaves / c), -FLT_MAX);
+    per_bin = (float)(c * kPerOctave);
+    root = exp2((threadIdx.x & 31) * (1.0 / 32) + 43.0);
   }
-  __device__ __forceinline__ double of(double t) const { return t >= -kOctaves ? exp2(t) : 0.0; }
+  __device__ __forceinline__ bool some(float l) const { return l >= cut; }
+  // of what has a weight; the sum rounds to a whole number
+  __device__ __forceinline__ int bin(float l) const {
+    const float y = fmaf(fminf(maxf - l, FLT_MAX), per_bin, 8388608.f);
+    return flat ? 0 : min(__float_as_int(y) - 0x4b000000, kBins - 1);
+  }
+  // 2^52 + the weight in units, of what has one
+  __device__ __forceinline__ double above(float l) const {
+    const double t = (widen(l) - max) * c;
+    constexpr double kRound = 6755399441055744.0;  // 1.5 2^52
+    double k = fma(t, 32.0, kRound);
+    const int n = __double2loint(k);
+    k -= kRound;
+    const double r = fma(k, -1.0 / 32, t);
+    double p = fma(r, 0.00133335581464284434, 0.00961812910762847716);
+    p = fma(r, p, 0.0555041086648215800);
+    p = fma(r, p, 0.240226506959100712);
+    p = fma(r, p, 0.693147180559945309);
+    p = fma(r, p, 1.0);
+    const int hi = __shfl_sync(0xffffffffu, __double2hiint(root), n), lo = __shfl_sync(0xffffffffu, __double2loint(root), n);
+    const double w = fma(__hiloint2double(hi + (n & ~31) * (1 << 15), lo), p, kUnits);
+    return flat ? kUnits + (double)kOne : w;
+  }
+  __device__ __forceinline__ u64 of(float l) const {
+    const double v = above(l);
+    return some(l) ? (u64)__double_as_longlong(v) - 0x4330000000000000ull : 0;
+  }
 };
-__device__ __forceinline__ u64 whole(double w) { return __double2ull_rn(w * kOne); }
-__device__ __forceinline__ int bin_of(double t) { return min((int)((float)t * -(float)kPerOctave), kBins - 1); }
 // the least whole sum that is at least x * sum, 1 .. sum
 __device__ __forceinline__ u64 share_of(float x, u64 sum) {
   if (!(x > 0.f)) return 1;
@@ -78,7 +141,16 @@ struct Pair {
   u64 sum;
 };
 __device__ __forceinline__ Pair operator+(const Pair& a, const Pair& b) { return {a.n + b.n, a.sum + b.sum}; }
-__device__ __forceinline__ Pair warp_scan(Pair v) {  // inclusive
+__device__ __forceinline__ u64 warp_scan(u64 v) {  // inclusive
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+__device__ __forceinline__ Pair warp_scan(Pair v) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -91,208 +163,253 @@ __device__ __forceinline__ Pair warp_scan(Pair v) {  // inclusive
 // What the cluster's first block tells the others: where a limit lies.
 struct Order {
   enum { kNone, kGather, kSelect } what;
-  bool by_rank;    // top-k is the limit, else top-p
-  int bin;         // the histogram's bin that it is in
-  u64 lo, hi;      // or the range of places
-  Pair before;     // what comes before the bin or range
-  unsigned in;     // tokens in it
-  u64 of, goal;    // the sum that top-p is a share of, and that share
+  bool by_rank;  // top-k is the limit, else top-p
+  int bin;       // the histogram's bin that it is in
+  u64 lo, hi;    // or the range of places
+  Pair before;   // what comes before the bin or range
+  unsigned in;   // tokens in it
+  u64 of, goal;  // the sum that top-p is a share of, and that share
 };
 
 struct Shared {
   unsigned count[kBins], low[kBins], high[kBins];  // of sums, the low and the high 32 bits
-  u64 list[kList], mass[kList];
+  u64 list[kList];
   Pair warps[kWarps];
-  u64 lo[kWarps], hi[kWarps];
-  u64 block_lo, block_hi, block_sum;
+  u64 sums[kWarps], lo[kWarps], hi[kWarps];
+  u64 block_lo, block_hi, block_sum, told;
   float max[kWarps], block_max;
-  unsigned listed, found;
+  int block_first;  // index of the block's first maximum
+  unsigned listed;
+  int found;
   Order order;
 };
 
-// Inclusive scan over the block of a value a thread; every thread is to call it.
+// Inclusive scans over the block of a value a thread; every thread is to call them.
 __device__ __forceinline__ Pair block_scan(Shared& s, Pair v, Pair* total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   v = warp_scan(v);
   if (lane == 31) s.warps[warp] = v;
   __syncthreads();
-  Pair w = warp_scan(lane < kWarps ? s.warps[lane] : Pair{0, 0});
+  const Pair w = warp_scan(lane < kWarps ? s.warps[lane] : Pair{0, 0});
   const int before = max(warp - 1, 0);
-  Pair at{__shfl_sync(0xffffffffu, w.n, before), __shfl_sync(0xffffffffu, w.sum, before)};
-  if (warp == 0) at = Pair{0, 0};
-  if (total) *total = Pair{__shfl_sync(0xffffffffu, w.n, kWarps - 1), __shfl_sync(0xffffffffu, w.sum, kWarps - 1)};
+  const Pair at{__shfl_sync(0xffffffffu, w.n, before), __shfl_sync(0xffffffffu, w.sum, before)};
+  *total = Pair{__shfl_sync(0xffffffffu, w.n, kWarps - 1), __shfl_sync(0xffffffffu, w.sum, kWarps - 1)};
   __syncthreads();
-  return at + v;
+  return warp ? at + v : v;
+}
+__device__ __forceinline__ u64 block_scan(Shared& s, u64 v, u64* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  v = warp_scan(v);
+  if (lane == 31) s.sums[warp] = v;
+  __syncthreads();
+  const u64 w = warp_scan(lane < kWarps ? s.sums[lane] : 0);
+  const u64 at = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+  *total = __shfl_sync(0xffffffffu, w, kWarps - 1);
+  __syncthreads();
+  return warp ? at + v : v;
 }
 
-__device__ __forceinline__ void clear_bins(Shared& s) {
-  for (int i = threadIdx.x; i < kBins; i += kThreads) s.count[i] = s.low[i] = s.high[i] = 0;
+__device__ __forceinline__ void clear_bins(Shared& s, bool sums) {
+  for (int i = threadIdx.x; i < kBins; i += kThreads) {
+    s.count[i] = 0;
+    if (sums) s.low[i] = s.high[i] = 0;
+  }
 }
 __device__ __forceinline__ void add_to_bin(Shared& s, int b, u64 w) {
   const unsigned lo = (unsigned)w;
-  atomicAdd(&s.count[b], 1u);
   const unsigned was = atomicAdd(&s.low[b], lo), hi = (unsigned)(w >> 32) + (was + lo < was ? 1u : 0u);
   if (hi) atomicAdd(&s.high[b], hi);
 }
-// The first block: takes the other blocks' bins in.
-__device__ __forceinline__ void merge_bins(Shared& s, int blocks) {
-  for (int i = threadIdx.x; i < kBins; i += kThreads) {
-    unsigned n = 0;
-    u64 sum = 0;
-    for (int c = 0; c < blocks; ++c) {
-      const Shared* o = dsmem_ptr(&s, c);
-      n += o->count[i];
-      sum += o->low[i] + ((u64)o->high[i] << 32);
-    }
-    s.count[i] = n;
-    s.low[i] = (unsigned)sum;
-    s.high[i] = (unsigned)(sum >> 32);
-  }
-  __syncthreads();
-}
 constexpr int kBinsPer = (kBins + kThreads - 1) / kThreads;
 
-// Descending, n a power of two.
-__device__ __forceinline__ void sort_list(u64* v, int n) {
-  for (int size = 2; size <= n; size <<= 1)
+// A list, 4 neighbouring tokens a thread, sorted descending; `all` is a power of two from 4 on, and what lies behind the
+// list's end is 0.  Steps of up to 64 places stay in a warp.
+__device__ __forceinline__ void sort_list(u64 (&v)[kEach], u64* buf, int all) {
+  const int i0 = threadIdx.x * kEach;
+  const bool in = (threadIdx.x & ~31) * kEach < all;  // the warp has a part in it
+  for (int size = 2; size <= all; size <<= 1)
     for (int step = size >> 1; step > 0; step >>= 1) {
-      for (int t = threadIdx.x; t < n / 2; t += kThreads) {
-        const int i = 2 * t - (t & (step - 1)), j = i + step;
-        const u64 a = v[i], b = v[j];
-        if ((a < b) == ((i & size) == 0)) {
-          v[i] = b;
-          v[j] = a;
+      if (step >= 32 * kEach) {
+        if (in) {
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) buf[e * kThreads + threadIdx.x] = v[e];
+        }
+        __syncthreads();
+        if (in) {
+          const bool most = !(i0 & step) == !(i0 & size);
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) {
+            const u64 o = buf[e * kThreads + (threadIdx.x ^ (step / kEach))];
+            if ((o > v[e]) == most) v[e] = o;
+          }
+        }
+        __syncthreads();
+      } else if (in && step >= kEach) {
+        const bool most = !(i0 & step) == !(i0 & size);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+          const u64 o = __shfl_xor_sync(0xffffffffu, v[e], step / kEach);
+          if ((o > v[e]) == most) v[e] = o;
+        }
+      } else if (in) {
+        auto order = [&](u64& a, u64& b, bool down) {
+          const u64 x = a, y = b;
+          if ((x < y) == down) a = y, b = x;
+        };
+        const bool down = !(i0 & size);
+        if (step == 2) {
+          order(v[0], v[2], down);
+          order(v[1], v[3], down);
+        } else {
+          order(v[0], v[1], down);
+          order(v[2], v[3], size == 2 ? !down : down);
         }
       }
-      __syncthreads();
     }
-}
-// Fills the list up with zeros to a power of two, sorts it, and leaves running sums of the weights in s.mass.
-// by_index: the list holds (~index, value) instead of (value, ~index).
-__device__ __forceinline__ void order_list(Shared& s, int n, const Weights& w, bool by_index) {
-  int all = 1;
-  while (all < n) all <<= 1;
-  for (int i = n + threadIdx.x; i < all; i += kThreads) s.list[i] = 0;
-  __syncthreads();
-  sort_list(s.list, all);
-  const int per = (n + kThreads - 1) / kThreads, i0 = threadIdx.x * per;
-  Pair mine{0, 0};
-  for (int i = i0; i < min(n, i0 + per); ++i) {
-    const unsigned key = by_index ? (unsigned)s.list[i] : (unsigned)(s.list[i] >> 32);
-    mine.sum += whole(w.of(w.log2_of(value_of(key))));
-    s.mass[i] = mine.sum;
-  }
-  const u64 before = block_scan(s, mine, nullptr).sum - mine.sum;
-  for (int i = i0; i < min(n, i0 + per); ++i) s.mass[i] += before;
-  __syncthreads();
-}
-// The first place in the list whose running sum reaches `sum`; the last if none does.
-__device__ __forceinline__ int reaches(Shared& s, int n, u64 sum) {
-  if (threadIdx.x == 0) s.found = n - 1;
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads)
-    if (s.mass[i] >= sum && (i == 0 || s.mass[i - 1] < sum)) s.found = i;
-  __syncthreads();
-  const int at = s.found;
-  __syncthreads();
-  return at;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_rows_kernel(const __grid_constant__ SampleRowsArgs a, int stretch, int staged) {
+__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_constant__ SampleRowsArgs a, int stretch, int staged) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ Shared s;
+  constexpr int kVec = Chunk<T>::kN;
   const int blocks = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
   const int r = blockIdx.x / blocks, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int i0 = min(a.vocab, rank * stretch), n = min(a.vocab, i0 + stretch) - i0;  // this block's stretch
-  constexpr int kVec = 16 / sizeof(T);
   pdl_wait();
+  const float temp = a.temperature ? __ldca(a.temperature + r) : 1.f;
+  const bool greedy = !(temp > 0.f);
+  const float coin = greedy ? 0.f : __ldca(a.coin + r);
+  const float top_p = greedy || !a.top_p ? 1.f : __ldca(a.top_p + r);
+  const int top_k = greedy || !a.top_k ? 0 : __ldca(a.top_k + r);
+  const float min_p = greedy || !a.min_p ? 0.f : __ldca(a.min_p + r);
+  const bool by_p = top_p < 1.f, by_k = top_k > 0 && top_k < a.vocab;
+  const u64 least = !(min_p > 0.f) ? 0 : min_p >= 1.f ? kOne : __double2ull_ru(min_p * (double)kOne);
+
+  // The stretch in chunks of 16 bytes, as they lie in memory: element 0 is the chunk 0's element `shift`, and what lies
+  // before and behind counts as -infinity.
   const T* g = static_cast<const T*>(a.logits) + (size_t)r * a.stride + i0;
-  // a stretch lies in shared memory as far from a 16-byte boundary as in memory
   const int shift = (int)(reinterpret_cast<uintptr_t>(g) / sizeof(T) % kVec);
-  T* x = staged ? reinterpret_cast<T*>(smem_raw) + shift : const_cast<T*>(g);
+  const int chunks = n > 0 ? (shift + n + kVec - 1) / kVec : 0;
+  const uint4* const from = reinterpret_cast<const uint4*>(g - shift);
+  uint4* const stage = reinterpret_cast<uint4*>(smem_raw);
+  auto fetch = [&](int c, bool again) -> Chunk<T> {
+    if (c * kVec >= shift && (c + 1) * kVec <= shift + n) return Chunk<T>(again ? __ldca(from + c) : __ldcs(from + c));
+    Chunk<T> v;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const int i = c * kVec + j - shift;
+      v.v[j] = i >= 0 && i < n ? g[i] : minus_infinity<T>();
+    }
+    return v;
+  };
   Weights w;
+  float own;  // the largest logit that this thread has read
   {
     float m = -INFINITY;
-    const int head = min(n, (kVec - shift) % kVec), body = (n - head) / kVec * kVec;
-    auto one = [&](int i) {
-      const T v = g[i];
-      if (staged) x[i] = v;
-      m = fmaxf(m, to_float(v));
-    };
-    if (threadIdx.x < head) one(threadIdx.x);
-    if (threadIdx.x < n - head - body) one(head + body + threadIdx.x);
     constexpr int kAhead = 4;
-    for (int i = threadIdx.x; i < body / kVec; i += kThreads * kAhead) {
-      uint4 v[kAhead];
+    for (int c = threadIdx.x; c < chunks; c += kThreads * kAhead) {
+      Chunk<T> v[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
-        if (i + k * kThreads < body / kVec) v[k] = __ldcs(reinterpret_cast<const uint4*>(g + head) + i + k * kThreads);
+        if (c + k * kThreads < chunks) v[k] = fetch(c + k * kThreads, !staged);
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
-        if (i + k * kThreads < body / kVec) {
-          if (staged) reinterpret_cast<uint4*>(x + head)[i + k * kThreads] = v[k];
-          const T* e = reinterpret_cast<const T*>(&v[k]);
+        if (c + k * kThreads < chunks) {
+          if (staged) stage[c + k * kThreads] = v[k].raw;
 #pragma unroll
-          for (int j = 0; j < kVec; ++j) m = fmaxf(m, to_float(e[j]));
+          for (int j = 0; j < kVec; ++j) m = fmaxf(m, v[k][j]);
         }
     }
-    m = fmaxf(m, -INFINITY);  // (NaN alone)
+    own = m;
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) s.max[warp] = m;
+    if (threadIdx.x == 0) s.block_first = a.vocab;
     __syncthreads();
     m = s.max[lane % kWarps];
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (greedy && own == m && m > -INFINITY) {  // the few threads that have met it look where
+      int first = a.vocab;
+      for (int c = threadIdx.x; c < chunks && first == a.vocab; c += kThreads) {
+        const Chunk<T> v = staged ? Chunk<T>(stage[c]) : fetch(c, true);
+#pragma unroll
+        for (int j = kVec - 1; j >= 0; --j)
+          if (v[j] == m) first = i0 + c * kVec + j - shift;
+      }
+      atomicMin(&s.block_first, first);
+    }
     if (threadIdx.x == 0) s.block_max = m;
     cluster_sync_all();
-    for (int c = 0; c < blocks; ++c) m = fmaxf(m, *dsmem_ptr(&s.block_max, c));
-    w.maxf = m;
+    // (lanes read the blocks of the cluster side by side: a trip to another block's memory each)
+    if (lane < blocks) m = fmaxf(m, *dsmem_ptr(&s.block_max, lane));
+    for (int o = kMaxCluster / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = __shfl_sync(0xffffffffu, m, 0);
+    w.init(m, temp);
   }
-  const float temp = a.temperature ? __ldca(a.temperature + r) : 1.f;
-  const bool greedy = !(temp > 0.f);
-  w.max = w.maxf;
-  w.flat = greedy || w.maxf == INFINITY;
-  w.c = 1.4426950408889634 / (double)temp;
-  const float coin = greedy ? 0.f : __ldca(a.coin + r);
-  const float given_min = greedy || !a.min_p ? 0.f : __ldca(a.min_p + r);
-  const float min_p = given_min > 0.f ? fminf(given_min, 1.f) : 0.f;
-  const float top_p = greedy || !a.top_p ? 1.f : __ldca(a.top_p + r);
-  const int top_k = greedy || !a.top_k ? 0 : __ldca(a.top_k + r);
-  const bool by_p = top_p < 1.f, by_k = top_k > 0 && top_k < a.vocab;
-  const double least = min_p;
-
   auto answer = [&](int token, float prob) {
     a.tokens[r] = token;
     if (a.prob) a.prob[r] = prob;
   };
-  if (w.maxf == -INFINITY) {  // nothing to draw
-    if (rank == 0 && threadIdx.x == 0) answer(0, 0.f);
-    cluster_sync_all();  // the others may still read this block's maximum
+  if (greedy || w.maxf == -INFINITY) {
+    if (rank == 0 && warp == 0) {
+      int first = a.vocab;
+      if (lane < blocks && w.maxf > -INFINITY && *dsmem_ptr(&s.block_max, lane) == w.maxf) first = *dsmem_ptr(&s.block_first, lane);
+      first = __reduce_min_sync(0xffffffffu, first);
+      if (lane == 0) answer(first < a.vocab ? first : 0, first < a.vocab ? 1.f : 0.f);  // (or there is nothing to draw)
+    }
+    cluster_sync_all();  // nobody leaves while others read its shared memory
     return;
   }
-  // A warp's part of the stretch: whole steps of 32 tokens, in the order of the row.
-  const int part = (n + kThreads - 1) / kThreads * 32, p0 = min(n, warp * part), p1 = min(n, p0 + part);
+  // A warp's part of the stretch; f is called by whole warps, with -infinity behind the end.
+  const int part = (chunks + kWarps - 1) / kWarps, c0 = min(chunks, warp * part), c1 = min(chunks, c0 + part);
+  auto chunk_at = [&](int c) -> Chunk<T> {
+    if (c < c1) return staged ? Chunk<T>(stage[c]) : fetch(c, true);
+    Chunk<T> v;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) v.v[j] = minus_infinity<T>();
+    return v;
+  };
+  auto index_of = [&](int c, int j) { return i0 + c * kVec + j - shift; };
+  // Four logits at a time, f(index of the first, logits).
+  auto each4 = [&](auto&& f) {
+    for (int b = c0; b < c1; b += 32) {
+      const Chunk<T> v = chunk_at(b + lane);
+#pragma unroll
+      for (int j = 0; j < kVec; j += 4) {
+        const float l[4] = {v[j], v[j + 1], v[j + 2], v[j + 3]};
+        f(index_of(b + lane, j), l);
+      }
+    }
+  };
   auto each = [&](auto&& f) {
-    for (int i = p0 + lane; i < p1; i += 32) f(i, to_float(x[i]));
+    each4([&](int i, const float (&l)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f(i + j, l[j]);
+    });
   };
   const Order* const told = dsmem_ptr(&s.order, 0);
   Shared* const first = const_cast<Shared*>(dsmem_ptr(&s, 0));
   // The first block merges the bins of all, and tells where `rank` (if any) or else the sum `goal` is reached; bin j is
-  // places hi - (j + 1) width + 1 .. hi - j width of the range, or of the logarithms (width 0).
+  // places hi - (j + 1) width + 1 .. hi - j width of the range, or of the first histogram's (width 0).
   auto find = [&](bool by_rank, Pair before, u64 goal, u64 of, u64 lo, u64 hi, u64 width) {
-    merge_bins(s, blocks);
     Pair mine{0, 0}, bin[kBinsPer], total;
 #pragma unroll
     for (int k = 0; k < kBinsPer; ++k) {
       const int b = threadIdx.x * kBinsPer + k;
-      bin[k] = b < kBins ? Pair{s.count[b], s.low[b] + ((u64)s.high[b] << 32)} : Pair{0, 0};
+      bin[k] = Pair{0, 0};
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) {  // all on their way at once
+        if (c >= blocks || b >= kBins) continue;
+        const Shared* o = dsmem_ptr(&s, c);
+        bin[k].n += o->count[b];
+        if (!by_rank) bin[k].sum += o->low[b] + ((u64)o->high[b] << 32);
+      }
       mine = mine + bin[k];
     }
     const Pair upto = block_scan(s, mine, &total);
     before = before + Pair{upto.n - mine.n, upto.sum - mine.sum};
     if (!width) {  // the first histogram: it holds all weights
-      if (!of) of = total.sum;
-      if (by_rank && (unsigned)top_k >= total.n) by_rank = false;
+      of = total.sum;
       goal = share_of(top_p, of);
     }
     if (threadIdx.x == 0) {
@@ -304,7 +421,7 @@ __global__ void __launch_bounds__(kThreads) sample_rows_kernel(const __grid_cons
     for (int k = 0; k < kBinsPer; ++k) {
       const Pair after = before + bin[k];
       const int b = threadIdx.x * kBinsPer + k;
-      if (by_rank ? before.n < (unsigned)top_k && (unsigned)top_k <= after.n : by_p && before.sum < goal && goal <= after.sum) {
+      if (by_rank ? before.n < (unsigned)top_k && (unsigned)top_k <= after.n : before.sum < goal && goal <= after.sum) {
         Order o;
         o.what = !width && after.n <= kList ? Order::kGather : Order::kSelect;
         o.by_rank = by_rank;
@@ -324,161 +441,270 @@ __global__ void __launch_bounds__(kThreads) sample_rows_kernel(const __grid_cons
     const unsigned to = atomicAdd(&first->listed, 1u);
     if (to < kList) first->list[to] = at;
   };
-  u64 limit = 0;  // places from here on are kept
-  if (by_k || by_p) {
-    bool want_k = by_k;
-    u64 of = 0;
-    for (;;) {  // once, or once for each limit
-      clear_bins(s);
+  // The first block's list, sorted, a thread's tokens in v.
+  u64 v[kEach];
+  const int v0 = threadIdx.x * kEach;
+  int listed = 0, all = kEach;
+  auto take_list = [&] {
+    listed = min((int)s.listed, kList);
+    while (all < listed) all <<= 1;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) v[e] = v0 + e < listed ? s.list[v0 + e] : 0;
+    __syncthreads();
+    sort_list(v, s.list, all);
+  };
+  // weights of v (by_index: the value is in the low half) and their running sums
+  u64 weight[kEach], upto[kEach];
+  auto sum_list = [&](bool by_index) {
+    u64 mine = 0, total;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      weight[e] = w.of(value_of(by_index ? (unsigned)v[e] : (unsigned)(v[e] >> 32)));
+      if (!v[e]) weight[e] = 0;
+      mine += weight[e];
+      upto[e] = mine;
+    }
+    const u64 before = block_scan(s, mine, &total) - mine;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) upto[e] += before;
+    return total;
+  };
+  // The list holds the first tokens, at least those that are kept: by rank, or else by the share of the sum `of`.
+  auto finish = [&](bool by_rank, u64 of) {
+    take_list();
+    sum_list(false);
+    int keep = by_rank ? min(top_k, listed) : listed;
+    if (by_p) {
+      if (by_rank && (keep - 1) / kEach == threadIdx.x) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+          if (v0 + e == keep - 1) s.told = upto[e];
+      }
       __syncthreads();
-      each([&](int, float l) {
-        const double t = w.log2_of(l);
-        const u64 v = whole(w.of(t));
-        if (v) add_to_bin(s, bin_of(t), v);
+      const u64 share = share_of(top_p, by_rank ? s.told : of);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (upto[e] >= share && upto[e] - weight[e] < share) s.found = v0 + e + 1;
+      __syncthreads();
+      keep = min(keep, s.found);
+    }
+    // the rest, in the order of the row
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) v[e] = v0 + e < keep && weight[e] >= least ? v[e] << 32 | v[e] >> 32 : 0;
+    sort_list(v, s.list, all);
+    const u64 sum = sum_list(true), share = share_of(coin, sum);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      if (upto[e] >= share && upto[e] - weight[e] < share)
+        answer((int)~(unsigned)(v[e] >> 32), (float)((double)weight[e] / (double)sum));
+  };
+  if (by_k) {
+    // The k-th largest of the threads' maxima is no larger than the k-th largest logit, and few tokens lie between the
+    // two: a histogram of 512 maxima a block instead of all its logits.
+    clear_bins(s, false);
+    __syncthreads();
+    if (w.some(own)) atomicAdd(&s.count[w.bin(own)], 1u);
+    cluster_sync_all();
+    if (rank == 0) find(true, Pair{0, 0}, 0, 0, 0, 0, 0);
+    cluster_sync_all();
+    const Order o = *told;
+    if (o.what == Order::kGather) {
+      each([&](int i, float l) {
+        if (w.some(l) && w.bin(l) <= o.bin) put(place_of(l, i));
       });
       cluster_sync_all();
-      if (rank == 0) find(want_k, Pair{0, 0}, 0, of, 0, 0, 0);
-      cluster_sync_all();
-      Order o = *told;
-      if (o.what == Order::kNone) break;  // as many are kept as there are
-      if (o.what == Order::kGather) {
-        each([&](int i, float l) {
-          const double t = w.log2_of(l);
-          if (bin_of(t) <= o.bin && whole(w.of(t))) put(place_of(l, i0 + i));
-        });
-        cluster_sync_all();
-        if (rank) return;
-        const int m = min((int)s.listed, kList);
-        order_list(s, m, w, false);
-        int keep = o.by_rank ? min(top_k, m) : m;
-        const u64 share = share_of(top_p, o.by_rank ? s.mass[keep - 1] : o.of);
-        if (by_p) keep = min(keep, reaches(s, m, share) + 1);
-        if (least > 0.0) {
-          if (threadIdx.x == 0) s.found = 1;
-          __syncthreads();
-          for (int i = threadIdx.x; i < keep; i += kThreads)
-            if (w.of(w.log2_of(value_of((unsigned)(s.list[i] >> 32)))) >= least) atomicMax(&s.found, i + 1u);
-          __syncthreads();
-          keep = (int)s.found;
-        }
-        const u64 sum = s.mass[keep - 1];
-        __syncthreads();
-        for (int i = threadIdx.x; i < keep; i += kThreads) s.list[i] = s.list[i] << 32 | s.list[i] >> 32;
-        order_list(s, keep, w, true);
-        const int at = reaches(s, keep, share_of(coin, sum));
-        if (threadIdx.x == 0)
-          answer((int)~(unsigned)(s.list[at] >> 32), (float)((double)(s.mass[at] - (at ? s.mass[at - 1] : 0)) / (double)sum));
+      const unsigned got = *dsmem_ptr(&s.listed, 0);
+      if (got <= kList) {
+        cluster_arrive();
+        if (rank == 0) finish(true, 0);
+        cluster_wait();
         return;
       }
-      // ---- the limit's own place, among too many: the ends of the bin's places first
-      u64 lo = ~0ull, hi = 0;
-      each([&](int i, float l) {
-        const double t = w.log2_of(l);
-        if (t >= -kOctaves && bin_of(t) == o.bin && whole(w.of(t))) {
-          const u64 at = place_of(l, i0 + i);
-          lo = at < lo ? at : lo;
-          hi = at > hi ? at : hi;
+    }
+  }
+  u64 limit = 0;  // places from here on are kept
+  auto in_limit = [&](int i, float l) { return !limit || place_of(l, i) >= limit; };
+  for (int kind = by_k ? 0 : 1; kind < (by_p ? 2 : 1); ++kind) {  // top-k, then (if that did not see to it) top-p
+    const bool by_rank = kind == 0;
+    clear_bins(s, !by_rank);
+    __syncthreads();
+    each4([&](int i, const float (&l)[4]) {
+      u64 v[4] = {0, 0, 0, 0};
+      if (!by_rank) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = w.of(l[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (w.some(l[j]) && in_limit(i + j, l[j])) {
+          const int b = w.bin(l[j]);
+          atomicAdd(&s.count[b], 1u);
+          if (v[j]) add_to_bin(s, b, v[j]);
         }
+    });
+    cluster_sync_all();
+    if (rank == 0) find(by_rank, Pair{0, 0}, 0, 0, 0, 0, 0);
+    cluster_sync_all();
+    Order o = *told;
+    if (o.what == Order::kNone) continue;  // no more than k tokens have a weight
+    if (o.what == Order::kGather) {
+      each([&](int i, float l) {
+        if (w.some(l) && w.bin(l) <= o.bin && in_limit(i, l)) put(place_of(l, i));
       });
+      cluster_sync_all();
+      if (rank) return;
+      finish(by_rank, o.of);
+      return;
+    }
+    // ---- the limit's own place, among too many: the ends of the bin's places first
+    u64 lo = ~0ull, hi = 0;
+    each([&](int i, float l) {
+      if (w.some(l) && w.bin(l) == o.bin && in_limit(i, l)) {
+        const u64 at = place_of(l, i);
+        lo = at < lo ? at : lo;
+        hi = at > hi ? at : hi;
+      }
+    });
+    auto ends = [](u64& lo, u64& hi) {  // of a warp's lanes
       for (int d = 16; d; d >>= 1) {
         const u64 l = __shfl_xor_sync(0xffffffffu, lo, d), h = __shfl_xor_sync(0xffffffffu, hi, d);
         lo = l < lo ? l : lo;
         hi = h > hi ? h : hi;
       }
-      if (lane == 0) {
-        s.lo[warp] = lo;
-        s.hi[warp] = hi;
+    };
+    ends(lo, hi);
+    if (lane == 0) {
+      s.lo[warp] = lo;
+      s.hi[warp] = hi;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int k = 1; k < kWarps; ++k) {
+        lo = s.lo[k] < lo ? s.lo[k] : lo;
+        hi = s.hi[k] > hi ? s.hi[k] : hi;
       }
+      s.block_lo = lo;
+      s.block_hi = hi;
+    }
+    cluster_sync_all();
+    lo = lane < blocks ? *dsmem_ptr(&s.block_lo, lane) : ~0ull;
+    hi = lane < blocks ? *dsmem_ptr(&s.block_hi, lane) : 0;
+    ends(lo, hi);
+    o.lo = lo;
+    o.hi = hi;
+    while (o.in > kList) {  // each round leaves one of kBins parts of a range that has at most 2^64 places
+      const u64 width = (o.hi - o.lo) / kBins + 1;
+      clear_bins(s, !by_rank);
       __syncthreads();
-      if (threadIdx.x == 0) {
-        for (int k = 1; k < kWarps; ++k) {
-          lo = s.lo[k] < lo ? s.lo[k] : lo;
-          hi = s.hi[k] > hi ? s.hi[k] : hi;
-        }
-        s.block_lo = lo;
-        s.block_hi = hi;
-      }
-      cluster_sync_all();
-      lo = ~0ull, hi = 0;
-      for (int c = 0; c < blocks; ++c) {
-        const u64 l = *dsmem_ptr(&s.block_lo, c), h = *dsmem_ptr(&s.block_hi, c);
-        lo = l < lo ? l : lo;
-        hi = h > hi ? h : hi;
-      }
-      o.lo = lo;
-      o.hi = hi;
-      while (o.in > kList) {  // each round leaves one of kBins parts of a range that has at most 2^64 places
-        const u64 width = (o.hi - o.lo) / kBins + 1;
-        clear_bins(s);
-        __syncthreads();
-        each([&](int i, float l) {
-          const u64 at = l == l ? place_of(l, i0 + i) : 0;
-          if (at >= o.lo && at <= o.hi) add_to_bin(s, (int)((o.hi - at) / width), whole(w.of(w.log2_of(l))));
-        });
-        cluster_sync_all();
-        if (rank == 0) find(o.by_rank, o.before, o.goal, o.of, o.lo, o.hi, width);
-        cluster_sync_all();
-        o = *told;
-      }
       each([&](int i, float l) {
-        const u64 at = l == l ? place_of(l, i0 + i) : 0;
-        if (at >= o.lo && at <= o.hi) put(at);
+        const u64 at = w.some(l) ? place_of(l, i) : 0;
+        const bool in = at >= o.lo && at <= o.hi;
+        const u64 v = !by_rank && __any_sync(0xffffffffu, in) ? w.of(l) : 0;
+        if (in) {
+          const int b = (int)((o.hi - at) / width);
+          atomicAdd(&s.count[b], 1u);
+          if (!by_rank && v) add_to_bin(s, b, v);
+        }
       });
       cluster_sync_all();
-      if (rank == 0) {
-        const int m = min((int)s.listed, kList);
-        order_list(s, m, w, false);
-        const int at = o.by_rank ? top_k - (int)o.before.n - 1 : reaches(s, m, o.goal - o.before.sum);
-        if (threadIdx.x == 0) {
-          s.order.lo = s.list[at];
-          s.order.of = o.before.sum + s.mass[at];
-        }
-      }
+      if (rank == 0) find(by_rank, o.before, o.goal, o.of, o.lo, o.hi, width);
       cluster_sync_all();
-      limit = told->lo;
-      of = told->of;
-      want_k = false;
-      if (!o.by_rank || !by_p) break;
+      o = *told;
     }
+    each([&](int i, float l) {
+      const u64 at = w.some(l) ? place_of(l, i) : 0;
+      if (at >= o.lo && at <= o.hi) put(at);
+    });
+    cluster_sync_all();
+    if (rank == 0) {
+      all = kEach;
+      take_list();
+      const u64 share = o.goal - o.before.sum;
+      if (!by_rank) sum_list(false);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (by_rank ? v0 + e == top_k - (int)o.before.n - 1 : upto[e] >= share && upto[e] - weight[e] < share) s.told = v[e];
+    }
+    cluster_sync_all();
+    limit = *dsmem_ptr(&s.told, 0);
   }
   // ---- the draw, in the order of the row
-  auto kept = [&](int i, float l) -> u64 {
-    if (limit && !(l == l && place_of(l, i) >= limit)) return 0;
-    const double v = w.of(w.log2_of(l));
-    return v >= least ? whole(v) : 0;
+  // Sums of a thread's weights, up to 2^20 / 8 / 512 of them, are whole numbers of 64-bit floating point.
+  const double least_above = kUnits + (double)least;
+  auto kept = [&](int i, const float (&l)[4], double (&v)[4]) {
+    bool in[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) in[j] = w.some(l[j]) && in_limit(i + j, l[j]);
+    const bool any = __any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = kUnits;
+    if (any) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = w.above(l[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = in[j] && v[j] >= least_above ? v[j] - kUnits : 0.0;
   };
-  u64 mine = 0;
-  each([&](int i, float l) { mine += kept(i0 + i, l); });
+  u64 mine;
+  {
+    double some = 0.0;
+    each4([&](int i, const float (&l)[4]) {
+      double v[4];
+      kept(i, l, v);
+      some += (v[0] + v[1]) + (v[2] + v[3]);
+    });
+    mine = __double2ull_rn(some);
+  }
   for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
   if (lane == 0) s.lo[warp] = mine;
   __syncthreads();
   u64 before = 0, sum = 0;
+#pragma unroll
   for (int k = 0; k < kWarps; ++k) {
     if (k == warp) before = sum;
     sum += s.lo[k];
   }
   if (threadIdx.x == 0) s.block_sum = sum;
   cluster_sync_all();
-  sum = 0;
-  for (int c = 0; c < blocks; ++c) {
-    if (c == rank) before += sum;
-    sum += *dsmem_ptr(&s.block_sum, c);
+  {
+    const u64 here = lane < blocks ? *dsmem_ptr(&s.block_sum, lane) : 0, upto = warp_scan(here);
+    before += __shfl_sync(0xffffffffu, upto - here, rank);
+    sum = __shfl_sync(0xffffffffu, upto, 31);
   }
-  const u64 goal = share_of(coin, sum);
-  if (before < goal && goal <= before + mine) {
-    for (int i = p0; i < p1; i += 32) {
-      const float l = i + lane < p1 ? to_float(x[i + lane]) : -INFINITY;
-      const u64 v = kept(i0 + i + lane, l);
-      const u64 upto = before + warp_scan(Pair{0, v}).sum;
-      const unsigned there = __ballot_sync(0xffffffffu, upto >= goal);
+  const u64 share = share_of(coin, sum);
+  if (before < share && share <= before + mine) {
+    for (int b = c0; b < c1; b += 32) {
+      const Chunk<T> x = chunk_at(b + lane);
+      u64 v[kVec], here = 0;
+#pragma unroll
+      for (int j = 0; j < kVec; j += 4) {
+        const float l[4] = {x[j], x[j + 1], x[j + 2], x[j + 3]};
+        double f[4];
+        kept(index_of(b + lane, j), l, f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) here += v[j + k] = __double2ull_rn(f[k]);
+      }
+      u64 upto = before + warp_scan(here);
+      const unsigned there = __ballot_sync(0xffffffffu, upto >= share);
       if (there) {
-        if (lane == __ffs(there) - 1) answer(i0 + i + lane, greedy ? 1.f : (float)((double)v / (double)sum));
+        if (lane == __ffs(there) - 1) {
+          upto -= here;
+          bool done = false;
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) {
+            upto += v[j];
+            if (!done && upto >= share) {
+              done = true;
+              answer(index_of(b + lane, j), (float)((double)v[j] / (double)sum));
+            }
+          }
+        }
         break;
       }
       before = __shfl_sync(0xffffffffu, upto, 31);
     }
   }
-  cluster_sync_all();  // nobody leaves while others read its shared memory
+  cluster_sync_all();
 }
 
 template <typename T>
@@ -487,7 +713,7 @@ cudaError_t launch(const SampleRowsArgs& a, int device, cudaStream_t s) {
   int blocks = 1;
   while (blocks < kMaxCluster && a.vocab > 4096 * blocks) blocks *= 2;
   const int stretch = ((a.vocab + blocks - 1) / blocks + 31) / 32 * 32;
-  const size_t bytes = (size_t)stretch * sizeof(T) + 16;
+  const size_t bytes = (size_t)stretch * sizeof(T) + 32;
   const int staged = bytes <= kMaxStage;
   const void* fn = reinterpret_cast<const void*>(&sample_rows_kernel<T>);
   static SmemCap cap;
