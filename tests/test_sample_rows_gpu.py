@@ -39,9 +39,9 @@ def _one(x, coin, T, k, p, least):
         return 0, 0.0
     if not T > 0:
         return int(np.argmax(x)), 1.0
+    T = min(max(T, 2.0 ** -60), 2.0 ** 90)
     with np.errstate(all="ignore"):
         w = (x == m).astype(np.float64) if m == np.inf else np.exp((x - m) / T)
-    w[np.isnan(w)] = 0.0  # -inf at an infinite temperature
     n = np.rint(w * ONE).astype(np.uint64)
     if 0 < k < len(x) or p < 1:
         order = np.lexsort((np.arange(len(x)), -x))

@@ -37,7 +37,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kOctaves = 44, kPerOctave = 16, kBins = kOctaves * kPerOctave;
 constexpr int kEach = 4, kList = kThreads * kEach;  // tokens of a list: 4 a thread
 constexpr u64 kOne = 1ull << 43;                    // the largest weight
-constexpr float kLeastTemperature = 0x1p-60f;
+constexpr float kLeastTemperature = 0x1p-60f, kMostTemperature = 0x1p90f;
 constexpr size_t kMaxStage = 160 * 1024;            // bytes of a row's stretch that shared memory takes
 constexpr int kMaxCluster = 8;
 
@@ -89,26 +89,40 @@ constexpr double kUnits = 4503599627370496.0;  // 2^52: added, it leaves a whole
 struct Weights {
   double max, c, root;  // the maximum, log2(e) / T, 2^(lane / 32 + 43)
   float maxf, cut;      // what lies below cut has no weight
+  float none;           // nor has this, which stands for all that lies below it, and for NaN
   float per_bin;        // bins a unit of l
-  bool flat;  // all that equal the maximum weigh the same, all else nothing (T is 0, or the maximum infinite)
+  // a number at or below all logits of the bins up to b that have a weight
+  __device__ __forceinline__ float floor_of_bins(int b) const {
+    return b == kBins - 1 ? cut : fmaxf(cut, __double2float_rd(max - (b + 1) * (double)(1.f + 0x1p-20f) / per_bin));
+  }
   __device__ __forceinline__ void init(float m, float temp) {
     maxf = m;
-    max = widen(m);
-    flat = !(temp > 0.f) || m == INFINITY;
-    c = 1.4426950408889634 / (double)fmaxf(temp, kLeastTemperature);
-    cut = flat ? m : fmaxf((float)((double)m - kOctaves / c), -FLT_MAX);
-    per_bin = (float)(c * kPerOctave);
+    max = widen(m);  // (2^128 for infinity)
     root = exp2((threadIdx.x & 31) * (1.0 / 32) + 43.0);
+    if (m == INFINITY) {  // the infinite ones weigh the same, the largest finite number 2^-50 of it
+      c = 50.0 * 0x1p-104;
+      cut = m;
+      none = FLT_MAX;
+      per_bin = 0.f;
+      return;
+    }
+    // Where the number below the maximum weighs nothing already, nothing changes down to 2^-50 of it: logarithms stay
+    // small enough for the exponents below.  (At |m| >= 2^127 that is so at every temperature; -infinity counts as -2^128.)
+    const unsigned u = __float_as_uint(m);
+    const double gap = max - widen(__uint_as_float(m > 0.f ? u - 1 : m < 0.f ? u + 1 : 0x80000001u));
+    c = fmin(1.4426950408889634 / (double)fminf(fmaxf(temp, kLeastTemperature), kMostTemperature), 50.0 / gap);
+    cut = fmaxf((float)(max - kOctaves / c), -FLT_MAX);
+    none = __double2float_rd(max - (kOctaves + 2) / c);
+    per_bin = (float)(c * kPerOctave);
   }
   __device__ __forceinline__ bool some(float l) const { return l >= cut; }
   // of what has a weight; the sum rounds to a whole number
   __device__ __forceinline__ int bin(float l) const {
-    const float y = fmaf(fminf(maxf - l, FLT_MAX), per_bin, 8388608.f);
-    return flat ? 0 : min(__float_as_int(y) - 0x4b000000, kBins - 1);
+    return min(__float_as_int(fmaf(fminf(maxf - l, FLT_MAX), per_bin, 8388608.f)) - 0x4b000000, kBins - 1);
   }
-  // 2^52 + the weight in units, of what has one
+  // 2^52 + the weight in units
   __device__ __forceinline__ double above(float l) const {
-    const double t = (widen(l) - max) * c;
+    const double t = (widen(fmaxf(l, none)) - max) * c;
     constexpr double kRound = 6755399441055744.0;  // 1.5 2^52
     double k = fma(t, 32.0, kRound);
     const int n = __double2loint(k);
@@ -120,12 +134,10 @@ struct Weights {
     p = fma(r, p, 0.693147180559945309);
     p = fma(r, p, 1.0);
     const int hi = __shfl_sync(0xffffffffu, __double2hiint(root), n), lo = __shfl_sync(0xffffffffu, __double2loint(root), n);
-    const double w = fma(__hiloint2double(hi + (n & ~31) * (1 << 15), lo), p, kUnits);
-    return flat ? kUnits + (double)kOne : w;
+    return fma(__hiloint2double(hi + (n & ~31) * (1 << 15), lo), p, kUnits);
   }
   __device__ __forceinline__ u64 of(float l) const {
-    const double v = above(l);
-    return some(l) ? (u64)__double_as_longlong(v) - 0x4330000000000000ull : 0;
+    return (u64)__double_as_longlong(above(l)) - 0x4330000000000000ull;
   }
 };
 // the least whole sum that is at least x * sum, 1 .. sum
@@ -268,8 +280,8 @@ __device__ __forceinline__ void sort_list(u64 (&v)[kEach], u64* buf, int all) {
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_constant__ SampleRowsArgs a, int stretch, int staged) {
+template <typename T, bool kStaged>
+__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_constant__ SampleRowsArgs a, int stretch) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ Shared s;
   constexpr int kVec = Chunk<T>::kN;
@@ -312,11 +324,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
       Chunk<T> v[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
-        if (c + k * kThreads < chunks) v[k] = fetch(c + k * kThreads, !staged);
+        if (c + k * kThreads < chunks) v[k] = fetch(c + k * kThreads, !kStaged);
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
         if (c + k * kThreads < chunks) {
-          if (staged) stage[c + k * kThreads] = v[k].raw;
+          if (kStaged) stage[c + k * kThreads] = v[k].raw;
 #pragma unroll
           for (int j = 0; j < kVec; ++j) m = fmaxf(m, v[k][j]);
         }
@@ -331,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     if (greedy && own == m && m > -INFINITY) {  // the few threads that have met it look where
       int first = a.vocab;
       for (int c = threadIdx.x; c < chunks && first == a.vocab; c += kThreads) {
-        const Chunk<T> v = staged ? Chunk<T>(stage[c]) : fetch(c, true);
+        const Chunk<T> v = kStaged ? Chunk<T>(stage[c]) : fetch(c, true);
 #pragma unroll
         for (int j = kVec - 1; j >= 0; --j)
           if (v[j] == m) first = i0 + c * kVec + j - shift;
@@ -363,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
   // A warp's part of the stretch; f is called by whole warps, with -infinity behind the end.
   const int part = (chunks + kWarps - 1) / kWarps, c0 = min(chunks, warp * part), c1 = min(chunks, c0 + part);
   auto chunk_at = [&](int c) -> Chunk<T> {
-    if (c < c1) return staged ? Chunk<T>(stage[c]) : fetch(c, true);
+    if (c < c1) return kStaged ? Chunk<T>(stage[c]) : fetch(c, true);
     Chunk<T> v;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) v.v[j] = minus_infinity<T>();
@@ -441,6 +453,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     const unsigned to = atomicAdd(&first->listed, 1u);
     if (to < kList) first->list[to] = at;
   };
+  auto gather = [&](float least_l) {  // all from a number on, and perhaps more than there is room for
+    each4([&](int i, const float (&l)[4]) {
+      if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= least_l) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (l[j] >= least_l) put(place_of(l[j], i + j));
+      }
+    });
+  };
   // The first block's list, sorted, a thread's tokens in v.
   u64 v[kEach];
   const int v0 = threadIdx.x * kEach;
@@ -509,9 +530,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     cluster_sync_all();
     const Order o = *told;
     if (o.what == Order::kGather) {
-      each([&](int i, float l) {
-        if (w.some(l) && w.bin(l) <= o.bin) put(place_of(l, i));
-      });
+      gather(w.floor_of_bins(o.bin));
       cluster_sync_all();
       const unsigned got = *dsmem_ptr(&s.listed, 0);
       if (got <= kList) {
@@ -632,27 +651,37 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
   // Sums of a thread's weights, up to 2^20 / 8 / 512 of them, are whole numbers of 64-bit floating point.
   const double least_above = kUnits + (double)least;
   auto kept = [&](int i, const float (&l)[4], double (&v)[4]) {
-    bool in[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) in[j] = w.some(l[j]) && in_limit(i + j, l[j]);
-    const bool any = __any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3]);
+    for (int j = 0; j < 4; ++j) v[j] = 0.0;
+    bool in[4] = {true, true, true, true};
+    if (limit) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = kUnits;
-    if (any) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = w.above(l[j]);
+      for (int j = 0; j < 4; ++j) in[j] = w.some(l[j]) && place_of(l[j], i + j) >= limit;
+      if (!__any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3])) return;
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = w.above(l[j]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = in[j] && v[j] >= least_above ? v[j] - kUnits : 0.0;
   };
   u64 mine;
   {
     double some = 0.0;
-    each4([&](int i, const float (&l)[4]) {
-      double v[4];
-      kept(i, l, v);
-      some += (v[0] + v[1]) + (v[2] + v[3]);
-    });
+    if (limit) {
+      each4([&](int i, const float (&l)[4]) {
+        double v[4];
+        kept(i, l, v);
+        some += (v[0] + v[1]) + (v[2] + v[3]);
+      });
+    } else {
+      each4([&](int, const float (&l)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const double v = w.above(l[j]);
+          if (v >= least_above) some += v - kUnits;
+        }
+      });
+    }
     mine = __double2ull_rn(some);
   }
   for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
@@ -712,16 +741,16 @@ cudaError_t launch(const SampleRowsArgs& a, int device, cudaStream_t s) {
   // blocks a row: enough that a stretch fits shared memory, and that a short row's passes are short
   int blocks = 1;
   while (blocks < kMaxCluster && a.vocab > 4096 * blocks) blocks *= 2;
-  const int stretch = ((a.vocab + blocks - 1) / blocks + 31) / 32 * 32;
+  int stretch = ((a.vocab + blocks - 1) / blocks + 31) / 32 * 32;
   const size_t bytes = (size_t)stretch * sizeof(T) + 32;
-  const int staged = bytes <= kMaxStage;
-  const void* fn = reinterpret_cast<const void*>(&sample_rows_kernel<T>);
+  const bool staged = bytes <= kMaxStage;
+  const void* fn = staged ? reinterpret_cast<const void*>(&sample_rows_kernel<T, true>)
+                          : reinterpret_cast<const void*>(&sample_rows_kernel<T, false>);
   static SmemCap cap;
-  const cudaError_t e = cap.raise(fn, device, kMaxStage);
+  const cudaError_t e = cap.raise(reinterpret_cast<const void*>(&sample_rows_kernel<T, true>), device, kMaxStage);
   if (e != cudaSuccess) return e;
   SampleRowsArgs p = a;
-  int st = stretch, sg = staged;
-  void* params[] = {&p, &st, &sg};
+  void* params[] = {&p, &stretch};
   return launch_cluster_params(fn, dim3((unsigned)(a.rows * blocks)), dim3(kThreads), staged ? bytes : 0, s, blocks, true, params);
 }
 
