@@ -111,6 +111,8 @@ CASES = [  # (cached, new, page size, spare pages, table width, rows)
     ([16 * (i % 3) for i in range(1024)], [1 if i % 5 else -1 for i in range(1024)], 16, 900, 4, 1030),
     ([16 * (i % 3) for i in range(1025)], [(i % 4) - 1 for i in range(1025)], 16, 900, 4, 2000),  # two kernels
     ([7], [8193], 64, 200, 200, 8193),  # two kernels for the rows' sake
+    ([5] * 9000, [(700 if i == 3 else 0) if i < 8000 else i % 3 for i in range(9000)], 16, 2000, 60, 3000),  # far apart
+    ([5] * 60000, [1 if i % 20000 == 7 else 0 for i in range(60000)], 16, 9, 2, 9000),
     ([i % 90 for i in range(20000)], [(i * 7) % 12 - 1 for i in range(20000)], 32, 30000, 4, 100000),
 ]
 

@@ -130,7 +130,7 @@ __device__ __forceinline__ long long paged_slot(const PagedPlanArgs& a, int p, i
   if (page < 0 || page >= a.n_pages) return -1;
   return ((long long)page << a.ps_log2) + (p & ((1 << a.ps_log2) - 1));
 }
-cudaError_t paged_plan(const PagedPlanArgs& a, cudaStream_t s);
+cudaError_t paged_plan(const PagedPlanArgs& a, int device, cudaStream_t s);
 
 int paged_attention_grid(int n_sms);  // blocks
 size_t paged_attention_scratch(int head_dim, int n_sms);

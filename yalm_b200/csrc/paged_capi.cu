@@ -190,7 +190,7 @@ extern "C" int yb_paged_plan_dev(const yb_paged_batch* b, const int* new_len_dev
   a.n_pages = b->n_pages;
   a.max_pages = b->max_pages;
   a.ps_log2 = p.ps_log2;
-  YB_CK(paged_plan(a, static_cast<cudaStream_t>(stream)));
+  YB_CK(paged_plan(a, dev, static_cast<cudaStream_t>(stream)));
   return 0;
 }
 

@@ -8,11 +8,11 @@
 // result is the same on every run: prefix sums, no atomics that hand out places.  A step that does not fit (pages,
 // rows, a sequence longer than its table) takes nothing and brings no tokens.
 //
-// Integers only, a few bytes a sequence and 12 a token: launches and chains of dependent loads are what it costs.  One
-// block does all of it for up to kBlockSeqs sequences and kBlockTokens rows, the starts in shared memory, where a
-// token's sequence is searched.  Larger batches: a cluster of 8 blocks does the sums and the pages, each block a
-// stretch of the sequences, with totals exchanged over distributed shared memory; a second kernel over the whole GPU
-// writes the tokens' positions and slots.
+// Integers only, a few bytes a sequence and 12 a token: launches and chains of dependent loads are what it costs, so
+// pages and tokens are shared out among all threads, each of which finds its sequence by a search of prefix sums in
+// shared memory.  One block does all of it for up to kBlockSeqs sequences and kBlockTokens rows.  Larger batches: a
+// cluster of 8 blocks does the sums and the pages, each block a stretch of the sequences, with totals exchanged over
+// distributed shared memory; a second kernel over the whole GPU writes the tokens' positions and slots.
 #include "cluster.cuh"
 #include "launch.h"
 #include "paged.cuh"
@@ -25,86 +25,80 @@ constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kCluster = 8;
 constexpr int kBlockSeqs = 1024, kBlockTokens = 8192;
+constexpr int kMostSeqs = 65536 / kCluster;  // of a block of the cluster
 
 struct Sums {
-  long long rows, more, back;  // tokens, pages taken, pages given back
+  long long rows;  // tokens
+  int more, back;  // pages taken; table entries of ended sequences (of a block at most 2^30)
 };
 __device__ __forceinline__ Sums operator+(const Sums& a, const Sums& b) { return {a.rows + b.rows, a.more + b.more, a.back + b.back}; }
+__device__ __forceinline__ Sums operator-(const Sums& a, const Sums& b) { return {a.rows - b.rows, a.more - b.more, a.back - b.back}; }
 
-// What a sequence brings: r < 0: it ends.  held: pages in its table before, more: pages that it takes.
-struct Wish {
-  int n, kv, held, more;
-  bool ends, too_long;
-};
-__device__ __forceinline__ Wish wish(const PagedPlanArgs& a, int s, bool there) {
-  Wish w{0, 0, 0, 0, false, false};
-  if (!there) return w;
-  const int r = __ldca(a.new_len + s), cap = a.max_pages << a.ps_log2, up = (1 << a.ps_log2) - 1;
-  w.kv = min(max(__ldca(a.kv_before + s), 0), cap);
-  w.held = (w.kv + up) >> a.ps_log2;
-  w.ends = r < 0;
-  w.n = max(r, 0);
-  w.too_long = w.n > cap - w.kv;
-  if (!w.too_long) w.more = ((w.kv + w.n + up) >> a.ps_log2) - w.held;
-  return w;
-}
-
-// The ended sequences' pages from `kept` on, those that are there, in order, by the whole warp.  lane i's sequence is
-// seq (ends: it is one); returns how many pages lane i's has, and stores them from free_pages[at] on if `at` >= 0.
-__device__ __forceinline__ int give_back(const PagedPlanArgs& a, int seq, const Wish& w, long long at) {
-  const int lane = threadIdx.x & 31;
-  int mine = 0;
-  for (unsigned todo = __ballot_sync(0xffffffffu, w.ends && w.held > 0); todo; todo &= todo - 1) {
-    const int src = __ffs(todo) - 1;
-    const int s = __shfl_sync(0xffffffffu, seq, src), held = __shfl_sync(0xffffffffu, w.held, src);
-    long long to = __shfl_sync(0xffffffffu, at, src);
-    const int* row = a.page_table + (size_t)s * a.max_pages;
-    int count = 0;
-    for (int j = min(max(a.kept ? __ldca(a.kept + s) : 0, 0), held) + lane; __any_sync(0xffffffffu, j < held); j += 32) {
-      const int page = j < held ? __ldca(row + j) : -1;
-      const bool real = page >= 0 && page < a.n_pages;
-      const unsigned which = __ballot_sync(0xffffffffu, real);
-      const long long mine_to = to + count + __popc(which & ((1u << lane) - 1));
-      if (at >= 0 && real && mine_to < a.n_pages) a.free_pages[mine_to] = page;
-      count += __popc(which);
-    }
-    if (lane == src) mine = count;
+// The last i < n with at[i] <= x, where at does not decrease and at[0] <= x: it has x, if any has.
+__device__ __forceinline__ int holder(const int* at, int n, int x) {
+  int lo = 0;
+  while (n - lo > 1) {
+    const int mid = (lo + n) / 2;
+    if (at[mid] <= x) lo = mid;
+    else n = mid;
   }
-  return mine;
+  return lo;
 }
-
-__device__ __forceinline__ long long shfl_up(long long v, int o) { return __shfl_up_sync(0xffffffffu, v, o); }
 
 template <bool kOne>  // one block and everything in it
 __global__ void __launch_bounds__(kThreads, 1) paged_plan_kernel(const __grid_constant__ PagedPlanArgs a) {
   __shared__ Sums s_warp[kWarps];
-  __shared__ int s_long[kWarps];
+  __shared__ int s_long[kWarps], s_found[kWarps];
   struct Total {
-    Sums sums;
+    Sums sums;     // back: pages that are there
     int too_long;  // the first sequence that is, or INT_MAX
   };
   __shared__ Total s_total;
-  __shared__ int s_row[kOne ? kBlockSeqs + 1 : 1], s_kv[kOne ? kBlockSeqs : 1];
+  // of each of the block's sequences: slots before; the first entry of the table that it takes a page for, or gives one
+  // back of; and the sums of the sequences before it: pages, entries, rows
+  extern __shared__ int s_dyn[];
+  __shared__ int s_one[kOne ? 5 * (kBlockSeqs + 1) : 1];
+  int* const s_kv = kOne ? s_one : s_dyn;
+  constexpr int kMost = kOne ? kBlockSeqs : kMostSeqs;
+  int* const s_from = s_kv + kMost + 1;
+  int* const s_take = s_from + kMost + 1;
+  int* const s_back = s_take + kMost + 1;
+  int* const s_row = s_back + kMost + 1;  // kOne alone
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kOne ? 0 : (int)cluster_ctarank(), blocks = kOne ? 1 : kCluster;
-  const int per = (a.n_seqs + blocks * kThreads - 1) / (blocks * kThreads);  // sequences of a thread
-  const int s0 = (rank * kThreads + threadIdx.x) * per;                      // (below 2^17)
+  const int mine = (a.n_seqs + blocks - 1) / blocks;  // sequences of a block
+  const int first = min(a.n_seqs, rank * mine), n = min(mine, a.n_seqs - first);
+  const int per = (n + kThreads - 1) / kThreads, i0 = min(n, (int)threadIdx.x * per), i1 = min(n, i0 + per);
+  const int cap = a.max_pages << a.ps_log2, up = (1 << a.ps_log2) - 1;
+  auto held_of = [&](int kv) { return (kv + up) >> a.ps_log2; };
   pdl_wait();
   const int n_free0 = min(max(__ldca(a.n_free_before), 0), a.n_pages);
 
-  Sums mine{0, 0, 0};
+  // ---- sums over the sequences
   int too_long = 0x7fffffff;
-  for (int i = 0; i < per; ++i) {
-    const int s = s0 + i;
-    const Wish w = wish(a, s, s < a.n_seqs);
-    if (w.too_long) too_long = min(too_long, s);
-    const int back = give_back(a, s, w, -1);
-    mine = mine + Sums{w.n, w.more, back};
-  }
-  Sums upto = mine;  // inclusive: of the warp's threads to this one
+  auto of_seq = [&](int i) {
+    const int s = first + i, r = __ldca(a.new_len + s), kept = a.kept ? __ldca(a.kept + s) : 0;
+    const int kv = min(max(__ldca(a.kv_before + s), 0), cap), held = held_of(kv);
+    Sums w{0, 0, 0};
+    s_kv[i] = kv;
+    s_from[i] = held;
+    if (r < 0) {
+      s_from[i] = min(max(kept, 0), held);
+      w.back = held - s_from[i];
+    } else {
+      w.rows = r;
+      if (r > cap - kv) too_long = min(too_long, s);
+      else w.more = held_of(kv + r) - held;
+    }
+    return w;
+  };
+  Sums own{0, 0, 0};
+  for (int i = i0; i < i1; ++i) own = own + of_seq(i);
+  Sums upto = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const Sums v{shfl_up(upto.rows, o), shfl_up(upto.more, o), shfl_up(upto.back, o)};
+    const Sums v{__shfl_up_sync(0xffffffffu, upto.rows, o), __shfl_up_sync(0xffffffffu, upto.more, o),
+                 __shfl_up_sync(0xffffffffu, upto.back, o)};
     if (lane >= o) upto = upto + v;
   }
   too_long = __reduce_min_sync(0xffffffffu, too_long);
@@ -117,131 +111,188 @@ __global__ void __launch_bounds__(kThreads, 1) paged_plan_kernel(const __grid_co
   too_long = __reduce_min_sync(0xffffffffu, s_long[lane]);
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const Sums v{shfl_up(sums.rows, o), shfl_up(sums.more, o), shfl_up(sums.back, o)};
+    const Sums v{__shfl_up_sync(0xffffffffu, sums.rows, o), __shfl_up_sync(0xffffffffu, sums.more, o),
+                 __shfl_up_sync(0xffffffffu, sums.back, o)};
     if (lane >= o) sums = sums + v;
   }
-  auto from = [&](long long v, int l) { return __shfl_sync(0xffffffffu, v, l); };
-  Sums all{from(sums.rows, 31), from(sums.more, 31), from(sums.back, 31)};
-  const int before_warp = max(warp - 1, 0);
-  Sums at{from(sums.rows, before_warp), from(sums.more, before_warp), from(sums.back, before_warp)};
+  auto from_lane = [&](const Sums& v, int l) {
+    return Sums{__shfl_sync(0xffffffffu, v.rows, l), __shfl_sync(0xffffffffu, v.more, l), __shfl_sync(0xffffffffu, v.back, l)};
+  };
+  const Sums block = from_lane(sums, 31);  // of the block
+  Sums at = from_lane(sums, max(warp - 1, 0));
   if (warp == 0) at = Sums{0, 0, 0};
-  at = Sums{at.rows + upto.rows - mine.rows, at.more + upto.more - mine.more, at.back + upto.back - mine.back};
-  if (!kOne) {
-    if (threadIdx.x == 0) s_total = Total{all, too_long};
-    cluster_sync_all();
-    all = Sums{0, 0, 0};
-    for (int c = 0; c < kCluster; ++c) {
-      const Total* t = dsmem_ptr(&s_total, c);
-      if (c < rank) at = at + t->sums;
-      all = all + t->sums;
-      too_long = min(too_long, t->too_long);
-    }
-    // (the next cluster barrier, which every block passes, comes after all of these loads)
-  }
-  const int top = (int)min(n_free0 + all.back, (long long)a.n_pages);
-  const bool ok = all.rows <= a.n_tokens && too_long == 0x7fffffff && all.more <= top;
-
-  if (all.back) {  // the same in every thread
-    long long to = n_free0 + at.back;
-    for (int i = 0; i < per; ++i) {
-      const int s = s0 + i;
-      to += give_back(a, s, wish(a, s, s < a.n_seqs), to);
+  at = at + upto - own;  // before this thread's sequences, in the block
+  {
+    Sums w = at;
+    for (int i = i0; i < i1; ++i) {
+      s_take[i] = w.more;
+      s_back[i] = w.back;
+      if (kOne) s_row[i] = (int)min(w.rows, 0x7fffffffll);
+      if (i + 1 < i1) w = w + of_seq(i);
     }
   }
-  // pages that one block gives back another may take
-  if (!kOne) cluster_sync_all();
-  else __syncthreads();
+  __syncthreads();
 
-  int row = ok ? (int)at.rows : 0;
-  long long take = top - 1 - at.more;  // the next page's place in the list
-  for (int i = 0; i < per; ++i) {
-    const int s = s0 + i;
-    const bool there = s < a.n_seqs;
-    const Wish w = wish(a, s, there);
-    const int more = ok ? w.more : 0;
-    // a page or two by the lane itself, more by the whole warp
-    if (more > 0 && more <= 2) {
-      int* to = a.page_table + (size_t)s * a.max_pages + w.held;
-      for (int j = 0; j < more; ++j) to[j] = __ldcg(a.free_pages + take - j);
-    }
-    for (unsigned todo = __ballot_sync(0xffffffffu, more > 2); todo; todo &= todo - 1) {
-      const int src = __ffs(todo) - 1, count = __shfl_sync(0xffffffffu, more, src);
-      const long long first = from(take, src);
-      int* to = a.page_table + (size_t)__shfl_sync(0xffffffffu, s, src) * a.max_pages + __shfl_sync(0xffffffffu, w.held, src);
-      for (int j = lane; j < count; j += 32) to[j] = __ldcg(a.free_pages + first - j);
-    }
-    take -= more;
-    if (there) {
-      a.q_start[s] = row;
-      if (kOne) {
-        s_row[s] = row;
-        s_kv[s] = w.kv;
+  // ---- pages of ended sequences, 1024 entries of their tables at a time, in order; where: the first one's place in the
+  // list, or -1 to count alone
+  auto give_back = [&](int where) {
+    int count = 0;
+    for (int b = 0; b < block.back; b += kThreads) {
+      const int x = b + threadIdx.x;
+      int page = -1;
+      if (x < block.back) {
+        const int i = holder(s_back, n, x);
+        page = __ldca(a.page_table + (size_t)(first + i) * a.max_pages + s_from[i] + x - s_back[i]);
       }
-      row += ok ? w.n : 0;
-      a.kv_len[s] = w.ends ? 0 : ok ? w.kv + w.n : w.kv;
-      if (s == a.n_seqs - 1) a.q_start[a.n_seqs] = row;
+      const bool there = page >= 0 && page < a.n_pages;
+      const unsigned which = __ballot_sync(0xffffffffu, there);
+      if (lane == 0) s_found[warp] = __popc(which);
+      __syncthreads();
+      int before = lane < warp ? s_found[lane] : 0, all = s_found[lane];
+      before = __reduce_add_sync(0xffffffffu, before) + __popc(which & ((1u << lane) - 1));
+      all = __reduce_add_sync(0xffffffffu, all);
+      if (where >= 0 && there && where + count + before < a.n_pages) a.free_pages[where + count + before] = page;
+      count += all;
+      __syncthreads();
+    }
+    return count;
+  };
+  const int gave = give_back(kOne ? n_free0 : -1);
+  long long rows = block.rows, back = gave, more = block.more, before_more = 0, before_rows = 0, before_back = 0;
+  if (!kOne) {
+    if (threadIdx.x == 0) s_total = Total{Sums{block.rows, block.more, gave}, too_long};
+    cluster_sync_all();
+    Total t{Sums{0, 0, 0}, 0x7fffffff};
+    if (lane < kCluster) t = *dsmem_ptr(&s_total, lane);
+    rows = back = more = 0;
+    for (int c = 0; c < kCluster; ++c) {
+      if (c == rank) before_rows = rows, before_more = more, before_back = back;
+      const Sums v = from_lane(t.sums, c);
+      rows += v.rows;
+      more += v.more;
+      back += v.back;
+    }
+    too_long = __reduce_min_sync(0xffffffffu, t.too_long);
+    if (gave) give_back((int)min(n_free0 + before_back, (long long)a.n_pages));
+    cluster_sync_all();  // pages that one block gives back another may take
+  }
+  const int top = (int)min(n_free0 + back, (long long)a.n_pages);
+  const bool ok = rows <= a.n_tokens && too_long == 0x7fffffff && more <= top;
+
+  // ---- the new pages (those given back are in the list: a barrier lies between)
+  if (ok)
+    for (int x = threadIdx.x; x < block.more; x += kThreads) {
+      const int i = holder(s_take, n, x);
+      a.page_table[(size_t)(first + i) * a.max_pages + s_from[i] + x - s_take[i]] =
+          __ldcg(a.free_pages + (top - 1 - (int)before_more - x));
+    }
+  {
+    long long row = ok ? before_rows + at.rows : 0;
+    for (int i = i0; i < i1; ++i) {
+      const int s = first + i, r = __ldca(a.new_len + s), kv = s_kv[i];
+      a.q_start[s] = (int)row;
+      if (ok) row += max(r, 0);
+      a.kv_len[s] = r < 0 ? 0 : ok ? kv + r : kv;
+      if (s == a.n_seqs - 1) a.q_start[a.n_seqs] = (int)row;
     }
   }
   if (rank == 0 && threadIdx.x == 0) {
     if (a.n_seqs == 0) a.q_start[0] = 0;
     auto short_by = [](long long need, long long have) { return (int)min(max(need - have, 0ll), 0x7fffffffll); };
-    a.n_free[0] = ok ? top - (int)all.more : top;
-    a.status[1] = short_by(all.more, top);
-    a.status[2] = short_by(all.rows, a.n_tokens);
+    a.n_free[0] = ok ? top - (int)more : top;
+    a.status[1] = short_by(more, top);
+    a.status[2] = short_by(rows, a.n_tokens);
     a.status[3] = too_long == 0x7fffffff ? -1 : too_long;
-    a.status[0] = (all.more > top ? kPlanPages : 0) | (all.rows > a.n_tokens ? kPlanRows : 0) |
+    a.status[0] = (more > top ? kPlanPages : 0) | (rows > a.n_tokens ? kPlanRows : 0) |
                   (too_long == 0x7fffffff ? 0 : kPlanTable);
   }
   if (kOne && ok && (a.pos || a.slots)) {
-    __syncthreads();  // the starts, and the table's new entries
-    for (int r = threadIdx.x; r < (int)all.rows; r += kThreads) {
-      int lo = 0, hi = a.n_seqs;  // the last sequence that starts at or before the row: it has it
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (s_row[mid] <= r) lo = mid;
-        else hi = mid;
+    __syncthreads();  // the table's new entries
+    constexpr int kAhead = 4;  // loads of the table under way
+    for (int r0 = threadIdx.x; r0 < (int)rows; r0 += kThreads * kAhead) {
+      int p[kAhead], page[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int r = r0 + k * kThreads;
+        if (r >= (int)rows) break;
+        const int i = holder(s_row, n, r);
+        p[k] = s_kv[i] + r - s_row[i];
+        if (a.slots) page[k] = __ldcg(a.page_table + (size_t)i * a.max_pages + (p[k] >> a.ps_log2));
       }
-      const int p = s_kv[lo] + r - s_row[lo];
-      if (a.pos) a.pos[r] = p;
-      if (a.slots) a.slots[r] = paged_slot(a, p, __ldcg(a.page_table + (size_t)lo * a.max_pages + (p >> a.ps_log2)));
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int r = r0 + k * kThreads;
+        if (r >= (int)rows) break;
+        if (a.pos) a.pos[r] = p[k];
+        if (a.slots) a.slots[r] = paged_slot(a, p[k], page[k]);
+      }
     }
   }
 }
 
-// Positions and slots of the rows of a large batch, which the first kernel has planned: a thread a row.
-constexpr int kRowThreads = 256;
+// Positions and slots of the rows of a large batch, which the first kernel has planned: a block has kBlockRows of them
+// and looks their sequences up in a window of starts and lengths in shared memory, from one probe by all its threads on.
+constexpr int kRowThreads = 256, kRowsEach = 4, kBlockRows = kRowThreads * kRowsEach;
+constexpr int kWindow = kBlockRows + 65536 / kRowThreads + 1;
 __global__ void __launch_bounds__(kRowThreads) paged_plan_rows_kernel(const __grid_constant__ PagedPlanArgs a) {
+  __shared__ int s_start[kWindow + 1], s_kv[kWindow];
   pdl_wait();
-  const int r0 = (blockIdx.x * kRowThreads + threadIdx.x) & ~31, r = r0 + (threadIdx.x & 31);
-  const int rows = __ldca(a.q_start + a.n_seqs);
+  const int rows = __ldca(a.q_start + a.n_seqs), r0 = blockIdx.x * kBlockRows;
   if (r0 >= rows) return;
-  PagedBatch b{};
-  b.q_start = a.q_start;
-  b.n_seqs = a.n_seqs;
-  int lo = paged_find_seq(b, r0), hi = paged_find_seq(b, min(r0 + 31, rows - 1)) + 1;
-  if (r >= rows) return;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (__ldca(a.q_start + mid) <= r) lo = mid;
-    else hi = mid;
+  const int step = (a.n_seqs + kRowThreads - 1) / kRowThreads, probe = threadIdx.x * step;
+  const int le = __syncthreads_count(probe < a.n_seqs && __ldca(a.q_start + probe) <= r0);
+  const int s0 = (le - 1) * step, n = min(kWindow, a.n_seqs - s0);  // (q_start[0] is 0)
+  for (int i = threadIdx.x; i <= n; i += kRowThreads) {
+    s_start[i] = __ldca(a.q_start + s0 + i);
+    if (i < n) s_kv[i] = __ldca(a.kv_len + s0 + i);
   }
-  const int p = __ldca(a.kv_len + lo) - __ldca(a.q_start + lo + 1) + r;
-  if (a.pos) a.pos[r] = p;
-  if (a.slots) a.slots[r] = paged_slot(a, p, __ldca(a.page_table + (size_t)lo * a.max_pages + (p >> a.ps_log2)));
+  __syncthreads();
+  int p[kRowsEach], page[kRowsEach];
+#pragma unroll
+  for (int k = 0; k < kRowsEach; ++k) {
+    const int r = r0 + k * kRowThreads + threadIdx.x;
+    if (r >= rows) break;
+    int s;
+    if (r < s_start[n]) {
+      const int i = holder(s_start, n, r);
+      s = s0 + i;
+      p[k] = s_kv[i] - s_start[i + 1] + r;
+    } else {  // behind the window: there are sequences without a token in it
+      s = s0 + n;
+      for (int hi = a.n_seqs; hi - s > 1;) {
+        const int mid = (s + hi) / 2;
+        if (__ldca(a.q_start + mid) <= r) s = mid;
+        else hi = mid;
+      }
+      p[k] = __ldca(a.kv_len + s) - __ldca(a.q_start + s + 1) + r;
+    }
+    if (a.slots) page[k] = __ldca(a.page_table + (size_t)s * a.max_pages + (p[k] >> a.ps_log2));
+  }
+#pragma unroll
+  for (int k = 0; k < kRowsEach; ++k) {
+    const int r = r0 + k * kRowThreads + threadIdx.x;
+    if (r >= rows) break;
+    if (a.pos) a.pos[r] = p[k];
+    if (a.slots) a.slots[r] = paged_slot(a, p[k], page[k]);
+  }
 }
 
 }  // namespace
 
-cudaError_t paged_plan(const PagedPlanArgs& a, cudaStream_t s) {
+cudaError_t paged_plan(const PagedPlanArgs& a, int device, cudaStream_t s) {
   PagedPlanArgs p = a;
   if (a.n_seqs <= kBlockSeqs && a.n_tokens <= kBlockTokens)
     return launch_kernel(reinterpret_cast<const void*>(&paged_plan_kernel<true>), dim3(1), dim3(kThreads), 0, s, true, &p);
   void* params[] = {&p};
-  const cudaError_t e = launch_cluster_params(reinterpret_cast<const void*>(&paged_plan_kernel<false>), dim3(kCluster),
-                                              dim3(kThreads), 0, s, kCluster, true, params);
+  const void* fn = reinterpret_cast<const void*>(&paged_plan_kernel<false>);
+  const size_t smem = 4 * (kMostSeqs + 1) * sizeof(int);
+  static SmemCap cap;
+  cudaError_t e = cap.raise(fn, device, smem);
+  if (e != cudaSuccess) return e;
+  e = launch_cluster_params(fn, dim3(kCluster), dim3(kThreads), smem, s, kCluster, true, params);
   if (e != cudaSuccess || (!a.pos && !a.slots) || a.n_tokens == 0) return e;
   return launch_kernel(reinterpret_cast<const void*>(&paged_plan_rows_kernel),
-                       dim3((a.n_tokens + kRowThreads - 1) / kRowThreads), dim3(kRowThreads), 0, s, true, &p);
+                       dim3((a.n_tokens + kBlockRows - 1) / kBlockRows), dim3(kRowThreads), 0, s, true, &p);
 }
 
 }  // namespace yb
