@@ -45,6 +45,28 @@ __device__ __forceinline__ int holder(const int* at, int n, int x) {
   return lo;
 }
 
+// Four neighbouring rows' positions and slots, r0 a multiple of 4.
+constexpr int kRowsEach = 4;
+__device__ __forceinline__ void write_rows(const PagedPlanArgs& a, int r0, int rows, const int (&p)[kRowsEach], const int (&page)[kRowsEach]) {
+  long long slot[kRowsEach];
+#pragma unroll
+  for (int k = 0; k < kRowsEach; ++k) slot[k] = a.slots ? paged_slot(a, p[k], page[k]) : 0;
+  const bool whole = r0 + kRowsEach <= rows;
+  if (a.pos && whole && (reinterpret_cast<uintptr_t>(a.pos) & 15) == 0) {
+    *reinterpret_cast<int4*>(a.pos + r0) = make_int4(p[0], p[1], p[2], p[3]);
+  } else if (a.pos) {
+    for (int k = 0; k < kRowsEach; ++k)
+      if (r0 + k < rows) a.pos[r0 + k] = p[k];
+  }
+  if (a.slots && whole && (reinterpret_cast<uintptr_t>(a.slots) & 15) == 0) {
+    reinterpret_cast<longlong2*>(a.slots + r0)[0] = make_longlong2(slot[0], slot[1]);
+    reinterpret_cast<longlong2*>(a.slots + r0)[1] = make_longlong2(slot[2], slot[3]);
+  } else if (a.slots) {
+    for (int k = 0; k < kRowsEach; ++k)
+      if (r0 + k < rows) a.slots[r0 + k] = slot[k];
+  }
+}
+
 template <bool kOne>  // one block and everything in it
 __global__ void __launch_bounds__(kThreads, 1) paged_plan_kernel(const __grid_constant__ PagedPlanArgs a) {
   __shared__ Sums s_warp[kWarps];
@@ -133,31 +155,44 @@ __global__ void __launch_bounds__(kThreads, 1) paged_plan_kernel(const __grid_co
   }
   __syncthreads();
 
-  // ---- pages of ended sequences, 1024 entries of their tables at a time, in order; where: the first one's place in the
-  // list, or -1 to count alone
-  auto give_back = [&](int where) {
-    int count = 0;
-    for (int b = 0; b < block.back; b += kThreads) {
-      const int x = b + threadIdx.x;
-      int page = -1;
-      if (x < block.back) {
-        const int i = holder(s_back, n, x);
-        page = __ldca(a.page_table + (size_t)(first + i) * a.max_pages + s_from[i] + x - s_back[i]);
-      }
-      const bool there = page >= 0 && page < a.n_pages;
-      const unsigned which = __ballot_sync(0xffffffffu, there);
-      if (lane == 0) s_found[warp] = __popc(which);
-      __syncthreads();
-      int before = lane < warp ? s_found[lane] : 0, all = s_found[lane];
-      before = __reduce_add_sync(0xffffffffu, before) + __popc(which & ((1u << lane) - 1));
-      all = __reduce_add_sync(0xffffffffu, all);
-      if (where >= 0 && there && where + count + before < a.n_pages) a.free_pages[where + count + before] = page;
-      count += all;
-      __syncthreads();
+  // A thread's part of `all` entries or pages, in order: f(sequence, the entry within its share, place among all).
+  auto share = [&](const int* sums_before, int all, auto&& f) {
+    const int each = (all + kThreads - 1) / kThreads, x0 = min(all, (int)threadIdx.x * each), x1 = min(all, x0 + each);
+    if (x0 >= x1) return;
+    int i = holder(sums_before, n, x0);
+    for (int x = x0; x < x1; ++x) {
+      while (i + 1 < n && sums_before[i + 1] <= x) ++i;
+      f(i, x - sums_before[i], x);
     }
-    return count;
   };
-  const int gave = give_back(kOne ? n_free0 : -1);
+  // ---- pages of ended sequences
+  auto entry = [&](int i, int j) { return __ldca(a.page_table + (size_t)(first + i) * a.max_pages + s_from[i] + j); };
+  int found = 0, gave = 0, gave_before = 0;  // pages that are there: of this thread, of the block, of the threads before
+  if (block.back) {
+    share(s_back, block.back, [&](int i, int j, int) {
+      const int page = entry(i, j);
+      found += page >= 0 && page < a.n_pages;
+    });
+    int v = found;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) s_found[warp] = v;
+    __syncthreads();
+    const int w = s_found[lane];
+    gave = __reduce_add_sync(0xffffffffu, w);
+    gave_before = __reduce_add_sync(0xffffffffu, lane < warp ? w : 0) + v - found;
+  }
+  auto give_back = [&](int where) {  // the block's first page's place in the list
+    where += gave_before;
+    if (found)
+      share(s_back, block.back, [&](int i, int j, int) {
+        const int page = entry(i, j);
+        if (page >= 0 && page < a.n_pages && where < a.n_pages) a.free_pages[where++] = page;
+      });
+  };
   long long rows = block.rows, back = gave, more = block.more, before_more = 0, before_rows = 0, before_back = 0;
   if (!kOne) {
     if (threadIdx.x == 0) s_total = Total{Sums{block.rows, block.more, gave}, too_long};
@@ -173,19 +208,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_plan_kernel(const __grid_co
       back += v.back;
     }
     too_long = __reduce_min_sync(0xffffffffu, t.too_long);
-    if (gave) give_back((int)min(n_free0 + before_back, (long long)a.n_pages));
-    cluster_sync_all();  // pages that one block gives back another may take
+    if (back) {  // (the same in all blocks)
+      give_back((int)min(n_free0 + before_back, (long long)a.n_pages));
+      cluster_sync_all();  // pages that one block gives back another may take
+    }
+  } else if (back) {
+    give_back(n_free0);
+    __syncthreads();
   }
   const int top = (int)min(n_free0 + back, (long long)a.n_pages);
   const bool ok = rows <= a.n_tokens && too_long == 0x7fffffff && more <= top;
 
   // ---- the new pages (those given back are in the list: a barrier lies between)
   if (ok)
-    for (int x = threadIdx.x; x < block.more; x += kThreads) {
-      const int i = holder(s_take, n, x);
-      a.page_table[(size_t)(first + i) * a.max_pages + s_from[i] + x - s_take[i]] =
-          __ldcg(a.free_pages + (top - 1 - (int)before_more - x));
-    }
+    share(s_take, block.more, [&](int i, int j, int x) {
+      a.page_table[(size_t)(first + i) * a.max_pages + s_from[i] + j] = __ldcg(a.free_pages + (top - 1 - (int)before_more - x));
+    });
   {
     long long row = ok ? before_rows + at.rows : 0;
     for (int i = i0; i < i1; ++i) {
@@ -196,6 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_plan_kernel(const __grid_co
       if (s == a.n_seqs - 1) a.q_start[a.n_seqs] = (int)row;
     }
   }
+  if (!kOne) cluster_sync_all();  // nobody leaves while others read its totals
   if (rank == 0 && threadIdx.x == 0) {
     if (a.n_seqs == 0) a.q_start[0] = 0;
     auto short_by = [](long long need, long long have) { return (int)min(max(need - have, 0ll), 0x7fffffffll); };
@@ -208,31 +247,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_plan_kernel(const __grid_co
   }
   if (kOne && ok && (a.pos || a.slots)) {
     __syncthreads();  // the table's new entries
-    constexpr int kAhead = 4;  // loads of the table under way
-    for (int r0 = threadIdx.x; r0 < (int)rows; r0 += kThreads * kAhead) {
-      int p[kAhead], page[kAhead];
+    for (int r0 = threadIdx.x * kRowsEach; r0 < (int)rows; r0 += kThreads * kRowsEach) {
+      int p[kRowsEach], page[kRowsEach], i = holder(s_row, n, r0);
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int r = r0 + k * kThreads;
-        if (r >= (int)rows) break;
-        const int i = holder(s_row, n, r);
-        p[k] = s_kv[i] + r - s_row[i];
+      for (int k = 0; k < kRowsEach; ++k) {
+        p[k] = page[k] = -1;
+        if (r0 + k >= (int)rows) continue;
+        while (i + 1 < n && s_row[i + 1] <= r0 + k) ++i;
+        p[k] = s_kv[i] + r0 + k - s_row[i];
         if (a.slots) page[k] = __ldcg(a.page_table + (size_t)i * a.max_pages + (p[k] >> a.ps_log2));
       }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int r = r0 + k * kThreads;
-        if (r >= (int)rows) break;
-        if (a.pos) a.pos[r] = p[k];
-        if (a.slots) a.slots[r] = paged_slot(a, p[k], page[k]);
-      }
+      write_rows(a, r0, (int)rows, p, page);
     }
   }
 }
 
 // Positions and slots of the rows of a large batch, which the first kernel has planned: a block has kBlockRows of them
 // and looks their sequences up in a window of starts and lengths in shared memory, from one probe by all its threads on.
-constexpr int kRowThreads = 256, kRowsEach = 4, kBlockRows = kRowThreads * kRowsEach;
+constexpr int kRowThreads = 256, kBlockRows = kRowThreads * kRowsEach;
 constexpr int kWindow = kBlockRows + 65536 / kRowThreads + 1;
 __global__ void __launch_bounds__(kRowThreads) paged_plan_rows_kernel(const __grid_constant__ PagedPlanArgs a) {
   __shared__ int s_start[kWindow + 1], s_kv[kWindow];
@@ -247,14 +279,17 @@ __global__ void __launch_bounds__(kRowThreads) paged_plan_rows_kernel(const __gr
     if (i < n) s_kv[i] = __ldca(a.kv_len + s0 + i);
   }
   __syncthreads();
-  int p[kRowsEach], page[kRowsEach];
+  const int t0 = r0 + threadIdx.x * kRowsEach;
+  if (t0 >= rows) return;
+  int p[kRowsEach], page[kRowsEach], i = holder(s_start, n, t0);
 #pragma unroll
   for (int k = 0; k < kRowsEach; ++k) {
-    const int r = r0 + k * kRowThreads + threadIdx.x;
-    if (r >= rows) break;
+    const int r = t0 + k;
+    p[k] = page[k] = -1;
+    if (r >= rows) continue;
     int s;
     if (r < s_start[n]) {
-      const int i = holder(s_start, n, r);
+      while (s_start[i + 1] <= r) ++i;
       s = s0 + i;
       p[k] = s_kv[i] - s_start[i + 1] + r;
     } else {  // behind the window: there are sequences without a token in it
@@ -268,13 +303,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_plan_rows_kernel(const __gr
     }
     if (a.slots) page[k] = __ldca(a.page_table + (size_t)s * a.max_pages + (p[k] >> a.ps_log2));
   }
-#pragma unroll
-  for (int k = 0; k < kRowsEach; ++k) {
-    const int r = r0 + k * kRowThreads + threadIdx.x;
-    if (r >= rows) break;
-    if (a.pos) a.pos[r] = p[k];
-    if (a.slots) a.slots[r] = paged_slot(a, p[k], page[k]);
-  }
+  write_rows(a, t0, rows, p, page);
 }
 
 }  // namespace

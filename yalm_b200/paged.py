@@ -23,6 +23,13 @@ def _dtype(t, name: str) -> int:
     return d
 
 
+def _raw_stream():
+    """A function from a GPU's index to torch's current stream there, as a cudaStream_t."""
+    import torch
+    # torch.cuda.current_stream makes a Stream object for it, which takes 1.2 us
+    return getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 class PagedBatch:
     """k_pages, v_pages [n_pages][n_kv_heads][page_size][head_dim] fp16 or bf16; page_table [n_seqs][max_pages],
     q_start [n_seqs + 1] and kv_len [n_seqs] int32; n_tokens: rows of the token-major tensors.  All on one
@@ -62,7 +69,7 @@ class PagedBatch:
         self._index = k_pages.get_device()
         import torch  # the caller's tensors are torch's; the package itself does not need it
         self._f32, self._i32, self._i64 = torch.float32, torch.int32, torch.int64
-        self._current = torch.cuda.current_stream
+        self._current = _raw_stream()
         self._q_shape = (self.n_tokens, self.n_heads * self.head_dim)
         self._qkv_shape = (self.n_tokens, (self.n_heads + 2 * self.n_kv_heads) * self.head_dim)
 
@@ -74,7 +81,7 @@ class PagedBatch:
         return row if self.n_tokens > 1 else shape[1]
 
     def _stream(self) -> int:
-        return self._current(self._index).cuda_stream if self._index >= 0 else 0
+        return self._current(self._index) if self._index >= 0 else 0
 
     def _vector(self, t, name: str, n: int, dtype):
         """Checks an optional vector and returns its address."""
