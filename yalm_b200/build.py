@@ -25,7 +25,7 @@ NVCC_FLAGS = ARCH + [
     "-Xcompiler", "-fPIC,-O3", "-I" + os.path.join(ROOT, "include"),
 ]
 CU_SOURCES = ["gemv.cu", "attention.cu", "persistent.cu", "engine.cu", "capi.cu", "noalloc.cu", "sampler.cu", "loader.cu", "prefill_gemm.cu", "prefill.cu", "prefill_attn_tc.cu", "prefill_run.cu",
-              "paged_append.cu", "paged_attn.cu", "paged_capi.cu", "paged_plan.cu", "paged_shared.cu", "sample_rows.cu", "sample_capi.cu"]
+              "paged_append.cu", "paged_attn.cu", "paged_capi.cu", "paged_plan.cu", "paged_shared.cu", "paged_few.cu", "sample_rows.cu", "sample_capi.cu"]
 HEADERS = ["common.cuh", "gemv.cuh", "attention.cuh", "persistent.cuh", "launch.h", "engine.h", "loader.h", "prefill.cuh",
            "prefill_gemm.cuh", "sampler.cuh", "tmap.h", "umma.cuh", "paged.cuh", "paged_axis.cuh", "cluster.cuh", "sample_rows.cuh", "checks.h", "paged_shared.cuh", "paged_shared_axis.cuh"]
 

@@ -265,6 +265,8 @@ struct PagedAttnParams {
   int n_groups;
   int part_rows;  // rows of a kv head in parts: of the tokens that have both
   float* parts;   // [prefixes, sequences][kv heads], a record of part_rows rows each
+  const float* few_recs;   // of sequences of few rows
+  const float* few_parts;
 };
 
 // Waits for the phase, or until the budget has run out, here or in another warp of the block, which *mark then tells.
@@ -948,13 +950,52 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     else hi = mid;
   }
   const SharedSeq own = paged_seq(a.shared, a.n_groups + lo);
-  if (token < own.row0 || token >= own.row0 + own.n) return;
+  if (token < own.row0 || token >= own.row0 + max(own.n, own.few)) return;
   const unsigned long long share = __ldca(&a.head->share);
   const int more = __ldca(&a.head->more);
   float mm = -INFINITY, ll = 0.f, acc[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+  auto join = [&](float m, float l, const float (&v)[8]) {
+    const float mn = fmaxf(mm, m);
+    const float old = mm == -INFINITY ? 0.f : ex2(mm - mn), w = m == -INFINITY ? 0.f : ex2(m - mn);
+    mm = mn;
+    ll = ll * old + l * w;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = acc[j] * old + v[j] * w;
+  };
   // a unit's parts: false if its outputs are in their place already
+  auto take_few = [&](const SharedSeq& q) {
+    const unsigned long long share = __ldca(&a.head->few_share), begin = q.few_begin + (unsigned long long)few_length(q) * head;
+    const int more = __ldca(&a.head->few_more);
+    const int first = block_of(share, more, begin), parts = block_of(share, more, begin + few_steps(q) - 1) - first + 1;
+    if (parts == 1 && q.part < 0) return false;
+    const int r = (token - q.row0) * a.gq + h;
+    const float* whole = a.few_parts + ((size_t)(q.part + token - q.row0) * b.n_heads + head * a.gq + h) * few_row_floats(HD);
+    for (int p0 = 0; p0 < parts; p0 += kMergeParts) {
+      float2 ml[kMergeParts];
+      float4 o[kMergeParts][2];
+#pragma unroll
+      for (int k = 0; k < kMergeParts; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.f);
+        o[k][0] = o[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int part = p0 + k;
+        if (part < parts) {
+          const float* rec = parts == 1 ? whole
+                                        : a.few_recs + (((size_t)(first + part) * 2 + (part == 0 ? 1 : 0)) * kFewRows + r) * few_row_floats(HD);
+          o[k][0] = __ldcg(reinterpret_cast<const float4*>(rec + 8 * c8));
+          o[k][1] = __ldcg(reinterpret_cast<const float4*>(rec + 8 * c8 + 4));
+          ml[k] = __ldcg(reinterpret_cast<const float2*>(rec + HD));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kMergeParts; ++k) {
+        const float v[8] = {o[k][0].x, o[k][0].y, o[k][0].z, o[k][0].w, o[k][1].x, o[k][1].y, o[k][1].z, o[k][1].w};
+        join(ml[k].x, ml[k].y, v);
+      }
+    }
+    return true;
+  };
   auto take = [&](const SharedSeq& q) {
     const int at = token - q.row0, unit = at / a.x.U;
     const Unit u = unit_of(a.x, q, unit);
@@ -988,17 +1029,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 #pragma unroll
       for (int k = 0; k < kMergeParts; ++k) {
         const float v[8] = {o[k][0].x, o[k][0].y, o[k][0].z, o[k][0].w, o[k][1].x, o[k][1].y, o[k][1].z, o[k][1].w};
-        const float mn = fmaxf(mm, m[k]);
-        const float old = mm == -INFINITY ? 0.f : ex2(mm - mn), w = m[k] == -INFINITY ? 0.f : ex2(m[k] - mn);
-        mm = mn;
-        ll = ll * old + l[k] * w;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = acc[j] * old + v[j] * w;
+        join(m[k], l[k], v);
       }
     }
     return true;
   };
-  if (!take(own)) return;
+  if (!(own.few ? take_few(own) : take(own))) return;
   if (own.part >= 0) take(paged_seq(a.shared, own.group));
   const float inv = ll != 0.f ? 1.f / ll : 0.f;
   T* out = static_cast<T*>(a.out) + (size_t)token * a.out_stride + (size_t)(head * a.gq + h) * HD + 8 * c8;
@@ -1025,8 +1061,15 @@ static size_t shared_plan_at(int head_dim, int n_sms) { return (paged_attention_
 static size_t shared_parts_at(const PagedBatch& b, int n_groups, int head_dim, int n_sms) {
   return shared_plan_at(head_dim, n_sms) + 256 + ((size_t)n_groups + b.n_seqs) * sizeof(SharedSeq);
 }
-size_t paged_shared_scratch(const PagedBatch& b, int n_groups, int head_dim, int n_sms) {
+static size_t few_parts_at(const PagedBatch& b, int n_groups, int head_dim, int n_sms) {
   return shared_parts_at(b, n_groups, head_dim, n_sms) + (size_t)2 * b.n_kv_heads * (head_dim + 2) * part_rows(b) * 4;
+}
+static size_t few_recs_at(const PagedBatch& b, int n_groups, int head_dim, int n_sms) {
+  return few_parts_at(b, n_groups, head_dim, n_sms) + (size_t)part_tokens(b) * b.n_heads * few_row_floats(head_dim) * 4;
+}
+size_t paged_shared_scratch(const PagedBatch& b, int n_groups, int head_dim, int n_sms) {
+  return few_recs_at(b, n_groups, head_dim, n_sms) +
+         (size_t)few_warps(paged_attention_grid(n_sms)) * 2 * kFewRows * few_row_floats(head_dim) * 4;
 }
 
 namespace {
@@ -1060,25 +1103,30 @@ cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cuda
   if constexpr (kShared) {
     char* const base = static_cast<char*>(a.scratch);
     const size_t plan = shared_plan_at(HD, a.n_sms);
-    SharedPlanArgs sp{a.b, a.group_start, a.prefix_len, a.n_groups, p.x, grid, part_tokens(a.b), reinterpret_cast<SharedHead*>(base + plan),
+    SharedPlanArgs sp{a.b, a.group_start, a.prefix_len, a.n_groups, p.x, grid, few_warps(grid), part_tokens(a.b), reinterpret_cast<SharedHead*>(base + plan),
                       reinterpret_cast<SharedSeq*>(base + plan + 256)};
     p.shared = SharedBatch{sp.seqs, a.n_groups + a.b.n_seqs};
     p.head = sp.head;
     p.n_groups = a.n_groups;
     p.part_rows = (int)part_rows(a.b);
     p.parts = reinterpret_cast<float*>(base + shared_parts_at(a.b, a.n_groups, HD, a.n_sms));
+    p.few_parts = reinterpret_cast<float*>(base + few_parts_at(a.b, a.n_groups, HD, a.n_sms));
+    p.few_recs = reinterpret_cast<float*>(base + few_recs_at(a.b, a.n_groups, HD, a.n_sms));
     if ((e = paged_shared_plan(sp, s)) != cudaSuccess) return e;
   }
   void* args[] = {&qm, &km, &vm, &p};
   // both kernels set up under the end of the one before (programmatic launch): 37.0 -> 33.1 us for one token over
   // 32767 slots, 47.8 -> 43.9 us for the chunk of 512
   if ((e = launch_kernel_params(fn, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, s, true, args)) != cudaSuccess) return e;
-  if (a.b.max_pages * ps <= kKT) return cudaSuccess;  // every unit is one key tile: nothing is cut
   if constexpr (kShared) {
+    const PagedFewArgs f{a.b, p.shared, p.head, a.q, a.out, a.k_pages, a.v_pages, a.q_stride, a.out_stride, K, gq, p.c,
+                         const_cast<float*>(p.few_recs), const_cast<float*>(p.few_parts)};
+    if ((e = paged_few(f, HD, bf16 ? 2 : 1, grid, s)) != cudaSuccess) return e;
     const long long items = (long long)a.b.n_tokens * gq * K * (HD / 8);
     return launch_kernel(reinterpret_cast<const void*>(&paged_join_kernel<HD, T>),
                          dim3((unsigned)((items + kJoinThreads - 1) / kJoinThreads)), dim3(kJoinThreads), 0, s, true, &p);
   }
+  if (a.b.max_pages * ps <= kKT) return cudaSuccess;  // every unit is one key tile: nothing is cut
   return launch_kernel(reinterpret_cast<const void*>(&paged_merge_kernel<HD, T>), dim3(grid, kMergeSlices),
                        dim3(kMergeThreads), 0, s, true, &p);
 }

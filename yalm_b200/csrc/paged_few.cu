@@ -1,0 +1,257 @@
+// Attention of sequences with few rows (up to 8: tokens x query heads of a kv head) over the paged cache, for batches
+// with shared prefixes, whose sequences' own slots are mostly few (paged_attn.cu has the prefixes and longer chunks).
+//
+// What bounds it is the cache's bytes, if starts and ends of many short units cost little: the tensor-core path pays
+// 4000 to 5500 clocks of a block for them, which for 3 tiles of own slots is as much as their bytes take.  Here a warp
+// works by itself, without shared memory or barriers: steps of 16 slots (of one page), K and V straight from memory into
+// the operands of mma.m16n8k16, for which the order of the dimensions inside a product is chosen so that every lane
+// loads 16 bytes at a time:
+//   S^T = K . Q^T   slots x rows; the product over dims takes dims 32c + 8q .. + 7 of lane q's chunk in any order, if K
+//                   and Q have the same one
+//   O^T += V^T . P^T  dims x rows; P^T is S^T's transpose in registers (movmatrix), V's operand pairs two slots of a
+//                   dimension, by byte permutes of two rows' chunks
+// Units (sequence, kv head) in order make an axis of steps that all warps share out evenly; a unit that is cut leaves
+// records, which the join puts together (paged_attn.cu).  Weights are rounded to the caches' type as there, fp16 with a
+// factor 2^7; the rest is fp32.
+#include <cuda_bf16.h>
+
+#include <math.h>
+#include <type_traits>
+
+#include "launch.h"
+#include "paged_shared.cuh"
+
+namespace yb {
+
+namespace {
+
+typedef unsigned long long u64;
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi, __half) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
+
+template <int HD, typename T>
+__global__ void __launch_bounds__(kFewThreads, kFewBlocks) paged_few_kernel(const __grid_constant__ PagedFewArgs a) {
+  constexpr int kC = HD / 32, kJ = HD / 64;  // chunks of 32 dims of K, of 64 of V
+  constexpr float kBias = std::is_same<T, __half>::value ? 7.f : 0.f;
+  const PagedBatch& b = a.b;
+  const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  const int warp = blockIdx.x * (kFewThreads / 32) + (threadIdx.x >> 5);
+  pdl_wait();
+  const u64 total = __ldca(&a.head->few_total), share = __ldca(&a.head->few_share);
+  const int more = __ldca(&a.head->few_more);
+  const u64 begin = block_begin(share, more, warp);
+  if (begin >= total) return;
+  int left = (int)min(share + (warp < more ? 1 : 0), total - begin);
+  // the last sequence that begins at or before this warp's part: those without rows here that begin there come earlier
+  int seq = 0;
+  for (int hi = a.shared.n_seqs; hi - seq > 1;) {
+    const int step = (hi - seq + 31) / 32, at = seq + (lane + 1) * step;
+    const int n = __popc(__ballot_sync(0xffffffffu, at < hi && __ldca(&a.shared.seqs[at].few_begin) <= begin));
+    seq += n * step;
+    hi = min(hi, seq + step);
+  }
+  SharedSeq sq = paged_seq(a.shared, seq);
+  int head, off;
+  {
+    const unsigned length = few_length(sq);
+    const u64 rem = begin - sq.few_begin;
+    head = (int)quot(rem, length);
+    off = (int)(rem - (u64)head * length);
+  }
+  const size_t row_elems = HD;
+  const int ps = 1 << b.ps_log2;
+  for (;;) {
+    // ---- a piece: steps [t0, t1) of the unit
+    const int steps = few_steps(sq), length = steps + kFewUnit, t0 = off, t1 = min(steps, off + left);
+    if (t0 < t1) {
+      const int rows = sq.few * a.gq;  // row r: token r / gq, head r % gq
+      const T* qrow = static_cast<const T*>(a.q);
+      uint4 qf[kC];
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        qf[c] = zero4();
+        if (g < rows)
+          qf[c] = __ldca(reinterpret_cast<const uint4*>(qrow + (size_t)(sq.row0 + g / a.gq) * a.q_stride +
+                                                        (size_t)(head * a.gq + g % a.gq) * HD + 32 * c + 8 * q4));
+      }
+      // the slots that rows 2 q4 and 2 q4 + 1 see end here
+      const int last0 = sq.kv - sq.few + (2 * q4) / a.gq + 1, last1 = sq.kv - sq.few + (2 * q4 + 1) / a.gq + 1;
+      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+      float o[2 * kC][4];  // o[4 j + i]: dims 64 j + 8 g + 2 i, + 1 of rows 2 q4, 2 q4 + 1
+#pragma unroll
+      for (int i = 0; i < 2 * kC; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      const int* table = b.page_table + (size_t)sq.table * b.max_pages;
+      const int slot_lo = sq.lo * kKT;
+      int pages = -1;  // lane i: the page of step (t & ~31) + i of the piece
+      for (int t = t0; t < t1; ++t) {
+        const int slot = slot_lo + t * kFewSlots;
+        if (((t - t0) & 31) == 0) {
+          const int s = slot + lane * kFewSlots;
+          pages = s < sq.kv && t + lane < t1 ? __ldca(table + (s >> b.ps_log2)) : -1;
+          if (pages >= b.n_pages) pages = -1;
+        }
+        const int page = __shfl_sync(0xffffffffu, pages, (t - t0) & 31);
+        if (page < 0) continue;
+        const size_t base = (((size_t)page * a.K + head) * ps + (slot & (ps - 1))) * row_elems;
+        const T* kp = static_cast<const T*>(a.k_pages) + base + (size_t)g * HD + 8 * q4;
+        const T* vp = static_cast<const T*>(a.v_pages) + base + (size_t)(2 * q4) * HD + 8 * g;
+        uint4 k0[kC], k1[kC], v[kJ][4];
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+          k0[c] = __ldcs(reinterpret_cast<const uint4*>(kp + 32 * c));
+          k1[c] = __ldcs(reinterpret_cast<const uint4*>(kp + 8 * HD + 32 * c));
+        }
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+          v[j][0] = __ldcs(reinterpret_cast<const uint4*>(vp + 64 * j));
+          v[j][1] = __ldcs(reinterpret_cast<const uint4*>(vp + HD + 64 * j));
+          v[j][2] = __ldcs(reinterpret_cast<const uint4*>(vp + 8 * HD + 64 * j));
+          v[j][3] = __ldcs(reinterpret_cast<const uint4*>(vp + 9 * HD + 64 * j));
+        }
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+          mma<T>(s, k0[c].x, k1[c].x, k0[c].y, k1[c].y, qf[c].x, qf[c].y);
+          mma<T>(s, k0[c].z, k1[c].z, k0[c].w, k1[c].w, qf[c].z, qf[c].w);
+        }
+        if (slot + kFewSlots > sq.kv - sq.few) {  // an edge
+          const int at = slot + g;
+          if (at >= last0) s[0] = -INFINITY;
+          if (at >= last1) s[1] = -INFINITY;
+          if (at + 8 >= last0) s[2] = -INFINITY;
+          if (at + 8 >= last1) s[3] = -INFINITY;
+          // what lies behind the last slot may be anything, and 0 of it has to be 0
+          const int n = sq.kv - slot - 2 * q4;
+#pragma unroll
+          for (int j = 0; j < kJ; ++j) {
+            if (n <= 0) v[j][0] = zero4();
+            if (n <= 1) v[j][1] = zero4();
+            if (n <= 8) v[j][2] = zero4();
+            if (n <= 9) v[j][3] = zero4();
+          }
+        }
+        float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+          x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+        }
+        const float n0 = fmaxf(m0, x0 * a.c), n1 = fmaxf(m1, x1 * a.c);
+        const float f0 = n0 == -INFINITY ? 0.f : n0 - kBias, f1 = n1 == -INFINITY ? 0.f : n1 - kBias;
+        if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
+          const float r0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0), r1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
+          l0 *= r0;
+          l1 *= r1;
+#pragma unroll
+          for (int i = 0; i < 2 * kC; ++i) {
+            o[i][0] *= r0;
+            o[i][1] *= r1;
+            o[i][2] *= r0;
+            o[i][3] *= r1;
+          }
+          m0 = n0;
+          m1 = n1;
+        }
+        s[0] = ex2(fmaf(s[0], a.c, -f0));
+        s[1] = ex2(fmaf(s[1], a.c, -f1));
+        s[2] = ex2(fmaf(s[2], a.c, -f0));
+        s[3] = ex2(fmaf(s[3], a.c, -f1));
+        l0 += s[0] + s[2];
+        l1 += s[1] + s[3];
+        const uint32_t p0 = movm_trans(pack(s[0], s[1], T())), p1 = movm_trans(pack(s[2], s[3], T()));
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+          const uint32_t w[4][4] = {{v[j][0].x, v[j][0].y, v[j][0].z, v[j][0].w}, {v[j][1].x, v[j][1].y, v[j][1].z, v[j][1].w},
+                                    {v[j][2].x, v[j][2].y, v[j][2].z, v[j][2].w}, {v[j][3].x, v[j][3].y, v[j][3].z, v[j][3].w}};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            mma<T>(o[4 * j + i], __byte_perm(w[0][i], w[1][i], 0x5410), __byte_perm(w[0][i], w[1][i], 0x7632),
+                   __byte_perm(w[2][i], w[3][i], 0x5410), __byte_perm(w[2][i], w[3][i], 0x7632), p0, p1);
+        }
+      }
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+      }
+      const bool whole = t0 == 0 && t1 == steps;
+      // ---- rows 2 q4 and 2 q4 + 1: the outputs, or a record
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 2 * q4 + e;
+        if (r >= rows) continue;
+        const float m = e ? m1 : m0, l = e ? l1 : l0;
+        const int token = r / a.gq, h = head * a.gq + r % a.gq;
+        if (whole && sq.part < 0) {
+          const float inv = l != 0.f ? 1.f / l : 0.f;
+          T* out = static_cast<T*>(a.out) + (size_t)(sq.row0 + token) * a.out_stride + (size_t)h * HD + 8 * g;
+#pragma unroll
+          for (int j = 0; j < kJ; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = pack(o[4 * j + i][e] * inv, o[4 * j + i][2 + e] * inv, T());
+            *reinterpret_cast<uint4*>(out + 64 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else {
+          float* rec = whole ? a.parts + ((size_t)(sq.part + token) * b.n_heads + h) * few_row_floats(HD)
+                             : a.recs + (((size_t)warp * 2 + (t0 == 0 ? 1 : 0)) * kFewRows + r) * few_row_floats(HD);
+#pragma unroll
+          for (int j = 0; j < kJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2)
+              *reinterpret_cast<float4*>(rec + 64 * j + 8 * g + 2 * i) =
+                  make_float4(o[4 * j + i][e], o[4 * j + i][2 + e], o[4 * j + i + 1][e], o[4 * j + i + 1][2 + e]);
+          if (g == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(m, l);
+        }
+      }
+    }
+    // ---- the next unit
+    left -= min(length - off, left);
+    if (left <= 0) return;
+    off = 0;
+    if (++head >= a.K) {
+      head = 0;
+      do {
+        if (++seq >= a.shared.n_seqs) return;
+        sq = paged_seq(a.shared, seq);
+      } while (sq.few <= 0);
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t paged_few(const PagedFewArgs& a, int head_dim, int type, int grid, cudaStream_t s) {
+  PagedFewArgs p = a;
+  const void* fn = head_dim == 128 ? (type == 1 ? reinterpret_cast<const void*>(&paged_few_kernel<128, __half>)
+                                                : reinterpret_cast<const void*>(&paged_few_kernel<128, __nv_bfloat16>))
+                                   : (type == 1 ? reinterpret_cast<const void*>(&paged_few_kernel<64, __half>)
+                                                : reinterpret_cast<const void*>(&paged_few_kernel<64, __nv_bfloat16>));
+  return launch_kernel(fn, dim3(grid * kFewBlocks), dim3(kFewThreads), 0, s, true, &p);
+}
+
+}  // namespace yb

@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
     }
   }
   __syncthreads();
-  const int all = a.n_groups + b.n_seqs;
+  const int all = a.n_groups + b.n_seqs, gq = b.n_heads / b.n_kv_heads;
   auto seq_at = [&](int v) {
     SharedSeq q{};
     q.part = -1;
@@ -116,12 +116,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
     const PagedSeq p = paged_seq(b, s);
     q.row0 = p.row0;
     q.n = p.n;
+    if (p.n * gq <= kFewRows) q.few = p.n, q.n = 0;
     q.kv = p.kv;
     q.table = s;
     if (p.n > 0 && g >= 0 && s_cut[g]) {
       int row0;
       const int rows = rows_of(g, row0), at = q.row0 - row0;
-      if (at >= 0 && at + q.n <= rows) {  // (else q_start decreases)
+      if (at >= 0 && at + p.n <= rows) {  // (else q_start decreases)
         q.lo = s_cut[g];
         q.part = s_part[g] + at;
         q.group = g;
@@ -130,19 +131,27 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
     return q;
   };
   const int per = (all + kThreads - 1) / kThreads, v0 = threadIdx.x * per;
-  u64 mine = 0, total;
-  for (int v = v0; v < min(all, v0 + per); ++v) mine += (u64)head_tiles(a.x, seq_at(v)) * a.x.K;
-  u64 at = block_sum(mine, s_warp, &total) - mine;
+  u64 mine = 0, few = 0, total, few_total;
+  for (int v = v0; v < min(all, v0 + per); ++v) {
+    const SharedSeq q = seq_at(v);
+    mine += (u64)head_tiles(a.x, q) * a.x.K;
+    few += (u64)few_length(q) * a.x.K;
+  }
+  u64 at = block_sum(mine, s_warp, &total) - mine, few_at = block_sum(few, s_warp, &few_total) - few;
   for (int v = v0; v < min(all, v0 + per); ++v) {
     SharedSeq q = seq_at(v);
     q.begin = at;
+    q.few_begin = few_at;
     at += (u64)head_tiles(a.x, q) * a.x.K;
+    few_at += (u64)few_length(q) * a.x.K;
     a.seqs[v] = q;
   }
   if (threadIdx.x == 0) {
     SharedHead h;
     h.total = total;
     share_out(total, a.grid, h.share, h.more);
+    h.few_total = few_total;
+    few_share(few_total, a.few_warps, h.few_share, h.few_more);
     *a.head = h;
   }
 }

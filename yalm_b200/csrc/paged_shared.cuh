@@ -9,10 +9,11 @@ namespace yb {
 
 constexpr int kMaxGroups = 2048;
 
-// How the axis is shared out (paged_axis.cuh).
+// How the axes are shared out (paged_axis.cuh).
 struct SharedHead {
   unsigned long long total, share;
-  int more;
+  unsigned long long few_total, few_share;
+  int more, few_more;
 };
 struct SharedPlanArgs {
   PagedBatch b;
@@ -21,11 +22,34 @@ struct SharedPlanArgs {
   int n_groups;
   Axis x;
   int grid;         // blocks of the attention
+  int few_warps;    // warps of the attention of few rows
   int part_tokens;  // tokens that the workspace has room for two parts of
   SharedHead* head;
   SharedSeq* seqs;  // [n_groups + n_seqs]
 };
 cudaError_t paged_shared_plan(const SharedPlanArgs& a, cudaStream_t s);
+
+// ---- sequences of few rows (paged_few.cu)
+constexpr int kFewThreads = 256, kFewBlocks = 2;  // of an SM
+inline int few_warps(int grid) { return grid * kFewBlocks * (kFewThreads / 32); }
+// A warp's records: 0 for a unit begun by an earlier warp, 1 for the one it leaves to later ones.  A row is o [head_dim],
+// m, l and two floats for alignment.
+inline __host__ __device__ size_t few_row_floats(int head_dim) { return (size_t)head_dim + 4; }
+struct PagedFewArgs {
+  PagedBatch b;
+  SharedBatch shared;
+  const SharedHead* head;
+  const void* q;
+  void* out;
+  const void* k_pages;
+  const void* v_pages;
+  long long q_stride, out_stride;
+  int K, gq;
+  float c;       // scale * log2(e)
+  float* recs;   // [warps][2][kFewRows] rows
+  float* parts;  // [tokens with a part][n_heads] rows
+};
+cudaError_t paged_few(const PagedFewArgs& a, int head_dim, int type, int grid, cudaStream_t s);
 
 __device__ __forceinline__ SharedSeq paged_seq(const SharedBatch& b, int v) {
   union {

@@ -1,6 +1,7 @@
 // The axis of the paged attention's work (paged_axis.cuh) for a batch in which groups of sequences share a prefix: before
 // the sequences come the groups' prefixes, as sequences of their own, whose tokens are those of the whole group, and
-// a sequence of a group begins behind the prefix.  Integer arithmetic alone; tests compile it for the host.
+// a sequence of a group begins behind the prefix.  Sequences of few rows (single tokens) lie on an axis of their own, in
+// steps of 16 slots, which warps share out (paged_few.cu).  Integer arithmetic alone; tests compile it for the host.
 #pragma once
 
 #include "paged_axis.cuh"
@@ -9,15 +10,17 @@ namespace yb {
 
 // A group's prefix or a sequence, as the kernel that plans a call (paged_shared.cu) leaves it in the workspace.
 struct __align__(16) SharedSeq {
-  int row0, n;   // tokens; of a prefix those of all its sequences
+  int row0, n;   // tokens, of a prefix those of all its sequences; n is 0 for a sequence of few rows,
+  int few;       // which has its tokens here
   int kv;        // slots, the prefix's among them
   int lo;        // first key tile: 0, or the tiles of the prefix that others look after
   int table;     // row of the page table
   int part;      // where its tokens' parts lie in the workspace; -1: there is no other part of them
   int group;     // of a sequence with a part: its prefix
   int all;       // a prefix: every token sees all of its slots
-  unsigned long long begin;  // where its units begin on the axis
-  unsigned long long pad;
+  int pad[3];
+  unsigned long long begin;      // where its units begin on the axis
+  unsigned long long few_begin;  // and on that of few rows
 };
 struct SharedBatch {
   const SharedSeq* seqs;
@@ -44,6 +47,18 @@ __device__ __forceinline__ unsigned head_tiles(const Axis& x, const SharedSeq& q
   if (q.n <= 0) return 0;
   const int nu = n_units(x, q);
   return units_before(x, q, nu - 1) + (unsigned)unit_of(x, q, nu - 1).cost + kUnitTiles;
+}
+
+// ---- few rows: a unit is (sequence, kv head), all its rows at once
+constexpr int kFewRows = 8;     // tokens x query heads of a kv head
+constexpr int kFewSlots = 16;   // slots of a step: of one page
+constexpr int kFewUnit = 4;     // what a unit's start and end cost, in steps
+constexpr int kFewLeast = 8;    // a warp's least share
+__device__ __forceinline__ int few_steps(const SharedSeq& q) { return max(1, ((q.kv + kFewSlots - 1) / kFewSlots) - q.lo * (kKT / kFewSlots)); }
+__device__ __forceinline__ unsigned few_length(const SharedSeq& q) { return q.few > 0 ? (unsigned)(few_steps(q) + kFewUnit) : 0u; }
+__device__ __forceinline__ void few_share(unsigned long long total, unsigned warps, unsigned long long& share, int& more) {
+  share_out(total, warps, share, more);
+  if (share < kFewLeast) share = kFewLeast, more = 0;
 }
 
 }  // namespace yb
