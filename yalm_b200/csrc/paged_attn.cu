@@ -140,8 +140,8 @@ __device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long lon
 // The same from a plan in the workspace, by one warp.
 __device__ void find_start(const SharedBatch& b, const SharedHead* head, const Axis& x, StartOf<SharedSeq>* s_start) {
   const int lane = threadIdx.x & 31, c = blockIdx.x;
-  const unsigned long long total = __ldca(&head->total), share = __ldca(&head->share);
-  const int more = __ldca(&head->more);
+  const unsigned long long total = __ldcg(&head->total), share = __ldcg(&head->share);
+  const int more = __ldcg(&head->more);
   const unsigned long long begin = block_begin(share, more, c);
   if (begin >= total) {
     if (lane == 0) s_start->left = 0;
@@ -151,7 +151,7 @@ __device__ void find_start(const SharedBatch& b, const SharedHead* head, const A
   int lo = 0, hi = b.n_seqs;
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
-    const bool le = at < hi && __ldca(&b.seqs[at].begin) <= begin;
+    const bool le = at < hi && __ldcg(&b.seqs[at].begin) <= begin;
     const int n = __popc(__ballot_sync(0xffffffffu, le));
     lo += n * step;
     hi = min(hi, lo + step);
@@ -336,6 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (kShared) return c.sq.table;
     else return c.seq;
   };
+  auto entry = [](const int* p) { return kShared ? __ldcg(p) : __ldca(p); };
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
                  : "memory");
@@ -352,7 +353,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       tma_prefetch_map(&vmap);
     }
   }
-  pdl_wait();  // up to here nothing of what earlier kernels write was touched
+  // up to here nothing of what earlier kernels write was touched
+  // With shared prefixes the kernel before is that of few rows, which runs beside this one on other SMs.  It has waited for
+  // all that comes before it when it lets this one start; what they wrote is read from L2.  The wait for its own end
+  // comes last, so that the join's is for both.
+  if constexpr (!kShared) pdl_wait();
   if constexpr (kShared) {
     if (warp == 0) find_start(a.shared, a.head, a.x, &s_start);
   } else {
@@ -386,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto there = [&](const PieceOf<Seq>& c, int t) {
       const int slot = ((c.u.tile0 + c.t0 + t) << 7) + lane * 16;
       int id = -1;
-      if (lane < 8 && slot < c.sq.kv) id = __ldca(b.page_table + (size_t)table_of(c) * b.max_pages + (slot >> b.ps_log2));
+      if (lane < 8 && slot < c.sq.kv) id = entry(b.page_table + (size_t)table_of(c) * b.max_pages + (slot >> b.ps_log2));
       return id >= 0 && id < b.n_pages;
     };
     bool more = walk.next(seqs, a.x, pc), nx = more && there(pc, 0);  // (a unit without a slot has one empty tile)
@@ -679,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // this lane's page of a key tile, and the row of the page pool where it starts (outside the pool: zeros)
       auto page_of = [&](int tile) {
         const int at = (tile << 7) + (lane << lg);
-        return lane < boxes && at < pc.sq.kv ? __ldca(table + (at >> lg)) : -1;
+        return lane < boxes && at < pc.sq.kv ? entry(table + (at >> lg)) : -1;
       };
       auto row_of = [&](int tile, int page) {
         if (page < 0 || page >= b.n_pages) return a.oob;
@@ -862,6 +867,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
+  if constexpr (kShared) pdl_wait();
 }
 
 // The units that were cut: out = sum_parts 2^(m - M) o / sum_parts 2^(m - M) l.  Blocks x look after the unit that
@@ -931,115 +937,114 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
 }
 
 // Shared prefixes: out = sum_parts 2^(m - M) o / sum_parts 2^(m - M) l over all parts of a row, those of its group's
-// prefix and those of its own slots, each a record in `parts` or, of a unit that was cut, several of the blocks'.  8
-// elements of a row are a thread's; neighbouring lanes have neighbouring rows, as the records hold them.
+// prefix and those of its own slots, each a record in `parts` or, of a unit that was cut, several of the blocks' or
+// warps'.  Blocks (x, y) look after sequence x; 8 elements of a row are a thread's.  A warp has 8 neighbouring rows,
+// whose elements lie side by side in the tensor-core kernel's records, and 4 neighbouring groups of 8, which do in the
+// others.
 constexpr int kJoinThreads = 128;
 template <int HD, typename T>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams a) {
   pdl_wait();
   const PagedBatch& b = a.b;
-  const long long item = (long long)blockIdx.x * kJoinThreads + threadIdx.x, rows = (long long)b.n_tokens * a.gq;
-  const int row = (int)(item % rows), token = row / a.gq, h = row % a.gq;
-  const long long rest = item / rows;
-  const int c8 = (int)(rest % (HD / 8)), head = (int)(rest / (HD / 8));
-  if (head >= a.x.K) return;
-  int lo = 0, hi = b.n_seqs;  // the last sequence that starts at or before the token
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (__ldca(b.q_start + mid) <= token) lo = mid;
-    else hi = mid;
+  const SharedSeq own = paged_seq(a.shared, a.n_groups + blockIdx.x);
+  const unsigned long long share = __ldcg(&a.head->share);
+  const int more = __ldcg(&a.head->more);
+  SharedSeq prefix{};
+  if (own.part >= 0) prefix = paged_seq(a.shared, own.group);
+  const int tokens = max(own.n, own.few), rows = tokens * b.n_heads;  // row: kv head, token, head of the group
+  const long long items = (rows + 7ll) / 8 * HD;
+  for (long long item = (long long)blockIdx.y * kJoinThreads + threadIdx.x; item < items; item += (long long)gridDim.y * kJoinThreads) {
+    const int row = (int)(item / HD) * 8 + (int)(item % 8), c8 = (int)(item / 8 % (HD / 8));
+    if (row >= rows) continue;
+    const int per_head = tokens * a.gq, head = row / per_head, token = own.row0 + row % per_head / a.gq, h = row % a.gq;
+    float mm = -INFINITY, ll = 0.f, acc[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+    auto join = [&](float m, float l, const float (&v)[8]) {
+      const float mn = fmaxf(mm, m);
+      const float old = mm == -INFINITY ? 0.f : ex2(mm - mn), w = m == -INFINITY ? 0.f : ex2(m - mn);
+      mm = mn;
+      ll = ll * old + l * w;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = acc[j] * old + v[j] * w;
+    };
+    // a unit's parts: false if its outputs are in their place already
+    auto take_few = [&](const SharedSeq& q) {
+      const unsigned long long share = __ldcg(&a.head->few_share), begin = q.few_begin + (unsigned long long)few_length(q) * head;
+      const int more = __ldcg(&a.head->few_more);
+      const int first = block_of(share, more, begin), parts = block_of(share, more, begin + few_steps(q) - 1) - first + 1;
+      if (parts == 1 && q.part < 0) return false;
+      const int r = (token - q.row0) * a.gq + h;
+      const float* whole = a.few_parts + ((size_t)(q.part + token - q.row0) * b.n_heads + head * a.gq + h) * few_row_floats(HD);
+      for (int p0 = 0; p0 < parts; p0 += kMergeParts) {
+        float2 ml[kMergeParts];
+        float4 o[kMergeParts][2];
+#pragma unroll
+        for (int k = 0; k < kMergeParts; ++k) {
+          ml[k] = make_float2(-INFINITY, 0.f);
+          o[k][0] = o[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+          const int part = p0 + k;
+          if (part < parts) {
+            const float* rec = parts == 1 ? whole
+                                          : a.few_recs + (((size_t)(first + part) * 2 + (part == 0 ? 1 : 0)) * kFewRows + r) * few_row_floats(HD);
+            o[k][0] = __ldcg(reinterpret_cast<const float4*>(rec + 8 * c8));
+            o[k][1] = __ldcg(reinterpret_cast<const float4*>(rec + 8 * c8 + 4));
+            ml[k] = __ldcg(reinterpret_cast<const float2*>(rec + HD));
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kMergeParts; ++k) {
+          const float v[8] = {o[k][0].x, o[k][0].y, o[k][0].z, o[k][0].w, o[k][1].x, o[k][1].y, o[k][1].z, o[k][1].w};
+          join(ml[k].x, ml[k].y, v);
+        }
+      }
+      return true;
+    };
+    auto take = [&](const SharedSeq& q) {
+      const int at = token - q.row0, unit = at / a.x.U;
+      const Unit u = unit_of(a.x, q, unit);
+      const unsigned long long begin = q.begin + (unsigned long long)head_tiles(a.x, q) * head + units_before(a.x, q, unit);
+      const int first = block_of(share, more, begin), parts = block_of(share, more, begin + u.cost - 1) - first + 1;
+      if (parts == 1 && q.part < 0) return false;
+      int rs = u.nq * a.gq, r = (at - u.q0) * a.gq + h;
+      const float* whole = nullptr;
+      if (parts == 1) {
+        rs = a.part_rows;
+        r = (q.part + at) * a.gq + h;
+        whole = a.parts + (size_t)((q.all ? 0 : a.x.K) + head) * (HD + 2) * rs;
+      }
+      for (int p0 = 0; p0 < parts; p0 += kMergeParts) {
+        float m[kMergeParts], l[kMergeParts];
+        float4 o[kMergeParts][2];
+#pragma unroll
+        for (int k = 0; k < kMergeParts; ++k) {
+          m[k] = -INFINITY;
+          l[k] = 0.f;
+          o[k][0] = o[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (p0 + k < parts) {
+            const float* rec = whole ? whole : a.recs + ((size_t)(first + p0 + k) * 2 + (p0 + k == 0 ? 1 : 0)) * rec_floats<HD>();
+            const float4* ro = reinterpret_cast<const float4*>(rec) + (size_t)(2 * c8) * rs + r;
+            o[k][0] = __ldcg(ro);
+            o[k][1] = __ldcg(ro + rs);
+            m[k] = __ldcg(rec + (size_t)HD * rs + r);
+            l[k] = __ldcg(rec + (size_t)(HD + 1) * rs + r);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kMergeParts; ++k) {
+          const float v[8] = {o[k][0].x, o[k][0].y, o[k][0].z, o[k][0].w, o[k][1].x, o[k][1].y, o[k][1].z, o[k][1].w};
+          join(m[k], l[k], v);
+        }
+      }
+      return true;
+    };
+    if (!(own.few ? take_few(own) : take(own))) continue;
+    if (own.part >= 0) take(prefix);
+    const float inv = ll != 0.f ? 1.f / ll : 0.f;
+    T* out = static_cast<T*>(a.out) + (size_t)token * a.out_stride + (size_t)(head * a.gq + h) * HD + 8 * c8;
+    *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv),
+                                                pack2<T>(acc[4] * inv, acc[5] * inv), pack2<T>(acc[6] * inv, acc[7] * inv));
   }
-  const SharedSeq own = paged_seq(a.shared, a.n_groups + lo);
-  if (token < own.row0 || token >= own.row0 + max(own.n, own.few)) return;
-  const unsigned long long share = __ldca(&a.head->share);
-  const int more = __ldca(&a.head->more);
-  float mm = -INFINITY, ll = 0.f, acc[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) acc[k] = 0.f;
-  auto join = [&](float m, float l, const float (&v)[8]) {
-    const float mn = fmaxf(mm, m);
-    const float old = mm == -INFINITY ? 0.f : ex2(mm - mn), w = m == -INFINITY ? 0.f : ex2(m - mn);
-    mm = mn;
-    ll = ll * old + l * w;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = acc[j] * old + v[j] * w;
-  };
-  // a unit's parts: false if its outputs are in their place already
-  auto take_few = [&](const SharedSeq& q) {
-    const unsigned long long share = __ldca(&a.head->few_share), begin = q.few_begin + (unsigned long long)few_length(q) * head;
-    const int more = __ldca(&a.head->few_more);
-    const int first = block_of(share, more, begin), parts = block_of(share, more, begin + few_steps(q) - 1) - first + 1;
-    if (parts == 1 && q.part < 0) return false;
-    const int r = (token - q.row0) * a.gq + h;
-    const float* whole = a.few_parts + ((size_t)(q.part + token - q.row0) * b.n_heads + head * a.gq + h) * few_row_floats(HD);
-    for (int p0 = 0; p0 < parts; p0 += kMergeParts) {
-      float2 ml[kMergeParts];
-      float4 o[kMergeParts][2];
-#pragma unroll
-      for (int k = 0; k < kMergeParts; ++k) {
-        ml[k] = make_float2(-INFINITY, 0.f);
-        o[k][0] = o[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        const int part = p0 + k;
-        if (part < parts) {
-          const float* rec = parts == 1 ? whole
-                                        : a.few_recs + (((size_t)(first + part) * 2 + (part == 0 ? 1 : 0)) * kFewRows + r) * few_row_floats(HD);
-          o[k][0] = __ldcg(reinterpret_cast<const float4*>(rec + 8 * c8));
-          o[k][1] = __ldcg(reinterpret_cast<const float4*>(rec + 8 * c8 + 4));
-          ml[k] = __ldcg(reinterpret_cast<const float2*>(rec + HD));
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kMergeParts; ++k) {
-        const float v[8] = {o[k][0].x, o[k][0].y, o[k][0].z, o[k][0].w, o[k][1].x, o[k][1].y, o[k][1].z, o[k][1].w};
-        join(ml[k].x, ml[k].y, v);
-      }
-    }
-    return true;
-  };
-  auto take = [&](const SharedSeq& q) {
-    const int at = token - q.row0, unit = at / a.x.U;
-    const Unit u = unit_of(a.x, q, unit);
-    const unsigned long long begin = q.begin + (unsigned long long)head_tiles(a.x, q) * head + units_before(a.x, q, unit);
-    const int first = block_of(share, more, begin), parts = block_of(share, more, begin + u.cost - 1) - first + 1;
-    if (parts == 1 && q.part < 0) return false;
-    int rs = u.nq * a.gq, r = (at - u.q0) * a.gq + h;
-    const float* whole = nullptr;
-    if (parts == 1) {
-      rs = a.part_rows;
-      r = (q.part + at) * a.gq + h;
-      whole = a.parts + (size_t)((q.all ? 0 : a.x.K) + head) * (HD + 2) * rs;
-    }
-    for (int p0 = 0; p0 < parts; p0 += kMergeParts) {
-      float m[kMergeParts], l[kMergeParts];
-      float4 o[kMergeParts][2];
-#pragma unroll
-      for (int k = 0; k < kMergeParts; ++k) {
-        m[k] = -INFINITY;
-        l[k] = 0.f;
-        o[k][0] = o[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (p0 + k < parts) {
-          const float* rec = whole ? whole : a.recs + ((size_t)(first + p0 + k) * 2 + (p0 + k == 0 ? 1 : 0)) * rec_floats<HD>();
-          const float4* ro = reinterpret_cast<const float4*>(rec) + (size_t)(2 * c8) * rs + r;
-          o[k][0] = __ldcg(ro);
-          o[k][1] = __ldcg(ro + rs);
-          m[k] = __ldcg(rec + (size_t)HD * rs + r);
-          l[k] = __ldcg(rec + (size_t)(HD + 1) * rs + r);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kMergeParts; ++k) {
-        const float v[8] = {o[k][0].x, o[k][0].y, o[k][0].z, o[k][0].w, o[k][1].x, o[k][1].y, o[k][1].z, o[k][1].w};
-        join(m[k], l[k], v);
-      }
-    }
-    return true;
-  };
-  if (!(own.few ? take_few(own) : take(own))) return;
-  if (own.part >= 0) take(paged_seq(a.shared, own.group));
-  const float inv = ll != 0.f ? 1.f / ll : 0.f;
-  T* out = static_cast<T*>(a.out) + (size_t)token * a.out_stride + (size_t)(head * a.gq + h) * HD + 8 * c8;
-  *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv),
-                                              pack2<T>(acc[4] * inv, acc[5] * inv), pack2<T>(acc[6] * inv, acc[7] * inv));
 }
 
 int paged_attention_grid(int n_sms) { return n_sms < kMaxGrid ? n_sms : kMaxGrid; }
@@ -1069,7 +1074,7 @@ static size_t few_recs_at(const PagedBatch& b, int n_groups, int head_dim, int n
 }
 size_t paged_shared_scratch(const PagedBatch& b, int n_groups, int head_dim, int n_sms) {
   return few_recs_at(b, n_groups, head_dim, n_sms) +
-         (size_t)few_warps(paged_attention_grid(n_sms)) * 2 * kFewRows * few_row_floats(head_dim) * 4;
+         (size_t)paged_attention_grid(n_sms) * kFewWarps * 2 * kFewRows * few_row_floats(head_dim) * 4;
 }
 
 namespace {
@@ -1103,7 +1108,7 @@ cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cuda
   if constexpr (kShared) {
     char* const base = static_cast<char*>(a.scratch);
     const size_t plan = shared_plan_at(HD, a.n_sms);
-    SharedPlanArgs sp{a.b, a.group_start, a.prefix_len, a.n_groups, p.x, grid, few_warps(grid), part_tokens(a.b), reinterpret_cast<SharedHead*>(base + plan),
+    SharedPlanArgs sp{a.b, a.group_start, a.prefix_len, a.n_groups, HD, p.x, grid, part_tokens(a.b), reinterpret_cast<SharedHead*>(base + plan),
                       reinterpret_cast<SharedSeq*>(base + plan + 256)};
     p.shared = SharedBatch{sp.seqs, a.n_groups + a.b.n_seqs};
     p.head = sp.head;
@@ -1113,18 +1118,21 @@ cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cuda
     p.few_parts = reinterpret_cast<float*>(base + few_parts_at(a.b, a.n_groups, HD, a.n_sms));
     p.few_recs = reinterpret_cast<float*>(base + few_recs_at(a.b, a.n_groups, HD, a.n_sms));
     if ((e = paged_shared_plan(sp, s)) != cudaSuccess) return e;
+    const PagedFewArgs f{a.b, p.shared, p.head, a.q, a.out, a.k_pages, a.v_pages, a.q_stride, a.out_stride, K, gq, p.c,
+                         const_cast<float*>(p.few_recs), const_cast<float*>(p.few_parts)};
+    if ((e = paged_few(f, HD, bf16 ? 2 : 1, grid, s)) != cudaSuccess) return e;
   }
   void* args[] = {&qm, &km, &vm, &p};
   // both kernels set up under the end of the one before (programmatic launch): 37.0 -> 33.1 us for one token over
   // 32767 slots, 47.8 -> 43.9 us for the chunk of 512
   if ((e = launch_kernel_params(fn, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, s, true, args)) != cudaSuccess) return e;
   if constexpr (kShared) {
-    const PagedFewArgs f{a.b, p.shared, p.head, a.q, a.out, a.k_pages, a.v_pages, a.q_stride, a.out_stride, K, gq, p.c,
-                         const_cast<float*>(p.few_recs), const_cast<float*>(p.few_parts)};
-    if ((e = paged_few(f, HD, bf16 ? 2 : 1, grid, s)) != cudaSuccess) return e;
-    const long long items = (long long)a.b.n_tokens * gq * K * (HD / 8);
+    // enough threads for all rows if they are spread evenly over the sequences
+    const long long items = (long long)a.b.n_tokens * a.b.n_heads * (HD / 8);
+    const long long slices = (items / a.b.n_seqs + kJoinThreads - 1) / kJoinThreads;
     return launch_kernel(reinterpret_cast<const void*>(&paged_join_kernel<HD, T>),
-                         dim3((unsigned)((items + kJoinThreads - 1) / kJoinThreads)), dim3(kJoinThreads), 0, s, true, &p);
+                         dim3(a.b.n_seqs, (unsigned)(slices < 1 ? 1 : slices < 1024 ? slices : 1024)), dim3(kJoinThreads), 0, s,
+                         true, &p);
   }
   if (a.b.max_pages * ps <= kKT) return cudaSuccess;  // every unit is one key tile: nothing is cut
   return launch_kernel(reinterpret_cast<const void*>(&paged_merge_kernel<HD, T>), dim3(grid, kMergeSlices),

@@ -10,8 +10,9 @@
 //                   and Q have the same one
 //   O^T += V^T . P^T  dims x rows; P^T is S^T's transpose in registers (movmatrix), V's operand pairs two slots of a
 //                   dimension, by byte permutes of two rows' chunks
-// Units (sequence, kv head) in order make an axis of steps that all warps share out evenly; a unit that is cut leaves
-// records, which the join puts together (paged_attn.cu).  Weights are rounded to the caches' type as there, fp16 with a
+// Units (sequence, kv head) in order make an axis of steps that warps share out evenly; a unit that is cut leaves
+// records, which the join puts together (paged_attn.cu).  It takes as many SMs as the plan gives it, and the tensor-core
+// kernel, which is started under it, has the others.  Weights are rounded to the caches' type as there, fp16 with a
 // factor 2^7; the rest is fp32.
 #include <cuda_bf16.h>
 
@@ -54,13 +55,14 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi, __nv_bfloat16) {
 __device__ __forceinline__ uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
 
 template <int HD, typename T>
-__global__ void __launch_bounds__(kFewThreads, kFewBlocks) paged_few_kernel(const __grid_constant__ PagedFewArgs a) {
+__global__ void __launch_bounds__(kFewThreads, 1) paged_few_kernel(const __grid_constant__ PagedFewArgs a) {
   constexpr int kC = HD / 32, kJ = HD / 64;  // chunks of 32 dims of K, of 64 of V
   constexpr float kBias = std::is_same<T, __half>::value ? 7.f : 0.f;
   const PagedBatch& b = a.b;
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
-  const int warp = blockIdx.x * (kFewThreads / 32) + (threadIdx.x >> 5);
+  const int warp = blockIdx.x * kFewWarps + (threadIdx.x >> 5);
   pdl_wait();
+  pdl_trigger();  // the attention kernel beside this one needs no more than the plan, which is there
   const u64 total = __ldca(&a.head->few_total), share = __ldca(&a.head->few_share);
   const int more = __ldca(&a.head->few_more);
   const u64 begin = block_begin(share, more, warp);
@@ -251,7 +253,7 @@ cudaError_t paged_few(const PagedFewArgs& a, int head_dim, int type, int grid, c
                                                 : reinterpret_cast<const void*>(&paged_few_kernel<128, __nv_bfloat16>))
                                    : (type == 1 ? reinterpret_cast<const void*>(&paged_few_kernel<64, __half>)
                                                 : reinterpret_cast<const void*>(&paged_few_kernel<64, __nv_bfloat16>));
-  return launch_kernel(fn, dim3(grid * kFewBlocks), dim3(kFewThreads), 0, s, true, &p);
+  return launch_kernel(fn, dim3(grid), dim3(kFewThreads), 0, s, true, &p);
 }
 
 }  // namespace yb

@@ -7,6 +7,8 @@
 // with U tokens a unit, sum_s ceil(n_s / U) >= 2 ceil(sum_s n_s / U).  Long chunks fill their units by themselves.
 //
 // One block: a few loads a sequence, prefix sums, and 48 bytes written for each.
+#include <math.h>
+
 #include "launch.h"
 #include "paged_shared.cuh"
 
@@ -146,13 +148,31 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
     few_at += (u64)few_length(q) * a.x.K;
     a.seqs[v] = q;
   }
-  if (threadIdx.x == 0) {
-    SharedHead h;
-    h.total = total;
-    share_out(total, a.grid, h.share, h.more);
-    h.few_total = few_total;
-    few_share(few_total, a.few_warps, h.few_share, h.few_more);
-    *a.head = h;
+  if (threadIdx.x < 32) {
+    // SMs for the one kernel and the other: the least of the longer time.  A key tile of two row tiles takes an SM 1.7 us, a
+    // step of few rows 0.11 us (of 8 KB, as fast as one SM reads), but all SMs together no less than 0.0013 us.
+    const float tiles = (float)total * 1.7f, steps = (float)few_total * (a.head_dim == 128 ? 1.f : 0.6f);
+    float best = INFINITY;
+    int blocks = 0;
+    for (int n = threadIdx.x; n <= a.grid; n += 32) {
+      const float t = fmaxf(n ? tiles / n : total ? INFINITY : 0.f,
+                            fmaxf(n < a.grid ? steps * 0.11f / (a.grid - n) : few_total ? INFINITY : 0.f, steps * 0.0013f));
+      if (t < best) best = t, blocks = n;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const float t = __shfl_xor_sync(0xffffffffu, best, o);
+      const int n = __shfl_xor_sync(0xffffffffu, blocks, o);
+      if (t < best || (t == best && n < blocks)) best = t, blocks = n;
+    }
+    if (threadIdx.x == 0) {
+      SharedHead h;
+      h.total = total;
+      share_out(total, max(blocks, 1), h.share, h.more);
+      h.few_total = few_total;
+      few_share(few_total, max(a.grid - blocks, 1) * kFewWarps, h.few_share, h.few_more);
+      *a.head = h;
+    }
   }
 }
 

@@ -9,7 +9,8 @@ namespace yb {
 
 constexpr int kMaxGroups = 2048;
 
-// How the axes are shared out (paged_axis.cuh).
+// How the axes are shared out (paged_axis.cuh): the first one among the first `blocks` blocks of its kernel, that of few
+// rows among the warps of the first grid - blocks blocks of its own, so that both run at the same time.
 struct SharedHead {
   unsigned long long total, share;
   unsigned long long few_total, few_share;
@@ -19,10 +20,9 @@ struct SharedPlanArgs {
   PagedBatch b;
   const int* group_start;  // [n_groups + 1] sequences
   const int* prefix_len;   // [n_groups] slots
-  int n_groups;
+  int n_groups, head_dim;
   Axis x;
-  int grid;         // blocks of the attention
-  int few_warps;    // warps of the attention of few rows
+  int grid;         // SMs, and blocks of either kernel
   int part_tokens;  // tokens that the workspace has room for two parts of
   SharedHead* head;
   SharedSeq* seqs;  // [n_groups + n_seqs]
@@ -30,8 +30,7 @@ struct SharedPlanArgs {
 cudaError_t paged_shared_plan(const SharedPlanArgs& a, cudaStream_t s);
 
 // ---- sequences of few rows (paged_few.cu)
-constexpr int kFewThreads = 256, kFewBlocks = 2;  // of an SM
-inline int few_warps(int grid) { return grid * kFewBlocks * (kFewThreads / 32); }
+constexpr int kFewThreads = 512, kFewWarps = kFewThreads / 32;  // one block an SM
 // A warp's records: 0 for a unit begun by an earlier warp, 1 for the one it leaves to later ones.  A row is o [head_dim],
 // m, l and two floats for alignment.
 inline __host__ __device__ size_t few_row_floats(int head_dim) { return (size_t)head_dim + 4; }
@@ -51,13 +50,14 @@ struct PagedFewArgs {
 };
 cudaError_t paged_few(const PagedFewArgs& a, int head_dim, int type, int grid, cudaStream_t s);
 
+// (from L2: the attention kernel starts while the one before it, which waits for the plan, still runs)
 __device__ __forceinline__ SharedSeq paged_seq(const SharedBatch& b, int v) {
   union {
     int4 w[sizeof(SharedSeq) / 16];
     SharedSeq q;
   } u;
 #pragma unroll
-  for (int i = 0; i < (int)sizeof(SharedSeq) / 16; ++i) u.w[i] = __ldca(reinterpret_cast<const int4*>(b.seqs + v) + i);
+  for (int i = 0; i < (int)sizeof(SharedSeq) / 16; ++i) u.w[i] = __ldcg(reinterpret_cast<const int4*>(b.seqs + v) + i);
   return u.q;
 }
 
