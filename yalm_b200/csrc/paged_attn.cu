@@ -938,112 +938,99 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
 
 // Shared prefixes: out = sum_parts 2^(m - M) o / sum_parts 2^(m - M) l over all parts of a row, those of its group's
 // prefix and those of its own slots, each a record in `parts` or, of a unit that was cut, several of the blocks' or
-// warps'.  Blocks (x, y) look after sequence x; 8 elements of a row are a thread's.  A warp has 8 neighbouring rows,
-// whose elements lie side by side in the tensor-core kernel's records, and 4 neighbouring groups of 8, which do in the
-// others.
-constexpr int kJoinThreads = 128;
+// warps'.  Blocks (x, y) look after sequence x.  A warp has 8 neighbouring rows, whose elements lie side by side in the
+// tensor-core kernel's records, by 4 lanes each, which take every fourth float4 of a row: side by side in the others.
+constexpr int kJoinThreads = 128, kJoinParts = 2;
 template <int HD, typename T>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams a) {
+  constexpr int kN = HD / 16;  // float4 of a thread
   pdl_wait();
   const PagedBatch& b = a.b;
   const SharedSeq own = paged_seq(a.shared, a.n_groups + blockIdx.x);
-  const unsigned long long share = __ldcg(&a.head->share);
-  const int more = __ldcg(&a.head->more);
+  const unsigned long long share = __ldcg(&a.head->share), few_share = __ldcg(&a.head->few_share);
+  const int more = __ldcg(&a.head->more), few_more = __ldcg(&a.head->few_more);
   SharedSeq prefix{};
   if (own.part >= 0) prefix = paged_seq(a.shared, own.group);
+  const int lane = threadIdx.x & 31, c = lane >> 3;
   const int tokens = max(own.n, own.few), rows = tokens * b.n_heads;  // row: kv head, token, head of the group
-  const long long items = (rows + 7ll) / 8 * HD;
-  for (long long item = (long long)blockIdx.y * kJoinThreads + threadIdx.x; item < items; item += (long long)gridDim.y * kJoinThreads) {
-    const int row = (int)(item / HD) * 8 + (int)(item % 8), c8 = (int)(item / 8 % (HD / 8));
+  const unsigned few_head = few_length(own), own_head = head_tiles(a.x, own), prefix_head = head_tiles(a.x, prefix);
+  for (int r8 = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); r8 < (rows + 7) / 8; r8 += gridDim.y * (kJoinThreads / 32)) {
+    const int row = r8 * 8 + (lane & 7);
     if (row >= rows) continue;
-    const int per_head = tokens * a.gq, head = row / per_head, token = own.row0 + row % per_head / a.gq, h = row % a.gq;
-    float mm = -INFINITY, ll = 0.f, acc[8];
+    const int per_head = tokens * a.gq, head = row / per_head, token = row % per_head / a.gq, h = row % a.gq;
+    float mm = -INFINITY, ll = 0.f;
+    float4 acc[kN];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) acc[k] = 0.f;
-    auto join = [&](float m, float l, const float (&v)[8]) {
-      const float mn = fmaxf(mm, m);
-      const float old = mm == -INFINITY ? 0.f : ex2(mm - mn), w = m == -INFINITY ? 0.f : ex2(m - mn);
-      mm = mn;
-      ll = ll * old + l * w;
+    for (int k = 0; k < kN; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    // parts first .. first + n - 1: at(part) is the record's first float4 of this thread, `step` float4 from one to the
+    // next, ml(part) its m and l
+    auto take = [&](int n, auto&& at, size_t step, auto&& ml) {
+      for (int p0 = 0; p0 < n; p0 += kJoinParts) {
+        float2 f[kJoinParts];
+        float4 o[kJoinParts][kN];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = acc[j] * old + v[j] * w;
-    };
-    // a unit's parts: false if its outputs are in their place already
-    auto take_few = [&](const SharedSeq& q) {
-      const unsigned long long share = __ldcg(&a.head->few_share), begin = q.few_begin + (unsigned long long)few_length(q) * head;
-      const int more = __ldcg(&a.head->few_more);
-      const int first = block_of(share, more, begin), parts = block_of(share, more, begin + few_steps(q) - 1) - first + 1;
-      if (parts == 1 && q.part < 0) return false;
-      const int r = (token - q.row0) * a.gq + h;
-      const float* whole = a.few_parts + ((size_t)(q.part + token - q.row0) * b.n_heads + head * a.gq + h) * few_row_floats(HD);
-      for (int p0 = 0; p0 < parts; p0 += kMergeParts) {
-        float2 ml[kMergeParts];
-        float4 o[kMergeParts][2];
+        for (int e = 0; e < kJoinParts; ++e) {
+          if (p0 + e >= n) break;
+          const float4* from = at(p0 + e);
 #pragma unroll
-        for (int k = 0; k < kMergeParts; ++k) {
-          ml[k] = make_float2(-INFINITY, 0.f);
-          o[k][0] = o[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-          const int part = p0 + k;
-          if (part < parts) {
-            const float* rec = parts == 1 ? whole
-                                          : a.few_recs + (((size_t)(first + part) * 2 + (part == 0 ? 1 : 0)) * kFewRows + r) * few_row_floats(HD);
-            o[k][0] = __ldcg(reinterpret_cast<const float4*>(rec + 8 * c8));
-            o[k][1] = __ldcg(reinterpret_cast<const float4*>(rec + 8 * c8 + 4));
-            ml[k] = __ldcg(reinterpret_cast<const float2*>(rec + HD));
+          for (int k = 0; k < kN; ++k) o[e][k] = __ldcg(from + k * step);
+          f[e] = ml(p0 + e);
+        }
+#pragma unroll
+        for (int e = 0; e < kJoinParts; ++e) {
+          if (p0 + e >= n) break;
+          const float mn = fmaxf(mm, f[e].x);
+          const float old = mm == -INFINITY ? 0.f : ex2(mm - mn), w = f[e].x == -INFINITY ? 0.f : ex2(f[e].x - mn);
+          mm = mn;
+          ll = ll * old + f[e].y * w;
+#pragma unroll
+          for (int k = 0; k < kN; ++k) {
+            acc[k].x = acc[k].x * old + o[e][k].x * w;
+            acc[k].y = acc[k].y * old + o[e][k].y * w;
+            acc[k].z = acc[k].z * old + o[e][k].z * w;
+            acc[k].w = acc[k].w * old + o[e][k].w * w;
           }
         }
-#pragma unroll
-        for (int k = 0; k < kMergeParts; ++k) {
-          const float v[8] = {o[k][0].x, o[k][0].y, o[k][0].z, o[k][0].w, o[k][1].x, o[k][1].y, o[k][1].z, o[k][1].w};
-          join(ml[k].x, ml[k].y, v);
-        }
       }
-      return true;
     };
-    auto take = [&](const SharedSeq& q) {
-      const int at = token - q.row0, unit = at / a.x.U;
+    // of the tensor-core kernel: false if the outputs are in their place already
+    auto take_unit = [&](const SharedSeq& q, unsigned per_head) {
+      const int at = own.row0 + token - q.row0, unit = at / a.x.U;
       const Unit u = unit_of(a.x, q, unit);
-      const unsigned long long begin = q.begin + (unsigned long long)head_tiles(a.x, q) * head + units_before(a.x, q, unit);
+      const unsigned long long begin = q.begin + (unsigned long long)per_head * head + units_before(a.x, q, unit);
       const int first = block_of(share, more, begin), parts = block_of(share, more, begin + u.cost - 1) - first + 1;
       if (parts == 1 && q.part < 0) return false;
-      int rs = u.nq * a.gq, r = (at - u.q0) * a.gq + h;
-      const float* whole = nullptr;
-      if (parts == 1) {
-        rs = a.part_rows;
-        r = (q.part + at) * a.gq + h;
-        whole = a.parts + (size_t)((q.all ? 0 : a.x.K) + head) * (HD + 2) * rs;
-      }
-      for (int p0 = 0; p0 < parts; p0 += kMergeParts) {
-        float m[kMergeParts], l[kMergeParts];
-        float4 o[kMergeParts][2];
-#pragma unroll
-        for (int k = 0; k < kMergeParts; ++k) {
-          m[k] = -INFINITY;
-          l[k] = 0.f;
-          o[k][0] = o[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (p0 + k < parts) {
-            const float* rec = whole ? whole : a.recs + ((size_t)(first + p0 + k) * 2 + (p0 + k == 0 ? 1 : 0)) * rec_floats<HD>();
-            const float4* ro = reinterpret_cast<const float4*>(rec) + (size_t)(2 * c8) * rs + r;
-            o[k][0] = __ldcg(ro);
-            o[k][1] = __ldcg(ro + rs);
-            m[k] = __ldcg(rec + (size_t)HD * rs + r);
-            l[k] = __ldcg(rec + (size_t)(HD + 1) * rs + r);
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < kMergeParts; ++k) {
-          const float v[8] = {o[k][0].x, o[k][0].y, o[k][0].z, o[k][0].w, o[k][1].x, o[k][1].y, o[k][1].z, o[k][1].w};
-          join(m[k], l[k], v);
-        }
-      }
+      const bool whole = parts == 1;
+      const int rs = whole ? a.part_rows : u.nq * a.gq, r = whole ? (q.part + at) * a.gq + h : (at - u.q0) * a.gq + h;
+      auto rec = [&](int p) -> const float* {
+        return whole ? a.parts + (size_t)((q.all ? 0 : a.x.K) + head) * (HD + 2) * rs
+                     : a.recs + ((size_t)(first + p) * 2 + (p == 0 ? 1 : 0)) * rec_floats<HD>();
+      };
+      take(parts, [&](int p) { return reinterpret_cast<const float4*>(rec(p)) + (size_t)c * rs + r; }, (size_t)4 * rs,
+           [&](int p) { return make_float2(__ldcg(rec(p) + (size_t)HD * rs + r), __ldcg(rec(p) + (size_t)(HD + 1) * rs + r)); });
       return true;
     };
-    if (!(own.few ? take_few(own) : take(own))) continue;
-    if (own.part >= 0) take(prefix);
+    // of the kernel of few rows
+    auto take_few = [&] {
+      const unsigned long long begin = own.few_begin + (unsigned long long)few_head * head;
+      const int first = block_of(few_share, few_more, begin);
+      const int parts = block_of(few_share, few_more, begin + few_steps(own) - 1) - first + 1;
+      if (parts == 1 && own.part < 0) return false;
+      auto rec = [&](int p) -> const float* {
+        return parts == 1 ? a.few_parts + ((size_t)(own.part + token) * b.n_heads + head * a.gq + h) * few_row_floats(HD)
+                          : a.few_recs + (((size_t)(first + p) * 2 + (p == 0 ? 1 : 0)) * kFewRows + token * a.gq + h) * few_row_floats(HD);
+      };
+      take(parts, [&](int p) { return reinterpret_cast<const float4*>(rec(p)) + c; }, 4,
+           [&](int p) { return __ldcg(reinterpret_cast<const float2*>(rec(p) + HD)); });
+      return true;
+    };
+    if (!(own.few ? take_few() : take_unit(own, own_head))) continue;
+    if (own.part >= 0) take_unit(prefix, prefix_head);
     const float inv = ll != 0.f ? 1.f / ll : 0.f;
-    T* out = static_cast<T*>(a.out) + (size_t)token * a.out_stride + (size_t)(head * a.gq + h) * HD + 8 * c8;
-    *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv),
-                                                pack2<T>(acc[4] * inv, acc[5] * inv), pack2<T>(acc[6] * inv, acc[7] * inv));
+    T* out = static_cast<T*>(a.out) + (size_t)(own.row0 + token) * a.out_stride + (size_t)(head * a.gq + h) * HD + 4 * c;
+#pragma unroll
+    for (int k = 0; k < kN; ++k)
+      *reinterpret_cast<uint2*>(out + 16 * k) = make_uint2(pack2<T>(acc[k].x * inv, acc[k].y * inv), pack2<T>(acc[k].z * inv, acc[k].w * inv));
   }
 }
 
@@ -1127,9 +1114,9 @@ cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cuda
   // 32767 slots, 47.8 -> 43.9 us for the chunk of 512
   if ((e = launch_kernel_params(fn, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, s, true, args)) != cudaSuccess) return e;
   if constexpr (kShared) {
-    // enough threads for all rows if they are spread evenly over the sequences
-    const long long items = (long long)a.b.n_tokens * a.b.n_heads * (HD / 8);
-    const long long slices = (items / a.b.n_seqs + kJoinThreads - 1) / kJoinThreads;
+    // enough warps for all rows if they are spread evenly over the sequences
+    const long long warps = ((long long)a.b.n_tokens * a.b.n_heads / a.b.n_seqs + 7) / 8;
+    const long long slices = (warps + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
     return launch_kernel(reinterpret_cast<const void*>(&paged_join_kernel<HD, T>),
                          dim3(a.b.n_seqs, (unsigned)(slices < 1 ? 1 : slices < 1024 ? slices : 1024)), dim3(kJoinThreads), 0, s,
                          true, &p);
