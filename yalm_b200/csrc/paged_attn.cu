@@ -936,14 +936,19 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
   }
 }
 
-// Shared prefixes: out = sum_parts 2^(m - M) o / sum_parts 2^(m - M) l over all parts of a row, those of its group's
-// prefix and those of its own slots, each a record in `parts` or, of a unit that was cut, several of the blocks' or
-// warps'.  Blocks (x, y) look after sequence x.  A warp has 8 neighbouring rows, whose elements lie side by side in the
-// tensor-core kernel's records, by 4 lanes each, which take every fourth float4 of a row: side by side in the others.
-constexpr int kJoinThreads = 128, kJoinParts = 2;
-template <int HD, typename T>
+// Shared prefixes: out = sum_parts 2^(m - M) o / sum_parts 2^(m - M) l over all parts of a row, those of its own slots and
+// those of its group's prefix, each a record in `parts` or, of a unit that was cut, several of the blocks' or warps'.
+// Blocks (x, y) look after sequence x.  Of a batch of many rows a warp has 8 neighbouring ones, by 4 lanes each, which
+// take every fourth float4.  Of a batch of few, whose units are cut over many blocks, it has one (kOne): 8 lanes share out
+// the parts, so that all are on their way at once, and their sum is scattered over them, a stage for each bit sending
+// the half that the other lane keeps.  16384 rows in 3 to 4 parts: 12 us with 8 rows a warp, 31 with one; 3904 in
+// up to 18 parts: 19 and 13.
+constexpr int kJoinThreads = 128, kJoinRows = 8192;
+template <int HD, typename T, bool kOne>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams a) {
-  constexpr int kN = HD / 16;  // float4 of a thread
+  constexpr int kN = HD / 16;         // float4 of a lane
+  constexpr int kA = kOne ? 1 : 2;    // parts that it loads at once
+  constexpr int kSubs = kOne ? 8 : 1;
   pdl_wait();
   const PagedBatch& b = a.b;
   const SharedSeq own = paged_seq(a.shared, a.n_groups + blockIdx.x);
@@ -951,86 +956,132 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   const int more = __ldcg(&a.head->more), few_more = __ldcg(&a.head->few_more);
   SharedSeq prefix{};
   if (own.part >= 0) prefix = paged_seq(a.shared, own.group);
-  const int lane = threadIdx.x & 31, c = lane >> 3;
+  const int lane = threadIdx.x & 31;
   const int tokens = max(own.n, own.few), rows = tokens * b.n_heads;  // row: kv head, token, head of the group
   const unsigned few_head = few_length(own), own_head = head_tiles(a.x, own), prefix_head = head_tiles(a.x, prefix);
-  for (int r8 = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); r8 < (rows + 7) / 8; r8 += gridDim.y * (kJoinThreads / 32)) {
-    const int row = r8 * 8 + (lane & 7);
+  // Where a unit's parts lie: n records, the first one apart; a row's float4 k is at k * step float4.
+  struct Parts {
+    int n;
+    const float *first, *rest;  // rest: the second one's
+    size_t next;                // floats from that to the one after it
+    int step, ml;               // where m is, and l is step floats from there
+  };
+  // of the tensor-core kernel
+  auto of_unit = [&](const SharedSeq& q, unsigned per_head, int head, int token, int h) {
+    const int at = own.row0 + token - q.row0, unit = at / a.x.U;
+    const Unit u = unit_of(a.x, q, unit);
+    const unsigned long long begin = q.begin + (unsigned long long)per_head * head + units_before(a.x, q, unit);
+    const int block = block_of(share, more, begin);
+    Parts p;
+    p.n = block_of(share, more, begin + u.cost - 1) - block + 1;
+    const bool whole = p.n == 1;
+    const int rs = whole ? a.part_rows : u.nq * a.gq, r = whole ? (q.part + at) * a.gq + h : (at - u.q0) * a.gq + h;
+    p.first = (whole ? a.parts + (size_t)((q.all ? 0 : a.x.K) + head) * (HD + 2) * rs
+                     : a.recs + ((size_t)block * 2 + 1) * rec_floats<HD>()) + 4 * (size_t)r;
+    p.rest = a.recs + (size_t)(block + 1) * 2 * rec_floats<HD>() + 4 * (size_t)r;
+    p.next = 2 * rec_floats<HD>();
+    p.step = rs;
+    p.ml = HD * rs - 3 * r;  // from 4 r on
+    return p;
+  };
+  // of the kernel of few rows
+  auto of_few = [&](int head, int token, int h) {
+    const unsigned long long begin = own.few_begin + (unsigned long long)few_head * head;
+    const int warp = block_of(few_share, few_more, begin);
+    Parts p;
+    p.n = block_of(few_share, few_more, begin + few_steps(own) - 1) - warp + 1;
+    const size_t row = (size_t)(token * a.gq + h) * few_row_floats(HD), rec = kFewRows * few_row_floats(HD);
+    p.first = p.n == 1 ? a.few_parts + ((size_t)(own.part + token) * b.n_heads + head * a.gq + h) * few_row_floats(HD)
+                       : a.few_recs + ((size_t)warp * 2 + 1) * rec + row;
+    p.rest = a.few_recs + (size_t)(warp + 1) * 2 * rec + row;
+    p.next = 2 * rec;
+    p.step = 1;
+    p.ml = HD;
+    return p;
+  };
+  const int warp = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5), warps = gridDim.y * (kJoinThreads / 32);
+  const int c = kOne ? lane & 3 : lane >> 3, sub = kOne ? lane >> 2 : 0;
+  for (int r = warp; r < (kOne ? rows : (rows + 7) / 8); r += warps) {
+    const int row = kOne ? r : r * 8 + (lane & 7);
     if (row >= rows) continue;
     const int per_head = tokens * a.gq, head = row / per_head, token = row % per_head / a.gq, h = row % a.gq;
-    float mm = -INFINITY, ll = 0.f;
-    float4 acc[kN];
+    const Parts one = own.few ? of_few(head, token, h) : of_unit(own, own_head, head, token, h);
+    if (one.n == 1 && own.part < 0) continue;  // the outputs are in their place
+    Parts two = one;
+    two.n = 0;
+    if (own.part >= 0) two = of_unit(prefix, prefix_head, head, token, h);
+    float mm = -INFINITY, ll = 0.f, acc[4 * kN];
 #pragma unroll
-    for (int k = 0; k < kN; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    // parts first .. first + n - 1: at(part) is the record's first float4 of this thread, `step` float4 from one to the
-    // next, ml(part) its m and l
-    auto take = [&](int n, auto&& at, size_t step, auto&& ml) {
-      for (int p0 = 0; p0 < n; p0 += kJoinParts) {
-        float2 f[kJoinParts];
-        float4 o[kJoinParts][kN];
+    for (int k = 0; k < 4 * kN; ++k) acc[k] = 0.f;
+    const int n = one.n + two.n;
+    for (int i0 = sub; i0 < n; i0 += kA * kSubs) {
+      float4 o[kA][kN];
+      float m[kA], l[kA];
 #pragma unroll
-        for (int e = 0; e < kJoinParts; ++e) {
-          if (p0 + e >= n) break;
-          const float4* from = at(p0 + e);
+      for (int e = 0; e < kA; ++e) {
+        const int i = i0 + e * kSubs;
+        if (i >= n) break;
+        const bool second = i >= one.n;
+        const int part = second ? i - one.n : i, step = second ? two.step : one.step, ml = second ? two.ml : one.ml;
+        const float* rec = part ? (second ? two.rest : one.rest) + (part - 1) * (second ? two.next : one.next)
+                                : second ? two.first : one.first;
 #pragma unroll
-          for (int k = 0; k < kN; ++k) o[e][k] = __ldcg(from + k * step);
-          f[e] = ml(p0 + e);
-        }
+        for (int k = 0; k < kN; ++k) o[e][k] = __ldcg(reinterpret_cast<const float4*>(rec) + (size_t)(4 * k + c) * step);
+        m[e] = __ldcg(rec + ml);
+        l[e] = __ldcg(rec + ml + step);
+      }
 #pragma unroll
-        for (int e = 0; e < kJoinParts; ++e) {
-          if (p0 + e >= n) break;
-          const float mn = fmaxf(mm, f[e].x);
-          const float old = mm == -INFINITY ? 0.f : ex2(mm - mn), w = f[e].x == -INFINITY ? 0.f : ex2(f[e].x - mn);
-          mm = mn;
-          ll = ll * old + f[e].y * w;
+      for (int e = 0; e < kA; ++e) {
+        if (i0 + e * kSubs >= n) break;
+        const float mn = fmaxf(mm, m[e]);
+        const float old = mm == -INFINITY ? 0.f : ex2(mm - mn), w = m[e] == -INFINITY ? 0.f : ex2(m[e] - mn);
+        mm = mn;
+        ll = ll * old + l[e] * w;
 #pragma unroll
-          for (int k = 0; k < kN; ++k) {
-            acc[k].x = acc[k].x * old + o[e][k].x * w;
-            acc[k].y = acc[k].y * old + o[e][k].y * w;
-            acc[k].z = acc[k].z * old + o[e][k].z * w;
-            acc[k].w = acc[k].w * old + o[e][k].w * w;
-          }
+        for (int k = 0; k < kN; ++k) {
+          acc[4 * k] = acc[4 * k] * old + o[e][k].x * w;
+          acc[4 * k + 1] = acc[4 * k + 1] * old + o[e][k].y * w;
+          acc[4 * k + 2] = acc[4 * k + 2] * old + o[e][k].z * w;
+          acc[4 * k + 3] = acc[4 * k + 3] * old + o[e][k].w * w;
         }
       }
-    };
-    // of the tensor-core kernel: false if the outputs are in their place already
-    auto take_unit = [&](const SharedSeq& q, unsigned per_head) {
-      const int at = own.row0 + token - q.row0, unit = at / a.x.U;
-      const Unit u = unit_of(a.x, q, unit);
-      const unsigned long long begin = q.begin + (unsigned long long)per_head * head + units_before(a.x, q, unit);
-      const int first = block_of(share, more, begin), parts = block_of(share, more, begin + u.cost - 1) - first + 1;
-      if (parts == 1 && q.part < 0) return false;
-      const bool whole = parts == 1;
-      const int rs = whole ? a.part_rows : u.nq * a.gq, r = whole ? (q.part + at) * a.gq + h : (at - u.q0) * a.gq + h;
-      auto rec = [&](int p) -> const float* {
-        return whole ? a.parts + (size_t)((q.all ? 0 : a.x.K) + head) * (HD + 2) * rs
-                     : a.recs + ((size_t)(first + p) * 2 + (p == 0 ? 1 : 0)) * rec_floats<HD>();
-      };
-      take(parts, [&](int p) { return reinterpret_cast<const float4*>(rec(p)) + (size_t)c * rs + r; }, (size_t)4 * rs,
-           [&](int p) { return make_float2(__ldcg(rec(p) + (size_t)HD * rs + r), __ldcg(rec(p) + (size_t)(HD + 1) * rs + r)); });
-      return true;
-    };
-    // of the kernel of few rows
-    auto take_few = [&] {
-      const unsigned long long begin = own.few_begin + (unsigned long long)few_head * head;
-      const int first = block_of(few_share, few_more, begin);
-      const int parts = block_of(few_share, few_more, begin + few_steps(own) - 1) - first + 1;
-      if (parts == 1 && own.part < 0) return false;
-      auto rec = [&](int p) -> const float* {
-        return parts == 1 ? a.few_parts + ((size_t)(own.part + token) * b.n_heads + head * a.gq + h) * few_row_floats(HD)
-                          : a.few_recs + (((size_t)(first + p) * 2 + (p == 0 ? 1 : 0)) * kFewRows + token * a.gq + h) * few_row_floats(HD);
-      };
-      take(parts, [&](int p) { return reinterpret_cast<const float4*>(rec(p)) + c; }, 4,
-           [&](int p) { return __ldcg(reinterpret_cast<const float2*>(rec(p) + HD)); });
-      return true;
-    };
-    if (!(own.few ? take_few() : take_unit(own, own_head))) continue;
-    if (own.part >= 0) take_unit(prefix, prefix_head);
-    const float inv = ll != 0.f ? 1.f / ll : 0.f;
-    T* out = static_cast<T*>(a.out) + (size_t)(own.row0 + token) * a.out_stride + (size_t)(head * a.gq + h) * HD + 4 * c;
+    }
+    T* out = static_cast<T*>(a.out) + (size_t)(own.row0 + token) * a.out_stride + (size_t)(head * a.gq + h) * HD;
+    if constexpr (!kOne) {
+      const float inv = ll != 0.f ? 1.f / ll : 0.f;
 #pragma unroll
-    for (int k = 0; k < kN; ++k)
-      *reinterpret_cast<uint2*>(out + 16 * k) = make_uint2(pack2<T>(acc[k].x * inv, acc[k].y * inv), pack2<T>(acc[k].z * inv, acc[k].w * inv));
+      for (int k = 0; k < kN; ++k)
+        *reinterpret_cast<uint2*>(out + 16 * k + 4 * c) =
+            make_uint2(pack2<T>(acc[4 * k] * inv, acc[4 * k + 1] * inv), pack2<T>(acc[4 * k + 2] * inv, acc[4 * k + 3] * inv));
+      continue;
+    }
+    float top = mm;
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float w = mm == -INFINITY ? 0.f : ex2(mm - top);
+    ll *= w;
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) ll += __shfl_xor_sync(0xffffffffu, ll, d);
+    const float scale = ll != 0.f ? w / ll : 0.f;
+#pragma unroll
+    for (int k = 0; k < 4 * kN; ++k) acc[k] *= scale;
+    auto stage = [&](auto left, int d) {  // bit d of sub keeps the upper half of what is left
+      constexpr int n = decltype(left)::value;
+      const bool up = (sub >> d) & 1;
+#pragma unroll
+      for (int k = 0; k < n; ++k) {
+        const float send = up ? acc[k] : acc[k + n], keep = up ? acc[k + n] : acc[k];
+        acc[k] = keep + __shfl_xor_sync(0xffffffffu, send, 4 << d);
+      }
+    };
+    stage(std::integral_constant<int, 2 * kN>(), 2);
+    stage(std::integral_constant<int, kN>(), 1);
+    stage(std::integral_constant<int, kN / 2>(), 0);
+    constexpr int kLeft = kN / 2;  // elements sub * kLeft .. of the lane's
+    const int e0 = sub * kLeft;
+    out += 4 * (4 * (e0 / 4) + c) + e0 % 4;
+#pragma unroll
+    for (int k = 0; k < kLeft; k += 2) *reinterpret_cast<uint32_t*>(out + k) = pack2<T>(acc[k], acc[k + 1]);
   }
 }
 
@@ -1115,9 +1166,11 @@ cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cuda
   if ((e = launch_kernel_params(fn, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, s, true, args)) != cudaSuccess) return e;
   if constexpr (kShared) {
     // enough warps for all rows if they are spread evenly over the sequences
-    const long long warps = ((long long)a.b.n_tokens * a.b.n_heads / a.b.n_seqs + 7) / 8;
-    const long long slices = (warps + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
-    return launch_kernel(reinterpret_cast<const void*>(&paged_join_kernel<HD, T>),
+    const long long rows = (long long)a.b.n_tokens * a.b.n_heads;
+    const bool one = rows <= kJoinRows;
+    const long long slices = (rows / a.b.n_seqs / (one ? 1 : 8) + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
+    return launch_kernel(one ? reinterpret_cast<const void*>(&paged_join_kernel<HD, T, true>)
+                             : reinterpret_cast<const void*>(&paged_join_kernel<HD, T, false>),
                          dim3(a.b.n_seqs, (unsigned)(slices < 1 ? 1 : slices < 1024 ? slices : 1024)), dim3(kJoinThreads), 0, s,
                          true, &p);
   }
