@@ -938,17 +938,15 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
 
 // Shared prefixes: out = sum_parts 2^(m - M) o / sum_parts 2^(m - M) l over all parts of a row, those of its own slots and
 // those of its group's prefix, each a record in `parts` or, of a unit that was cut, several of the blocks' or warps'.
-// Blocks (x, y) look after sequence x.  Of a batch of many rows a warp has 8 neighbouring ones, by 4 lanes each, which
-// take every fourth float4.  Of a batch of few, whose units are cut over many blocks, it has one (kOne): 8 lanes share out
-// the parts, so that all are on their way at once, and their sum is scattered over them, a stage for each bit sending
-// the half that the other lane keeps.  16384 rows in 3 to 4 parts: 12 us with 8 rows a warp, 31 with one; 3904 in
-// up to 18 parts: 19 and 13.
-constexpr int kJoinThreads = 128, kJoinRows = 8192;
-template <int HD, typename T, bool kOne>
+// Blocks (x, y) look after sequence x, a warp after up to 8 rows of a kv head: where their parts lie is found once for
+// them.  A row has 32 / rows lanes, which take turns at its float4, so that records of either kind are read by pieces of
+// 64 bytes and more, four parts at once.  (A warp a row, with the parts shared out among its lanes, took 945
+// instructions a row, mostly for that search: 64 single tokens 8.6 us.)
+constexpr int kJoinThreads = 128, kJoinRows = 8, kJoinParts = 8;
+template <int HD, typename T>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams a) {
-  constexpr int kN = HD / 16;         // float4 of a lane
-  constexpr int kA = kOne ? 1 : 2;    // parts that it loads at once
-  constexpr int kSubs = kOne ? 8 : 1;
+  constexpr int kF = HD / 4;  // float4 of a row
+  constexpr int kN = 4;       // of a lane at once
   pdl_wait();
   const PagedBatch& b = a.b;
   const SharedSeq own = paged_seq(a.shared, a.n_groups + blockIdx.x);
@@ -957,7 +955,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   SharedSeq prefix{};
   if (own.part >= 0) prefix = paged_seq(a.shared, own.group);
   const int lane = threadIdx.x & 31;
-  const int tokens = max(own.n, own.few), rows = tokens * b.n_heads;  // row: kv head, token, head of the group
+  const int tokens = max(own.n, own.few), rows = tokens * a.gq;  // of a kv head
+  if (!tokens) return;
+  const int groups = (rows + kJoinRows - 1) / kJoinRows, items = groups * a.x.K;
+  // lanes of a row: a power of two
+  const int log_rows = rows > 4 ? 3 : rows > 2 ? 2 : rows - 1, lanes = 32 >> log_rows;
+  const int c = lane & (lanes - 1);
   const unsigned few_head = few_length(own), own_head = head_tiles(a.x, own), prefix_head = head_tiles(a.x, prefix);
   // Where a unit's parts lie: n records, the first one apart; a row's float4 k is at k * step float4.
   struct Parts {
@@ -999,89 +1002,72 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     p.ml = HD;
     return p;
   };
-  const int warp = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5), warps = gridDim.y * (kJoinThreads / 32);
-  const int c = kOne ? lane & 3 : lane >> 3, sub = kOne ? lane >> 2 : 0;
-  for (int r = warp; r < (kOne ? rows : (rows + 7) / 8); r += warps) {
-    const int row = kOne ? r : r * 8 + (lane & 7);
+  const int warps = gridDim.y * (kJoinThreads / 32);
+  for (int item = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); item < items; item += warps) {
+    const int head = item / groups, row = (item - head * groups) * kJoinRows + lane / lanes;
     if (row >= rows) continue;
-    const int per_head = tokens * a.gq, head = row / per_head, token = row % per_head / a.gq, h = row % a.gq;
+    const int token = row / a.gq, h = row - token * a.gq;
     const Parts one = own.few ? of_few(head, token, h) : of_unit(own, own_head, head, token, h);
     if (one.n == 1 && own.part < 0) continue;  // the outputs are in their place
     Parts two = one;
     two.n = 0;
     if (own.part >= 0) two = of_unit(prefix, prefix_head, head, token, h);
-    float mm = -INFINITY, ll = 0.f, acc[4 * kN];
-#pragma unroll
-    for (int k = 0; k < 4 * kN; ++k) acc[k] = 0.f;
     const int n = one.n + two.n;
-    for (int i0 = sub; i0 < n; i0 += kA * kSubs) {
-      float4 o[kA][kN];
-      float m[kA], l[kA];
+    T* out = static_cast<T*>(a.out) + (size_t)(own.row0 + token) * a.out_stride + (size_t)(head * a.gq + h) * HD;
+    for (int f0 = c; f0 < kF; f0 += kN * lanes) {
+      float mm = -INFINITY, ll = 0.f;
+      float4 acc[kN];
 #pragma unroll
-      for (int e = 0; e < kA; ++e) {
-        const int i = i0 + e * kSubs;
-        if (i >= n) break;
-        const bool second = i >= one.n;
-        const int part = second ? i - one.n : i, step = second ? two.step : one.step, ml = second ? two.ml : one.ml;
-        const float* rec = part ? (second ? two.rest : one.rest) + (part - 1) * (second ? two.next : one.next)
-                                : second ? two.first : one.first;
+      for (int k = 0; k < kN; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int p0 = 0; p0 < n; p0 += kJoinParts) {
+        float4 o[kJoinParts][kN];
+        float m[kJoinParts], l[kJoinParts];
 #pragma unroll
-        for (int k = 0; k < kN; ++k) o[e][k] = __ldcg(reinterpret_cast<const float4*>(rec) + (size_t)(4 * k + c) * step);
-        m[e] = __ldcg(rec + ml);
-        l[e] = __ldcg(rec + ml + step);
-      }
+        for (int e = 0; e < kJoinParts; ++e) {
+          m[e] = -INFINITY;
+          l[e] = 0.f;
 #pragma unroll
-      for (int e = 0; e < kA; ++e) {
-        if (i0 + e * kSubs >= n) break;
-        const float mn = fmaxf(mm, m[e]);
-        const float old = mm == -INFINITY ? 0.f : ex2(mm - mn), w = m[e] == -INFINITY ? 0.f : ex2(m[e] - mn);
+          for (int k = 0; k < kN; ++k) o[e][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          const int i = p0 + e;
+          if (i >= n) continue;
+          const bool second = i >= one.n;
+          const int part = second ? i - one.n : i, step = second ? two.step : one.step, ml = second ? two.ml : one.ml;
+          const float* rec = part ? (second ? two.rest : one.rest) + (part - 1) * (second ? two.next : one.next)
+                                  : second ? two.first : one.first;
+#pragma unroll
+          for (int k = 0; k < kN; ++k)
+            if (f0 + k * lanes < kF) o[e][k] = __ldcg(reinterpret_cast<const float4*>(rec) + (size_t)(f0 + k * lanes) * step);
+          m[e] = __ldcg(rec + ml);
+          l[e] = __ldcg(rec + ml + step);
+        }
+        float mn = mm;
+#pragma unroll
+        for (int e = 0; e < kJoinParts; ++e) mn = fmaxf(mn, m[e]);
+        const float old = mm == -INFINITY ? 0.f : ex2(mm - mn);
         mm = mn;
-        ll = ll * old + l[e] * w;
+        ll *= old;
 #pragma unroll
-        for (int k = 0; k < kN; ++k) {
-          acc[4 * k] = acc[4 * k] * old + o[e][k].x * w;
-          acc[4 * k + 1] = acc[4 * k + 1] * old + o[e][k].y * w;
-          acc[4 * k + 2] = acc[4 * k + 2] * old + o[e][k].z * w;
-          acc[4 * k + 3] = acc[4 * k + 3] * old + o[e][k].w * w;
+        for (int k = 0; k < kN; ++k) acc[k] = make_float4(acc[k].x * old, acc[k].y * old, acc[k].z * old, acc[k].w * old);
+#pragma unroll
+        for (int e = 0; e < kJoinParts; ++e) {
+          const float w = m[e] == -INFINITY ? 0.f : ex2(m[e] - mn);
+          ll = fmaf(l[e], w, ll);
+#pragma unroll
+          for (int k = 0; k < kN; ++k) {
+            acc[k].x = fmaf(o[e][k].x, w, acc[k].x);
+            acc[k].y = fmaf(o[e][k].y, w, acc[k].y);
+            acc[k].z = fmaf(o[e][k].z, w, acc[k].z);
+            acc[k].w = fmaf(o[e][k].w, w, acc[k].w);
+          }
         }
       }
-    }
-    T* out = static_cast<T*>(a.out) + (size_t)(own.row0 + token) * a.out_stride + (size_t)(head * a.gq + h) * HD;
-    if constexpr (!kOne) {
       const float inv = ll != 0.f ? 1.f / ll : 0.f;
 #pragma unroll
       for (int k = 0; k < kN; ++k)
-        *reinterpret_cast<uint2*>(out + 16 * k + 4 * c) =
-            make_uint2(pack2<T>(acc[4 * k] * inv, acc[4 * k + 1] * inv), pack2<T>(acc[4 * k + 2] * inv, acc[4 * k + 3] * inv));
-      continue;
+        if (f0 + k * lanes < kF)
+          *reinterpret_cast<uint2*>(out + 4 * (f0 + k * lanes)) =
+              make_uint2(pack2<T>(acc[k].x * inv, acc[k].y * inv), pack2<T>(acc[k].z * inv, acc[k].w * inv));
     }
-    float top = mm;
-#pragma unroll
-    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    const float w = mm == -INFINITY ? 0.f : ex2(mm - top);
-    ll *= w;
-#pragma unroll
-    for (int d = 4; d < 32; d <<= 1) ll += __shfl_xor_sync(0xffffffffu, ll, d);
-    const float scale = ll != 0.f ? w / ll : 0.f;
-#pragma unroll
-    for (int k = 0; k < 4 * kN; ++k) acc[k] *= scale;
-    auto stage = [&](auto left, int d) {  // bit d of sub keeps the upper half of what is left
-      constexpr int n = decltype(left)::value;
-      const bool up = (sub >> d) & 1;
-#pragma unroll
-      for (int k = 0; k < n; ++k) {
-        const float send = up ? acc[k] : acc[k + n], keep = up ? acc[k + n] : acc[k];
-        acc[k] = keep + __shfl_xor_sync(0xffffffffu, send, 4 << d);
-      }
-    };
-    stage(std::integral_constant<int, 2 * kN>(), 2);
-    stage(std::integral_constant<int, kN>(), 1);
-    stage(std::integral_constant<int, kN / 2>(), 0);
-    constexpr int kLeft = kN / 2;  // elements sub * kLeft .. of the lane's
-    const int e0 = sub * kLeft;
-    out += 4 * (4 * (e0 / 4) + c) + e0 % 4;
-#pragma unroll
-    for (int k = 0; k < kLeft; k += 2) *reinterpret_cast<uint32_t*>(out + k) = pack2<T>(acc[k], acc[k + 1]);
   }
 }
 
@@ -1166,13 +1152,10 @@ cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cuda
   if ((e = launch_kernel_params(fn, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, s, true, args)) != cudaSuccess) return e;
   if constexpr (kShared) {
     // enough warps for all rows if they are spread evenly over the sequences
-    const long long rows = (long long)a.b.n_tokens * a.b.n_heads;
-    const bool one = rows <= kJoinRows;
-    const long long slices = (rows / a.b.n_seqs / (one ? 1 : 8) + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
-    return launch_kernel(one ? reinterpret_cast<const void*>(&paged_join_kernel<HD, T, true>)
-                             : reinterpret_cast<const void*>(&paged_join_kernel<HD, T, false>),
-                         dim3(a.b.n_seqs, (unsigned)(slices < 1 ? 1 : slices < 1024 ? slices : 1024)), dim3(kJoinThreads), 0, s,
-                         true, &p);
+    const long long items = (((long long)a.b.n_tokens * gq / a.b.n_seqs + kJoinRows - 1) / kJoinRows + 1) * K;
+    const long long slices = (items + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
+    return launch_kernel(reinterpret_cast<const void*>(&paged_join_kernel<HD, T>), dim3(a.b.n_seqs, (unsigned)(slices < 1024 ? slices : 1024)),
+                         dim3(kJoinThreads), 0, s, true, &p);
   }
   if (a.b.max_pages * ps <= kKT) return cudaSuccess;  // every unit is one key tile: nothing is cut
   return launch_kernel(reinterpret_cast<const void*>(&paged_merge_kernel<HD, T>), dim3(grid, kMergeSlices),

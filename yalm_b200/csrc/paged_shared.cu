@@ -6,7 +6,7 @@
 // group sees all of it and no mask is needed.  It is computed once if that halves its passes over the prefix at least:
 // with U tokens a unit, sum_s ceil(n_s / U) >= 2 ceil(sum_s n_s / U).  Long chunks fill their units by themselves.
 //
-// One block: a few loads a sequence, prefix sums, and 48 bytes written for each.
+// One block, for small batches of few threads: a few loads a sequence, prefix sums, and 64 bytes written for each.
 #include <math.h>
 
 #include "launch.h"
@@ -16,38 +16,19 @@ namespace yb {
 
 namespace {
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32;
 typedef unsigned long long u64;
 
-// Inclusive sum over the block.
-__device__ __forceinline__ u64 block_sum(u64 v, u64* s_warp, u64* total) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
-  }
-  if (lane == 31) s_warp[warp] = v;
-  __syncthreads();
-  u64 w = s_warp[lane];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 u = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += u;
-  }
-  const u64 before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
-  *total = __shfl_sync(0xffffffffu, w, kWarps - 1);
-  __syncthreads();
-  return v + (warp ? before : 0);
-}
-
+template <int kThreads>
 __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __grid_constant__ SharedPlanArgs a) {
+  constexpr int kWarps = kThreads / 32;
   __shared__ int s_start[kMaxGroups + 1];  // first sequences
   __shared__ int s_cut[kMaxGroups];        // slots, then key tiles of the prefix that are computed once
-  __shared__ int s_units[kMaxGroups];      // units of the sequences, each by itself
-  __shared__ int s_part[kMaxGroups];       // where the group's tokens' parts begin
-  __shared__ u64 s_warp[kWarps];
+  __shared__ int s_units[kMaxGroups];      // units of the sequences, each by itself, then where their tokens' parts begin
+  __shared__ int s_row0[kMaxGroups], s_rows[kMaxGroups];  // the group's tokens
+  int* const s_part = s_units;
+  __shared__ u64 s_warp[2][kWarps];
   const PagedBatch& b = a.b;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = b.n_heads / b.n_kv_heads;
   pdl_wait();
   for (int g = threadIdx.x; g <= a.n_groups; g += kThreads) {
     s_start[g] = min(max(__ldca(a.group_start + g), 0), b.n_seqs);
@@ -67,6 +48,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
     }
     return lo < a.n_groups && s_start[lo] <= s && s < s_start[lo + 1] ? lo : -1;
   };
+  auto row_of = [&](int s) { return min(max(__ldca(b.q_start + s), 0), b.n_tokens); };
+  for (int g = threadIdx.x; g < a.n_groups; g += kThreads) {
+    s_row0[g] = row_of(s_start[g]);
+    s_rows[g] = s_start[g + 1] > s_start[g] ? max(row_of(s_start[g + 1]) - s_row0[g], 0) : 0;
+  }
   for (int s = threadIdx.x; s < b.n_seqs; s += kThreads) {
     const PagedSeq q = paged_seq(b, s);
     const int g = q.n > 0 ? group_of(s) : -1;
@@ -76,38 +62,39 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
     }
   }
   __syncthreads();
-  // rows of a group's tokens
-  auto row_of = [&](int s) { return min(max(__ldca(b.q_start + s), 0), b.n_tokens); };
-  auto rows_of = [&](int g, int& row0) {
-    row0 = row_of(s_start[g]);
-    return s_start[g + 1] > s_start[g] ? max(row_of(s_start[g + 1]) - row0, 0) : 0;
-  };
-  {
-    const int per = (a.n_groups + kThreads - 1) / kThreads, g0 = threadIdx.x * per;
-    u64 mine = 0, total;
-    for (int g = g0; g < min(a.n_groups, g0 + per); ++g) {
-      int row0;
-      const int rows = rows_of(g, row0), tiles = max(s_cut[g], 0) / kKT;
-      s_cut[g] = rows && s_units[g] >= 2 * ((rows + a.x.U - 1) / a.x.U) ? tiles : 0;
-      if (s_cut[g]) mine += rows;
-    }
-    u64 at = block_sum(mine, s_warp, &total) - mine;
-    for (int g = g0; g < min(a.n_groups, g0 + per); ++g) {
-      int row0;
-      const int rows = s_cut[g] ? rows_of(g, row0) : 0;
-      if (at + rows > (u64)a.part_tokens) s_cut[g] = 0;  // (groups that overlap, which the caller must not give)
-      s_part[g] = (int)at;
-      at += rows;
+  if (warp == 0) {
+    int at = 0;
+    for (int g0 = 0; g0 < a.n_groups; g0 += 32) {
+      const int g = g0 + lane;
+      int rows = 0, tiles = 0;
+      if (g < a.n_groups) {
+        rows = s_rows[g];
+        tiles = max(s_cut[g], 0) / kKT;
+        if (!rows || s_units[g] < 2 * ((rows + a.x.U - 1) / a.x.U)) tiles = 0;
+        if (!tiles) rows = 0;
+      }
+      int upto = rows;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += u;
+      }
+      // (groups that overlap, which the caller must not give, could have more than there is room for)
+      if (g < a.n_groups) {
+        s_part[g] = at + upto - rows;
+        s_cut[g] = at + upto <= a.part_tokens ? tiles : 0;
+      }
+      at = min(at + __shfl_sync(0xffffffffu, upto, 31), 1 << 21);
     }
   }
   __syncthreads();
-  const int all = a.n_groups + b.n_seqs, gq = b.n_heads / b.n_kv_heads;
+  const int all = a.n_groups + b.n_seqs;
   auto seq_at = [&](int v) {
     SharedSeq q{};
     q.part = -1;
     if (v < a.n_groups) {
-      q.n = rows_of(v, q.row0);
-      if (!s_cut[v]) q.n = 0;
+      q.row0 = s_row0[v];
+      q.n = s_cut[v] ? s_rows[v] : 0;
       q.kv = s_cut[v] * kKT;
       q.table = s_start[v];
       q.part = s_part[v];
@@ -122,9 +109,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
     q.kv = p.kv;
     q.table = s;
     if (p.n > 0 && g >= 0 && s_cut[g]) {
-      int row0;
-      const int rows = rows_of(g, row0), at = q.row0 - row0;
-      if (at >= 0 && at + p.n <= rows) {  // (else q_start decreases)
+      const int at = q.row0 - s_row0[g];
+      if (at >= 0 && at + p.n <= s_rows[g]) {  // (else q_start decreases)
         q.lo = s_cut[g];
         q.part = s_part[g] + at;
         q.group = g;
@@ -132,31 +118,51 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
     }
     return q;
   };
-  const int per = (all + kThreads - 1) / kThreads, v0 = threadIdx.x * per;
-  u64 mine = 0, few = 0, total, few_total;
-  for (int v = v0; v < min(all, v0 + per); ++v) {
-    const SharedSeq q = seq_at(v);
-    mine += (u64)head_tiles(a.x, q) * a.x.K;
-    few += (u64)few_length(q) * a.x.K;
+  const int per = (all + kThreads - 1) / kThreads, v0 = min(all, (int)threadIdx.x * per), v1 = min(all, v0 + per);
+  SharedSeq one{};
+  u64 mine = 0, few = 0;
+  for (int v = v0; v < v1; ++v) {
+    one = seq_at(v);
+    mine += (u64)head_tiles(a.x, one) * a.x.K;
+    few += (u64)few_length(one) * a.x.K;
   }
-  u64 at = block_sum(mine, s_warp, &total) - mine, few_at = block_sum(few, s_warp, &few_total) - few;
-  for (int v = v0; v < min(all, v0 + per); ++v) {
-    SharedSeq q = seq_at(v);
+  u64 at = mine, few_at = few;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, at, o), y = __shfl_up_sync(0xffffffffu, few_at, o);
+    if (lane >= o) at += x, few_at += y;
+  }
+  if (lane == 31) {
+    s_warp[0][warp] = at;
+    s_warp[1][warp] = few_at;
+  }
+  __syncthreads();
+  u64 total = 0, few_total = 0;
+  at -= mine;
+  few_at -= few;
+  for (int i = 0; i < kWarps; ++i) {
+    if (i == warp) at += total, few_at += few_total;
+    total += s_warp[0][i];
+    few_total += s_warp[1][i];
+  }
+  for (int v = v0; v < v1; ++v) {
+    SharedSeq q = per == 1 ? one : seq_at(v);
     q.begin = at;
     q.few_begin = few_at;
     at += (u64)head_tiles(a.x, q) * a.x.K;
     few_at += (u64)few_length(q) * a.x.K;
     a.seqs[v] = q;
   }
-  if (threadIdx.x < 32) {
-    // SMs for the one kernel and the other: the least of the longer time.  A key tile of two row tiles takes an SM 1.7 us, a
-    // step of few rows 0.11 us (of 8 KB, as fast as one SM reads), but all SMs together no less than 0.0013 us.
-    const float tiles = (float)total * 1.7f, steps = (float)few_total * (a.head_dim == 128 ? 1.f : 0.6f);
+  if (warp == kWarps - 1) {
+    // SMs for the one kernel and the other: the least of the longer time.  An SM takes 6 us and 2.2 us a key tile, or 3 us and
+    // 0.136 us a step of few rows (of 8 KB, as fast as one SM reads); all SMs together no less than 0.0013 us a step.
+    const float tiles = (float)total * 2.2f, steps = (float)few_total * (a.head_dim == 128 ? 1.f : 0.6f);
     float best = INFINITY;
     int blocks = 0;
-    for (int n = threadIdx.x; n <= a.grid; n += 32) {
-      const float t = fmaxf(n ? tiles / n : total ? INFINITY : 0.f,
-                            fmaxf(n < a.grid ? steps * 0.11f / (a.grid - n) : few_total ? INFINITY : 0.f, steps * 0.0013f));
+    for (int n = lane; n <= a.grid; n += 32) {
+      const float t = fmaxf(n ? 6.f + __fdividef(tiles, (float)n) : total ? INFINITY : 0.f,
+                            fmaxf(n < a.grid ? 3.f + __fdividef(steps * 0.136f, (float)(a.grid - n)) : few_total ? INFINITY : 0.f,
+                                  steps * 0.0013f));
       if (t < best) best = t, blocks = n;
     }
 #pragma unroll
@@ -165,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
       const int n = __shfl_xor_sync(0xffffffffu, blocks, o);
       if (t < best || (t == best && n < blocks)) best = t, blocks = n;
     }
-    if (threadIdx.x == 0) {
+    if (lane == 0) {
       SharedHead h;
       h.total = total;
       share_out(total, max(blocks, 1), h.share, h.more);
@@ -180,7 +186,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
 
 cudaError_t paged_shared_plan(const SharedPlanArgs& a, cudaStream_t s) {
   SharedPlanArgs p = a;
-  return launch_kernel(reinterpret_cast<const void*>(&paged_shared_plan_kernel), dim3(1), dim3(kThreads), 0, s, true, &p);
+  // a thread for each prefix and sequence where 1024 are enough: sums over few warps are short
+  const int all = a.n_groups + a.b.n_seqs, threads = all <= 256 ? 256 : all <= 512 ? 512 : 1024;
+  const void* fn = threads == 256   ? reinterpret_cast<const void*>(&paged_shared_plan_kernel<256>)
+                   : threads == 512 ? reinterpret_cast<const void*>(&paged_shared_plan_kernel<512>)
+                                    : reinterpret_cast<const void*>(&paged_shared_plan_kernel<1024>);
+  return launch_kernel(fn, dim3(1), dim3(threads), 0, s, true, &p);
 }
 
 }  // namespace yb
