@@ -3,9 +3,9 @@
 //
 // What bounds it is the cache's bytes, if starts and ends of many short units cost little: the tensor-core path pays
 // 4000 to 5500 clocks of a block for them, which for 3 tiles of own slots is as much as their bytes take.  Here a warp
-// works by itself, without shared memory or barriers: steps of 16 slots (of one page), K and V straight from memory into
-// the operands of mma.m16n8k16, for which the order of the dimensions inside a product is chosen so that every lane
-// loads 16 bytes at a time:
+// works by itself: steps of 16 slots (of one page), whose K and V, 4 KB each for heads of 128, come by a bulk copy into a
+// ring of its own, also across units; and from there straight into the operands of mma.m16n8k16, for which the order of
+// the dimensions inside a product is chosen so that every lane loads 16 bytes at a time:
 //   S^T = K . Q^T   slots x rows; the product over dims takes dims 32c + 8q .. + 7 of lane q's chunk in any order, if K
 //                   and Q have the same one
 //   O^T += V^T . P^T  dims x rows; P^T is S^T's transpose in registers (movmatrix), V's operand pairs two slots of a
@@ -52,6 +52,11 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi, __nv_bfloat16) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
 
 template <int HD, typename T>
@@ -84,8 +89,74 @@ __global__ void __launch_bounds__(kFewThreads, 1) paged_few_kernel(const __grid_
     head = (int)quot(rem, length);
     off = (int)(rem - (u64)head * length);
   }
-  const size_t row_elems = HD;
   const int ps = 1 << b.ps_log2;
+  // ---- this warp's ring
+  constexpr int kStages = few_stages(HD);
+  constexpr uint32_t kBytes = kFewSlots * HD * 2;  // of K, and of V
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t s_bars[kFewWarps][kStages];
+  const int w = threadIdx.x >> 5;
+  const uint32_t ring = smem_u32(smem_raw) + (uint32_t)w * kStages * 2 * kBytes, bars = smem_u32(&s_bars[w][0]);
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init_s(bars + 8 * i, 1);
+    mbar_fence_init();
+  }
+  __syncwarp();
+  // The steps of this warp's part in order, copied kStages ahead of those that are worked on.  A wait that runs out ends
+  // the warp, once what it has under way has landed.
+  struct {
+    SharedSeq sq;
+    int seq, head, off, left, pages;  // pages: lane i has that of step t with t % 32 == i
+    unsigned count, there;            // steps issued; by count % 32, whether the page is there
+    bool fresh;
+  } ahead{sq, seq, head, off, left, -1, 0, 0, true};
+  unsigned done = 0;  // steps worked on
+  bool dead = false;
+  auto issue = [&] {
+    for (;;) {
+      if (ahead.left <= 0) return;
+      const int steps = few_steps(ahead.sq);
+      if (ahead.off < steps) break;
+      ahead.left -= steps + kFewUnit - ahead.off;
+      if (ahead.left <= 0) return;
+      ahead.off = 0;
+      ahead.fresh = true;
+      if (++ahead.head >= a.K) {
+        ahead.head = 0;
+        do {
+          if (++ahead.seq >= a.shared.n_seqs) {
+            ahead.left = 0;
+            return;
+          }
+          ahead.sq = paged_seq(a.shared, ahead.seq);
+        } while (ahead.sq.few <= 0);
+      }
+    }
+    const int t = ahead.off, slot = ahead.sq.lo * kKT + t * kFewSlots;
+    if (ahead.fresh || (t & 31) == 0) {
+      const int at = ahead.sq.lo * kKT + ((t & ~31) + lane) * kFewSlots;
+      ahead.pages = at < ahead.sq.kv ? __ldca(b.page_table + (size_t)ahead.sq.table * b.max_pages + (at >> b.ps_log2)) : -1;
+      ahead.fresh = false;
+    }
+    const int page = __shfl_sync(0xffffffffu, ahead.pages, t & 31);
+    const bool ok = page >= 0 && page < b.n_pages;
+    const unsigned bit = 1u << (ahead.count & 31);
+    ahead.there = ok ? ahead.there | bit : ahead.there & ~bit;
+    if (ok && lane == 0) {
+      const int stage = ahead.count % kStages;
+      const size_t from = (((size_t)page * a.K + ahead.head) * ps + (slot & (ps - 1))) * HD;
+      const uint32_t to = ring + stage * 2 * kBytes, bar = bars + 8 * stage;
+      mbar_arrive_expect_tx_s(bar, 2 * kBytes);
+      bulk_g2s_nohint_s(to, static_cast<const T*>(a.k_pages) + from, kBytes, bar);
+      bulk_g2s_nohint_s(to + kBytes, static_cast<const T*>(a.v_pages) + from, kBytes, bar);
+    }
+    ++ahead.count;
+    ++ahead.off;
+    --ahead.left;
+  };
+  unsigned phases = 0;  // by stage, the parity that its next copy completes
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) issue();
   for (;;) {
     // ---- a piece: steps [t0, t1) of the unit
     const int steps = few_steps(sq), length = steps + kFewUnit, t0 = off, t1 = min(steps, off + left);
@@ -106,55 +177,37 @@ __global__ void __launch_bounds__(kFewThreads, 1) paged_few_kernel(const __grid_
       float o[2 * kC][4];  // o[4 j + i]: dims 64 j + 8 g + 2 i, + 1 of rows 2 q4, 2 q4 + 1
 #pragma unroll
       for (int i = 0; i < 2 * kC; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-      const int* table = b.page_table + (size_t)sq.table * b.max_pages;
       const int slot_lo = sq.lo * kKT;
-      int pages = -1;  // lane i: the page of step (t & ~31) + i of the piece
       for (int t = t0; t < t1; ++t) {
         const int slot = slot_lo + t * kFewSlots;
-        if (((t - t0) & 31) == 0) {
-          const int s = slot + lane * kFewSlots;
-          pages = s < sq.kv && t + lane < t1 ? __ldca(table + (s >> b.ps_log2)) : -1;
-          if (pages >= b.n_pages) pages = -1;
+        const int stage = done % kStages;
+        const bool here = (ahead.there >> (done & 31)) & 1u;
+        ++done;
+        if (!here) {
+          issue();
+          continue;
         }
-        const int page = __shfl_sync(0xffffffffu, pages, (t - t0) & 31);
-        if (page < 0) continue;
-        const size_t base = (((size_t)page * a.K + head) * ps + (slot & (ps - 1))) * row_elems;
-        const T* kp = static_cast<const T*>(a.k_pages) + base + (size_t)g * HD + 8 * q4;
-        const T* vp = static_cast<const T*>(a.v_pages) + base + (size_t)(2 * q4) * HD + 8 * g;
-        uint4 k0[kC], k1[kC], v[kJ][4];
+        if (!__all_sync(0xffffffffu, mbar_wait_s(bars + 8 * stage, (phases >> stage) & 1u, a.status))) {
+          dead = true;
+          break;
+        }
+        phases ^= 1u << stage;
+        const uint32_t kv = ring + stage * 2 * kBytes, kat = kv + g * (HD * 2) + q4 * 16, vat = kv + kBytes + q4 * (HD * 4) + g * 16;
+        float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
-          k0[c] = __ldcs(reinterpret_cast<const uint4*>(kp + 32 * c));
-          k1[c] = __ldcs(reinterpret_cast<const uint4*>(kp + 8 * HD + 32 * c));
+          const uint4 k0 = lds16(kat + 64 * c), k1 = lds16(kat + 8 * HD * 2 + 64 * c);
+          mma<T>(s, k0.x, k1.x, k0.y, k1.y, qf[c].x, qf[c].y);
+          mma<T>(s2, k0.z, k1.z, k0.w, k1.w, qf[c].z, qf[c].w);
         }
 #pragma unroll
-        for (int j = 0; j < kJ; ++j) {
-          v[j][0] = __ldcs(reinterpret_cast<const uint4*>(vp + 64 * j));
-          v[j][1] = __ldcs(reinterpret_cast<const uint4*>(vp + HD + 64 * j));
-          v[j][2] = __ldcs(reinterpret_cast<const uint4*>(vp + 8 * HD + 64 * j));
-          v[j][3] = __ldcs(reinterpret_cast<const uint4*>(vp + 9 * HD + 64 * j));
-        }
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < kC; ++c) {
-          mma<T>(s, k0[c].x, k1[c].x, k0[c].y, k1[c].y, qf[c].x, qf[c].y);
-          mma<T>(s, k0[c].z, k1[c].z, k0[c].w, k1[c].w, qf[c].z, qf[c].w);
-        }
+        for (int k = 0; k < 4; ++k) s[k] += s2[k];
         if (slot + kFewSlots > sq.kv - sq.few) {  // an edge
           const int at = slot + g;
           if (at >= last0) s[0] = -INFINITY;
           if (at >= last1) s[1] = -INFINITY;
           if (at + 8 >= last0) s[2] = -INFINITY;
           if (at + 8 >= last1) s[3] = -INFINITY;
-          // what lies behind the last slot may be anything, and 0 of it has to be 0
-          const int n = sq.kv - slot - 2 * q4;
-#pragma unroll
-          for (int j = 0; j < kJ; ++j) {
-            if (n <= 0) v[j][0] = zero4();
-            if (n <= 1) v[j][1] = zero4();
-            if (n <= 8) v[j][2] = zero4();
-            if (n <= 9) v[j][3] = zero4();
-          }
         }
         float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
 #pragma unroll
@@ -187,14 +240,24 @@ __global__ void __launch_bounds__(kFewThreads, 1) paged_few_kernel(const __grid_
         const uint32_t p0 = movm_trans(pack(s[0], s[1], T())), p1 = movm_trans(pack(s[2], s[3], T()));
 #pragma unroll
         for (int j = 0; j < kJ; ++j) {
-          const uint32_t w[4][4] = {{v[j][0].x, v[j][0].y, v[j][0].z, v[j][0].w}, {v[j][1].x, v[j][1].y, v[j][1].z, v[j][1].w},
-                                    {v[j][2].x, v[j][2].y, v[j][2].z, v[j][2].w}, {v[j][3].x, v[j][3].y, v[j][3].z, v[j][3].w}};
+          uint32_t w[4][4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // slots 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9
+            const int at = (k & 1) + (k >> 1) * 8;
+            uint4 v = lds16(vat + at * (HD * 2) + 128 * j);
+            // what lies behind the last slot may be anything, and 0 of it has to be 0
+            if (slot + 2 * q4 + at >= sq.kv) v = zero4();
+            w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
+          }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             mma<T>(o[4 * j + i], __byte_perm(w[0][i], w[1][i], 0x5410), __byte_perm(w[0][i], w[1][i], 0x7632),
                    __byte_perm(w[2][i], w[3][i], 0x5410), __byte_perm(w[2][i], w[3][i], 0x7632), p0, p1);
         }
+        __syncwarp();  // all have read the stage
+        issue();
       }
+      if (dead) break;
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) {
         l0 += __shfl_xor_sync(0xffffffffu, l0, d);
@@ -243,17 +306,27 @@ __global__ void __launch_bounds__(kFewThreads, 1) paged_few_kernel(const __grid_
       } while (sq.few <= 0);
     }
   }
+  // (only after a wait that ran out) nobody leaves while a copy may still be landing: that of the failed step and later
+  for (unsigned i = done - 1; i != ahead.count; ++i)
+    if ((ahead.there >> (i & 31)) & 1u) {
+      mbar_wait_s(bars + 8 * (i % kStages), (phases >> (i % kStages)) & 1u, a.status);
+      phases ^= 1u << (i % kStages);
+    }
 }
 
 }  // namespace
 
-cudaError_t paged_few(const PagedFewArgs& a, int head_dim, int type, int grid, cudaStream_t s) {
+cudaError_t paged_few(const PagedFewArgs& a, int head_dim, int type, int device, int grid, cudaStream_t s) {
   PagedFewArgs p = a;
-  const void* fn = head_dim == 128 ? (type == 1 ? reinterpret_cast<const void*>(&paged_few_kernel<128, __half>)
-                                                : reinterpret_cast<const void*>(&paged_few_kernel<128, __nv_bfloat16>))
-                                   : (type == 1 ? reinterpret_cast<const void*>(&paged_few_kernel<64, __half>)
-                                                : reinterpret_cast<const void*>(&paged_few_kernel<64, __nv_bfloat16>));
-  return launch_kernel(fn, dim3(grid), dim3(kFewThreads), 0, s, true, &p);
+  static SmemCap caps[4];
+  const int which = (head_dim == 128 ? 2 : 0) + (type == 1 ? 1 : 0);
+  const void* const fns[4] = {
+      reinterpret_cast<const void*>(&paged_few_kernel<64, __nv_bfloat16>), reinterpret_cast<const void*>(&paged_few_kernel<64, __half>),
+      reinterpret_cast<const void*>(&paged_few_kernel<128, __nv_bfloat16>), reinterpret_cast<const void*>(&paged_few_kernel<128, __half>)};
+  const size_t smem = (size_t)kFewWarps * few_stages(head_dim) * 2 * kFewSlots * head_dim * 2;
+  const cudaError_t e = caps[which].raise(fns[which], device, smem);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(fns[which], dim3(grid), dim3(kFewThreads), smem, s, true, &p);
 }
 
 }  // namespace yb

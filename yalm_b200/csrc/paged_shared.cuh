@@ -30,7 +30,8 @@ struct SharedPlanArgs {
 cudaError_t paged_shared_plan(const SharedPlanArgs& a, cudaStream_t s);
 
 // ---- sequences of few rows (paged_few.cu)
-constexpr int kFewThreads = 512, kFewWarps = kFewThreads / 32;  // one block an SM
+constexpr int kFewThreads = 384, kFewWarps = kFewThreads / 32;  // one block an SM
+constexpr __host__ __device__ int few_stages(int head_dim) { return head_dim == 128 ? 2 : 4; }
 // A warp's records: 0 for a unit begun by an earlier warp, 1 for the one it leaves to later ones.  A row is o [head_dim],
 // m, l and two floats for alignment.
 inline __host__ __device__ size_t few_row_floats(int head_dim) { return (size_t)head_dim + 4; }
@@ -47,8 +48,9 @@ struct PagedFewArgs {
   float c;       // scale * log2(e)
   float* recs;   // [warps][2][kFewRows] rows
   float* parts;  // [tokens with a part][n_heads] rows
+  unsigned* status;
 };
-cudaError_t paged_few(const PagedFewArgs& a, int head_dim, int type, int grid, cudaStream_t s);
+cudaError_t paged_few(const PagedFewArgs& a, int head_dim, int type, int device, int grid, cudaStream_t s);
 
 // (from L2: the attention kernel starts while the one before it, which waits for the plan, still runs)
 __device__ __forceinline__ SharedSeq paged_seq(const SharedBatch& b, int v) {
