@@ -13,9 +13,10 @@ pytestmark = pytest.mark.gpu
 
 
 class Shared(Step):
-    """A Step whose sequences from starts[g] to starts[g + 1] have the first one's pages for prefix[g] slots."""
+    """A Step whose sequences from starts[g] to starts[g + 1] have the first one's pages for prefix[g] slots.  wide: its
+    table is so long that sharing could save the 64 MB from which on prefixes are computed apart."""
 
-    def __init__(self, starts, prefix, own, new, nh, nkv, hd, ps, dtype, seed, **kw):
+    def __init__(self, starts, prefix, own, new, nh, nkv, hd, ps, dtype, seed, wide=True, **kw):
         import torch
         S = len(own)
         group = [next((g for g in range(len(prefix)) if starts[g] <= s < starts[g + 1]), None) for s in range(S)]
@@ -35,6 +36,11 @@ class Shared(Step):
                     self.k[page], self.v[page] = math.nan, math.nan
         i32 = dict(dtype=torch.int32, device="cuda")
         self.page_table = torch.tensor(self.table, **i32)
+        if wide and S > 1:
+            width = min(int(64e6 / ((S - 1) * nkv * hd * 4) / ps) + 1, (1 << 21) // ps)
+            if width > self.page_table.shape[1]:
+                more = torch.full((S, width - self.page_table.shape[1]), -1, **i32)
+                self.page_table = torch.cat((self.page_table, more), 1).contiguous()
         self.group_start, self.prefix_len = torch.tensor(starts, **i32), torch.tensor(prefix, **i32)
 
     def attend(self, window=0, scale=None, out=None, q=None, scratch=None, batch=None):
@@ -172,6 +178,14 @@ def test_results_repeat_and_take_a_dirty_workspace(gpu):
     ref, tol = st.attend64()
     assert ((out.double() - ref).abs() <= tol).all()
     assert b.status(scratch) == 0
+
+
+def test_small_batches_take_the_other_call(gpu):
+    import torch
+    st = Shared([0, 9], [1000], _ragged(9, 300, 6), [1] * 9, 8, 2, 128, 16, "f16", seed=16, wide=False)
+    assert torch.equal(st.check().half(), Step.attend(st))
+    wide = Shared([0, 9], [1000], _ragged(9, 300, 6), [1] * 9, 8, 2, 128, 16, "f16", seed=16)
+    assert not torch.equal(wide.check().half(), Step.attend(st))  # (sums are split elsewhere)
 
 
 def test_without_groups_it_is_the_other_call(gpu):

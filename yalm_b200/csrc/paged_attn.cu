@@ -337,6 +337,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     else return c.seq;
   };
   auto entry = [](const int* p) { return kShared ? __ldcg(p) : __ldca(p); };
+  if constexpr (kShared) {
+    if (block_begin(__ldcg(&a.head->share), __ldcg(&a.head->more), blockIdx.x) >= __ldcg(&a.head->total)) {
+      pdl_wait();  // nothing to do here: its SM was the other kernel's
+      return;
+    }
+  }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
                  : "memory");
@@ -956,12 +962,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   if (own.part >= 0) prefix = paged_seq(a.shared, own.group);
   const int lane = threadIdx.x & 31;
   const int tokens = max(own.n, own.few), rows = tokens * a.gq;  // of a kv head
+  const unsigned few_head = few_length(own), own_head = head_tiles(a.x, own), prefix_head = head_tiles(a.x, prefix);
   if (!tokens) return;
   const int groups = (rows + kJoinRows - 1) / kJoinRows, items = groups * a.x.K;
   // lanes of a row: a power of two
   const int log_rows = rows > 4 ? 3 : rows > 2 ? 2 : rows - 1, lanes = 32 >> log_rows;
   const int c = lane & (lanes - 1);
-  const unsigned few_head = few_length(own), own_head = head_tiles(a.x, own), prefix_head = head_tiles(a.x, prefix);
   // Where a unit's parts lie: n records, the first one apart; a row's float4 k is at k * step float4.
   struct Parts {
     int n;

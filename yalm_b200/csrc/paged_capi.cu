@@ -274,7 +274,12 @@ extern "C" int yb_paged_attention_shared_dev(const yb_paged_batch* b, int n_grou
                                              long long q_stride, float scale, void* scratch_dev, void* stream) {
   int rc = check_groups(n_groups);
   if (rc) return rc;
-  if (n_groups == 0)  // nothing is shared
+  // Where nothing is shared, or reading it once can save no more than 64 MB (every sequence's whole table but one), its
+  // kernels cost more than they save.  32 heads of 128 on 8 kv heads, prefix of 4096 and 100 own slots: 4 sequences (50
+  // MB) 19.4 us without, 32.9 with; 8 (117 MB) 27.1 and 31.3; 16 (252 MB) 42.9 and 31.5.  8 heads of 64 on 2: 32 (65 MB)
+  // 24.3 and 25.2, 64 (132 MB) 37.7 and 25.3.
+  if (b && b->n_seqs > 0 && (b->n_seqs - 1.0) * b->max_pages * b->page_size * b->n_kv_heads * b->head_dim * 4.0 < 64e6) n_groups = 0;
+  if (n_groups == 0)
     return yb_paged_attention_dev(b, out, out_stride, q, q_stride, scale, 0, scratch_dev, stream);
   PagedAttnArgs a{};
   bool empty = false;

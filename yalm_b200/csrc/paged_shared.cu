@@ -29,6 +29,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
   __shared__ u64 s_warp[2][kWarps];
   const PagedBatch& b = a.b;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = b.n_heads / b.n_kv_heads;
+  pdl_trigger();  // the next kernel waits for this one's end
   pdl_wait();
   for (int g = threadIdx.x; g <= a.n_groups; g += kThreads) {
     s_start[g] = min(max(__ldca(a.group_start + g), 0), b.n_seqs);
