@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <initializer_list>
 #include <string>
 #include <utility>
@@ -26,6 +27,22 @@ inline int check_device(int dev, std::initializer_list<std::pair<const char*, co
       return set_error(YB_E_INVALID, std::string(b.first) + " is not memory of the current device");
   }
   return 0;
+}
+
+// SMs of a device, asked for once (148 without one, so that sizes can be computed anywhere)
+inline int device_sms(int dev) {
+  static std::atomic<int> known[64];
+  if (dev >= 0 && dev < 64) {
+    const int n = known[dev].load(std::memory_order_relaxed);
+    if (n) return n;
+  }
+  int n = 0;
+  if (dev < 0 || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    return 148;
+  }
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 }  // namespace yb

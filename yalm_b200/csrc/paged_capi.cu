@@ -59,22 +59,6 @@ int check_rows(const char* name, const void* p, long long stride, long long widt
   return 0;
 }
 
-// SMs of a device, asked for once (148 without one, so that sizes can be computed anywhere)
-int device_sms(int dev) {
-  static std::atomic<int> known[64];
-  if (dev >= 0 && dev < 64) {
-    const int n = known[dev].load(std::memory_order_relaxed);
-    if (n) return n;
-  }
-  int n = 0;
-  if (dev < 0 || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
-    cudaGetLastError();
-    return 148;
-  }
-  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
-  return n;
-}
-
 // What one of the attention's blocks may have to walk is counted in 31 bits: the units (blocks of up to 2 * (128 /
 // query heads per kv head) queries) of every sequence and kv head, with the key tiles of 128 slots of the longest cache
 // and 3 more each, shared out over the blocks.

@@ -37,6 +37,6 @@ extern "C" int yb_sample_rows_dev(int* tokens_dev, float* prob_dev, const void* 
   a.top_k = top_k_dev;
   a.top_p = top_p_dev;
   a.min_p = min_p_dev;
-  YB_CK(sample_rows(a, dtype, dev, static_cast<cudaStream_t>(stream)));
+  YB_CK(sample_rows(a, dtype, dev, device_sms(dev), static_cast<cudaStream_t>(stream)));
   return 0;
 }

@@ -36,6 +36,7 @@ typedef unsigned long long u64;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kOctaves = 44, kPerOctave = 16, kBins = kOctaves * kPerOctave;
 constexpr int kEach = 4, kList = kThreads * kEach;  // tokens of a list: 4 a thread
+constexpr int kBinsPer = (kBins + kThreads - 1) / kThreads;
 constexpr u64 kOne = 1ull << 43;                    // the largest weight
 constexpr float kLeastTemperature = 0x1p-60f, kMostTemperature = 0x1p90f;
 constexpr size_t kMaxStage = 160 * 1024;            // bytes of a row's stretch that shared memory takes
@@ -91,7 +92,10 @@ struct Weights {
   float maxf, cut;      // what lies below cut has no weight
   float none;           // nor has this, which stands for all that lies below it, and for NaN
   float per_bin;        // bins a unit of l
-  // a number at or below all logits of the bins up to b that have a weight
+  // a number at or below all logits of the bins up to b that have a weight, and one above those of bin b > 0
+  __device__ __forceinline__ float ceiling_of_bin(int b) const {
+    return fminf(maxf, __double2float_ru(max - (b - 1) * (double)(1.f - 0x1p-20f) / per_bin));
+  }
   __device__ __forceinline__ float floor_of_bins(int b) const {
     return b == kBins - 1 ? cut : fmaxf(cut, __double2float_rd(max - (b + 1) * (double)(1.f + 0x1p-20f) / per_bin));
   }
@@ -184,11 +188,12 @@ struct Order {
 };
 
 struct Shared {
-  unsigned count[kBins], low[kBins], high[kBins];  // of sums, the low and the high 32 bits
+  // of sums of weights 15 bits, the next 15, and the rest, each summed by itself: up to 2^17 of them (2^20 / 8) fit 32 bits
+  unsigned count[kBins], low[kBins], mid[kBins], high[kBins];
   u64 list[kList];
   Pair warps[kWarps];
   u64 sums[kWarps], lo[kWarps], hi[kWarps];
-  u64 block_lo, block_hi, block_sum, told;
+  u64 block_sum, told;
   float max[kWarps], block_max;
   int block_first;  // index of the block's first maximum
   unsigned listed;
@@ -224,15 +229,16 @@ __device__ __forceinline__ u64 block_scan(Shared& s, u64 v, u64* total) {
 __device__ __forceinline__ void clear_bins(Shared& s, bool sums) {
   for (int i = threadIdx.x; i < kBins; i += kThreads) {
     s.count[i] = 0;
-    if (sums) s.low[i] = s.high[i] = 0;
+    if (sums) s.low[i] = s.mid[i] = s.high[i] = 0;
   }
 }
-__device__ __forceinline__ void add_to_bin(Shared& s, int b, u64 w) {
-  const unsigned lo = (unsigned)w;
-  const unsigned was = atomicAdd(&s.low[b], lo), hi = (unsigned)(w >> 32) + (was + lo < was ? 1u : 0u);
+__device__ __forceinline__ void add_to_bin(Shared& s, int b, double above) {  // 2^52 + the weight
+  const unsigned lo = (unsigned)__double2loint(above), hi = (lo >> 30) | (unsigned)(__double2hiint(above) - 0x43300000) << 2;
+  atomicAdd(&s.count[b], 1u);
+  atomicAdd(&s.low[b], lo & 0x7fffu);
+  atomicAdd(&s.mid[b], (lo >> 15) & 0x7fffu);
   if (hi) atomicAdd(&s.high[b], hi);
 }
-constexpr int kBinsPer = (kBins + kThreads - 1) / kThreads;
 
 // A list, 4 neighbouring tokens a thread, sorted descending; `all` is a power of two from 4 on, and what lies behind the
 // list's end is 0.  Steps of up to 64 places stay in a warp.
@@ -278,6 +284,93 @@ __device__ __forceinline__ void sort_list(u64 (&v)[kEach], u64* buf, int all) {
         }
       }
     }
+}
+
+// The same for n tokens (0 behind them), by way of bins of the list's own range: a token's place is the number of those in
+// bins before its own, and of larger ones in it.  Short lists, and those with many tokens in a bin, are sorted as above.
+constexpr int kShortList = 64, kFullBin = 48;
+__device__ __forceinline__ void order_list(Shared& s, u64 (&v)[kEach], int n) {
+  int all = kShortList;
+  while (all < n) all <<= 1;
+  if (n <= kShortList) {
+    sort_list(v, s.list, all);
+    return;
+  }
+  const int v0 = threadIdx.x * kEach, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  u64 lo = ~0ull, hi = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e)
+    if (v[e]) {
+      lo = v[e] < lo ? v[e] : lo;
+      hi = v[e] > hi ? v[e] : hi;
+    }
+  for (int d = 16; d; d >>= 1) {
+    const u64 l = __shfl_xor_sync(0xffffffffu, lo, d), h = __shfl_xor_sync(0xffffffffu, hi, d);
+    lo = l < lo ? l : lo;
+    hi = h > hi ? h : hi;
+  }
+  if (lane == 0) {
+    s.lo[warp] = lo;
+    s.hi[warp] = hi;
+  }
+  for (int i = threadIdx.x; i < kBins; i += kThreads) s.count[i] = 0;
+  __syncthreads();
+  lo = s.lo[lane % kWarps];
+  hi = s.hi[lane % kWarps];
+  for (int d = kWarps / 2; d; d >>= 1) {
+    const u64 l = __shfl_xor_sync(0xffffffffu, lo, d), h = __shfl_xor_sync(0xffffffffu, hi, d);
+    lo = l < lo ? l : lo;
+    hi = h > hi ? h : hi;
+  }
+  const float per = (float)kBins / ((float)(hi - lo) + 1.f);  // (roundings keep the order)
+  int bin[kEach];
+  unsigned slot[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    bin[e] = min((int)((float)(hi - v[e]) * per), kBins - 1);
+    if (v[e]) slot[e] = atomicAdd(&s.count[bin[e]], 1u);
+  }
+  __syncthreads();
+  const int b0 = threadIdx.x * kBinsPer;
+  unsigned count[kBinsPer], mine = 0;
+  bool full = false;
+#pragma unroll
+  for (int k = 0; k < kBinsPer; ++k) {
+    count[k] = b0 + k < kBins ? s.count[b0 + k] : 0;
+    full |= count[k] > kFullBin;
+    mine += count[k];
+  }
+  u64 total;
+  unsigned before = (unsigned)block_scan(s, (u64)mine, &total) - mine;
+#pragma unroll
+  for (int k = 0; k < kBinsPer; ++k) {
+    if (b0 + k < kBins) s.low[b0 + k] = before;
+    before += count[k];
+  }
+  if (__syncthreads_or(full)) {
+    sort_list(v, s.list, all);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < kEach; ++e)
+    if (v[e]) s.list[s.low[bin[e]] + slot[e]] = v[e];
+  __syncthreads();
+  unsigned place[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    if (!v[e]) continue;
+    place[e] = s.low[bin[e]];
+    const unsigned from = place[e], to = from + s.count[bin[e]];
+    for (unsigned i = from; i < to; ++i) place[e] += s.list[i] > v[e];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kEach; ++e)
+    if (v[e]) s.list[place[e]] = v[e];
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) v[e] = v0 + e < (int)total ? s.list[v0 + e] : 0;
+  __syncthreads();
 }
 
 template <typename T, bool kStaged>
@@ -414,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
         if (c >= blocks || b >= kBins) continue;
         const Shared* o = dsmem_ptr(&s, c);
         bin[k].n += o->count[b];
-        if (!by_rank) bin[k].sum += o->low[b] + ((u64)o->high[b] << 32);
+        if (!by_rank) bin[k].sum += o->low[b] + ((u64)o->mid[b] << 15) + ((u64)o->high[b] << 30);
       }
       mine = mine + bin[k];
     }
@@ -453,26 +546,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     const unsigned to = atomicAdd(&first->listed, 1u);
     if (to < kList) first->list[to] = at;
   };
-  auto gather = [&](float least_l) {  // all from a number on, and perhaps more than there is room for
+  // Lists what is at least least_l and passes a test.
+  auto pick = [&](float least_l, auto&& test) {
     each4([&](int i, const float (&l)[4]) {
       if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= least_l) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (l[j] >= least_l) put(place_of(l[j], i + j));
+          if (l[j] >= least_l && test(i + j, l[j])) put(place_of(l[j], i + j));
       }
     });
   };
   // The first block's list, sorted, a thread's tokens in v.
   u64 v[kEach];
   const int v0 = threadIdx.x * kEach;
-  int listed = 0, all = kEach;
+  int listed = 0;
   auto take_list = [&] {
     listed = min((int)s.listed, kList);
-    while (all < listed) all <<= 1;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) v[e] = v0 + e < listed ? s.list[v0 + e] : 0;
     __syncthreads();
-    sort_list(v, s.list, all);
+    order_list(s, v, listed);
   };
   // weights of v (by_index: the value is in the low half) and their running sums
   u64 weight[kEach], upto[kEach];
@@ -512,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     // the rest, in the order of the row
 #pragma unroll
     for (int e = 0; e < kEach; ++e) v[e] = v0 + e < keep && weight[e] >= least ? v[e] << 32 | v[e] >> 32 : 0;
-    sort_list(v, s.list, all);
+    order_list(s, v, listed);
     const u64 sum = sum_list(true), share = share_of(coin, sum);
 #pragma unroll
     for (int e = 0; e < kEach; ++e)
@@ -530,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     cluster_sync_all();
     const Order o = *told;
     if (o.what == Order::kGather) {
-      gather(w.floor_of_bins(o.bin));
+      pick(w.floor_of_bins(o.bin), [](int, float) { return true; });  // (and perhaps more than there is room for)
       cluster_sync_all();
       const unsigned got = *dsmem_ptr(&s.listed, 0);
       if (got <= kList) {
@@ -541,102 +634,72 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
       }
     }
   }
-  u64 limit = 0;  // places from here on are kept
-  auto in_limit = [&](int i, float l) { return !limit || place_of(l, i) >= limit; };
+  u64 limit = 0;  // places from here on are kept: larger values, and of this one the indices up to limit_i
+  float limit_l = 0.f;
+  int limit_i = 0;
+  auto in_limit = [&](int i, float l) { return l > limit_l || (l == limit_l && i <= limit_i); };
   for (int kind = by_k ? 0 : 1; kind < (by_p ? 2 : 1); ++kind) {  // top-k, then (if that did not see to it) top-p
     const bool by_rank = kind == 0;
     clear_bins(s, !by_rank);
     __syncthreads();
-    each4([&](int i, const float (&l)[4]) {
-      u64 v[4] = {0, 0, 0, 0};
-      if (!by_rank) {
+    if (by_rank) {
+      each([&](int, float l) {
+        if (w.some(l)) atomicAdd(&s.count[w.bin(l)], 1u);
+      });
+    } else {
+      each4([&](int i, const float (&l)[4]) {
+        bool in[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = w.of(l[j]);
-      }
+        for (int j = 0; j < 4; ++j) in[j] = limit ? in_limit(i + j, l[j]) : w.some(l[j]);
+        if (!__any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3])) return;
+        double v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (w.some(l[j]) && in_limit(i + j, l[j])) {
-          const int b = w.bin(l[j]);
-          atomicAdd(&s.count[b], 1u);
-          if (v[j]) add_to_bin(s, b, v[j]);
-        }
-    });
+        for (int j = 0; j < 4; ++j) v[j] = w.above(l[j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (in[j]) add_to_bin(s, w.bin(l[j]), v[j]);
+      });
+    }
     cluster_sync_all();
     if (rank == 0) find(by_rank, Pair{0, 0}, 0, 0, 0, 0, 0);
     cluster_sync_all();
     Order o = *told;
     if (o.what == Order::kNone) continue;  // no more than k tokens have a weight
     if (o.what == Order::kGather) {
-      each([&](int i, float l) {
-        if (w.some(l) && w.bin(l) <= o.bin && in_limit(i, l)) put(place_of(l, i));
-      });
+      pick(w.floor_of_bins(o.bin), [&](int i, float l) { return w.bin(l) <= o.bin && (!limit || in_limit(i, l)); });
       cluster_sync_all();
       if (rank) return;
       finish(by_rank, o.of);
       return;
     }
-    // ---- the limit's own place, among too many: the ends of the bin's places first
-    u64 lo = ~0ull, hi = 0;
-    each([&](int i, float l) {
-      if (w.some(l) && w.bin(l) == o.bin && in_limit(i, l)) {
-        const u64 at = place_of(l, i);
-        lo = at < lo ? at : lo;
-        hi = at > hi ? at : hi;
-      }
-    });
-    auto ends = [](u64& lo, u64& hi) {  // of a warp's lanes
-      for (int d = 16; d; d >>= 1) {
-        const u64 l = __shfl_xor_sync(0xffffffffu, lo, d), h = __shfl_xor_sync(0xffffffffu, hi, d);
-        lo = l < lo ? l : lo;
-        hi = h > hi ? h : hi;
-      }
-    };
-    ends(lo, hi);
-    if (lane == 0) {
-      s.lo[warp] = lo;
-      s.hi[warp] = hi;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int k = 1; k < kWarps; ++k) {
-        lo = s.lo[k] < lo ? s.lo[k] : lo;
-        hi = s.hi[k] > hi ? s.hi[k] : hi;
-      }
-      s.block_lo = lo;
-      s.block_hi = hi;
-    }
-    cluster_sync_all();
-    lo = lane < blocks ? *dsmem_ptr(&s.block_lo, lane) : ~0ull;
-    hi = lane < blocks ? *dsmem_ptr(&s.block_hi, lane) : 0;
-    ends(lo, hi);
-    o.lo = lo;
-    o.hi = hi;
+    // ---- the limit's own place, among too many: a range of values that holds the bin's, whatever index they have
+    const int only = o.bin;  // of the first histogram, whose bins these tokens are in
+    const float floor_l = w.floor_of_bins(only);
+    o.lo = (u64)key_of(floor_l) << 32;
+    o.hi = (u64)key_of(only ? w.ceiling_of_bin(only) : w.maxf) << 32 | 0xffffffffu;
+    auto in_range = [&](float l, u64 at) { return w.bin(l) == only && at >= o.lo && at <= o.hi; };
     while (o.in > kList) {  // each round leaves one of kBins parts of a range that has at most 2^64 places
       const u64 width = (o.hi - o.lo) / kBins + 1;
       clear_bins(s, !by_rank);
       __syncthreads();
       each([&](int i, float l) {
-        const u64 at = w.some(l) ? place_of(l, i) : 0;
-        const bool in = at >= o.lo && at <= o.hi;
-        const u64 v = !by_rank && __any_sync(0xffffffffu, in) ? w.of(l) : 0;
-        if (in) {
-          const int b = (int)((o.hi - at) / width);
-          atomicAdd(&s.count[b], 1u);
-          if (!by_rank && v) add_to_bin(s, b, v);
-        }
+        const u64 at = l >= floor_l ? place_of(l, i) : 0;
+        const bool in = l >= floor_l && (!limit || in_limit(i, l)) && in_range(l, at);
+        if (!__any_sync(0xffffffffu, in)) return;
+        const double v = by_rank ? 0.0 : w.above(l);
+        if (!in) return;
+        const int b = (int)((o.hi - at) / width);
+        if (by_rank) atomicAdd(&s.count[b], 1u);
+        else add_to_bin(s, b, v);
       });
       cluster_sync_all();
       if (rank == 0) find(by_rank, o.before, o.goal, o.of, o.lo, o.hi, width);
       cluster_sync_all();
       o = *told;
     }
-    each([&](int i, float l) {
-      const u64 at = w.some(l) ? place_of(l, i) : 0;
-      if (at >= o.lo && at <= o.hi) put(at);
-    });
+    pick(floor_l, [&](int i, float l) { return (!limit || in_limit(i, l)) && in_range(l, place_of(l, i)); });
     cluster_sync_all();
     if (rank == 0) {
-      all = kEach;
       take_list();
       const u64 share = o.goal - o.before.sum;
       if (!by_rank) sum_list(false);
@@ -646,6 +709,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     }
     cluster_sync_all();
     limit = *dsmem_ptr(&s.told, 0);
+    limit_l = value_of((unsigned)(limit >> 32));
+    limit_i = (int)~(unsigned)limit;
   }
   // ---- the draw, in the order of the row
   // Sums of a thread's weights, up to 2^20 / 8 / 512 of them, are whole numbers of 64-bit floating point.
@@ -656,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     bool in[4] = {true, true, true, true};
     if (limit) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) in[j] = w.some(l[j]) && place_of(l[j], i + j) >= limit;
+      for (int j = 0; j < 4; ++j) in[j] = in_limit(i + j, l[j]);
       if (!__any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3])) return;
     }
 #pragma unroll
@@ -737,13 +802,25 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
 }
 
 template <typename T>
-cudaError_t launch(const SampleRowsArgs& a, int device, cudaStream_t s) {
-  // blocks a row: enough that a stretch fits shared memory, and that a short row's passes are short
-  int blocks = 1;
-  while (blocks < kMaxCluster && a.vocab > 4096 * blocks) blocks *= 2;
-  int stretch = ((a.vocab + blocks - 1) / blocks + 31) / 32 * 32;
+cudaError_t launch(const SampleRowsArgs& a, int device, int n_sms, cudaStream_t s) {
+  // Blocks a row, the cheapest of 1 to 8 by what was measured (in us): a wave of blocks takes 3.2 (4.2 and 5.2 in clusters
+  // of 4 and 8) and 0.39 for each 1000 logits that an SM's blocks have, 0.5 if there is one alone, 1.15 times as much for
+  // rows that shared memory does not take.  61 rows of 49999: 16 us with 4 blocks a row, 23 with 8; 64 rows of 131072 in
+  // 16 bits: 28 and 34; 256 rows of 32000: 28 with one, 68 with 8.
+  int blocks = 1, stretch = 0;
+  bool staged = false;
+  float best = FLT_MAX;
+  for (int c = 1; c <= kMaxCluster; c *= 2) {
+    if (c > 1 && a.vocab < 2048 * c) break;
+    const int st = ((a.vocab + c - 1) / c + 31) / 32 * 32;
+    const size_t bytes = (size_t)st * sizeof(T) + 32;
+    const bool in = bytes <= kMaxStage;
+    const int per_sm = in && bytes > kMaxStage / 2 ? 1 : 2, waves = (int)(((long long)a.rows * c + n_sms * per_sm - 1) / (n_sms * per_sm));
+    const bool alone = per_sm == 1 || (long long)a.rows * c <= n_sms;
+    const float t = waves * ((c < 4 ? 3.2f : c < 8 ? 4.2f : 5.2f) + st * (alone ? 0.5e-3f : 0.78e-3f) * (in ? 1.f : 1.15f));
+    if (t < best) best = t, blocks = c, stretch = st, staged = in;
+  }
   const size_t bytes = (size_t)stretch * sizeof(T) + 32;
-  const bool staged = bytes <= kMaxStage;
   const void* fn = staged ? reinterpret_cast<const void*>(&sample_rows_kernel<T, true>)
                           : reinterpret_cast<const void*>(&sample_rows_kernel<T, false>);
   static SmemCap cap;
@@ -756,10 +833,10 @@ cudaError_t launch(const SampleRowsArgs& a, int device, cudaStream_t s) {
 
 }  // namespace
 
-cudaError_t sample_rows(const SampleRowsArgs& a, int type, int device, cudaStream_t s) {
-  if (type == 0) return launch<float>(a, device, s);
-  if (type == 1) return launch<__half>(a, device, s);
-  return launch<__nv_bfloat16>(a, device, s);
+cudaError_t sample_rows(const SampleRowsArgs& a, int type, int device, int n_sms, cudaStream_t s) {
+  if (type == 0) return launch<float>(a, device, n_sms, s);
+  if (type == 1) return launch<__half>(a, device, n_sms, s);
+  return launch<__nv_bfloat16>(a, device, n_sms, s);
 }
 
 }  // namespace yb

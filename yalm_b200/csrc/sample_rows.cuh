@@ -20,6 +20,6 @@ struct SampleRowsArgs {
   const float* min_p;
 };
 // type: of the logits, 0 fp32, 1 fp16, 2 bf16
-cudaError_t sample_rows(const SampleRowsArgs& a, int type, int device, cudaStream_t s);
+cudaError_t sample_rows(const SampleRowsArgs& a, int type, int device, int n_sms, cudaStream_t s);
 
 }  // namespace yb
