@@ -12,10 +12,12 @@
 // that are read again, from L2); every later pass reads that.  The limits are found on a histogram of the distance
 // to the maximum, 16 bins an octave of the weight, whose bins are stretches of the sorted order: of counts for top-k,
 // which needs no weights, of counts and sums for top-p alone.  The cluster's first block merges the blocks' bins.
-// Where the limit's bin and all before it hold at most kList tokens, as a usual top-k or top-p has, they are gathered
-// in the first block, sorted, and the rest happens there.  Else the limit's place is narrowed down by histograms of
-// the range (value, then place in the row, as one 64-bit number) until at most kList tokens are in it, and the draw
-// is one more pass over the row in its order.
+// Where the limit's bin and all before it hold at most kList tokens, as a usual top-k or top-p has, they are listed in
+// the first block, and the rest happens there: by comparing each with each where they are few, else by histograms of
+// the list's own range, which a round or three narrow down to one token.  (Sorting the list took 2.5 us for 64 tokens and
+// 8 to 13 us for 2048, twice.)  Else the limit's place is narrowed down by histograms of the range (value, then place
+// in the row, as one 64-bit number) until at most kList tokens are in it, and the draw is one more pass over the row in
+// its order.
 #include "sample_rows.cuh"
 
 #include <cuda_bf16.h>
@@ -37,6 +39,8 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kOctaves = 44, kPerOctave = 16, kBins = kOctaves * kPerOctave;
 constexpr int kEach = 4, kList = kThreads * kEach;  // tokens of a list: 4 a thread
 constexpr int kBinsPer = (kBins + kThreads - 1) / kThreads;
+constexpr int kShortList = 128;
+constexpr int kRounds = 8;  // kBins^7 is more than 2^64, the places that a range may have
 constexpr u64 kOne = 1ull << 43;                    // the largest weight
 constexpr float kLeastTemperature = 0x1p-60f, kMostTemperature = 0x1p90f;
 constexpr size_t kMaxStage = 160 * 1024;            // bytes of a row's stretch that shared memory takes
@@ -99,10 +103,14 @@ struct Weights {
   __device__ __forceinline__ float floor_of_bins(int b) const {
     return b == kBins - 1 ? cut : fmaxf(cut, __double2float_rd(max - (b + 1) * (double)(1.f + 0x1p-20f) / per_bin));
   }
-  __device__ __forceinline__ void init(float m, float temp) {
+  double of_t;  // log2(e) / T before the maximum is known
+  __device__ __forceinline__ void prepare(float temp) {
+    root = exp2((threadIdx.x & 31) * (1.0 / 32) + 43.0);
+    of_t = 1.4426950408889634 / (double)fminf(fmaxf(temp, kLeastTemperature), kMostTemperature);
+  }
+  __device__ __forceinline__ void init(float m) {
     maxf = m;
     max = widen(m);  // (2^128 for infinity)
-    root = exp2((threadIdx.x & 31) * (1.0 / 32) + 43.0);
     if (m == INFINITY) {  // the infinite ones weigh the same, the largest finite number 2^-50 of it
       c = 50.0 * 0x1p-104;
       cut = m;
@@ -114,9 +122,10 @@ struct Weights {
     // small enough for the exponents below.  (At |m| >= 2^127 that is so at every temperature; -infinity counts as -2^128.)
     const unsigned u = __float_as_uint(m);
     const double gap = max - widen(__uint_as_float(m > 0.f ? u - 1 : m < 0.f ? u + 1 : 0x80000001u));
-    c = fmin(1.4426950408889634 / (double)fminf(fmaxf(temp, kLeastTemperature), kMostTemperature), 50.0 / gap);
-    cut = fmaxf((float)(max - kOctaves / c), -FLT_MAX);
-    none = __double2float_rd(max - (kOctaves + 2) / c);
+    c = fmin(of_t, (double)__fdividef(50.f, (float)gap));
+    const double octave = (double)__frcp_rn((float)c);
+    cut = fmaxf((float)(max - kOctaves * octave), -FLT_MAX);
+    none = __double2float_rd(max - (kOctaves + 2) * octave);
     per_bin = (float)(c * kPerOctave);
   }
   __device__ __forceinline__ bool some(float l) const { return l >= cut; }
@@ -194,6 +203,8 @@ struct Shared {
   Pair warps[kWarps];
   u64 sums[kWarps], lo[kWarps], hi[kWarps];
   u64 block_sum, told;
+  Pair found_before;
+  unsigned mine;  // tokens that the block has listed for the first one
   float max[kWarps], block_max;
   int block_first;  // index of the block's first maximum
   unsigned listed;
@@ -214,18 +225,6 @@ __device__ __forceinline__ Pair block_scan(Shared& s, Pair v, Pair* total) {
   __syncthreads();
   return warp ? at + v : v;
 }
-__device__ __forceinline__ u64 block_scan(Shared& s, u64 v, u64* total) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  v = warp_scan(v);
-  if (lane == 31) s.sums[warp] = v;
-  __syncthreads();
-  const u64 w = warp_scan(lane < kWarps ? s.sums[lane] : 0);
-  const u64 at = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
-  *total = __shfl_sync(0xffffffffu, w, kWarps - 1);
-  __syncthreads();
-  return warp ? at + v : v;
-}
-
 __device__ __forceinline__ void clear_bins(Shared& s, bool sums) {
   for (int i = threadIdx.x; i < kBins; i += kThreads) {
     s.count[i] = 0;
@@ -240,137 +239,95 @@ __device__ __forceinline__ void add_to_bin(Shared& s, int b, double above) {  //
   if (hi) atomicAdd(&s.high[b], hi);
 }
 
-// A list, 4 neighbouring tokens a thread, sorted descending; `all` is a power of two from 4 on, and what lies behind the
-// list's end is 0.  Steps of up to 64 places stay in a warp.
-__device__ __forceinline__ void sort_list(u64 (&v)[kEach], u64* buf, int all) {
-  const int i0 = threadIdx.x * kEach;
-  const bool in = (threadIdx.x & ~31) * kEach < all;  // the warp has a part in it
-  for (int size = 2; size <= all; size <<= 1)
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      if (step >= 32 * kEach) {
-        if (in) {
-#pragma unroll
-          for (int e = 0; e < kEach; ++e) buf[e * kThreads + threadIdx.x] = v[e];
-        }
-        __syncthreads();
-        if (in) {
-          const bool most = !(i0 & step) == !(i0 & size);
-#pragma unroll
-          for (int e = 0; e < kEach; ++e) {
-            const u64 o = buf[e * kThreads + (threadIdx.x ^ (step / kEach))];
-            if ((o > v[e]) == most) v[e] = o;
-          }
-        }
-        __syncthreads();
-      } else if (in && step >= kEach) {
-        const bool most = !(i0 & step) == !(i0 & size);
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          const u64 o = __shfl_xor_sync(0xffffffffu, v[e], step / kEach);
-          if ((o > v[e]) == most) v[e] = o;
-        }
-      } else if (in) {
-        auto order = [&](u64& a, u64& b, bool down) {
-          const u64 x = a, y = b;
-          if ((x < y) == down) a = y, b = x;
-        };
-        const bool down = !(i0 & size);
-        if (step == 2) {
-          order(v[0], v[2], down);
-          order(v[1], v[3], down);
-        } else {
-          order(v[0], v[1], down);
-          order(v[2], v[3], size == 2 ? !down : down);
-        }
-      }
-    }
+__device__ __forceinline__ void add_to_bin(Shared& s, int b, u64 w) {
+  atomicAdd(&s.low[b], (unsigned)w & 0x7fffu);
+  atomicAdd(&s.mid[b], (unsigned)(w >> 15) & 0x7fffu);
+  if (w >> 30) atomicAdd(&s.high[b], (unsigned)(w >> 30));
 }
-
-// The same for n tokens (0 behind them), by way of bins of the list's own range: a token's place is the number of those in
-// bins before its own, and of larger ones in it.  Short lists, and those with many tokens in a bin, are sorted as above.
-constexpr int kShortList = 64, kFullBin = 48;
-__device__ __forceinline__ void order_list(Shared& s, u64 (&v)[kEach], int n) {
-  int all = kShortList;
-  while (all < n) all <<= 1;
-  if (n <= kShortList) {
-    sort_list(v, s.list, all);
-    return;
-  }
-  const int v0 = threadIdx.x * kEach, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  u64 lo = ~0ull, hi = 0;
+__device__ __forceinline__ u64 block_sum(Shared& s, u64 v) {
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  if ((threadIdx.x & 31) == 0) s.sums[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = s.sums[threadIdx.x & (kWarps - 1)];
+  for (int d = kWarps / 2; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  __syncthreads();
+  return v;
+}
+// Of a list of different numbers, 4 a thread (0: none), the one at which, from the largest down, `rank` (by_rank) or the
+// sum `goal` of their weights is reached.  Each round leaves one of kBins parts of the range that is still in question.
+__device__ __forceinline__ u64 select(Shared& s, u64 (&v)[kEach], const u64 (&weight)[kEach], bool by_rank, unsigned rank, u64 goal) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b0 = threadIdx.x * kBinsPer;
+  for (int round = 0;; ++round) {
+    u64 lo = ~0ull, hi = 0;
 #pragma unroll
-  for (int e = 0; e < kEach; ++e)
-    if (v[e]) {
-      lo = v[e] < lo ? v[e] : lo;
-      hi = v[e] > hi ? v[e] : hi;
+    for (int e = 0; e < kEach; ++e)
+      if (v[e]) {
+        lo = v[e] < lo ? v[e] : lo;
+        hi = v[e] > hi ? v[e] : hi;
+      }
+    auto ends = [&](int d) {
+      for (; d; d >>= 1) {
+        const u64 l = __shfl_xor_sync(0xffffffffu, lo, d), h = __shfl_xor_sync(0xffffffffu, hi, d);
+        lo = l < lo ? l : lo;
+        hi = h > hi ? h : hi;
+      }
+    };
+    ends(16);
+    if (lane == 0) {
+      s.lo[warp] = lo;
+      s.hi[warp] = hi;
     }
-  for (int d = 16; d; d >>= 1) {
-    const u64 l = __shfl_xor_sync(0xffffffffu, lo, d), h = __shfl_xor_sync(0xffffffffu, hi, d);
-    lo = l < lo ? l : lo;
-    hi = h > hi ? h : hi;
-  }
-  if (lane == 0) {
-    s.lo[warp] = lo;
-    s.hi[warp] = hi;
-  }
-  for (int i = threadIdx.x; i < kBins; i += kThreads) s.count[i] = 0;
-  __syncthreads();
-  lo = s.lo[lane % kWarps];
-  hi = s.hi[lane % kWarps];
-  for (int d = kWarps / 2; d; d >>= 1) {
-    const u64 l = __shfl_xor_sync(0xffffffffu, lo, d), h = __shfl_xor_sync(0xffffffffu, hi, d);
-    lo = l < lo ? l : lo;
-    hi = h > hi ? h : hi;
-  }
-  const float per = (float)kBins / ((float)(hi - lo) + 1.f);  // (roundings keep the order)
-  int bin[kEach];
-  unsigned slot[kEach];
+    clear_bins(s, !by_rank);
+    if (threadIdx.x == 0) s.found = -1;  // (a goal beyond the sum would end with none)
+    __syncthreads();
+    lo = s.lo[lane % kWarps];
+    hi = s.hi[lane % kWarps];
+    ends(kWarps / 2);
+    if (lo >= hi || round == kRounds) {
+      __syncthreads();
+      return hi;
+    }
+    const float per = (float)kBins / ((float)(hi - lo) + 1.f);  // (roundings keep the order)
+    int bin[kEach];
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    bin[e] = min((int)((float)(hi - v[e]) * per), kBins - 1);
-    if (v[e]) slot[e] = atomicAdd(&s.count[bin[e]], 1u);
+    for (int e = 0; e < kEach; ++e) {
+      bin[e] = min((int)((float)(hi - v[e]) * per), kBins - 1);
+      if (!v[e]) continue;
+      if (by_rank) atomicAdd(&s.count[bin[e]], 1u);
+      else add_to_bin(s, bin[e], weight[e]);
+    }
+    __syncthreads();
+    Pair part[kBinsPer], mine{0, 0}, total;
+#pragma unroll
+    for (int k = 0; k < kBinsPer; ++k) {
+      const int b = b0 + k;
+      part[k] = Pair{0, 0};
+      if (b < kBins) {
+        if (by_rank) part[k].n = s.count[b];
+        else part[k].sum = s.low[b] + ((u64)s.mid[b] << 15) + ((u64)s.high[b] << 30);
+      }
+      mine = mine + part[k];
+    }
+    Pair before = block_scan(s, mine, &total);
+    before = Pair{before.n - mine.n, before.sum - mine.sum};
+#pragma unroll
+    for (int k = 0; k < kBinsPer; ++k) {
+      const Pair after = before + part[k];
+      if (by_rank ? before.n < rank && rank <= after.n : before.sum < goal && goal <= after.sum) {
+        s.found = b0 + k;
+        s.found_before = before;
+      }
+      before = after;
+    }
+    __syncthreads();
+    const int found = s.found;
+    rank -= s.found_before.n;
+    goal -= s.found_before.sum;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      if (bin[e] != found) v[e] = 0;
+    __syncthreads();
   }
-  __syncthreads();
-  const int b0 = threadIdx.x * kBinsPer;
-  unsigned count[kBinsPer], mine = 0;
-  bool full = false;
-#pragma unroll
-  for (int k = 0; k < kBinsPer; ++k) {
-    count[k] = b0 + k < kBins ? s.count[b0 + k] : 0;
-    full |= count[k] > kFullBin;
-    mine += count[k];
-  }
-  u64 total;
-  unsigned before = (unsigned)block_scan(s, (u64)mine, &total) - mine;
-#pragma unroll
-  for (int k = 0; k < kBinsPer; ++k) {
-    if (b0 + k < kBins) s.low[b0 + k] = before;
-    before += count[k];
-  }
-  if (__syncthreads_or(full)) {
-    sort_list(v, s.list, all);
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < kEach; ++e)
-    if (v[e]) s.list[s.low[bin[e]] + slot[e]] = v[e];
-  __syncthreads();
-  unsigned place[kEach];
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    if (!v[e]) continue;
-    place[e] = s.low[bin[e]];
-    const unsigned from = place[e], to = from + s.count[bin[e]];
-    for (unsigned i = from; i < to; ++i) place[e] += s.list[i] > v[e];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int e = 0; e < kEach; ++e)
-    if (v[e]) s.list[place[e]] = v[e];
-  __syncthreads();
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) v[e] = v0 + e < (int)total ? s.list[v0 + e] : 0;
-  __syncthreads();
 }
 
 template <typename T, bool kStaged>
@@ -409,6 +366,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     return v;
   };
   Weights w;
+  w.prepare(temp);
   float own;  // the largest logit that this thread has read
   {
     float m = -INFINITY;
@@ -449,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     if (lane < blocks) m = fmaxf(m, *dsmem_ptr(&s.block_max, lane));
     for (int o = kMaxCluster / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     m = __shfl_sync(0xffffffffu, m, 0);
-    w.init(m, temp);
+    w.init(m);
   }
   auto answer = [&](int token, float prob) {
     a.tokens[r] = token;
@@ -494,20 +452,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
   };
   const Order* const told = dsmem_ptr(&s.order, 0);
   Shared* const first = const_cast<Shared*>(dsmem_ptr(&s, 0));
-  // The first block merges the bins of all, and tells where `rank` (if any) or else the sum `goal` is reached; bin j is
-  // places hi - (j + 1) width + 1 .. hi - j width of the range, or of the first histogram's (width 0).
-  auto find = [&](bool by_rank, Pair before, u64 goal, u64 of, u64 lo, u64 hi, u64 width) {
+  // Merges the bins of all blocks, and tells where `rank` (if any) or else the sum `goal` is reached; bin j is places
+  // hi - (j + 1) width + 1 .. hi - j width of the range, or of the first histogram's (width 0).  Counts the first block
+  // reads from all; of counts and sums, four words a bin, each block sums up a part and leaves it in the first one's list.
+  auto tell = [&](bool by_rank, Pair before, u64 goal, u64 of, u64 lo, u64 hi, u64 width) {
     Pair mine{0, 0}, bin[kBinsPer], total;
 #pragma unroll
     for (int k = 0; k < kBinsPer; ++k) {
       const int b = threadIdx.x * kBinsPer + k;
       bin[k] = Pair{0, 0};
+      if (!by_rank) {
+        if (b < kBins) bin[k] = Pair{(unsigned)s.list[kBins + b], s.list[b]};
+      } else {
 #pragma unroll
-      for (int c = 0; c < kMaxCluster; ++c) {  // all on their way at once
-        if (c >= blocks || b >= kBins) continue;
-        const Shared* o = dsmem_ptr(&s, c);
-        bin[k].n += o->count[b];
-        if (!by_rank) bin[k].sum += o->low[b] + ((u64)o->mid[b] << 15) + ((u64)o->high[b] << 30);
+        for (int c = 0; c < kMaxCluster; ++c)  // all on their way at once
+          if (c < blocks && b < kBins) bin[k].n += dsmem_ptr(&s, c)->count[b];
       }
       mine = mine + bin[k];
     }
@@ -519,6 +478,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     }
     if (threadIdx.x == 0) {
       s.order.what = Order::kNone;
+      s.order.in = 0;
       s.listed = 0;
     }
     __syncthreads();
@@ -542,75 +502,133 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
       before = after;
     }
   };
-  auto put = [&](u64 at) {  // (the counts leave room for all that come)
-    const unsigned to = atomicAdd(&first->listed, 1u);
-    if (to < kList) first->list[to] = at;
+  auto find = [&](bool by_rank, Pair before, u64 goal, u64 of, u64 lo, u64 hi, u64 width) {
+    cluster_sync_all();
+    if (!by_rank) {
+      const int per = (kBins + blocks - 1) / blocks, end = min(kBins, (rank + 1) * per);
+      for (int b = rank * per + threadIdx.x; b < end; b += kThreads) {
+        unsigned n = 0;
+        u64 sum = 0;
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c) {
+          if (c >= blocks) continue;
+          const Shared* o = dsmem_ptr(&s, c);
+          n += o->count[b];
+          sum += o->low[b] + ((u64)o->mid[b] << 15) + ((u64)o->high[b] << 30);
+        }
+        first->list[b] = sum;
+        first->list[kBins + b] = n;
+      }
+      cluster_sync_all();
+    }
+    if (rank == 0) tell(by_rank, before, goal, of, lo, hi, width);
+    cluster_sync_all();
   };
-  // Lists what is at least least_l and passes a test.
+  // Lists in the first block what is at least least_l and passes a test (the counts leave room for all, or s.listed tells):
+  // every block in its own list, which is then copied to a place behind those of others.
   auto pick = [&](float least_l, auto&& test) {
+    unsigned* const listed = rank ? &s.mine : &s.listed;
+    if (rank && threadIdx.x == 0) s.mine = 0;
+    __syncthreads();
     each4([&](int i, const float (&l)[4]) {
       if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= least_l) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (l[j] >= least_l && test(i + j, l[j])) put(place_of(l[j], i + j));
+          if (l[j] >= least_l && test(i + j, l[j])) {
+            const unsigned to = atomicAdd(listed, 1u);
+            if (to < kList) s.list[to] = place_of(l[j], i + j);
+          }
       }
     });
+    if (rank) {
+      __syncthreads();
+      if (threadIdx.x == 0) s.found = (int)atomicAdd(&first->listed, s.mine);
+      __syncthreads();
+      for (unsigned i = threadIdx.x; i < min(s.mine, (unsigned)kList); i += kThreads)
+        if (s.found + i < kList) first->list[s.found + i] = s.list[i];
+    }
+    cluster_sync_all();
   };
-  // The first block's list, sorted, a thread's tokens in v.
-  u64 v[kEach];
-  const int v0 = threadIdx.x * kEach;
+  // The first block's list, 4 tokens a thread, and their weights.
+  u64 v[kEach], weight[kEach];
   int listed = 0;
   auto take_list = [&] {
     listed = min((int)s.listed, kList);
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) v[e] = v0 + e < listed ? s.list[v0 + e] : 0;
-    __syncthreads();
-    order_list(s, v, listed);
-  };
-  // weights of v (by_index: the value is in the low half) and their running sums
-  u64 weight[kEach], upto[kEach];
-  auto sum_list = [&](bool by_index) {
-    u64 mine = 0, total;
-#pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      weight[e] = w.of(value_of(by_index ? (unsigned)v[e] : (unsigned)(v[e] >> 32)));
+      const int i = e * kThreads + threadIdx.x;
+      v[e] = i < listed ? s.list[i] : 0;
+      weight[e] = 0;
+      if (e * kThreads < listed) weight[e] = w.of(value_of((unsigned)(v[e] >> 32)));
       if (!v[e]) weight[e] = 0;
-      mine += weight[e];
-      upto[e] = mine;
     }
-    const u64 before = block_scan(s, mine, &total) - mine;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) upto[e] += before;
-    return total;
+    __syncthreads();
   };
   // The list holds the first tokens, at least those that are kept: by rank, or else by the share of the sum `of`.
   auto finish = [&](bool by_rank, u64 of) {
     take_list();
-    sum_list(false);
-    int keep = by_rank ? min(top_k, listed) : listed;
-    if (by_p) {
-      if (by_rank && (keep - 1) / kEach == threadIdx.x) {
-#pragma unroll
-        for (int e = 0; e < kEach; ++e)
-          if (v0 + e == keep - 1) s.told = upto[e];
+    if (listed <= kShortList) {  // each with each: the larger ones' number and sum, then the sum of those of a lower index
+      u64* const weights = reinterpret_cast<u64*>(s.low);
+      const int i = threadIdx.x;
+      if (i < listed) weights[i] = weight[0];
+      __syncthreads();
+      int larger = 0;
+      u64 before = 0, lower = 0, sum = 0;
+      if (i < listed)
+        for (int j = 0; j < listed; ++j) {
+          const bool more = s.list[j] > v[0];
+          larger += more;
+          before += more ? weights[j] : 0;
+        }
+      bool keep = i < listed && (!by_rank || larger < top_k);
+      if (by_p) {
+        const u64 all = by_rank ? block_sum(s, keep ? weight[0] : 0) : of;
+        keep = keep && before < share_of(top_p, all);
       }
+      keep = keep && weight[0] >= least && weight[0];
       __syncthreads();
-      const u64 share = share_of(top_p, by_rank ? s.told : of);
-#pragma unroll
-      for (int e = 0; e < kEach; ++e)
-        if (upto[e] >= share && upto[e] - weight[e] < share) s.found = v0 + e + 1;
+      if (i < listed) weights[i] = keep ? weight[0] : 0;
       __syncthreads();
-      keep = min(keep, s.found);
+      if (keep) {
+        for (int j = 0; j < listed; ++j) {
+          sum += weights[j];
+          lower += (unsigned)s.list[j] > (unsigned)v[0] ? weights[j] : 0;  // (indices are held inverted)
+        }
+        const u64 share = share_of(coin, sum);
+        if (lower < share && share <= lower + weight[0])
+          answer((int)~(unsigned)v[0], (float)((double)weight[0] / (double)sum));
+      }
+      return;
     }
-    // the rest, in the order of the row
+    u64 from = 0, x[kEach];
+    auto all_from = [&] {
+      u64 sum = 0;
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) v[e] = v0 + e < keep && weight[e] >= least ? v[e] << 32 | v[e] >> 32 : 0;
-    order_list(s, v, listed);
-    const u64 sum = sum_list(true), share = share_of(coin, sum);
+      for (int e = 0; e < kEach; ++e) {
+        x[e] = v[e] >= from ? v[e] : 0;
+        sum += x[e] ? weight[e] : 0;
+      }
+      return sum;
+    };
+    if (by_rank && top_k < listed) {
+      all_from();
+      from = select(s, x, weight, true, (unsigned)top_k, 0);
+    }
+    if (by_p) {
+      u64 sum = all_from();
+      if (by_rank) of = block_sum(s, sum);
+      from = select(s, x, weight, false, 0, share_of(top_p, of));
+    }
+    u64 mine = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {  // in the order of the row
+      x[e] = v[e] && v[e] >= from && weight[e] >= least && weight[e] ? v[e] << 32 | v[e] >> 32 : 0;
+      mine += x[e] ? weight[e] : 0;
+    }
+    const u64 sum = block_sum(s, mine), at = select(s, x, weight, false, 0, share_of(coin, sum));
 #pragma unroll
     for (int e = 0; e < kEach; ++e)
-      if (upto[e] >= share && upto[e] - weight[e] < share)
-        answer((int)~(unsigned)(v[e] >> 32), (float)((double)weight[e] / (double)sum));
+      if (v[e] && (v[e] << 32 | v[e] >> 32) == at) answer((int)~(unsigned)v[e], (float)((double)weight[e] / (double)sum));
   };
   if (by_k) {
     // The k-th largest of the threads' maxima is no larger than the k-th largest logit, and few tokens lie between the
@@ -618,13 +636,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     clear_bins(s, false);
     __syncthreads();
     if (w.some(own)) atomicAdd(&s.count[w.bin(own)], 1u);
-    cluster_sync_all();
-    if (rank == 0) find(true, Pair{0, 0}, 0, 0, 0, 0, 0);
-    cluster_sync_all();
+    find(true, Pair{0, 0}, 0, 0, 0, 0, 0);
     const Order o = *told;
     if (o.what == Order::kGather) {
-      pick(w.floor_of_bins(o.bin), [](int, float) { return true; });  // (and perhaps more than there is room for)
-      cluster_sync_all();
+      pick(w.floor_of_bins(o.bin), [](int, float) { return true; });  // (perhaps more than there is room for)
       const unsigned got = *dsmem_ptr(&s.listed, 0);
       if (got <= kList) {
         cluster_arrive();
@@ -660,14 +675,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
           if (in[j]) add_to_bin(s, w.bin(l[j]), v[j]);
       });
     }
-    cluster_sync_all();
-    if (rank == 0) find(by_rank, Pair{0, 0}, 0, 0, 0, 0, 0);
-    cluster_sync_all();
+    find(by_rank, Pair{0, 0}, 0, 0, 0, 0, 0);
     Order o = *told;
     if (o.what == Order::kNone) continue;  // no more than k tokens have a weight
     if (o.what == Order::kGather) {
       pick(w.floor_of_bins(o.bin), [&](int i, float l) { return w.bin(l) <= o.bin && (!limit || in_limit(i, l)); });
-      cluster_sync_all();
       if (rank) return;
       finish(by_rank, o.of);
       return;
@@ -678,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     o.lo = (u64)key_of(floor_l) << 32;
     o.hi = (u64)key_of(only ? w.ceiling_of_bin(only) : w.maxf) << 32 | 0xffffffffu;
     auto in_range = [&](float l, u64 at) { return w.bin(l) == only && at >= o.lo && at <= o.hi; };
-    while (o.in > kList) {  // each round leaves one of kBins parts of a range that has at most 2^64 places
+    for (int round = 0; o.in > kList && round < kRounds; ++round) {  // each leaves one of kBins parts of the range
       const u64 width = (o.hi - o.lo) / kBins + 1;
       clear_bins(s, !by_rank);
       __syncthreads();
@@ -692,20 +704,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
         if (by_rank) atomicAdd(&s.count[b], 1u);
         else add_to_bin(s, b, v);
       });
-      cluster_sync_all();
-      if (rank == 0) find(by_rank, o.before, o.goal, o.of, o.lo, o.hi, width);
-      cluster_sync_all();
+      find(by_rank, o.before, o.goal, o.of, o.lo, o.hi, width);
       o = *told;
     }
     pick(floor_l, [&](int i, float l) { return (!limit || in_limit(i, l)) && in_range(l, place_of(l, i)); });
-    cluster_sync_all();
     if (rank == 0) {
       take_list();
-      const u64 share = o.goal - o.before.sum;
-      if (!by_rank) sum_list(false);
-#pragma unroll
-      for (int e = 0; e < kEach; ++e)
-        if (by_rank ? v0 + e == top_k - (int)o.before.n - 1 : upto[e] >= share && upto[e] - weight[e] < share) s.told = v[e];
+      const u64 at = select(s, v, weight, by_rank, (unsigned)top_k - o.before.n, o.goal - o.before.sum);
+      if (threadIdx.x == 0) s.told = at;
     }
     cluster_sync_all();
     limit = *dsmem_ptr(&s.told, 0);
