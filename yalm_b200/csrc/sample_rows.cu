@@ -210,6 +210,7 @@ struct Shared {
   unsigned listed;
   int found;
   Order order;
+  __device__ __forceinline__ u64* of_list() { return reinterpret_cast<u64*>(low); }  // weights of a short list
 };
 
 // Inclusive scans over the block of a value a thread; every thread is to call them.
@@ -254,7 +255,8 @@ __device__ __forceinline__ u64 block_sum(Shared& s, u64 v) {
   return v;
 }
 // Of a list of different numbers, 4 a thread (0: none), the one at which, from the largest down, `rank` (by_rank) or the
-// sum `goal` of their weights is reached.  Each round leaves one of kBins parts of the range that is still in question.
+// sum `goal` of their weights is reached.  Each round leaves one of kBins parts of the range that is still in question,
+// until few are left (they take the place of what is in s.list), which are compared each with each.
 __device__ __forceinline__ u64 select(Shared& s, u64 (&v)[kEach], const u64 (&weight)[kEach], bool by_rank, unsigned rank, u64 goal) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b0 = threadIdx.x * kBinsPer;
   for (int round = 0;; ++round) {
@@ -278,7 +280,11 @@ __device__ __forceinline__ u64 select(Shared& s, u64 (&v)[kEach], const u64 (&we
       s.hi[warp] = hi;
     }
     clear_bins(s, !by_rank);
-    if (threadIdx.x == 0) s.found = -1;  // (a goal beyond the sum would end with none)
+    if (threadIdx.x == 0) {
+      s.found = -1;  // (a goal beyond the sum would end with none)
+      s.mine = 0;
+      s.told = 0;
+    }
     __syncthreads();
     lo = s.lo[lane % kWarps];
     hi = s.hi[lane % kWarps];
@@ -323,10 +329,36 @@ __device__ __forceinline__ u64 select(Shared& s, u64 (&v)[kEach], const u64 (&we
     const int found = s.found;
     rank -= s.found_before.n;
     goal -= s.found_before.sum;
+    u64* const weights = s.of_list();
 #pragma unroll
-    for (int e = 0; e < kEach; ++e)
+    for (int e = 0; e < kEach; ++e) {
       if (bin[e] != found) v[e] = 0;
+      if (!v[e]) continue;
+      const unsigned to = atomicAdd(&s.mine, 1u);
+      if (to < kShortList) {
+        s.list[to] = v[e];
+        weights[to] = weight[e];
+      }
+    }
     __syncthreads();
+    const int left = (int)s.mine;
+    if (left <= kShortList) {
+      if (threadIdx.x < left) {
+        const u64 own = s.list[threadIdx.x];
+        unsigned larger = 0;
+        u64 before = 0;
+        for (int j = 0; j < left; ++j) {
+          const bool more = s.list[j] > own;
+          larger += more;
+          before += more ? weights[j] : 0;
+        }
+        if (by_rank ? larger + 1 == rank : before < goal && goal <= before + weights[threadIdx.x]) s.told = own;
+      }
+      __syncthreads();
+      const u64 at = s.told;
+      __syncthreads();
+      return at;
+    }
   }
 }
 
@@ -425,8 +457,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
   }
   // A warp's part of the stretch; f is called by whole warps, with -infinity behind the end.
   const int part = (chunks + kWarps - 1) / kWarps, c0 = min(chunks, warp * part), c1 = min(chunks, c0 + part);
-  auto chunk_at = [&](int c) -> Chunk<T> {
-    if (c < c1) return kStaged ? Chunk<T>(stage[c]) : fetch(c, true);
+  auto chunk_at = [&](int c, int end) -> Chunk<T> {
+    if (c < end) return kStaged ? Chunk<T>(stage[c]) : fetch(c, true);
     Chunk<T> v;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) v.v[j] = minus_infinity<T>();
@@ -436,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
   // Four logits at a time, f(index of the first, logits).
   auto each4 = [&](auto&& f) {
     for (int b = c0; b < c1; b += 32) {
-      const Chunk<T> v = chunk_at(b + lane);
+      const Chunk<T> v = chunk_at(b + lane, c1);
 #pragma unroll
       for (int j = 0; j < kVec; j += 4) {
         const float l[4] = {v[j], v[j + 1], v[j + 2], v[j + 3]};
@@ -524,9 +556,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     if (rank == 0) tell(by_rank, before, goal, of, lo, hi, width);
     cluster_sync_all();
   };
-  // Lists in the first block what is at least least_l and passes a test (the counts leave room for all, or s.listed tells):
+  // Lists in the first block what is from least_l to most_l and passes a test (the counts leave room for all, or s.listed tells):
   // every block in its own list, which is then copied to a place behind those of others.
-  auto pick = [&](float least_l, auto&& test) {
+  auto pick = [&](float least_l, float most_l, auto&& test) {
     unsigned* const listed = rank ? &s.mine : &s.listed;
     if (rank && threadIdx.x == 0) s.mine = 0;
     __syncthreads();
@@ -534,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
       if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= least_l) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (l[j] >= least_l && test(i + j, l[j])) {
+          if (l[j] >= least_l && l[j] <= most_l && test(i + j, l[j])) {
             const unsigned to = atomicAdd(listed, 1u);
             if (to < kList) s.list[to] = place_of(l[j], i + j);
           }
@@ -568,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
   auto finish = [&](bool by_rank, u64 of) {
     take_list();
     if (listed <= kShortList) {  // each with each: the larger ones' number and sum, then the sum of those of a lower index
-      u64* const weights = reinterpret_cast<u64*>(s.low);
+      u64* const weights = s.of_list();
       const int i = threadIdx.x;
       if (i < listed) weights[i] = weight[0];
       __syncthreads();
@@ -639,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     find(true, Pair{0, 0}, 0, 0, 0, 0, 0);
     const Order o = *told;
     if (o.what == Order::kGather) {
-      pick(w.floor_of_bins(o.bin), [](int, float) { return true; });  // (perhaps more than there is room for)
+      pick(w.floor_of_bins(o.bin), INFINITY, [](int, float) { return true; });  // (perhaps more than there is room for)
       const unsigned got = *dsmem_ptr(&s.listed, 0);
       if (got <= kList) {
         cluster_arrive();
@@ -679,25 +711,25 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     Order o = *told;
     if (o.what == Order::kNone) continue;  // no more than k tokens have a weight
     if (o.what == Order::kGather) {
-      pick(w.floor_of_bins(o.bin), [&](int i, float l) { return w.bin(l) <= o.bin && (!limit || in_limit(i, l)); });
+      pick(w.floor_of_bins(o.bin), INFINITY, [&](int i, float l) { return w.bin(l) <= o.bin && (!limit || in_limit(i, l)); });
       if (rank) return;
       finish(by_rank, o.of);
       return;
     }
     // ---- the limit's own place, among too many: a range of values that holds the bin's, whatever index they have
     const int only = o.bin;  // of the first histogram, whose bins these tokens are in
-    const float floor_l = w.floor_of_bins(only);
+    const float floor_l = w.floor_of_bins(only), ceiling_l = only ? w.ceiling_of_bin(only) : w.maxf;
     o.lo = (u64)key_of(floor_l) << 32;
-    o.hi = (u64)key_of(only ? w.ceiling_of_bin(only) : w.maxf) << 32 | 0xffffffffu;
+    o.hi = (u64)key_of(ceiling_l) << 32 | 0xffffffffu;
     auto in_range = [&](float l, u64 at) { return w.bin(l) == only && at >= o.lo && at <= o.hi; };
     for (int round = 0; o.in > kList && round < kRounds; ++round) {  // each leaves one of kBins parts of the range
       const u64 width = (o.hi - o.lo) / kBins + 1;
       clear_bins(s, !by_rank);
       __syncthreads();
       each([&](int i, float l) {
+        if (!__any_sync(0xffffffffu, l >= floor_l && l <= ceiling_l)) return;
         const u64 at = l >= floor_l ? place_of(l, i) : 0;
         const bool in = l >= floor_l && (!limit || in_limit(i, l)) && in_range(l, at);
-        if (!__any_sync(0xffffffffu, in)) return;
         const double v = by_rank ? 0.0 : w.above(l);
         if (!in) return;
         const int b = (int)((o.hi - at) / width);
@@ -707,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
       find(by_rank, o.before, o.goal, o.of, o.lo, o.hi, width);
       o = *told;
     }
-    pick(floor_l, [&](int i, float l) { return (!limit || in_limit(i, l)) && in_range(l, place_of(l, i)); });
+    pick(floor_l, ceiling_l, [&](int i, float l) { return (!limit || in_limit(i, l)) && in_range(l, place_of(l, i)); });
     if (rank == 0) {
       take_list();
       const u64 at = select(s, v, weight, by_rank, (unsigned)top_k - o.before.n, o.goal - o.before.sum);
@@ -758,24 +790,28 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
   for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
   if (lane == 0) s.lo[warp] = mine;
   __syncthreads();
-  u64 before = 0, sum = 0;
+  u64 sum = 0;
 #pragma unroll
-  for (int k = 0; k < kWarps; ++k) {
-    if (k == warp) before = sum;
-    sum += s.lo[k];
-  }
+  for (int k = 0; k < kWarps; ++k) sum += s.lo[k];
   if (threadIdx.x == 0) s.block_sum = sum;
   cluster_sync_all();
+  u64 before, all;  // of the blocks before this one, of the row
   {
     const u64 here = lane < blocks ? *dsmem_ptr(&s.block_sum, lane) : 0, upto = warp_scan(here);
-    before += __shfl_sync(0xffffffffu, upto - here, rank);
-    sum = __shfl_sync(0xffffffffu, upto, 31);
+    before = __shfl_sync(0xffffffffu, upto - here, rank);
+    all = __shfl_sync(0xffffffffu, upto, 31);
   }
-  const u64 share = share_of(coin, sum);
-  if (before < share && share <= before + mine) {
-    for (int b = c0; b < c1; b += 32) {
-      const Chunk<T> x = chunk_at(b + lane);
-      u64 v[kVec], here = 0;
+  const u64 share = share_of(coin, all);
+  if (before < share && share <= before + sum) {  // the token is in this block
+    int owner = 0;
+    while (share > before + s.lo[owner]) before += s.lo[owner++];
+    // all warps look after a sixteenth each of that warp's part
+    const int o0 = min(chunks, owner * part), o1 = min(chunks, o0 + part), sub = (o1 - o0 + kWarps - 1) / kWarps;
+    const int s0 = min(o1, o0 + warp * sub), s1 = min(o1, s0 + sub);
+    u64 v[kVec], here = 0;
+    auto weights_at = [&](int b) {
+      const Chunk<T> x = chunk_at(b + lane, s1);
+      here = 0;
 #pragma unroll
       for (int j = 0; j < kVec; j += 4) {
         const float l[4] = {x[j], x[j + 1], x[j + 2], x[j + 3]};
@@ -784,25 +820,38 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
 #pragma unroll
         for (int k = 0; k < 4; ++k) here += v[j + k] = __double2ull_rn(f[k]);
       }
-      u64 upto = before + warp_scan(here);
-      const unsigned there = __ballot_sync(0xffffffffu, upto >= share);
-      if (there) {
-        if (lane == __ffs(there) - 1) {
-          upto -= here;
-          bool done = false;
+    };
+    mine = 0;
+    for (int b = s0; b < s1; b += 32) {
+      weights_at(b);
+      mine += here;
+    }
+    for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+    if (lane == 0) s.hi[warp] = mine;
+    __syncthreads();
+    for (int k = 0; k < warp; ++k) before += s.hi[k];
+    if (before < share && share <= before + mine)
+      for (int b = s0; b < s1; b += 32) {
+        weights_at(b);
+        u64 upto = before + warp_scan(here);
+        const unsigned there = __ballot_sync(0xffffffffu, upto >= share);
+        if (there) {
+          if (lane == __ffs(there) - 1) {
+            upto -= here;
+            bool done = false;
 #pragma unroll
-          for (int j = 0; j < kVec; ++j) {
-            upto += v[j];
-            if (!done && upto >= share) {
-              done = true;
-              answer(index_of(b + lane, j), (float)((double)v[j] / (double)sum));
+            for (int j = 0; j < kVec; ++j) {
+              upto += v[j];
+              if (!done && upto >= share) {
+                done = true;
+                answer(index_of(b + lane, j), (float)((double)v[j] / (double)all));
+              }
             }
           }
+          break;
         }
-        break;
+        before = __shfl_sync(0xffffffffu, upto, 31);
       }
-      before = __shfl_sync(0xffffffffu, upto, 31);
-    }
   }
   cluster_sync_all();
 }
