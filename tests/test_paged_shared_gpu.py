@@ -7,7 +7,7 @@ import random
 import pytest
 
 from test_paged_gpu import Step, _types
-from yalm_b200 import YalmB200Error
+from yalm_b200 import PagedBatch, YalmB200Error
 
 pytestmark = pytest.mark.gpu
 
@@ -82,6 +82,9 @@ CASES = [
     ([0, 5, 11, 40, 41, 60], [4096, 128, 333, 2000, 700], _ragged(60, 500, 12), _ragged(60, 3, 13, 1), 64, 8, 128, 32,
      "bf16"),
     ([0, 6], [5000], [0, 0, 0, 0, 0, 0], [1] * 6, 4, 1, 128, 64, "f16"),  # few rows over many blocks
+    ([0, 20], [900], _ragged(20, 300, 14), _ragged(20, 8, 15, 1), 16, 16, 128, 16, "f16"),  # up to 8 tokens of one head
+    ([0, 20], [900], _ragged(20, 300, 16), _ragged(20, 8, 17, 1), 4, 4, 64, 64, "bf16"),
+    ([0, 12], [700], [0] * 12, [1] * 12, 16, 2, 128, 256, "f16"),
     ([0, 3], [512], [100, 200, 0], [300, 257, 900], 8, 2, 128, 16, "f16"),  # chunks, which do not share
     ([0, 10], [2000], [100] * 10, [400] + [1] * 9, 32, 8, 128, 16, "bf16"),  # one long chunk among single tokens
     ([0, 40], [2000], [100] * 40, [200] + [1] * 39, 32, 8, 128, 16, "f16"),
@@ -260,3 +263,81 @@ def test_refusals(gpu):
     many = torch.zeros(2050, **i32)
     with pytest.raises(YalmB200Error):
         b.attend_shared(st.q, out, w, many, many[:2049])
+
+
+@pytest.fixture
+def wait_budget():
+    """Sets the clocks that a wait may take; the default comes back at the end."""
+    from yalm_b200 import _lib
+
+    def use(clocks):
+        _lib.check(_lib.lib().yb_paged_attention_wait_budget(clocks))
+    yield use
+    use(0)
+
+
+@pytest.mark.parametrize("clocks", [1, 500, 2000, 6000])
+@pytest.mark.parametrize("new", [[1] * 30, [1] * 20 + [40, 300] + [1] * 8])
+def test_a_wait_that_runs_out_ends_the_call(gpu, wait_budget, new, clocks):
+    """In either kernel: told in the workspace's first word, with nothing in flight, and the next call is right."""
+    import torch
+    st = Shared([0, 30], [1500], _ragged(30, 400, 21), new, 16, 4, 128, 16, "f16", seed=22)
+    b = st.batch()
+    scratch = torch.zeros(b.shared_scratch_bytes(1), dtype=torch.uint8, device="cuda")
+    want, out = st.check(scratch=scratch, batch=b), torch.empty_like(st.q)
+    for _ in range(3):
+        wait_budget(clocks)
+        b.attend_shared(st.q, out, scratch, st.group_start, st.prefix_len)
+        bits = b.status(scratch)
+        assert bits in ((1,) if clocks == 1 else (0, 1))
+        if not bits:
+            assert torch.equal(out.double(), want)
+        wait_budget(0)
+        assert torch.equal(st.attend(scratch=scratch, batch=b).double(), want)
+
+
+def test_pools_past_32_bit_offsets(gpu):
+    """Pages whose elements lie past 2^31 and whose bytes lie past 2^32, of the prefix and of the sequences' own."""
+    import torch
+    st = Shared([0, 12], [512], _ragged(12, 300, 23, 1), [1] * 12, 16, 8, 128, 256, "f16", seed=24)
+    n_pages = 11000
+    k = torch.empty(n_pages, 8, 256, 128, dtype=torch.float16, device="cuda")
+    v = torch.empty_like(k)
+    assert k.numel() > 2 ** 31
+    old = st.page_table.clone()
+    for i, page in enumerate(sorted(set(old.flatten().tolist()) - {-1})):
+        to = 10999 - 7 * i
+        k[to], v[to] = st.k[page], st.v[page]
+        st.page_table[old == page] = to
+    st.k, st.v, st.n_pages = k, v, n_pages
+    st.check()
+
+
+@pytest.mark.parametrize("slots,hd,dtype", [(1 << 20, 64, "f16"), (300_000, 128, "bf16")])
+def test_long_sums_of_few_rows(gpu, slots, hd, dtype):
+    """As many loose sequences as warps have room for, over the same pages, values of one sign: a warp carries one
+    row's sums over thousands of steps, which must not lose what an addition of the tensor cores cuts off."""
+    import torch
+    from test_paged_gpu import U
+    n, ps, dt = 1300, 256, _types()[dtype]
+    g = torch.Generator(device="cuda").manual_seed(25)
+    pages = -(-slots // ps)
+    k = (torch.randn(pages, 1, ps, hd, generator=g, device="cuda") * 0.3).to(dt)
+    v = (torch.rand(pages, 1, ps, hd, generator=g, device="cuda") + 0.5).to(dt)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table = torch.randperm(pages, generator=g, device="cuda").int().expand(n, -1).contiguous()
+    b = PagedBatch(k, v, table, torch.arange(n + 1, **i32), torch.full((n,), slots, **i32), 2, n)
+    q = torch.randn(n, 2 * hd, generator=g, device="cuda").to(dt)
+    out, scratch = torch.empty_like(q), torch.zeros(b.shared_scratch_bytes(1), dtype=torch.uint8, device="cuda")
+    b.attend_shared(q, out, scratch, torch.tensor([0, 0], **i32), torch.zeros(1, **i32))
+    assert b.status(scratch) == 0
+    keys, values = (x[table[0].long(), 0].reshape(-1, hd)[:slots].double() for x in (k, v))
+    for i in (0, 1, n // 2, n - 1):
+        for h in range(2):
+            sc = keys @ q[i, h * hd: (h + 1) * hd].double() / math.sqrt(hd)
+            w = torch.softmax(sc, 0)
+            mag = float((keys.abs() @ q[i, h * hd: (h + 1) * hd].double().abs()).max()) / math.sqrt(hd)
+            o = w @ values
+            # the weights' roundings average over the slots: the output's own, and those of the sums
+            tol = U[dtype] * o.abs() + (2.0 ** -15 + 2 * 2.0 ** -20 * mag) * (w @ values.abs())
+            assert ((out[i, h * hd: (h + 1) * hd].double() - o).abs() <= tol).all()

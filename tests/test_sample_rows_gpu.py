@@ -116,6 +116,15 @@ def test_rows_match_the_definition(gpu, kind, dtype, R, V):
     _check(_logits(R, V, dtype, R + V), rng.random(R).tolist(), **par)
 
 
+@pytest.mark.parametrize("kind", ["all", "top_p", "plain"])
+@pytest.mark.parametrize("R,V,dtype", [(260, 20000, "f32"), (256, 32000, "bf16"), (300, 60000, "f32"), (300, 131072, "f16")])
+def test_batches_of_many_rows(gpu, kind, R, V, dtype):
+    """As many rows as take one or two blocks each, staged in shared memory or not."""
+    rng = np.random.default_rng(R + V)
+    par = {k: [v[r % len(v)] for r in range(R)] for k, v in KINDS[kind].items()}
+    _check(_logits(R, V, dtype, 9), rng.random(R).tolist(), **par)
+
+
 @pytest.mark.parametrize("V", [300000, 1 << 20])  # longer than shared memory takes
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_long_rows(gpu, dtype, V):

@@ -1,7 +1,10 @@
-"""Refusals of the plan and the sampler (yb_paged_plan_dev, yb_sample_rows_dev): every bad size, NULL or alignment
-returns an error code with a message before any CUDA call, so without a GPU too; a dummy non-NULL address is never
-dereferenced on these paths."""
+"""Refusals of the plan, the attention over shared prefixes and the sampler (yb_paged_plan_dev,
+yb_paged_attention_shared_dev, yb_sample_rows_dev): every bad size, NULL or alignment returns an error code with a
+message before any CUDA call, so without a GPU too; a dummy non-NULL address is never dereferenced on these paths.  And
+the arithmetic by which the attention shares out its work, against counting."""
 import ctypes
+import os
+import subprocess
 
 import pytest
 
@@ -46,6 +49,57 @@ def test_bad_plan_arguments_are_refused(kw):
 def test_bad_batches_are_refused_by_the_plan(kw, code):
     assert _plan(_batch(**kw)) == code
     assert _lib.last_error()
+
+
+def _shared(b, **kw):
+    c = dict(n_groups=1, group_start=P, prefix_len=P, out=P, out_stride=512, q=P, q_stride=512, scale=0.125, scratch=P)
+    c.update(kw)
+    return _lib.lib().yb_paged_attention_shared_dev(ctypes.byref(b) if b else None, *c.values(), None)
+
+
+WIDE = dict(n_seqs=40, max_pages=4000)  # a table so long that prefixes are computed apart
+
+
+@pytest.mark.parametrize("kw,code", [
+    ({"n_groups": -1}, _lib.YB_E_INVALID), ({"n_groups": 2049}, _lib.YB_E_UNSUPPORTED), ({"group_start": None}, _lib.YB_E_INVALID),
+    ({"prefix_len": None}, _lib.YB_E_INVALID), ({"group_start": P + 1}, _lib.YB_E_INVALID),
+    ({"prefix_len": P + 2}, _lib.YB_E_INVALID), ({"out": None}, _lib.YB_E_INVALID), ({"q": P + 8}, _lib.YB_E_INVALID),
+    ({"out_stride": 500}, _lib.YB_E_INVALID), ({"scale": 0.0}, _lib.YB_E_INVALID), ({"scratch": None}, _lib.YB_E_INVALID),
+    ({"scratch": P + 8}, _lib.YB_E_INVALID)])
+def test_bad_shared_attention_arguments_are_refused(kw, code):
+    assert _shared(_batch(**WIDE), **kw) == code
+    assert _lib.last_error()
+
+
+def test_bad_batches_are_refused_by_the_shared_attention():
+    for kw, code in (({"head_dim": 80}, _lib.YB_E_UNSUPPORTED), ({"n_heads": 7}, _lib.YB_E_INVALID),
+                     ({"page_table_dev": None}, _lib.YB_E_INVALID), ({"page_size": 8}, _lib.YB_E_UNSUPPORTED)):
+        assert _shared(_batch(**{**WIDE, **kw})) == code
+        assert _lib.lib().yb_paged_attention_shared_scratch_bytes(ctypes.byref(_batch(**{**WIDE, **kw})), 1) == 0
+    big = dict(n_seqs=65536, n_tokens=65536, n_heads=512, n_kv_heads=512, max_pages=(1 << 21) // 16)
+    assert _shared(_batch(**big), out_stride=512 * 64, q_stride=512 * 64) == _lib.YB_E_UNSUPPORTED
+    assert _shared(None) == _lib.YB_E_INVALID
+
+
+def test_the_shared_workspace_serves_the_other_call_too():
+    for kw in (WIDE, {}, dict(n_seqs=3, n_tokens=900, head_dim=128)):
+        b = _batch(**kw)
+        plain = _lib.lib().yb_paged_attention_scratch_bytes(ctypes.byref(b))
+        assert 0 < plain < _lib.lib().yb_paged_attention_shared_scratch_bytes(ctypes.byref(b), 1)
+
+
+def test_empty_shared_batches_need_no_gpu():
+    for kw in ({"n_seqs": 0}, {"n_tokens": 0}):
+        assert _shared(_batch(**{**WIDE, **kw})) == 0
+
+
+def test_shared_work_axis_against_counting(tmp_path):
+    here, csrc = os.path.dirname(os.path.abspath(__file__)), os.path.join(os.path.dirname(_lib.__file__), "csrc")
+    exe = str(tmp_path / "axis")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover", "-I" + csrc, "-o", exe,
+                    os.path.join(here, "paged_shared_axis_check.cpp")], check=True, timeout=300)
+    r = subprocess.run([exe, "20000"], capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0 and r.stdout == "ok\n", r.stdout + r.stderr
 
 
 def test_null_batch_is_refused():

@@ -1149,7 +1149,7 @@ cudaError_t launch(const PagedAttnArgs& a, int device, int grid, bool bf16, cuda
     p.few_recs = reinterpret_cast<float*>(base + few_recs_at(a.b, a.n_groups, HD, a.n_sms));
     if ((e = paged_shared_plan(sp, s)) != cudaSuccess) return e;
     const PagedFewArgs f{a.b, p.shared, p.head, a.q, a.out, a.k_pages, a.v_pages, a.q_stride, a.out_stride, K, gq, p.c,
-                         const_cast<float*>(p.few_recs), const_cast<float*>(p.few_parts), p.status};
+                         const_cast<float*>(p.few_recs), const_cast<float*>(p.few_parts), p.status, a.wait_budget};
     if ((e = paged_few(f, HD, bf16 ? 2 : 1, device, grid, s)) != cudaSuccess) return e;
   }
   void* args[] = {&qm, &km, &vm, &p};

@@ -28,6 +28,10 @@ namespace {
 
 typedef unsigned long long u64;
 
+// Steps in a sum of the tensor cores: of values of one sign it loses 2^-24 of itself a step, on average over its growth (sums
+// of 1024 were 6e-5 too small, a quarter of an fp16 rounding).
+constexpr int kFewSum = 256;
+
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same<T, __half>::value)
@@ -51,6 +55,18 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi, __half) {
 __device__ __forceinline__ uint32_t pack(float lo, float hi, __nv_bfloat16) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Waits for a copy; false, and told, when the clocks have run out.  (Less than the default: without try_wait, which may
+// suspend a warp for longer.)
+__device__ __forceinline__ bool landed(uint64_t* bar, unsigned parity, long long clocks, unsigned* status) {
+  if (mbar_test_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!(clocks < kWaitBudgetCycles ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity)))
+    if (clock64() - t0 > clocks) {
+      atomicOr(status, kStatusMbarTimeout);
+      return false;
+    }
+  return true;
 }
 __device__ __forceinline__ uint4 lds16(uint32_t at) {
   uint4 v;
@@ -173,126 +189,149 @@ __global__ void __launch_bounds__(kFewThreads, 1) paged_few_kernel(const __grid_
       }
       // the slots that rows 2 q4 and 2 q4 + 1 see end here
       const int last0 = sq.kv - sq.few + (2 * q4) / a.gq + 1, last1 = sq.kv - sq.few + (2 * q4 + 1) / a.gq + 1;
-      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-      float o[2 * kC][4];  // o[4 j + i]: dims 64 j + 8 g + 2 i, + 1 of rows 2 q4, 2 q4 + 1
-#pragma unroll
-      for (int i = 0; i < 2 * kC; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
       const int slot_lo = sq.lo * kKT;
-      for (int t = t0; t < t1; ++t) {
-        const int slot = slot_lo + t * kFewSlots;
-        const int stage = done % kStages;
-        const bool here = (ahead.there >> (done & 31)) & 1u;
-        ++done;
-        if (!here) {
-          issue();
-          continue;
-        }
-        if (!__all_sync(0xffffffffu, mbar_wait_s(bars + 8 * stage, (phases >> stage) & 1u, a.status))) {
-          dead = true;
-          break;
-        }
-        phases ^= 1u << stage;
-        const uint32_t kv = ring + stage * 2 * kBytes, kat = kv + g * (HD * 2) + q4 * 16, vat = kv + kBytes + q4 * (HD * 4) + g * 16;
-        float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+      // The tensor cores' additions cut off what does not fit: a sum of theirs ends after kFewSum of them, and is joined
+      // to those before in fp32 (paged_axis.cuh, kSumTiles).
+      float had_m[2], had_l[2];  // of those before, whose o this lane has left in the record
+      for (int u0 = t0, u1; u0 < t1; u0 = u1) {
+        u1 = min(t1, u0 + kFewSum);
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+        float o[2 * kC][4];  // o[4 j + i]: dims 64 j + 8 g + 2 i, + 1 of rows 2 q4, 2 q4 + 1
 #pragma unroll
-        for (int c = 0; c < kC; ++c) {
-          const uint4 k0 = lds16(kat + 64 * c), k1 = lds16(kat + 8 * HD * 2 + 64 * c);
-          mma<T>(s, k0.x, k1.x, k0.y, k1.y, qf[c].x, qf[c].y);
-          mma<T>(s2, k0.z, k1.z, k0.w, k1.w, qf[c].z, qf[c].w);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) s[k] += s2[k];
-        if (slot + kFewSlots > sq.kv - sq.few) {  // an edge
-          const int at = slot + g;
-          if (at >= last0) s[0] = -INFINITY;
-          if (at >= last1) s[1] = -INFINITY;
-          if (at + 8 >= last0) s[2] = -INFINITY;
-          if (at + 8 >= last1) s[3] = -INFINITY;
-        }
-        float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-          x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
-        }
-        const float n0 = fmaxf(m0, x0 * a.c), n1 = fmaxf(m1, x1 * a.c);
-        const float f0 = n0 == -INFINITY ? 0.f : n0 - kBias, f1 = n1 == -INFINITY ? 0.f : n1 - kBias;
-        if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
-          const float r0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0), r1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
-          l0 *= r0;
-          l1 *= r1;
-#pragma unroll
-          for (int i = 0; i < 2 * kC; ++i) {
-            o[i][0] *= r0;
-            o[i][1] *= r1;
-            o[i][2] *= r0;
-            o[i][3] *= r1;
+        for (int i = 0; i < 2 * kC; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        for (int t = u0; t < u1; ++t) {
+          const int slot = slot_lo + t * kFewSlots;
+          const int stage = done % kStages;
+          const bool here = (ahead.there >> (done & 31)) & 1u;
+          ++done;
+          if (!here) {
+            issue();
+            continue;
           }
-          m0 = n0;
-          m1 = n1;
-        }
-        s[0] = ex2(fmaf(s[0], a.c, -f0));
-        s[1] = ex2(fmaf(s[1], a.c, -f1));
-        s[2] = ex2(fmaf(s[2], a.c, -f0));
-        s[3] = ex2(fmaf(s[3], a.c, -f1));
-        l0 += s[0] + s[2];
-        l1 += s[1] + s[3];
-        const uint32_t p0 = movm_trans(pack(s[0], s[1], T())), p1 = movm_trans(pack(s[2], s[3], T()));
+          if (!__all_sync(0xffffffffu, landed(&s_bars[w][stage], (phases >> stage) & 1u, a.wait_budget, a.status))) {
+            dead = true;
+            break;
+          }
+          phases ^= 1u << stage;
+          const uint32_t kv = ring + stage * 2 * kBytes, kat = kv + g * (HD * 2) + q4 * 16, vat = kv + kBytes + q4 * (HD * 4) + g * 16;
+          float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < kJ; ++j) {
-          uint32_t w[4][4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {  // slots 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9
-            const int at = (k & 1) + (k >> 1) * 8;
-            uint4 v = lds16(vat + at * (HD * 2) + 128 * j);
-            // what lies behind the last slot may be anything, and 0 of it has to be 0
-            if (slot + 2 * q4 + at >= sq.kv) v = zero4();
-            w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
+          for (int c = 0; c < kC; ++c) {
+            const uint4 k0 = lds16(kat + 64 * c), k1 = lds16(kat + 8 * HD * 2 + 64 * c);
+            mma<T>(s, k0.x, k1.x, k0.y, k1.y, qf[c].x, qf[c].y);
+            mma<T>(s2, k0.z, k1.z, k0.w, k1.w, qf[c].z, qf[c].w);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            mma<T>(o[4 * j + i], __byte_perm(w[0][i], w[1][i], 0x5410), __byte_perm(w[0][i], w[1][i], 0x7632),
-                   __byte_perm(w[2][i], w[3][i], 0x5410), __byte_perm(w[2][i], w[3][i], 0x7632), p0, p1);
-        }
-        __syncwarp();  // all have read the stage
-        issue();
-      }
-      if (dead) break;
+          for (int k = 0; k < 4; ++k) s[k] += s2[k];
+          if (slot + kFewSlots > sq.kv - sq.few) {  // an edge
+            const int at = slot + g;
+            if (at >= last0) s[0] = -INFINITY;
+            if (at >= last1) s[1] = -INFINITY;
+            if (at + 8 >= last0) s[2] = -INFINITY;
+            if (at + 8 >= last1) s[3] = -INFINITY;
+          }
+          float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, d);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, d);
-      }
-      const bool whole = t0 == 0 && t1 == steps;
-      // ---- rows 2 q4 and 2 q4 + 1: the outputs, or a record
+          for (int d = 4; d < 32; d <<= 1) {
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+          }
+          const float n0 = fmaxf(m0, x0 * a.c), n1 = fmaxf(m1, x1 * a.c);
+          const float f0 = n0 == -INFINITY ? 0.f : n0 - kBias, f1 = n1 == -INFINITY ? 0.f : n1 - kBias;
+          if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
+            const float r0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0), r1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
+            l0 *= r0;
+            l1 *= r1;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = 2 * q4 + e;
-        if (r >= rows) continue;
-        const float m = e ? m1 : m0, l = e ? l1 : l0;
-        const int token = r / a.gq, h = head * a.gq + r % a.gq;
-        if (whole && sq.part < 0) {
-          const float inv = l != 0.f ? 1.f / l : 0.f;
-          T* out = static_cast<T*>(a.out) + (size_t)(sq.row0 + token) * a.out_stride + (size_t)h * HD + 8 * g;
+            for (int i = 0; i < 2 * kC; ++i) {
+              o[i][0] *= r0;
+              o[i][1] *= r1;
+              o[i][2] *= r0;
+              o[i][3] *= r1;
+            }
+            m0 = n0;
+            m1 = n1;
+          }
+          s[0] = ex2(fmaf(s[0], a.c, -f0));
+          s[1] = ex2(fmaf(s[1], a.c, -f1));
+          s[2] = ex2(fmaf(s[2], a.c, -f0));
+          s[3] = ex2(fmaf(s[3], a.c, -f1));
+          l0 += s[0] + s[2];
+          l1 += s[1] + s[3];
+          const uint32_t p0 = movm_trans(pack(s[0], s[1], T())), p1 = movm_trans(pack(s[2], s[3], T()));
 #pragma unroll
           for (int j = 0; j < kJ; ++j) {
-            uint32_t w[4];
+            uint32_t w[4][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = pack(o[4 * j + i][e] * inv, o[4 * j + i][2 + e] * inv, T());
-            *reinterpret_cast<uint4*>(out + 64 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int k = 0; k < 4; ++k) {  // slots 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9
+              const int at = (k & 1) + (k >> 1) * 8;
+              uint4 v = lds16(vat + at * (HD * 2) + 128 * j);
+              // what lies behind the last slot may be anything, and 0 of it has to be 0
+              if (slot + 2 * q4 + at >= sq.kv) v = zero4();
+              w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              mma<T>(o[4 * j + i], __byte_perm(w[0][i], w[1][i], 0x5410), __byte_perm(w[0][i], w[1][i], 0x7632),
+                     __byte_perm(w[2][i], w[3][i], 0x5410), __byte_perm(w[2][i], w[3][i], 0x7632), p0, p1);
           }
-        } else {
-          float* rec = whole ? a.parts + ((size_t)(sq.part + token) * b.n_heads + h) * few_row_floats(HD)
-                             : a.recs + (((size_t)warp * 2 + (t0 == 0 ? 1 : 0)) * kFewRows + r) * few_row_floats(HD);
+          __syncwarp();  // all have read the stage
+          issue();
+        }
+        if (dead) break;
 #pragma unroll
-          for (int j = 0; j < kJ; ++j)
+        for (int d = 4; d < 32; d <<= 1) {
+          l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+          l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+        }
+        const bool whole = t0 == 0 && u1 == steps;
+        // ---- rows 2 q4 and 2 q4 + 1: the outputs, or a record
 #pragma unroll
-            for (int i = 0; i < 4; i += 2)
-              *reinterpret_cast<float4*>(rec + 64 * j + 8 * g + 2 * i) =
-                  make_float4(o[4 * j + i][e], o[4 * j + i][2 + e], o[4 * j + i + 1][e], o[4 * j + i + 1][2 + e]);
-          if (g == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(m, l);
+        for (int e = 0; e < 2; ++e) {
+          const int r = 2 * q4 + e;
+          if (r >= rows) continue;
+          float m = e ? m1 : m0, l = e ? l1 : l0;
+          const int token = r / a.gq, h = head * a.gq + r % a.gq;
+          float* const mine = a.recs + (((size_t)warp * 2 + (t0 == 0 ? 1 : 0)) * kFewRows + r) * few_row_floats(HD);
+          if (u0 > t0) {  // what the sums before this one have left
+            const float mm = fmaxf(m, had_m[e]), f = m == -INFINITY ? 0.f : ex2(m - mm);
+            const float fo = had_m[e] == -INFINITY ? 0.f : ex2(had_m[e] - mm);
+            m = mm;
+            l = l * f + had_l[e] * fo;
+#pragma unroll
+            for (int j = 0; j < kJ; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float* was = mine + 64 * j + 8 * g + 2 * i;
+                o[4 * j + i][e] = o[4 * j + i][e] * f + was[0] * fo;
+                o[4 * j + i][2 + e] = o[4 * j + i][2 + e] * f + was[1] * fo;
+              }
+          }
+          had_m[e] = m;
+          had_l[e] = l;
+          if (whole && sq.part < 0) {
+            const float inv = l != 0.f ? 1.f / l : 0.f;
+            T* out = static_cast<T*>(a.out) + (size_t)(sq.row0 + token) * a.out_stride + (size_t)h * HD + 8 * g;
+#pragma unroll
+            for (int j = 0; j < kJ; ++j) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) w[i] = pack(o[4 * j + i][e] * inv, o[4 * j + i][2 + e] * inv, T());
+              *reinterpret_cast<uint4*>(out + 64 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+            float* rec = whole ? a.parts + ((size_t)(sq.part + token) * b.n_heads + h) * few_row_floats(HD) : mine;
+#pragma unroll
+            for (int j = 0; j < kJ; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; i += 2)
+                *reinterpret_cast<float4*>(rec + 64 * j + 8 * g + 2 * i) =
+                    make_float4(o[4 * j + i][e], o[4 * j + i][2 + e], o[4 * j + i + 1][e], o[4 * j + i + 1][2 + e]);
+            if (g == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(m, l);
+          }
         }
       }
+      if (dead) break;
     }
     // ---- the next unit
     left -= min(length - off, left);

@@ -49,6 +49,7 @@ struct PagedFewArgs {
   float* recs;   // [warps][2][kFewRows] rows
   float* parts;  // [tokens with a part][n_heads] rows
   unsigned* status;
+  long long wait_budget;
 };
 cudaError_t paged_few(const PagedFewArgs& a, int head_dim, int type, int device, int grid, cudaStream_t s);
 
