@@ -258,6 +258,8 @@ extern "C" int yb_paged_attention_shared_dev(const yb_paged_batch* b, int n_grou
                                              long long q_stride, float scale, void* scratch_dev, void* stream) {
   int rc = check_groups(n_groups);
   if (rc) return rc;
+  if (n_groups && (!group_start_dev || !prefix_len_dev || !aligned4(group_start_dev) || !aligned4(prefix_len_dev)))
+    return set_error(YB_E_INVALID, "group_start_dev and prefix_len_dev must be 4-byte aligned buffers");
   // Where nothing is shared, or reading it once can save no more than 64 MB (every sequence's whole table but one), its
   // kernels cost more than they save.  32 heads of 128 on 8 kv heads, prefix of 4096 and 100 own slots: 4 sequences (50
   // MB) 19.4 us without, 32.9 with; 8 (117 MB) 27.1 and 31.3; 16 (252 MB) 42.9 and 31.5.  8 heads of 64 on 2: 32 (65 MB)
@@ -268,8 +270,6 @@ extern "C" int yb_paged_attention_shared_dev(const yb_paged_batch* b, int n_grou
   PagedAttnArgs a{};
   bool empty = false;
   if ((rc = check_attention(b, &a, &empty, out, out_stride, q, q_stride, scale, scratch_dev))) return rc;
-  if (!group_start_dev || !prefix_len_dev || !aligned4(group_start_dev) || !aligned4(prefix_len_dev))
-    return set_error(YB_E_INVALID, "group_start_dev and prefix_len_dev must be 4-byte aligned buffers");
   if (empty) return 0;
   if ((rc = check_share(b, a.b, current_device(), n_groups))) return rc;
   int dev = 0;

@@ -2,7 +2,7 @@
 `build/test -bk {matmul,matmul-wide,mha,ffn}`, src/test.cpp:339-405).
 
     python -m yalm_b200.kbench [--kernel gemv|gateup|qkv|attention|prefill_attention|prefill_gemm|prefill|
-                               paged_append|paged_attention|all]
+                               paged_plan|paged_append|paged_attention|paged_shared|sample|all]
                                [--iters N] [--warm W] [--quick]
 
 Each launch goes through the C ABI (yb_gemv_dev, yb_gateup_dev, yb_qkv_dev, yb_attention_dev) on
@@ -269,6 +269,75 @@ def bench_paged_attention(new, kv, nh, nkv, hd, ps, iters, seed=0):
             "tflops": round(4.0 * pairs * nh * hd / (ms / 1000) / 1e12, 2), **_LAST_SPREAD}
 
 
+def bench_paged_plan(seqs, new, kv, ps, iters, seed=0):
+    """The plan of a step (yb_paged_plan_dev): `seqs` sequences that bring `new` tokens over kv cached slots each."""
+    import torch
+    from .paged import PagedBatch
+    _fresh()
+    held, then = -(-kv // ps), -(-(kv + new) // ps)
+    pages, i32 = seqs * then, dict(dtype=torch.int32, device="cuda")
+    order = torch.randperm(pages, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)).int()
+    table = torch.full((seqs, then), -1, **i32)
+    table[:, :held] = order[: seqs * held].view(seqs, held)
+    free = torch.cat((order[seqs * held:], torch.full((seqs * held,), -1, **i32)))
+    k = torch.empty(pages, 1, ps, 64, dtype=torch.float16, device="cuda")
+    b = PagedBatch(k, k, table, torch.zeros(seqs + 1, **i32), torch.zeros(seqs, **i32), 1, seqs * new)
+    before, n_free, n_before = torch.full((seqs,), kv, **i32), torch.zeros(1, **i32), torch.full((1,), pages - seqs * held, **i32)
+    new_len, status, pos = torch.full((seqs,), new, **i32), torch.zeros(4, **i32), torch.zeros(seqs * new, **i32)
+    slots, stream = torch.zeros(seqs * new, dtype=torch.int64, device="cuda"), torch.cuda.current_stream().cuda_stream
+
+    def fn(i):
+        b.plan(new_len, free, n_free, status, kv_before=before, n_free_before=n_before, pos=pos, slots=slots, stream=stream)
+    ms = _time(fn, iters)
+    return {"kernel": "paged_plan", "sequences": seqs, "tokens": seqs * new, "page": ps, "us": round(ms * 1000, 2), **_LAST_SPREAD}
+
+
+def bench_paged_shared(seqs, prefix, own, nh, nkv, hd, ps, iters, seed=0):
+    """Attention of single tokens over a shared prefix and `own` slots each (yb_paged_attention_shared_dev), fp16."""
+    import torch
+    _fresh()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    b = _paged([1] * seqs, [prefix + own] * seqs, nh, nkv, hd, ps, torch.float16, seed)
+    table = b._keep[2]
+    table[:, : prefix // ps] = table[0, : prefix // ps]
+    q = torch.randn(seqs, nh * hd, device="cuda").half()
+    out, scratch = torch.empty_like(q), torch.zeros(b.shared_scratch_bytes(1), dtype=torch.uint8, device="cuda")
+    groups, lens = torch.tensor([0, seqs], **i32), torch.tensor([prefix // ps * ps], **i32)
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def fn(i):
+        b.attend_shared(q, out, scratch, groups, lens, stream=stream)
+    ms = _time(fn, iters)
+    slots = prefix // ps * ps + seqs * (prefix % ps + own)
+    return {"kernel": "paged_shared", "sequences": seqs, "prefix": prefix, "own": own, "n_heads": nh, "n_kv_heads": nkv,
+            "head_dim": hd, "page": ps, "us": round(ms * 1000, 2),
+            "gbs": round((4 * slots * nkv + 4 * seqs * nh) * hd / (ms / 1000) / 1e9, 1), **_LAST_SPREAD}
+
+
+def bench_sample(rows, vocab, dtype, iters, seed=0, **limits):
+    """A token for every row of logits (yb_sample_rows_dev), N(0, 2) with 40 likely ones."""
+    import torch
+    from .sampling import sample_rows
+    _fresh()
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    size = torch.finfo(dtype).bits // 8
+    n = min(16, _copies(rows * vocab * size))
+    x = []
+    for _ in range(n):
+        t = torch.randn(rows, vocab, device="cuda", generator=g) * 2
+        at = torch.randint(0, vocab, (rows, 40), device="cuda", generator=g)
+        x.append(t.scatter(1, at, 2 + 9 * torch.rand(rows, 40, device="cuda", generator=g)).to(dtype))
+    coin, tokens = torch.rand(rows, device="cuda", generator=g), torch.zeros(rows, dtype=torch.int32, device="cuda")
+    par = {k: torch.full((rows,), v, dtype=torch.int32 if k == "top_k" else torch.float32, device="cuda") for k, v in limits.items()}
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def fn(i):
+        sample_rows(x[i % n], coin, tokens, stream=stream, **par)
+    ms = _time(fn, iters)
+    return {"kernel": "sample", "rows": rows, "vocab": vocab, "dtype": str(dtype).split(".")[1], **limits, "us": round(ms * 1000, 2),
+            "gbs": round(rows * vocab * size / (ms / 1000) / 1e9, 1), **_LAST_SPREAD}
+
+
 def bench_prefill(tokens, iters, config="mistral-7b", seed=0):
     """The whole batched prompt pass (yb_prefill, every layer's GEMMs, norms, RoPE / KV append and
     attention, then the classifier) of the seeded synthetic checkpoint.  Per prompt length one
@@ -310,7 +379,7 @@ def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("--kernel", default="all",
                     choices=["gemv", "gateup", "qkv", "attention", "prefill_attention", "prefill_gemm", "prefill",
-                             "paged_append", "paged_attention", "all"])
+                             "paged_plan", "paged_append", "paged_attention", "paged_shared", "sample", "all"])
     ap.add_argument("--iters", type=int, default=200)
     ap.add_argument("--quick", action="store_true", help="one shape per kernel (for profiler captures)")
     ap.add_argument("--kv-lens", default="", help="attention: comma-separated kv_len values")
@@ -354,6 +423,19 @@ def main(argv=None):
                                                       ([512], [3202]), ([2048], [16384])]
         for new, kv in cases:
             rows.append(bench_paged_attention(new, kv, 32, 8, 128, 16, max(3, args.iters // (20 if sum(new) > 64 else 1))))
+    if args.kernel in ("paged_plan", "all"):
+        for seqs, new, kv in [(256, 1, 1000)] if args.quick else [(1, 1, 36), (256, 1, 1000), (256, 30, 1000), (16384, 27, 250)]:
+            rows.append(bench_paged_plan(seqs, new, kv, 16, args.iters))
+    if args.kernel in ("paged_shared", "all"):
+        cases = [(64, 4096, 350)] if args.quick else [(64, 4096, 350), (64, 16384, 350), (256, 4096, 350)]
+        for seqs, prefix, own in cases:
+            rows.append(bench_paged_shared(seqs, prefix, own, 32, 8, 128, 16, args.iters))
+    if args.kernel in ("sample", "all"):
+        shapes = [(64, 131072, torch.bfloat16)] if args.quick else [(1, 32000, torch.float32), (64, 131072, torch.bfloat16),
+                                                                    (256, 131072, torch.float32)]
+        for r, v, t in shapes:
+            for limits in ({"temperature": 0.0}, {"temperature": 0.8}, {"top_k": 50, "top_p": 0.95}, {"top_p": 0.9}):
+                rows.append(bench_sample(r, v, t, args.iters, **limits))
     if args.kernel == "prefill_gemm":
         T = int(args.tokens.split(",")[0]) if args.tokens else 3202
         for planes in (1, 2):
