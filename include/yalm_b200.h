@@ -402,13 +402,15 @@ size_t yb_paged_attention_scratch_bytes(const yb_paged_batch* b); /* 0 for a bat
 /* The same attention, without a window, for a batch in which groups of sequences begin with the same pages (a system
  * prompt, a document, samples of one prompt): a group's prefix is read once for all of its sequences.  Sequences
  * group_start_dev[g] .. group_start_dev[g + 1] - 1 form group g of n_groups (up to 2048); their rows of the table hold
- * the same pages for the first prefix_len_dev[g] slots, which are read through the first one's row.  Sequences before
- * group_start_dev[0] and from group_start_dev[n_groups] on share nothing, nor does a group with prefix_len_dev 0.  Both
- * are read on the device; group_start must not decrease, and is taken as clamped to [0, n_seqs], prefix_len to what
- * every sequence of the group with new tokens has cached before them.
+ * the same pages for the first prefix_len_dev[g] slots, which are read through the row of the first that has new tokens
+ * (those that have none count for nothing, whatever their rows hold).  Sequences before group_start_dev[0] and from
+ * group_start_dev[n_groups] on share nothing, nor does a group with prefix_len_dev 0.  Both are read on the device;
+ * group_start must not decrease, and is taken as clamped to [0, n_seqs], prefix_len to what every sequence of the group
+ * with new tokens has cached before them.
  * The result is that of yb_paged_attention_dev on the same batch, to the rounding of sums that are split in other
  * places; a prefix is computed apart only where that pays: whole tiles of 128 slots of it, for groups of which several
- * sequences fit a unit of 2 * floor(128 * n_kv_heads / n_heads) queries.  With n_groups 0 it is that call.
+ * sequences fit a unit of 2 * floor(128 * n_kv_heads / n_heads) queries, in batches whose n_seqs - 1 other rows of the
+ * table span 64 MB of the cache at least.  With n_groups 0 it is that call.
  * scratch_dev: yb_paged_attention_shared_scratch_bytes(b, n_groups) bytes, 16-byte aligned, which also grows with
  * n_seqs and n_tokens; what is said of that call's workspace and of its first word holds here too. */
 int yb_paged_attention_shared_dev(const yb_paged_batch* b, int n_groups, const int* group_start_dev,

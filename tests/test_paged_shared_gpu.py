@@ -154,6 +154,17 @@ def test_a_prefix_longer_than_what_is_cached(gpu):
     assert want.shape == (20, 8 * 128)
 
 
+def test_sequences_that_bring_nothing_may_come_first(gpu):
+    """A group's pages are read through a row that means something: that of an ended sequence may hold anything."""
+    new = [0, 0] + [1] * 18 + [0, 0, 0] + [2] * 17
+    st = Shared([0, 20, 40], [1000, 700], [0, 0] + [40] * 18 + [0] * 3 + [9] * 17, new, 8, 2, 128, 16, "f16", seed=11)
+    for s in range(40):
+        if not new[s]:
+            st.page_table[s, :] = st.n_pages + s if s % 2 else -1
+            st.kv_len[s] = st.kv[s] = 0
+    st.check()
+
+
 def test_group_starts_out_of_range(gpu):
     import torch
     st = Shared([0, 20], [1024], _ragged(20, 300, 4), [1] * 20, 8, 2, 128, 16, "f16", seed=11)

@@ -946,7 +946,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
 // those of its group's prefix, each a record in `parts` or, of a unit that was cut, several of the blocks' or warps'.
 // Blocks (x, y) look after sequence x, a warp after up to 8 rows of a kv head: where their parts lie is found once for
 // them.  A row has 32 / rows lanes, which take turns at its float4, so that records of either kind are read by pieces of
-// 64 bytes and more, four parts at once.  (A warp a row, with the parts shared out among its lanes, took 945
+// 64 bytes and more, up to 8 parts at once.  (A warp a row, with the parts shared out among its lanes, took 945
 // instructions a row, mostly for that search: 64 single tokens 8.6 us.)
 constexpr int kJoinThreads = 128, kJoinRows = 8, kJoinParts = 8;
 template <int HD, typename T>

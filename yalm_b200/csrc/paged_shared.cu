@@ -24,7 +24,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
   __shared__ int s_start[kMaxGroups + 1];  // first sequences
   __shared__ int s_cut[kMaxGroups];        // slots, then key tiles of the prefix that are computed once
   __shared__ int s_units[kMaxGroups];      // units of the sequences, each by itself, then where their tokens' parts begin
-  __shared__ int s_row0[kMaxGroups], s_rows[kMaxGroups];  // the group's tokens
+  __shared__ int s_row0[kMaxGroups + 1];  // first rows
+  __shared__ int s_first[kMaxGroups];     // the first sequence with new tokens, whose row of the table is read
   int* const s_part = s_units;
   __shared__ u64 s_warp[2][kWarps];
   const PagedBatch& b = a.b;
@@ -36,6 +37,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
     if (g < a.n_groups) {
       s_cut[g] = min(max(__ldca(a.prefix_len + g), 0), b.max_pages << b.ps_log2);
       s_units[g] = 0;
+      s_first[g] = b.n_seqs - 1;
     }
   }
   __syncthreads();
@@ -50,16 +52,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
     return lo < a.n_groups && s_start[lo] <= s && s < s_start[lo + 1] ? lo : -1;
   };
   auto row_of = [&](int s) { return min(max(__ldca(b.q_start + s), 0), b.n_tokens); };
-  for (int g = threadIdx.x; g < a.n_groups; g += kThreads) {
-    s_row0[g] = row_of(s_start[g]);
-    s_rows[g] = s_start[g + 1] > s_start[g] ? max(row_of(s_start[g + 1]) - s_row0[g], 0) : 0;
-  }
+  for (int g = threadIdx.x; g <= a.n_groups; g += kThreads) s_row0[g] = row_of(s_start[g]);
+  auto rows_of = [&](int g) { return s_start[g + 1] > s_start[g] ? max(s_row0[g + 1] - s_row0[g], 0) : 0; };
   for (int s = threadIdx.x; s < b.n_seqs; s += kThreads) {
     const PagedSeq q = paged_seq(b, s);
     const int g = q.n > 0 ? group_of(s) : -1;
     if (g >= 0) {
       atomicMin(&s_cut[g], q.kv - q.n);
       atomicAdd(&s_units[g], (q.n + a.x.U - 1) / a.x.U);
+      atomicMin(&s_first[g], s);
     }
   }
   __syncthreads();
@@ -69,7 +70,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
       const int g = g0 + lane;
       int rows = 0, tiles = 0;
       if (g < a.n_groups) {
-        rows = s_rows[g];
+        rows = rows_of(g);
         tiles = max(s_cut[g], 0) / kKT;
         if (!rows || s_units[g] < 2 * ((rows + a.x.U - 1) / a.x.U)) tiles = 0;
         if (!tiles) rows = 0;
@@ -95,9 +96,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
     q.part = -1;
     if (v < a.n_groups) {
       q.row0 = s_row0[v];
-      q.n = s_cut[v] ? s_rows[v] : 0;
+      q.n = s_cut[v] ? rows_of(v) : 0;
       q.kv = s_cut[v] * kKT;
-      q.table = s_start[v];
+      q.table = s_first[v];
       q.part = s_part[v];
       q.all = 1;
       return q;
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
     q.table = s;
     if (p.n > 0 && g >= 0 && s_cut[g]) {
       const int at = q.row0 - s_row0[g];
-      if (at >= 0 && at + p.n <= s_rows[g]) {  // (else q_start decreases)
+      if (at >= 0 && at + p.n <= rows_of(g)) {  // (else q_start decreases)
         q.lo = s_cut[g];
         q.part = s_part[g] + at;
         q.group = g;
