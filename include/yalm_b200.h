@@ -431,8 +431,9 @@ int yb_paged_attention_wait_budget(long long clocks);
  *   with min_p > 0: of those the ones of w_i >= min_p (more than 1 counts as 1, so the first always stays);
  * and of those, by index, the first whose running sum reaches coin times their sum (a coin up to 0 counts as the least
  * there is, one from 1 on as 1).  temperature <= 0 or NaN: the first index of the maximum, whatever the other
- * settings are; others count as at least 2^-60 and at most 2^90.  A top_p <= 0 keeps the first token alone.  NaN logits are never drawn (they count as -infinity); where
- * the maximum is +infinity, its tokens share the draw.  A row without a logit above -infinity gives token 0 and probability 0.
+ * settings are; others count as at least 2^-60 and at most 2^90.  A top_p <= 0 keeps the first token alone.  NaN logits
+ * are never drawn (they count as -infinity); where the maximum is +infinity, its tokens share the draw.  A row without a
+ * logit above -infinity gives token 0 and probability 0.
  * coin_dev [rows]; temperature_dev, top_k_dev, top_p_dev, min_p_dev [rows], each may be NULL: 1, and no limit.  A NaN
  * among coins counts as 0, among limits as none.  tokens_dev [rows] gets the tokens, prob_dev [rows] (or NULL) their
  * probability among those that were kept (1 where temperature <= 0).
