@@ -133,6 +133,20 @@ def test_long_rows(gpu, dtype, V):
     _check(_logits(8, V, dtype, 7), rng.random(8).tolist(), **par)
 
 
+def test_batches_of_long_rows(gpu):
+    """As many rows as there are places for blocks, each longer than the 2^17 logits whose weights a block's sums hold."""
+    import torch
+    R, V = 290, 1 << 20
+    x = torch.zeros(R, V, dtype=torch.bfloat16, device="cuda")
+    x[1::2] = _logits(1, V, "bf16", 8, 1e-2, peaks=False)
+    rng = np.random.default_rng(8)
+    coin, p = rng.random(R).tolist(), [(0.5, 0.9, 1.0, 0.3)[r // 2 % 4] for r in range(R)]
+    tokens, prob = _run(x, coin, top_p=p)
+    for r in (0, 1, 2, 3, 4, 5, 6, 7, 144, 145, 288, 289):
+        t, q = _one(x[r].float().cpu().numpy().astype(np.float64), float(np.float32(coin[r])), 1.0, 0, float(np.float32(p[r])), 0.0)
+        assert tokens[r] == t and abs(prob[r] - q) <= 2.0 ** -24 * q + 2.0 ** -42, (r, tokens[r], t, prob[r], q)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("spread", [0.0, 1e-3, 0.02, 0.5])
 def test_limits_among_many_tokens_alike(gpu, dtype, spread):

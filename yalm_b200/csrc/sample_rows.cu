@@ -45,6 +45,7 @@ constexpr u64 kOne = 1ull << 43;                    // the largest weight
 constexpr float kLeastTemperature = 0x1p-60f, kMostTemperature = 0x1p90f;
 constexpr size_t kMaxStage = 160 * 1024;            // bytes of a row's stretch that shared memory takes
 constexpr int kMaxCluster = 8;
+constexpr int kMostLogits = kSampleMaxVocab / kMaxCluster;  // of a block: sums by parts of weights are sized for them
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
@@ -197,7 +198,7 @@ struct Order {
 };
 
 struct Shared {
-  // of sums of weights 15 bits, the next 15, and the rest, each summed by itself: up to 2^17 of them (2^20 / 8) fit 32 bits
+  // of sums of weights 15 bits, the next 15, and the rest, each summed by itself: kMostLogits (2^17) of them fit 32 bits
   unsigned count[kBins], low[kBins], mid[kBins], high[kBins];
   u64 list[kList];
   Pair warps[kWarps];
@@ -751,7 +752,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     limit_i = (int)~(unsigned)limit;
   }
   // ---- the draw, in the order of the row
-  // Sums of a thread's weights, up to 2^20 / 8 / 512 of them, are whole numbers of 64-bit floating point.
+  // Sums of a thread's weights, up to kMostLogits / 512 of them, are whole numbers of 64-bit floating point.
   const double least_above = kUnits + (double)least;
   auto kept = [&](int i, const float (&l)[4], double (&v)[4]) {
 #pragma unroll
@@ -868,6 +869,7 @@ cudaError_t launch(const SampleRowsArgs& a, int device, int n_sms, cudaStream_t 
   for (int c = 1; c <= kMaxCluster; c *= 2) {
     if (c > 1 && a.vocab < 2048 * c) break;
     const int st = ((a.vocab + c - 1) / c + 31) / 32 * 32;
+    if (st > kMostLogits) continue;
     const size_t bytes = (size_t)st * sizeof(T) + 32;
     const bool in = bytes <= kMaxStage;
     const int per_sm = in && bytes > kMaxStage / 2 ? 1 : 2, waves = (int)(((long long)a.rows * c + n_sms * per_sm - 1) / (n_sms * per_sm));
