@@ -40,6 +40,7 @@ constexpr int kOctaves = 44, kPerOctave = 16, kBins = kOctaves * kPerOctave;
 constexpr int kEach = 4, kList = kThreads * kEach;  // tokens of a list: 4 a thread
 constexpr int kBinsPer = (kBins + kThreads - 1) / kThreads;
 constexpr int kShortList = 128;
+constexpr int kPart = 14;  // kMostLogits of 2^kPart, and 2 % more, fit 32 bits
 constexpr int kRounds = 8;  // kBins^7 is more than 2^64, the places that a range may have
 constexpr u64 kOne = 1ull << 43;                    // the largest weight
 constexpr float kLeastTemperature = 0x1p-60f, kMostTemperature = 0x1p90f;
@@ -130,9 +131,16 @@ struct Weights {
     per_bin = (float)(c * kPerOctave);
   }
   __device__ __forceinline__ bool some(float l) const { return l >= cut; }
-  // of what has a weight; the sum rounds to a whole number
-  __device__ __forceinline__ int bin(float l) const {
-    return min(__float_as_int(fmaf(fminf(maxf - l, FLT_MAX), per_bin, 8388608.f)) - 0x4b000000, kBins - 1);
+  // 2^23 + the bin (or more than the last one's) of what has a weight; the sum rounds to a whole number
+  __device__ __forceinline__ float bin_above(float l) const { return fmaf(fminf(maxf - l, FLT_MAX), per_bin, 8388608.f); }
+  __device__ __forceinline__ int bin(float l) const { return min(__float_as_int(bin_above(l)) - 0x4b000000, kBins - 1); }
+  // The same, and about 2^kPart times the weight's ratio to that of the bin's middle: 2^-x by its series up to x^2, |x| <= 1/32.
+  __device__ __forceinline__ int bin_and_part(float l, unsigned* part) const {
+    const float d = fminf(maxf - l, FLT_MAX), b = fmaf(d, per_bin, 8388608.f), x = fmaf(d, per_bin, 8388608.f - b);
+    constexpr float kSlope = 0.69314718f / kPerOctave, kScale = 1 << kPart;
+    const float y = fmaf(x, fmaf(x, 0.5f * kSlope * kSlope * kScale, -kSlope * kScale), kScale + 8388608.f);
+    *part = (unsigned)(__float_as_int(y) - 0x4b000000);
+    return min(__float_as_int(b) - 0x4b000000, kBins - 1);
   }
   // 2^52 + the weight in units
   __device__ __forceinline__ double above(float l) const {
@@ -206,6 +214,7 @@ struct Shared {
   u64 block_sum, told;
   Pair found_before;
   unsigned mine;  // tokens that the block has listed for the first one
+  u64 weights, before;  // of the block's logits: all, those of the bins before the limit's
   float max[kWarps], block_max;
   int block_first;  // index of the block's first maximum
   unsigned listed;
@@ -468,8 +477,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
   auto index_of = [&](int c, int j) { return i0 + c * kVec + j - shift; };
   // Four logits at a time, f(index of the first, logits).
   auto each4 = [&](auto&& f) {
+    Chunk<T> next;
+    if (!kStaged) next = chunk_at(c0 + lane, c1);
     for (int b = c0; b < c1; b += 32) {
-      const Chunk<T> v = chunk_at(b + lane, c1);
+      const Chunk<T> v = kStaged ? chunk_at(b + lane, c1) : next;
+      if (!kStaged) next = chunk_at(b + 32 + lane, c1);
 #pragma unroll
       for (int j = 0; j < kVec; j += 4) {
         const float l[4] = {v[j], v[j + 1], v[j + 2], v[j + 3]};
@@ -557,21 +569,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     if (rank == 0) tell(by_rank, before, goal, of, lo, hi, width);
     cluster_sync_all();
   };
-  // Lists in the first block what is from least_l to most_l and passes a test (the counts leave room for all, or s.listed tells):
+  // Lists in the first block what f(list) lists of the block's logits (the counts leave room for all, or s.listed tells):
   // every block in its own list, which is then copied to a place behind those of others.
-  auto pick = [&](float least_l, float most_l, auto&& test) {
+  auto collect = [&](auto&& f) {
     unsigned* const listed = rank ? &s.mine : &s.listed;
     if (rank && threadIdx.x == 0) s.mine = 0;
     __syncthreads();
-    each4([&](int i, const float (&l)[4]) {
-      if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= least_l) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (l[j] >= least_l && l[j] <= most_l && test(i + j, l[j])) {
-            const unsigned to = atomicAdd(listed, 1u);
-            if (to < kList) s.list[to] = place_of(l[j], i + j);
-          }
-      }
+    f([&](int i, float l) {
+      const unsigned to = atomicAdd(listed, 1u);
+      if (to < kList) s.list[to] = place_of(l, i);
     });
     if (rank) {
       __syncthreads();
@@ -581,6 +587,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
         if (s.found + i < kList) first->list[s.found + i] = s.list[i];
     }
     cluster_sync_all();
+  };
+  // What is from least_l to most_l and passes a test.
+  auto pick = [&](float least_l, float most_l, auto&& test) {
+    collect([&](auto&& list) {
+      each4([&](int i, const float (&l)[4]) {
+        if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= least_l) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (l[j] >= least_l && l[j] <= most_l && test(i + j, l[j])) list(i + j, l[j]);
+        }
+      });
+    });
   };
   // The first block's list, 4 tokens a thread, and their weights.
   u64 v[kEach], weight[kEach];
@@ -686,7 +704,130 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
   float limit_l = 0.f;
   int limit_i = 0;
   auto in_limit = [&](int i, float l) { return l > limit_l || (l == limit_l && i <= limit_i); };
-  for (int kind = by_k ? 0 : 1; kind < (by_p ? 2 : 1); ++kind) {  // top-k, then (if that did not see to it) top-p
+  auto set_limit = [&](u64 at) {
+    limit = at;
+    limit_l = value_of((unsigned)(limit >> 32));
+    limit_i = (int)~(unsigned)limit;
+  };
+  const double least_above = kUnits + (double)least;
+  bool summed = false;  // s.lo holds the sums of what the warps' parts of the row keep
+  if (by_p && !by_k) {
+    // One histogram of about the weights, an atomic a logit, says in which bin the limit should lie; then a pass sums
+    // exactly the weights before that bin, and all, and lists the bin.  The sums tell if the limit is in it: else, and
+    // where the bin has too many, what is below does it by exact histograms.
+    clear_bins(s, false);
+    __syncthreads();
+    each4([&](int, const float (&l)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (w.some(l[j])) {
+          unsigned some;
+          const int b = w.bin_and_part(l[j], &some);
+          atomicAdd(&s.count[b], some);
+        }
+    });
+    cluster_sync_all();
+    const int per = (kBins + blocks - 1) / blocks, end = min(kBins, (rank + 1) * per);
+    for (int b = rank * per + threadIdx.x; b < end; b += kThreads) {
+      u64 some = 0;
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c)
+        if (c < blocks) some += dsmem_ptr(&s, c)->count[b];
+      first->list[b] = __float2ull_rn((float)some * exp2f(20.f - b * (1.f / kPerOctave)));
+      first->list[kBins + b] = (some + (1u << (kPart - 1))) >> kPart;  // to 2 %
+    }
+    cluster_sync_all();
+    if (rank == 0) tell(false, Pair{0, 0}, 0, 0, 0, 0, 0);
+    cluster_sync_all();
+    const Order o = *told;
+    if (o.in <= kList) {
+      const bool whole = o.before.n + o.in <= kList * 7 / 8;  // what comes before the bin is listed, too
+      const float upper = o.bin == kBins - 1 ? INFINITY : 8388608.f + (float)o.bin, edge = whole ? 0.f : 8388608.f + (float)o.bin;
+      double all = 0.0, before = 0.0, keep = 0.0;
+      collect([&](auto&& list) {
+        each4([&](int i, const float (&l)[4]) {
+          double v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = w.above(l[j]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float b = w.bin_above(l[j]);
+            const double u = v[j] - kUnits;
+            all += u;
+            if (b < edge) {
+              before += u;
+              if (v[j] >= least_above) keep += u;
+            } else if (b <= upper && w.some(l[j])) {
+              list(i + j, l[j]);
+            }
+          }
+        });
+        const u64 all_sum = block_sum(s, __double2ull_rn(all)), before_sum = block_sum(s, __double2ull_rn(before));
+        if (threadIdx.x == 0) {
+          s.weights = all_sum;
+          s.before = before_sum;
+        }
+      });
+      u64 kept_sum = __double2ull_rn(keep);
+      for (int d = 16; d; d >>= 1) kept_sum += __shfl_xor_sync(0xffffffffu, kept_sum, d);
+      if (rank == 0) {
+        u64 sum = 0, prior = 0;
+        for (int c = 0; c < blocks; ++c) {
+          sum += *dsmem_ptr(&s.weights, c);
+          prior += *dsmem_ptr(&s.before, c);
+        }
+        const bool fits = s.listed <= kList;
+        take_list();
+        const u64 goal = share_of(top_p, sum), here = block_sum(s, (weight[0] + weight[1]) + (weight[2] + weight[3]));
+        u64 at = 0;
+        if (whole) {
+          at = fits && goal <= here ? sum : 0;
+        } else if (fits && prior < goal && goal <= prior + here) {
+          u64 x[kEach];
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) x[e] = v[e];
+          at = select(s, x, weight, false, 0, goal - prior);
+        }
+        if (threadIdx.x == 0) s.told = at;
+      }
+      if (threadIdx.x < kWarps && rank) s.low[threadIdx.x] = s.mid[threadIdx.x] = s.high[threadIdx.x] = 0;
+      cluster_sync_all();
+      const u64 at = *dsmem_ptr(&s.told, 0);
+      if (at && whole) {
+        cluster_arrive();
+        if (rank == 0) finish(false, at);
+        cluster_wait();
+        return;
+      }
+      if (at) {
+        set_limit(at);
+        if (rank == 0) {
+          if (threadIdx.x < kWarps) s.low[threadIdx.x] = s.mid[threadIdx.x] = s.high[threadIdx.x] = 0;
+          __syncthreads();
+        }
+        // the listed ones that are kept, to the sum of the warp whose part they are in
+        auto add = [&](u64 place, u64 of) {
+          const int i = (int)~(unsigned)place - i0;
+          if (place >= limit && of >= least && i < n) add_to_bin(s, (i + shift) / kVec / part, of);
+        };
+        if (rank == 0) {
+#pragma unroll
+          for (int e = 0; e < kEach; ++e)
+            if (v[e]) add(v[e], weight[e]);
+        } else {
+          const int listed = (int)s.mine;
+          for (int b = warp * 32; b < listed; b += kThreads) {
+            const u64 place = b + lane < listed ? s.list[b + lane] : 0, of = w.of(value_of((unsigned)(place >> 32)));
+            if (place) add(place, of);
+          }
+        }
+        __syncthreads();
+        if (lane == 0) s.lo[warp] = kept_sum + s.low[warp] + ((u64)s.mid[warp] << 15) + ((u64)s.high[warp] << 30);
+        summed = true;
+      }
+    }
+  }
+  for (int kind = by_k ? 0 : 1; kind < (by_p && !summed ? 2 : 1); ++kind) {  // top-k, then (if that did not see to it) top-p
     const bool by_rank = kind == 0;
     clear_bins(s, !by_rank);
     __syncthreads();
@@ -747,13 +888,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
       if (threadIdx.x == 0) s.told = at;
     }
     cluster_sync_all();
-    limit = *dsmem_ptr(&s.told, 0);
-    limit_l = value_of((unsigned)(limit >> 32));
-    limit_i = (int)~(unsigned)limit;
+    set_limit(*dsmem_ptr(&s.told, 0));
   }
   // ---- the draw, in the order of the row
   // Sums of a thread's weights, up to kMostLogits / 512 of them, are whole numbers of 64-bit floating point.
-  const double least_above = kUnits + (double)least;
   auto kept = [&](int i, const float (&l)[4], double (&v)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = 0.0;
@@ -769,7 +907,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     for (int j = 0; j < 4; ++j) v[j] = in[j] && v[j] >= least_above ? v[j] - kUnits : 0.0;
   };
   u64 mine;
-  {
+  if (!summed) {
     double some = 0.0;
     if (limit) {
       each4([&](int i, const float (&l)[4]) {
@@ -787,9 +925,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
       });
     }
     mine = __double2ull_rn(some);
+    for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+    if (lane == 0) s.lo[warp] = mine;
   }
-  for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-  if (lane == 0) s.lo[warp] = mine;
   __syncthreads();
   u64 sum = 0;
 #pragma unroll
