@@ -215,6 +215,9 @@ struct Shared {
   Pair found_before;
   unsigned mine;  // tokens that the block has listed for the first one
   u64 weights, before;  // of the block's logits: all, those of the bins before the limit's
+  float coin, top_p;  // the row's settings
+  int top_k;
+  u64 least;  // weight
   float max[kWarps], block_max;
   int block_first;  // index of the block's first maximum
   unsigned listed;
@@ -383,12 +386,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
   pdl_wait();
   const float temp = a.temperature ? __ldca(a.temperature + r) : 1.f;
   const bool greedy = !(temp > 0.f);
-  const float coin = greedy ? 0.f : __ldca(a.coin + r);
-  const float top_p = greedy || !a.top_p ? 1.f : __ldca(a.top_p + r);
-  const int top_k = greedy || !a.top_k ? 0 : __ldca(a.top_k + r);
-  const float min_p = greedy || !a.min_p ? 0.f : __ldca(a.min_p + r);
-  const bool by_p = top_p < 1.f, by_k = top_k > 0 && top_k < a.vocab;
-  const u64 least = !(min_p > 0.f) ? 0 : min_p >= 1.f ? kOne : __double2ull_ru(min_p * (double)kOne);
 
   // The stretch in chunks of 16 bytes, as they lie in memory: element 0 is the chunk 0's element `shift`, and what lies
   // before and behind counts as -infinity.
@@ -427,6 +424,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
         }
     }
     own = m;
+    if (threadIdx.x == 0) {  // (registers are short)
+      const float min_p = a.min_p ? __ldca(a.min_p + r) : 0.f;
+      s.coin = __ldca(a.coin + r);
+      s.top_p = a.top_p ? __ldca(a.top_p + r) : 1.f;
+      s.top_k = a.top_k ? __ldca(a.top_k + r) : 0;
+      s.least = !(min_p > 0.f) ? 0 : min_p >= 1.f ? kOne : __double2ull_ru(min_p * (double)kOne);
+    }
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) s.max[warp] = m;
     if (threadIdx.x == 0) s.block_first = a.vocab;
@@ -465,6 +469,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     cluster_sync_all();  // nobody leaves while others read its shared memory
     return;
   }
+  const bool by_p = s.top_p < 1.f, by_k = s.top_k > 0 && s.top_k < a.vocab;
   // A warp's part of the stretch; f is called by whole warps, with -infinity behind the end.
   const int part = (chunks + kWarps - 1) / kWarps, c0 = min(chunks, warp * part), c1 = min(chunks, c0 + part);
   auto chunk_at = [&](int c, int end) -> Chunk<T> {
@@ -519,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     before = before + Pair{upto.n - mine.n, upto.sum - mine.sum};
     if (!width) {  // the first histogram: it holds all weights
       of = total.sum;
-      goal = share_of(top_p, of);
+      goal = share_of(s.top_p, of);
     }
     if (threadIdx.x == 0) {
       s.order.what = Order::kNone;
@@ -531,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     for (int k = 0; k < kBinsPer; ++k) {
       const Pair after = before + bin[k];
       const int b = threadIdx.x * kBinsPer + k;
-      if (by_rank ? before.n < (unsigned)top_k && (unsigned)top_k <= after.n : before.sum < goal && goal <= after.sum) {
+      if (by_rank ? before.n < (unsigned)s.top_k && (unsigned)s.top_k <= after.n : before.sum < goal && goal <= after.sum) {
         Order o;
         o.what = !width && after.n <= kList ? Order::kGather : Order::kSelect;
         o.by_rank = by_rank;
@@ -631,12 +636,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
           larger += more;
           before += more ? weights[j] : 0;
         }
-      bool keep = i < listed && (!by_rank || larger < top_k);
+      bool keep = i < listed && (!by_rank || larger < s.top_k);
       if (by_p) {
         const u64 all = by_rank ? block_sum(s, keep ? weight[0] : 0) : of;
-        keep = keep && before < share_of(top_p, all);
+        keep = keep && before < share_of(s.top_p, all);
       }
-      keep = keep && weight[0] >= least && weight[0];
+      keep = keep && weight[0] >= s.least && weight[0];
       __syncthreads();
       if (i < listed) weights[i] = keep ? weight[0] : 0;
       __syncthreads();
@@ -645,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
           sum += weights[j];
           lower += (unsigned)s.list[j] > (unsigned)v[0] ? weights[j] : 0;  // (indices are held inverted)
         }
-        const u64 share = share_of(coin, sum);
+        const u64 share = share_of(s.coin, sum);
         if (lower < share && share <= lower + weight[0])
           answer((int)~(unsigned)v[0], (float)((double)weight[0] / (double)sum));
       }
@@ -661,22 +666,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
       }
       return sum;
     };
-    if (by_rank && top_k < listed) {
+    if (by_rank && s.top_k < listed) {
       all_from();
-      from = select(s, x, weight, true, (unsigned)top_k, 0);
+      from = select(s, x, weight, true, (unsigned)s.top_k, 0);
     }
     if (by_p) {
       u64 sum = all_from();
       if (by_rank) of = block_sum(s, sum);
-      from = select(s, x, weight, false, 0, share_of(top_p, of));
+      from = select(s, x, weight, false, 0, share_of(s.top_p, of));
     }
     u64 mine = 0;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {  // in the order of the row
-      x[e] = v[e] && v[e] >= from && weight[e] >= least && weight[e] ? v[e] << 32 | v[e] >> 32 : 0;
+      x[e] = v[e] && v[e] >= from && weight[e] >= s.least && weight[e] ? v[e] << 32 | v[e] >> 32 : 0;
       mine += x[e] ? weight[e] : 0;
     }
-    const u64 sum = block_sum(s, mine), at = select(s, x, weight, false, 0, share_of(coin, sum));
+    const u64 sum = block_sum(s, mine), at = select(s, x, weight, false, 0, share_of(s.coin, sum));
 #pragma unroll
     for (int e = 0; e < kEach; ++e)
       if (v[e] && (v[e] << 32 | v[e] >> 32) == at) answer((int)~(unsigned)v[e], (float)((double)weight[e] / (double)sum));
@@ -709,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     limit_l = value_of((unsigned)(limit >> 32));
     limit_i = (int)~(unsigned)limit;
   };
-  const double least_above = kUnits + (double)least;
+  const double least_above = kUnits + (double)s.least;
   bool summed = false;  // s.lo holds the sums of what the warps' parts of the row keep
   if (by_p && !by_k) {
     // One histogram of about the weights, an atomic a logit, says in which bin the limit should lie; then a pass sums
@@ -778,7 +783,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
         }
         const bool fits = s.listed <= kList;
         take_list();
-        const u64 goal = share_of(top_p, sum), here = block_sum(s, (weight[0] + weight[1]) + (weight[2] + weight[3]));
+        const u64 goal = share_of(s.top_p, sum), here = block_sum(s, (weight[0] + weight[1]) + (weight[2] + weight[3]));
         u64 at = 0;
         if (whole) {
           at = fits && goal <= here ? sum : 0;
@@ -808,7 +813,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
         // the listed ones that are kept, to the sum of the warp whose part they are in
         auto add = [&](u64 place, u64 of) {
           const int i = (int)~(unsigned)place - i0;
-          if (place >= limit && of >= least && i < n) add_to_bin(s, (i + shift) / kVec / part, of);
+          if (place >= limit && of >= s.least && i < n) add_to_bin(s, (i + shift) / kVec / part, of);
         };
         if (rank == 0) {
 #pragma unroll
@@ -884,7 +889,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     pick(floor_l, ceiling_l, [&](int i, float l) { return (!limit || in_limit(i, l)) && in_range(l, place_of(l, i)); });
     if (rank == 0) {
       take_list();
-      const u64 at = select(s, v, weight, by_rank, (unsigned)top_k - o.before.n, o.goal - o.before.sum);
+      const u64 at = select(s, v, weight, by_rank, (unsigned)s.top_k - o.before.n, o.goal - o.before.sum);
       if (threadIdx.x == 0) s.told = at;
     }
     cluster_sync_all();
@@ -940,7 +945,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     before = __shfl_sync(0xffffffffu, upto - here, rank);
     all = __shfl_sync(0xffffffffu, upto, 31);
   }
-  const u64 share = share_of(coin, all);
+  const u64 share = share_of(s.coin, all);
   if (before < share && share <= before + sum) {  // the token is in this block
     int owner = 0;
     while (share > before + s.lo[owner]) before += s.lo[owner++];
