@@ -10,14 +10,21 @@
 //
 // A cluster of blocks has a row, each block a stretch of it, which is read once into shared memory (rows too long for
 // that are read again, from L2); every later pass reads that.  The limits are found on a histogram of the distance
-// to the maximum, 16 bins an octave of the weight, whose bins are stretches of the sorted order: of counts for top-k,
-// which needs no weights, of counts and sums for top-p alone.  The cluster's first block merges the blocks' bins.
-// Where the limit's bin and all before it hold at most kList tokens, as a usual top-k or top-p has, they are listed in
-// the first block, and the rest happens there: by comparing each with each where they are few, else by histograms of
+// to the maximum, 16 bins an octave of the weight, whose bins are stretches of the sorted order:
+//   top-k: of counts of maxima of parts of the row, which need no weights; what lies above the limit's bin is listed;
+//   top-p alone: of about the weights, in 32 bits, one atomic a logit; then one pass of exact sums (all, those before the
+//     limit's bin, those that are kept by warp) that lists the bin, or all up to it where they are few.  The sums tell
+//     whether the bin was the right one.  (Exact weights in the histogram took four atomics a logit, 17 us of 63 for 64
+//     rows of 131072, and a further pass over them.)
+//   what does not fit the list, kList tokens in the first block: by exact histograms, of the limit's own range of (value,
+//     place in the row, as one 64-bit number) until it does.
+// A list is worked on in the first block: by comparing each with each where they are few, else by histograms of
 // the list's own range, which a round or three narrow down to one token.  (Sorting the list took 2.5 us for 64 tokens and
-// 8 to 13 us for 2048, twice.)  Else the limit's place is narrowed down by histograms of the range (value, then place
-// in the row, as one 64-bit number) until at most kList tokens are in it, and the draw is one more pass over the row in
-// its order.
+// 8 to 13 us for 2048, twice.)  Without such a list the draw is a pass over the row in its order.
+//
+// What it costs: bytes for the largest logit alone (temperature 0: 64 rows of 131072 in 16 bits 6.6 us), else about 39
+// instructions a logit for a weight in 64 bits and its sum (26 us), 15 more and an atomic for top-p (50 to 55), and 5 to
+// 10 phases of a cluster, about 1 us each (one row of 32000: 3.8 us at temperature 0, 7.7 without limits, 9 with top-k).
 #include "sample_rows.cuh"
 
 #include <cuda_bf16.h>
@@ -40,6 +47,7 @@ constexpr int kOctaves = 44, kPerOctave = 16, kBins = kOctaves * kPerOctave;
 constexpr int kEach = 4, kList = kThreads * kEach;  // tokens of a list: 4 a thread
 constexpr int kBinsPer = (kBins + kThreads - 1) / kThreads;
 constexpr int kShortList = 128;
+constexpr int kMaxima = 4;  // of a thread, of each fourth chunk that it reads
 constexpr int kPart = 14;  // kMostLogits of 2^kPart, and 2 % more, fit 32 bits
 constexpr int kRounds = 8;  // kBins^7 is more than 2^64, the places that a range may have
 constexpr u64 kOne = 1ull << 43;                    // the largest weight
@@ -408,8 +416,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
   w.prepare(temp);
   float own;  // the largest logit that this thread has read
   {
-    float m = -INFINITY;
-    constexpr int kAhead = 4;
+    constexpr int kAhead = kMaxima;
+    float part[kMaxima];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) part[k] = -INFINITY;
     for (int c = threadIdx.x; c < chunks; c += kThreads * kAhead) {
       Chunk<T> v[kAhead];
 #pragma unroll
@@ -420,9 +430,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
         if (c + k * kThreads < chunks) {
           if (kStaged) stage[c + k * kThreads] = v[k].raw;
 #pragma unroll
-          for (int j = 0; j < kVec; ++j) m = fmaxf(m, v[k][j]);
+          for (int j = 0; j < kVec; ++j) part[k] = fmaxf(part[k], v[k][j]);
         }
     }
+    reinterpret_cast<float4*>(s.list)[threadIdx.x] = make_float4(part[0], part[1], part[2], part[3]);
+    float m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
     own = m;
     if (threadIdx.x == 0) {  // (registers are short)
       const float min_p = a.min_p ? __ldca(a.min_p + r) : 0.f;
@@ -687,11 +699,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
       if (v[e] && (v[e] << 32 | v[e] >> 32) == at) answer((int)~(unsigned)v[e], (float)((double)weight[e] / (double)sum));
   };
   if (by_k) {
-    // The k-th largest of the threads' maxima is no larger than the k-th largest logit, and few tokens lie between the
-    // two: a histogram of 512 maxima a block instead of all its logits.
+    // The k-th largest of the threads' maxima, of every fourth chunk each, is no larger than the k-th largest logit, and few
+    // tokens lie between the two: a histogram of 2048 maxima a block instead of all its logits.  (With one maximum a
+    // thread, 1000 tokens of 61 rows of 49999 in 2 blocks a row took 34 us.)
     clear_bins(s, false);
     __syncthreads();
-    if (w.some(own)) atomicAdd(&s.count[w.bin(own)], 1u);
+    const float4 part = reinterpret_cast<const float4*>(s.list)[threadIdx.x];
+    for (const float l : {part.x, part.y, part.z, part.w})
+      if (w.some(l)) atomicAdd(&s.count[w.bin(l)], 1u);
     find(true, Pair{0, 0}, 0, 0, 0, 0, 0);
     const Order o = *told;
     if (o.what == Order::kGather) {
@@ -1002,10 +1017,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
 
 template <typename T>
 cudaError_t launch(const SampleRowsArgs& a, int device, int n_sms, cudaStream_t s) {
-  // Blocks a row, the cheapest of 1 to 8 by what was measured (in us): a wave of blocks takes 3.2 (4.2 and 5.2 in clusters
-  // of 4 and 8) and 0.39 for each 1000 logits that an SM's blocks have, 0.5 if there is one alone, 1.15 times as much for
-  // rows that shared memory does not take.  61 rows of 49999: 16 us with 4 blocks a row, 23 with 8; 64 rows of 131072 in
-  // 16 bits: 28 and 34; 256 rows of 32000: 28 with one, 68 with 8.
+  // Blocks a row, the cheapest of 1 to 8 by what was measured without limits (in us): a wave of blocks takes 6.5 to 6.8 (8 in
+  // clusters of 8 that fill more than half of the SMs) and 0.29 for each 1000 logits of a block, 0.32 if other waves
+  // follow, 0.57 if an SM has two blocks, 1.15 times as much for rows in 32 bits that shared memory does not take.  The last
+  // wave counts by its part.  Clusters of 4 that have their SMs for themselves, and those of 8, leave an eighth of
+  // the places empty.  (Where 2 and 4 are near, rows of mixed settings gain by 4: 61 of 49999 33 with 2, 31 with 4.)  Measured with 1, 2, 4, 8 blocks a row: 61 rows of 49999: 24, 14.8, 16, 23; 64 of 131072 in 16 bits: 44, 26, 26,
+  // 37; 256 of those: 81, 101, 94, 128; 64 of 131072 in 32 bits: 51, 30, 34, 34; one row of 32000: 15.4, 11.6, 8.8, 7.7.
   int blocks = 1, stretch = 0;
   bool staged = false;
   float best = FLT_MAX;
@@ -1014,10 +1031,13 @@ cudaError_t launch(const SampleRowsArgs& a, int device, int n_sms, cudaStream_t 
     const int st = ((a.vocab + c - 1) / c + 31) / 32 * 32;
     if (st > kMostLogits) continue;
     const size_t bytes = (size_t)st * sizeof(T) + 32;
-    const bool in = bytes <= kMaxStage;
-    const int per_sm = in && bytes > kMaxStage / 2 ? 1 : 2, waves = (int)(((long long)a.rows * c + n_sms * per_sm - 1) / (n_sms * per_sm));
-    const bool alone = per_sm == 1 || (long long)a.rows * c <= n_sms;
-    const float t = waves * ((c < 4 ? 3.2f : c < 8 ? 4.2f : 5.2f) + st * (alone ? 0.5e-3f : 0.78e-3f) * (in ? 1.f : 1.15f));
+    const bool in = bytes <= kMaxStage, one = in && bytes > kMaxStage / 2;  // one: block on an SM
+    const float all = (float)a.rows * c, places = (one ? 1.f : 2.f) * n_sms * (c == 8 || (c == 4 && one) ? 0.875f : 1.f);
+    const float waves = all <= places ? 1.f : 0.45f * ceilf(all / places) + 0.55f * all / places;
+    const bool alone = all <= (c == 8 ? 0.5f : 1.f) * n_sms;
+    const float start = c == 1 ? 6.5f : c < 8 || alone ? 6.8f : 8.f;
+    const float each = (alone ? 0.29e-3f : one ? 0.32e-3f : 0.57e-3f) * (in || sizeof(T) == 2 ? 1.f : 1.15f);
+    const float t = waves * (start + (float)st * each);
     if (t < best) best = t, blocks = c, stretch = st, staged = in;
   }
   const size_t bytes = (size_t)stretch * sizeof(T) + 32;
