@@ -23,8 +23,8 @@
 // 8 to 13 us for 2048, twice.)  Without such a list the draw is a pass over the row in its order.
 //
 // What it costs: bytes for the largest logit alone (temperature 0: 64 rows of 131072 in 16 bits 6.6 us), else about 39
-// instructions a logit for a weight in 64 bits and its sum (26 us), 15 more and an atomic for top-p (50 to 55), and 5 to
-// 10 phases of a cluster, about 1 us each (one row of 32000: 3.8 us at temperature 0, 7.7 without limits, 9 with top-k).
+// instructions a logit for a weight in 64 bits and its sum (26 us), 105 in all for top-p (50 to 55), and 5 to 10 phases of
+// a cluster, about 1 us each (one row of 32000: 3.8 us at temperature 0, 7.7 without limits, 9 with top-k).
 #include "sample_rows.cuh"
 
 #include <cuda_bf16.h>
