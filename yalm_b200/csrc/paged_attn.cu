@@ -140,6 +140,9 @@ __device__ void find_start(const PagedBatch& b, const Axis& x, unsigned long lon
 // The same from a plan in the workspace, by one warp.
 __device__ void find_start(const SharedBatch& b, const SharedHead* head, const Axis& x, StartOf<SharedSeq>* s_start) {
   const int lane = threadIdx.x & 31, c = blockIdx.x;
+  // (the search's first round is on its way beside the head)
+  const int step0 = (b.n_seqs + 31) / 32, at0 = (lane + 1) * step0;
+  const unsigned long long probe0 = at0 < b.n_seqs ? __ldcg(&b.seqs[at0].begin) : ~0ull;
   const unsigned long long total = __ldcg(&head->total), share = __ldcg(&head->share);
   const int more = __ldcg(&head->more);
   const unsigned long long begin = block_begin(share, more, c);
@@ -148,7 +151,7 @@ __device__ void find_start(const SharedBatch& b, const SharedHead* head, const A
     return;
   }
   // the last prefix or sequence that begins at or before the block: one that begins there and has no length comes earlier
-  int lo = 0, hi = b.n_seqs;
+  int lo = __popc(__ballot_sync(0xffffffffu, probe0 <= begin)) * step0, hi = min(b.n_seqs, lo + step0);
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
     const bool le = at < hi && __ldcg(&b.seqs[at].begin) <= begin;

@@ -84,14 +84,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) paged_few_kernel(const __grid_
   const int warp = blockIdx.x * kFewWarps + (threadIdx.x >> 5);
   pdl_wait();
   pdl_trigger();  // the attention kernel beside this one needs no more than the plan, which is there
+  // (the search's first round is on its way beside the head)
+  const int step0 = (a.shared.n_seqs + 31) / 32, at0 = (lane + 1) * step0;
+  const u64 probe0 = at0 < a.shared.n_seqs ? __ldca(&a.shared.seqs[at0].few_begin) : ~0ull;
   const u64 total = __ldca(&a.head->few_total), share = __ldca(&a.head->few_share);
   const int more = __ldca(&a.head->few_more);
   const u64 begin = block_begin(share, more, warp);
   if (begin >= total) return;
   int left = (int)min(share + (warp < more ? 1 : 0), total - begin);
   // the last sequence that begins at or before this warp's part: those without rows here that begin there come earlier
-  int seq = 0;
-  for (int hi = a.shared.n_seqs; hi - seq > 1;) {
+  int seq = __popc(__ballot_sync(0xffffffffu, probe0 <= begin)) * step0;
+  for (int hi = min(a.shared.n_seqs, seq + step0); hi - seq > 1;) {
     const int step = (hi - seq + 31) / 32, at = seq + (lane + 1) * step;
     const int n = __popc(__ballot_sync(0xffffffffu, at < hi && __ldca(&a.shared.seqs[at].few_begin) <= begin));
     seq += n * step;

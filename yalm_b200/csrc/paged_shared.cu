@@ -32,6 +32,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = b.n_heads / b.n_kv_heads;
   pdl_trigger();  // the next kernel waits for this one's end
   pdl_wait();
+  // (on its way beside the groups)
+  const PagedSeq ahead = (int)threadIdx.x < b.n_seqs ? paged_seq(b, threadIdx.x) : PagedSeq{};
   for (int g = threadIdx.x; g <= a.n_groups; g += kThreads) {
     s_start[g] = min(max(__ldca(a.group_start + g), 0), b.n_seqs);
     if (g < a.n_groups) {
@@ -55,7 +57,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_shared_plan_kernel(const __
   for (int g = threadIdx.x; g <= a.n_groups; g += kThreads) s_row0[g] = row_of(s_start[g]);
   auto rows_of = [&](int g) { return s_start[g + 1] > s_start[g] ? max(s_row0[g + 1] - s_row0[g], 0) : 0; };
   for (int s = threadIdx.x; s < b.n_seqs; s += kThreads) {
-    const PagedSeq q = paged_seq(b, s);
+    const PagedSeq q = s == (int)threadIdx.x ? ahead : paged_seq(b, s);
     const int g = q.n > 0 ? group_of(s) : -1;
     if (g >= 0) {
       atomicMin(&s_cut[g], q.kv - q.n);
