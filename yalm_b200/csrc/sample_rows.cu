@@ -220,6 +220,9 @@ struct Shared {
   Pair warps[kWarps];
   u64 sums[kWarps], lo[kWarps], hi[kWarps];
   u64 block_sum, told;
+  // What the first block found, for the others.  Nothing that it does by itself after cluster_arrive (finish, and select,
+  // which has `told` for its own threads) writes this or `listed`: the others may read them as late as they leave.
+  u64 verdict;
   Pair found_before;
   unsigned mine;  // tokens that the block has listed for the first one
   u64 weights, before;  // of the block's logits: all, those of the bins before the limit's
@@ -808,11 +811,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
           for (int e = 0; e < kEach; ++e) x[e] = v[e];
           at = select(s, x, weight, false, 0, goal - prior);
         }
-        if (threadIdx.x == 0) s.told = at;
+        if (threadIdx.x == 0) s.verdict = at;
       }
       if (threadIdx.x < kWarps && rank) s.low[threadIdx.x] = s.mid[threadIdx.x] = s.high[threadIdx.x] = 0;
       cluster_sync_all();
-      const u64 at = *dsmem_ptr(&s.told, 0);
+      const u64 at = *dsmem_ptr(&s.verdict, 0);
       if (at && whole) {
         cluster_arrive();
         if (rank == 0) finish(false, at);
@@ -905,10 +908,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     if (rank == 0) {
       take_list();
       const u64 at = select(s, v, weight, by_rank, (unsigned)s.top_k - o.before.n, o.goal - o.before.sum);
-      if (threadIdx.x == 0) s.told = at;
+      if (threadIdx.x == 0) s.verdict = at;
     }
     cluster_sync_all();
-    set_limit(*dsmem_ptr(&s.told, 0));
+    set_limit(*dsmem_ptr(&s.verdict, 0));
   }
   // ---- the draw, in the order of the row
   // Sums of a thread's weights, up to kMostLogits / 512 of them, are whole numbers of 64-bit floating point.
