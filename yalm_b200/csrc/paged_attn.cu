@@ -652,15 +652,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     make_uint4(pack2<T>(v[8 * k], v[8 * k + 1]), pack2<T>(v[8 * k + 2], v[8 * k + 3]),
                                pack2<T>(v[8 * k + 4], v[8 * k + 5]), pack2<T>(v[8 * k + 6], v[8 * k + 7]));
             } else {
-              float4* o = reinterpret_cast<float4*>(to_rec) + (size_t)(c0 / 4) * to_rows + to_at;
+              float4* o = reinterpret_cast<float4*>(to_rec + record_sum(to_rows, to_at, c0 / 4));
 #pragma unroll
               for (int k = 0; k < 8; ++k) o[(size_t)k * to_rows] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
             }
           }
         }
         if (!final && valid) {
-          to_rec[(size_t)HD * to_rows + to_at] = m;
-          to_rec[(size_t)(HD + 1) * to_rows + to_at] = l;
+          to_rec[record_m(HD, to_rows, to_at)] = m;
+          to_rec[record_l(HD, to_rows, to_at)] = l;
         }
         tc_fence_before();
         __syncwarp();
@@ -976,7 +976,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     int n;
     const float *first, *rest;  // rest: the second one's
     size_t next;                // floats from that to the one after it
-    int step, ml;               // where m is, and l is step floats from there
+    RecordRow row;
   };
   // of the tensor-core kernel
   auto of_unit = [&](const SharedSeq& q, unsigned per_head, int head, int token, int h) {
@@ -989,11 +989,10 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     const bool whole = p.n == 1;
     const int rs = whole ? a.part_rows : u.nq * a.gq, r = whole ? (q.part + at) * a.gq + h : (at - u.q0) * a.gq + h;
     p.first = (whole ? a.parts + (size_t)((q.all ? 0 : a.x.K) + head) * (HD + 2) * rs
-                     : a.recs + ((size_t)block * 2 + 1) * rec_floats<HD>()) + 4 * (size_t)r;
-    p.rest = a.recs + (size_t)(block + 1) * 2 * rec_floats<HD>() + 4 * (size_t)r;
+                     : a.recs + ((size_t)block * 2 + 1) * rec_floats<HD>()) + record_sum(rs, r, 0);
+    p.rest = a.recs + (size_t)(block + 1) * 2 * rec_floats<HD>() + record_sum(rs, r, 0);
     p.next = 2 * rec_floats<HD>();
-    p.step = rs;
-    p.ml = HD * rs - 3 * r;  // from 4 r on
+    p.row = record_row(HD, rs, r);
     return p;
   };
   // of the kernel of few rows
@@ -1007,8 +1006,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
                        : a.few_recs + ((size_t)warp * 2 + 1) * rec + row;
     p.rest = a.few_recs + (size_t)(warp + 1) * 2 * rec + row;
     p.next = 2 * rec;
-    p.step = 1;
-    p.ml = HD;
+    p.row = RecordRow{1, HD};
     return p;
   };
   const int warps = gridDim.y * (kJoinThreads / 32);
@@ -1040,14 +1038,15 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
           const int i = p0 + e;
           if (i >= n) continue;
           const bool second = i >= one.n;
-          const int part = second ? i - one.n : i, step = second ? two.step : one.step, ml = second ? two.ml : one.ml;
+          const int part = second ? i - one.n : i, step = second ? two.row.step : one.row.step;
+          const long long m_at = second ? two.row.m : one.row.m;
           const float* rec = part ? (second ? two.rest : one.rest) + (part - 1) * (second ? two.next : one.next)
                                   : second ? two.first : one.first;
 #pragma unroll
           for (int k = 0; k < kN; ++k)
             if (f0 + k * lanes < kF) o[e][k] = __ldcg(reinterpret_cast<const float4*>(rec) + (size_t)(f0 + k * lanes) * step);
-          m[e] = __ldcg(rec + ml);
-          l[e] = __ldcg(rec + ml + step);
+          m[e] = __ldcg(rec + m_at);
+          l[e] = __ldcg(rec + m_at + step);
         }
         float mn = mm;
 #pragma unroll

@@ -49,6 +49,19 @@ __device__ __forceinline__ unsigned head_tiles(const Axis& x, const SharedSeq& q
   return units_before(x, q, nu - 1) + (unsigned)unit_of(x, q, nu - 1).cost + kUnitTiles;
 }
 
+// ---- records of rows whose sums other parts join: head_dim sums as float4, then m, then l, each of all `rows` side by
+// side.  Places in floats; a record of parts has up to 2^24 rows, 2^31 sums of head_dim 128.
+__device__ __forceinline__ size_t record_sum(int rows, int r, int k) { return 4 * ((size_t)k * rows + r); }  // float4 k
+__device__ __forceinline__ size_t record_m(int head_dim, int rows, int r) { return (size_t)head_dim * rows + r; }
+__device__ __forceinline__ size_t record_l(int head_dim, int rows, int r) { return (size_t)(head_dim + 1) * rows + r; }
+// The same from the row's float4 0 on, as the join goes through it: the next float4 `step` float4 further, m at `m`, l `step`
+// floats behind that.
+struct RecordRow {
+  int step;
+  long long m;
+};
+__device__ __forceinline__ RecordRow record_row(int head_dim, int rows, int r) { return {rows, (long long)head_dim * rows - 3ll * r}; }
+
 // ---- few rows: a unit is (sequence, kv head), all its rows at once
 constexpr int kFewRows = 8;     // tokens x query heads of a kv head
 constexpr int kFewSlots = 16;   // slots of a step: of one page
