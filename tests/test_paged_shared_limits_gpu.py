@@ -43,3 +43,24 @@ def test_room_for_the_most_tokens_and_heads(gpu):
         tol = u * o.abs() + (u + 2.0 ** -16 + 2 * 2.0 ** -20 * mag) * (w @ values.abs()) + TINY
         assert ((out[s].double().view(16, hd) - o).abs() <= tol).all(), s
     assert (out[live:] == 7).all()
+
+
+@pytest.mark.parametrize("width", [8, 60000])  # of the table: prefixes are computed apart with the second
+@pytest.mark.parametrize("host", ["group_start", "prefix_len"])
+def test_groups_are_the_devices_memory_whatever_the_batch(gpu, width, host):
+    import torch
+    from yalm_b200 import _lib
+    i32 = dict(dtype=torch.int32, device="cuda")
+    k = torch.zeros(8, 2, 16, 64, dtype=torch.float16, device="cuda")
+    b = PagedBatch(k, k.clone(), torch.zeros(3, width, **i32), torch.arange(4, **i32), torch.full((3,), 20, **i32), 4, 3)
+    q = torch.zeros(3, 256, dtype=torch.float16, device="cuda")
+    out, scratch = torch.empty_like(q), torch.zeros(b.shared_scratch_bytes(1), dtype=torch.uint8, device="cuda")
+    t = dict(group_start=torch.tensor([0, 3], **i32), prefix_len=torch.tensor([16], **i32))
+
+    def call():
+        return _lib.lib().yb_paged_attention_shared_dev(b._ref, 1, t["group_start"].data_ptr(), t["prefix_len"].data_ptr(),
+                                                        out.data_ptr(), 256, q.data_ptr(), 256, 0.125, scratch.data_ptr(), None)
+    torch.cuda.synchronize()
+    assert call() == 0 and b.status(scratch) == 0
+    t[host] = t[host].cpu()
+    assert call() == _lib.YB_E_INVALID and host in _lib.last_error()

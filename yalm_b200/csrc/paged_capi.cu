@@ -260,18 +260,18 @@ extern "C" int yb_paged_attention_shared_dev(const yb_paged_batch* b, int n_grou
   if (rc) return rc;
   if (n_groups && (!group_start_dev || !prefix_len_dev || !aligned4(group_start_dev) || !aligned4(prefix_len_dev)))
     return set_error(YB_E_INVALID, "group_start_dev and prefix_len_dev must be 4-byte aligned buffers");
-  // Where nothing is shared, or reading it once can save no more than 64 MB (every sequence's whole table but one), its
-  // kernels cost more than they save.  32 heads of 128 on 8 kv heads, prefix of 4096 and 100 own slots: 4 sequences (50
-  // MB) 19.4 us without, 32.9 with; 8 (117 MB) 27.1 and 31.3; 16 (252 MB) 42.9 and 31.5.  8 heads of 64 on 2: 32 (65 MB)
-  // 24.3 and 25.2, 64 (132 MB) 37.7 and 25.3.
-  if (b && b->n_seqs > 0 && (b->n_seqs - 1.0) * b->max_pages * b->page_size * b->n_kv_heads * b->head_dim * 4.0 < 64e6) n_groups = 0;
   if (n_groups == 0)
     return yb_paged_attention_dev(b, out, out_stride, q, q_stride, scale, 0, scratch_dev, stream);
   PagedAttnArgs a{};
   bool empty = false;
   if ((rc = check_attention(b, &a, &empty, out, out_stride, q, q_stride, scale, scratch_dev))) return rc;
   if (empty) return 0;
-  if ((rc = check_share(b, a.b, current_device(), n_groups))) return rc;
+  // Where reading a prefix once can save no more than 64 MB (every sequence's whole table but one), the kernels for it
+  // cost more than they save.  32 heads of 128 on 8 kv heads, prefix of 4096 and 100 own slots: 4 sequences (50
+  // MB) 19.4 us without, 32.9 with; 8 (117 MB) 27.1 and 31.3; 16 (252 MB) 42.9 and 31.5.  8 heads of 64 on 2: 32 (65 MB)
+  // 24.3 and 25.2, 64 (132 MB) 37.7 and 25.3.
+  const bool apart = (b->n_seqs - 1.0) * b->max_pages * b->page_size * b->n_kv_heads * b->head_dim * 4.0 >= 64e6;
+  if ((rc = check_share(b, a.b, current_device(), apart ? n_groups : 0))) return rc;
   int dev = 0;
   YB_CK(cudaGetDevice(&dev));
   if ((rc = check_attention_device(dev, b, out, q, scratch_dev)) ||
@@ -282,6 +282,8 @@ extern "C" int yb_paged_attention_shared_dev(const yb_paged_batch* b, int n_grou
   a.prefix_len = prefix_len_dev;
   a.n_groups = n_groups;
   a.n_sms = device_sms(dev);
-  YB_CK(paged_attention_shared(a, b->head_dim, b->dtype, dev, static_cast<cudaStream_t>(stream)));
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  YB_CK(apart ? paged_attention_shared(a, b->head_dim, b->dtype, dev, s)
+              : paged_attention(a, b->head_dim, b->dtype, dev, a.n_sms, s));
   return 0;
 }
