@@ -170,12 +170,18 @@ struct Weights {
     return (u64)__double_as_longlong(above(l)) - 0x4330000000000000ull;
   }
 };
-// the least whole sum that is at least x * sum, 1 .. sum
+// The least whole sum that is at least x * sum, 1 .. sum: in whole numbers, x = m 2^-d with 24 bits m, since a sum of up to 2^63
+// does not fit the 53 bits of a 64-bit floating-point number.
 __device__ __forceinline__ u64 share_of(float x, u64 sum) {
   if (!(x > 0.f)) return 1;
   if (x >= 1.f) return sum;
-  const u64 v = __double2ull_ru((double)x * __ull2double_rn(sum));
-  return v < 1 ? 1 : v < sum ? v : sum;
+  const unsigned u = __float_as_uint(x), e = u >> 23;
+  const u64 m = e ? (u & 0x7fffffu) | 0x800000u : u;
+  const unsigned d = 150 - (e ? e : 1);  // 24 .. 149
+  const u64 lo = m * sum, hi = __umul64hi(m, sum);  // hi < 2^24
+  if (d >= 88) return 1;  // the whole product is below 2^87
+  if (d >= 64) return (hi >> (d - 64)) + (lo || (hi & ((1ull << (d - 64)) - 1)));
+  return (hi << (64 - d) | lo >> d) + ((lo & ((1ull << d) - 1)) != 0);
 }
 
 struct Pair {
