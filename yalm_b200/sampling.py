@@ -27,7 +27,8 @@ def sample_rows(logits, coin, tokens, *, prob=None, temperature=None, top_k=None
     global _stream
     if _stream is None:
         import torch
-        _stream, _codes["f32"], _codes["i32"] = _raw_stream(), torch.float32, torch.int32
+        _codes["f32"], _codes["i32"] = torch.float32, torch.int32
+        _stream = _raw_stream()  # last: calls of other threads go by it
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits must be [rows][vocab] with unit column stride")
     rows, vocab = logits.shape
