@@ -412,7 +412,9 @@ size_t yb_paged_attention_scratch_bytes(const yb_paged_batch* b); /* 0 for a bat
  * sequences fit a unit of 2 * floor(128 * n_kv_heads / n_heads) queries, in batches whose n_seqs - 1 other rows of the
  * table span 64 MB of the cache at least.  With n_groups 0 it is that call.
  * scratch_dev: yb_paged_attention_shared_scratch_bytes(b, n_groups) bytes, 16-byte aligned, which also grows with
- * n_seqs and n_tokens; what is said of that call's workspace and of its first word holds here too. */
+ * n_seqs and n_tokens; what is said of that call's workspace and of its first word holds here too.
+ * Refused (YB_E_UNSUPPORTED) is a batch whose prefixes may be computed apart from a fifth of that call's share of work for
+ * one SM on, with n_groups and a second n_tokens / U added to the units. */
 int yb_paged_attention_shared_dev(const yb_paged_batch* b, int n_groups, const int* group_start_dev,
                                   const int* prefix_len_dev, void* out, long long out_stride, const void* q,
                                   long long q_stride, float scale, void* scratch_dev, void* stream);

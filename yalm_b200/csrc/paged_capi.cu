@@ -62,13 +62,15 @@ int check_rows(const char* name, const void* p, long long stride, long long widt
 // What one of the attention's blocks may have to walk is counted in 31 bits: the units (blocks of up to 2 * (128 /
 // query heads per kv head) queries) of every sequence and kv head, with the key tiles of 128 slots of the longest cache
 // and 3 more each, shared out over the blocks.
-// With `groups` > 0 shared prefixes, which are units of their own.
+// With `groups` > 0 shared prefixes, which are units of their own, two kernels share the blocks' SMs, by a choice (paged_shared.cu)
+// that lets neither take longer than half of the SMs would.  At its rates of 2.2 us a key tile and 0.08 us a step of few rows
+// (16 slots, 12 warps a block) a block then has up to twice this count of tiles, a warp up to 4.5 times as many steps.
 int check_share(const yb_paged_batch* b, const PagedBatch& p, int dev, int groups = 0) {
   const long long queries = 2 * (128 / (b->n_heads / b->n_kv_heads));
   long long units = b->n_tokens / queries + (b->n_seqs < b->n_tokens ? b->n_seqs : b->n_tokens);
   if (groups) units += b->n_tokens / queries + groups;
   const long long tiles = (((long long)b->max_pages << p.ps_log2) >> 7) + 3;
-  if (units * b->n_kv_heads * tiles / paged_attention_grid(device_sms(dev)) >= INT_MAX)
+  if (units * b->n_kv_heads * tiles / paged_attention_grid(device_sms(dev)) >= (groups ? INT_MAX / 5 : INT_MAX))
     return set_error(YB_E_UNSUPPORTED, "the batch may have too many slots to attend to on this device "
                                        "((n_tokens / queries of a unit + n_seqs) * n_kv_heads * max_pages * page_size)");
   return 0;
