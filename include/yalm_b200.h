@@ -420,8 +420,9 @@ int yb_paged_attention_shared_dev(const yb_paged_batch* b, int n_groups, const i
                                   long long q_stride, float scale, void* scratch_dev, void* stream);
 size_t yb_paged_attention_shared_scratch_bytes(const yb_paged_batch* b, int n_groups); /* 0: refused */
 
-/* Diagnostics: the SM clocks that a wait in the kernel of later yb_paged_attention_dev calls of this process may take
- * before it gives up (0: the default of 4e9, about 2 s, which is also the most).  A healthy wait takes microseconds. */
+/* Diagnostics: the SM clocks that a wait in the kernels of later yb_paged_attention_dev and yb_paged_attention_shared_dev
+ * calls of this process may take before it gives up (0: the default of 4e9, about 2 s, which is also the most).  What is
+ * still in flight after a wait has run out is waited for with the default.  A healthy wait takes microseconds. */
 int yb_paged_attention_wait_budget(long long clocks);
 
 /* ---------------------------------------------------------------- a token for every row of logits
