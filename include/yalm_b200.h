@@ -410,7 +410,7 @@ size_t yb_paged_attention_scratch_bytes(const yb_paged_batch* b); /* 0 for a bat
  * The result is that of yb_paged_attention_dev on the same batch, to the rounding of sums that are split in other
  * places; a prefix is computed apart only where that pays: whole tiles of 128 slots of it, for groups of which several
  * sequences fit a unit of 2 * floor(128 * n_kv_heads / n_heads) queries, in batches whose n_seqs - 1 other rows of the
- * table span 64 MB of the cache at least.  With n_groups 0 it is that call.
+ * table span 64 MB of the cache at least (by their width, whatever they hold).  With n_groups 0 it is that call.
  * scratch_dev: yb_paged_attention_shared_scratch_bytes(b, n_groups) bytes, 16-byte aligned, which also grows with
  * n_seqs and n_tokens; what is said of that call's workspace and of its first word holds here too.
  * Refused (YB_E_UNSUPPORTED) is a batch whose prefixes may be computed apart from a fifth of that call's share of work for

@@ -782,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (pc.u.none) continue;
       const bool two = pc.u.nq > QB;
       const int first = pc.u.tile0 + pc.t0, nk = pc.t1 - pc.t0, n = two ? 2 * nk : nk;
-      const int qb = two ? p : buf;
+      const int qb = query_buffer(two, p, buf);
       // each pipeline's warp keeps count of both buffers, whichever it reads
       for (int t = two ? 0 : buf; t <= (two ? 1 : buf); ++t) {
         if (t == qb) wait(&q_full[t], uses[t] & 1);
@@ -835,8 +835,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         umma_commit_if(e, &s_full[p][u]);
         if (ends(i)) umma_commit_if(e, &empty[kslot]);
         if (i == n - 1) {
-          umma_commit_if(e, &q_empty[two ? 0 : qb]);
-          if (two) umma_commit_if(e, &q_empty[1]);
+          umma_commit_if(e, &q_empty[qb]);
+          if (query_releases(two) == 2) umma_commit_if(e, &q_empty[qb]);
         }
       };
       // a buffer of S is free again once the product that reads P from it is issued: they execute in order

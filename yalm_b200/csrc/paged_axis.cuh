@@ -130,6 +130,13 @@ __device__ __forceinline__ int block_of(unsigned long long share, int more, unsi
   return x < cut ? (int)quot(x, share + 1) : more + (int)quot(x - cut, share);
 }
 
+// The block's two query buffers.  A unit of two row tiles has one tile in each, which that pipeline alone reads; a unit of one
+// has them in turn, and both pipelines read it.  A buffer is free again after two arrivals, one of each that reads it or
+// two of the only one: an arrival of a pipeline that does not wait for the buffer could come for the next unit before the
+// other one's for this unit, and free it under that one's products.
+__device__ __forceinline__ int query_buffer(bool two, int pipeline, int turn) { return two ? pipeline : turn; }
+__device__ __forceinline__ int query_releases(bool two) { return two ? 2 : 1; }  // of a pipeline that has read its buffer
+
 // The next piece of this block's share: tiles [t0, t1) of a unit, of which the block has those from `from` on.
 template <typename Seq>
 struct PieceOf {

