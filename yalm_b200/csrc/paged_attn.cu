@@ -783,7 +783,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool two = pc.u.nq > QB;
       const int first = pc.u.tile0 + pc.t0, nk = pc.t1 - pc.t0, n = two ? 2 * nk : nk;
       const int qb = query_buffer(two, p, buf);
-      // each pipeline's warp keeps count of both buffers, whichever it reads
+      // each pipeline's warp keeps count of both buffers, whichever it reads.  (One that it did not wait for is full by then: the
+      // pipelines' softmaxes take turns, so this one has ended the unit before only after the other's products read it.)
       for (int t = two ? 0 : buf; t <= (two ? 1 : buf); ++t) {
         if (t == qb) wait(&q_full[t], uses[t] & 1);
         ++uses[t];
